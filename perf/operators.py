@@ -290,7 +290,8 @@ def _plain_distill(st):
     log_p = d.gather(1, ids) - torch.log(total)
     kl = torch.where(q > 0, q * (log_q - log_p), 0.0).sum(-1)
     grad = (e / total).scatter_add_(1, ids, torch.where(live, -q, 0.0))
-    w = st["weights"]
+    w = torch.where(live.any(-1), st["weights"], 0.0)  # a frame without alternatives teaches nothing
+    grad = torch.where(w[:, None] > 0, grad, 0.0)
     return [w * tau * tau * kl, (grad * (w * tau)[:, None]).to(_type(case))]
 
 
@@ -394,6 +395,8 @@ def _exact_logprobs(case, t, rows):
 def _exact_distill(case, t, rows):
     tau, lp = case["temperature"], _exact_logits(case, t, rows)
     ids, w = t["ids"][rows].long(), t["weights"][rows].double()
+    w[(ids < 0).all(-1)] = 0.0
+    ids[:, 0] = torch.where((ids < 0).all(-1), 0, ids[:, 0])
     lq = torch.log_softmax((t["scores"][rows].double() / tau).masked_fill(ids < 0, -math.inf), -1)
     q = lq.exp()
     full = torch.zeros_like(lp).scatter_add(1, ids.clamp_min(0), q)
