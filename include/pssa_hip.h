@@ -51,6 +51,9 @@ extern "C" {
 #define PSSA_HIP_F32 0
 #define PSSA_HIP_BF16 1
 
+/* "No token": a target that is not scored, a teacher entry or an alternative that is not there. */
+#define PSSA_HIP_NO_TOKEN 0xFFFFFFFFu
+
 /* Weight initialisation modes (pssa_hip_weights_init). */
 #define PSSA_HIP_INIT_REFERENCE 0 /* PSSALayerV2::new draw order, src/pssa.rs:2019-2072 */
 #define PSSA_HIP_INIT_BASELINE 1  /* seeded N(0, 0.02) for every matrix; log-spaced rates with
@@ -581,6 +584,65 @@ int pssa_hip_model_get_hybrid(pssa_hip_model* model, size_t layer, float* gate, 
  * arrays of `cap` entries (either may be NULL); returns the number of stages. */
 int pssa_hip_lanes_stage_times(pssa_hip_lanes* lanes, int enable, const char** names, float* ms,
                                size_t cap);
+
+/* --------------------------------------------- language-model operators
+ * On device-resident arrays (plain device pointers from any allocator),
+ * asynchronous on the context stream: work that other streams do on these
+ * arrays has to be complete before the call, and pssa_hip_synchronize
+ * completes it.  `dtype` is PSSA_HIP_F32 or PSSA_HIP_BF16; sums, statistics and states are
+ * fp32.  They have no counterpart in the reference's backend.
+ */
+
+/* Log probabilities of given tokens under log softmax(logits / temperature),
+ * with the distribution's entropy and its top alternatives.
+ * logits [rows, vocab], row r at d_logits + r*ld elements (ld >= vocab; rows
+ * may start at any element).  d_targets [rows] or NULL: d_logprobs[r] is the
+ * log probability of token d_targets[r], 0 for PSSA_HIP_NO_TOKEN, NaN for any
+ * other id >= vocab.  d_entropy [rows] (natural units) or NULL.  top_k <= 64:
+ * d_top_ids / d_top_logprobs [rows, top_k] list the tokens of the largest
+ * logits in descending order, equal logits by ascending id.
+ * A logit of -inf is a token that cannot occur: it has log probability -inf
+ * and is never an alternative (places left over hold PSSA_HIP_NO_TOKEN and
+ * -inf).  A row of nothing else has entropy 0.  A row with a NaN or +inf has
+ * NaN in every value and no alternatives.  temperature in [1e-6, 1e6]. */
+int pssa_hip_token_logprobs_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t rows, size_t vocab,
+                                     size_t ld, const uint32_t* d_targets, float temperature, size_t top_k,
+                                     float* d_logprobs, float* d_entropy, uint32_t* d_top_ids,
+                                     float* d_top_logprobs, char* err, size_t err_len);
+
+/* Distillation from a teacher's top logits, forward and backward: with q the
+ * softmax of the row's teacher entries / temperature and p that of the whole
+ * student row / temperature,
+ *   losses[r] = w_r temperature^2 sum_j q_j (log q_j - log p[id_j])
+ *   grad[r]   = d losses[r] / d logits[r] = w_r temperature (p - q).
+ * d_teacher_ids, d_teacher_logits [rows, teacher_k], teacher_k <= 1024; an
+ * entry with id PSSA_HIP_NO_TOKEN or logit -inf is none, an id listed twice
+ * has both entries' weight.  d_row_weights [rows] or NULL (1).  d_grad (the
+ * logits' type, row r at d_grad + r*ld_grad) or NULL for the loss alone; it
+ * may be d_logits itself with ld_grad = ld, and must not overlap it
+ * otherwise.  A row of weight 0, or without teacher entries, has loss 0 and
+ * gradient 0 whatever it holds.  A teacher's token whose student logit is
+ * -inf gives the loss +inf (and a finite gradient); a NaN or +inf among the
+ * student's or teacher's logits, or a teacher id >= vocab, makes the row's
+ * loss and gradient NaN.  temperature in [1e-6, 1e6]. */
+int pssa_hip_distill_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t rows, size_t vocab,
+                              size_t ld, const uint32_t* d_teacher_ids, const float* d_teacher_logits,
+                              size_t teacher_k, float temperature, const float* d_row_weights, float* d_losses,
+                              void* d_grad, size_t ld_grad, char* err, size_t err_len);
+
+/* The same on the logits that the last pssa_hip_batch_forward of these lanes
+ * left on the device, host arrays in and out, rows in that call's packed
+ * token order (n_tokens of them, which must be its token count).
+ * targets NULL: the batch's own targets.  Any output may be NULL. */
+int pssa_hip_batch_token_logprobs(pssa_hip_lanes* lanes, const uint32_t* targets, size_t n_tokens, float temperature,
+                                  size_t top_k, float* logprobs, float* entropy, uint32_t* top_ids,
+                                  float* top_logprobs, char* err, size_t err_len);
+/* teacher_ids, teacher_logits [n_tokens, teacher_k], row_weights [n_tokens]
+ * or NULL; losses [n_tokens], grad_logits [n_tokens, V] or NULL (the adjoint
+ * that the head's pssa_hip_gemm_nn and pssa_hip_gemm_tn_accumulate take). */
+int pssa_hip_batch_distill(pssa_hip_lanes* lanes, const uint32_t* teacher_ids, const float* teacher_logits,
+                           size_t n_tokens, size_t teacher_k, float temperature, const float* row_weights,
+                           float* losses, float* grad_logits, char* err, size_t err_len);
 
 #ifdef __cplusplus
 }

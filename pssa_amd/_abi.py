@@ -20,6 +20,7 @@ EUNSUPPORTED = -5
 
 F32 = 0
 BF16 = 1
+NO_TOKEN = 0xFFFFFFFF
 INIT_REFERENCE = 0
 INIT_BASELINE = 1
 H2D, D2H, D2D = 0, 1, 2
@@ -189,6 +190,12 @@ def lib() -> C.CDLL:
         "pssa_hip_lanes_stage_times": ([vp, C.c_int, C.POINTER(C.c_char_p), fp, sz], C.c_int),
         "pssa_hip_decode": ([vp, u32p, sz, sz, C.c_int, u32p, sz, fp, sz, err_t, sz], C.c_int),
         "pssa_hip_model_get_plastic": ([vp, sz, fp, fp, fp, fp, fp, u64p, u64p, u64p, u64p, err_t, sz], C.c_int),
+        "pssa_hip_token_logprobs_resident": ([vp, vp, C.c_int, sz, sz, sz, vp, C.c_float, sz, vp, vp, vp, vp, err_t, sz],
+                                             C.c_int),
+        "pssa_hip_distill_resident": ([vp, vp, C.c_int, sz, sz, sz, vp, vp, sz, C.c_float, vp, vp, vp, sz, err_t, sz],
+                                      C.c_int),
+        "pssa_hip_batch_token_logprobs": ([vp, u32p, sz, C.c_float, sz, fp, fp, u32p, fp, err_t, sz], C.c_int),
+        "pssa_hip_batch_distill": ([vp, u32p, fp, sz, sz, C.c_float, fp, fp, fp, err_t, sz], C.c_int),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)

@@ -9,6 +9,7 @@
 #include "gemm.h"
 #include "memory.h"
 #include "model.h"
+#include "operators.h"
 #include "ssm.h"
 
 namespace pssa {
@@ -203,6 +204,7 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_retrieve_attributes());
     PSSA_RETURN_IF(pssa::init_decode_attributes());
     PSSA_RETURN_IF(pssa::init_dense_scan_attributes());
+    PSSA_RETURN_IF(pssa::init_operator_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));
     *out = ctx.release();
     return Status::Ok();
@@ -1485,6 +1487,7 @@ int pssa_hip_batch_forward(pssa_hip_lanes* L, const pssa_hip_sequence* seqs, siz
       PSSA_RETURN_IF(L->tok_loss.alloc(L->max_tokens * 4));
     }
     L->logit_lanes = 0;  // lanes->logits no longer follows a prefill
+    L->tok_row.clear();
 
     std::vector<size_t> offset(n_seqs);  // packed token offsets in the given order
     std::vector<uint64_t> lens(n_seqs), lane_of(n_seqs);
@@ -1507,12 +1510,17 @@ int pssa_hip_batch_forward(pssa_hip_lanes* L, const pssa_hip_sequence* seqs, siz
 
     RaggedPlan p;
     plan_ragged(L, lens, lane_of, p);
-    std::vector<uint32_t> ids_h(tokens), meta_h(2 * tokens);
+    std::vector<uint32_t> ids_h(tokens), meta_h(2 * tokens), row_h(tokens), target_h(tokens);
     for (size_t l = 0; l < p.order.size(); ++l) {
       const pssa_hip_sequence& q = seqs[p.order[l]];
       std::memcpy(&ids_h[p.row[l]], q.inputs, q.len * 4);
       std::memcpy(&meta_h[p.row[l]], q.targets, q.len * 4);
-      for (size_t t = 0; t < q.len; ++t) meta_h[tokens + p.row[l] + t] = (uint32_t)(offset[p.order[l]] + t);
+      for (size_t t = 0; t < q.len; ++t) {
+        const size_t at = offset[p.order[l]] + t;
+        meta_h[tokens + p.row[l] + t] = (uint32_t)at;
+        row_h[at] = (uint32_t)(p.row[l] + t);
+        target_h[at] = q.targets[t];
+      }
     }
     PSSA_RETURN_IF(L->ctx->stage.to_device(L->ids.p, ids_h.data(), tokens * 4, L->ctx->stream));
     PSSA_RETURN_IF(L->ctx->stage.to_device(L->tok_meta.p, meta_h.data(), 2 * tokens * 4, L->ctx->stream));
@@ -1531,6 +1539,8 @@ int pssa_hip_batch_forward(pssa_hip_lanes* L, const pssa_hip_sequence* seqs, siz
         PSSA_RETURN_IF(L->ctx->stage.to_host(logits + offset[p.order[l]] * V,
                                              L->tok_logits.as<float>() + p.row[l] * V, lens[p.order[l]] * V * 4, st));
     PSSA_RETURN_IF(sync(L->ctx));
+    L->tok_row.swap(row_h);
+    L->tok_target.swap(target_h);
     // The token mean in packed order, summed left to right in f32
     // (stage_logits_loss, src/gpu_batch.rs:1246-1249).
     float total = 0.0f;
@@ -2007,6 +2017,239 @@ int pssa_hip_dense_scan_reserve(pssa_hip_ctx* ctx, size_t batch, size_t seq_len,
     return bind_dense_scan_scratch(ctx, (int)batch, (int)seq_len, (int)d_state);
   };
   return pssa::finish(body(), err, err_len);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------- language-model operators
+
+namespace {
+
+// Runs an entry point's body; no C++ exception leaves it.
+template <class Body>
+int guarded(Body body, char* err, size_t err_len) {
+  try {
+    return pssa::finish(body(), err, err_len);
+  } catch (const std::exception& e) {
+    return pssa::finish(Status::NoMem(std::string("host: ") + e.what()), err, err_len);
+  }
+}
+
+bool temperature_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
+bool dtype_ok(int dtype) { return dtype == PSSA_HIP_F32 || dtype == PSSA_HIP_BF16; }
+size_t dtype_size(int dtype) { return dtype == PSSA_HIP_BF16 ? 2 : 4; }
+bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// A matrix of logit rows: its type, extent and alignment.
+Status check_rows(const void* p, int dtype, size_t rows, size_t vocab, size_t ld, const char* what) {
+  PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+  if (!rows || !vocab) return Status::Invalid(std::string(what) + ": dimensions must be positive");
+  if (vocab > ((size_t)1 << 24) || rows > INT32_MAX) return Status::Invalid(std::string(what) + ": too large");
+  if (ld < vocab) return Status::Invalid(std::string(what) + ": row stride below the vocabulary");
+  size_t n = 0;
+  PSSA_RETURN_IF(pssa::checked_count({rows, ld}, &n, what));
+  if (!aligned_to(p, dtype_size(dtype))) return Status::Invalid(std::string(what) + ": misaligned buffer");
+  return Status::Ok();
+}
+
+// Rows of `width` words between packed token order (host) and the device
+// rows of the last batch forward.
+template <class T>
+void rows_to_device_order(const std::vector<uint32_t>& row, const T* in, size_t width, std::vector<T>& out) {
+  out.resize(row.size() * width);
+  for (size_t i = 0; i < row.size(); ++i) std::memcpy(&out[row[i] * width], in + i * width, width * sizeof(T));
+}
+
+// A device array in batch-row order, copied to `out` in packed token order.
+template <class T>
+Status rows_to_host(pssa_hip_lanes* L, T* out, const DevBuf& buf, size_t width) {
+  std::vector<T> h(L->tok_row.size() * width);
+  PSSA_RETURN_IF(download(L->ctx, h.data(), buf, h.size() * sizeof(T)));
+  PSSA_RETURN_IF(sync(L->ctx));
+  for (size_t i = 0; i < L->tok_row.size(); ++i)
+    std::memcpy(out + i * width, &h[L->tok_row[i] * width], width * sizeof(T));
+  return Status::Ok();
+}
+
+Status check_batch(const pssa_hip_lanes* L, size_t n_tokens) {
+  PSSA_RETURN_IF(need(!L->tok_row.empty(), "no batch forward has left logits on these lanes"));
+  return need(n_tokens == L->tok_row.size(), "token count must be the last batch forward's");
+}
+
+}  // namespace
+
+extern "C" {
+
+int pssa_hip_token_logprobs_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t rows, size_t vocab,
+                                     size_t ld, const uint32_t* d_targets, float temperature, size_t top_k,
+                                     float* d_logprobs, float* d_entropy, uint32_t* d_top_ids,
+                                     float* d_top_logprobs, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_logits != nullptr, "token logprobs: null buffer"));
+    PSSA_RETURN_IF(check_rows(d_logits, dtype, rows, vocab, ld, "token logprobs"));
+    PSSA_RETURN_IF(need(temperature_ok(temperature), "token logprobs: temperature must be in [1e-6, 1e6]"));
+    PSSA_RETURN_IF(need(top_k <= (size_t)pssa::kMaxAlternatives, "token logprobs: top_k must be at most 64"));
+    PSSA_RETURN_IF(need(!top_k || (d_top_ids && d_top_logprobs), "token logprobs: top_k needs both of its outputs"));
+    PSSA_RETURN_IF(need(!d_logprobs || d_targets, "token logprobs: log probabilities need targets"));
+    PSSA_RETURN_IF(need(d_logprobs || d_entropy || top_k, "token logprobs: no output asked for"));
+    PSSA_RETURN_IF(need(aligned_to(d_targets, 4) && aligned_to(d_logprobs, 4) && aligned_to(d_entropy, 4) &&
+                            aligned_to(d_top_ids, 4) && aligned_to(d_top_logprobs, 4),
+                        "token logprobs: misaligned buffer"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::LogprobArgs a;
+    a.logits = d_logits;
+    a.ld = ld;
+    a.vocab = (int)vocab;
+    a.targets = d_targets;
+    a.temperature = temperature;
+    a.top_k = (int)top_k;
+    a.logprobs = d_logprobs;
+    a.entropy = d_entropy;
+    a.top_ids = d_top_ids;
+    a.top_logprobs = d_top_logprobs;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return pssa::launch_token_logprobs(ctx->stream, dtype, a, rows);
+  }, err, err_len);
+}
+
+int pssa_hip_distill_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t rows, size_t vocab,
+                              size_t ld, const uint32_t* d_teacher_ids, const float* d_teacher_logits,
+                              size_t teacher_k, float temperature, const float* d_row_weights, float* d_losses,
+                              void* d_grad, size_t ld_grad, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_logits && d_teacher_ids && d_teacher_logits && d_losses, "distill: null buffer"));
+    PSSA_RETURN_IF(check_rows(d_logits, dtype, rows, vocab, ld, "distill"));
+    PSSA_RETURN_IF(need(teacher_k >= 1 && teacher_k <= (size_t)pssa::kMaxTeacher,
+                        "distill: teacher_k must be in 1..=1024"));
+    PSSA_RETURN_IF(need(temperature_ok(temperature), "distill: temperature must be in [1e-6, 1e6]"));
+    PSSA_RETURN_IF(need(aligned_to(d_teacher_ids, 4) && aligned_to(d_teacher_logits, 4) &&
+                            aligned_to(d_row_weights, 4) && aligned_to(d_losses, 4),
+                        "distill: misaligned buffer"));
+    if (d_grad) {
+      PSSA_RETURN_IF(check_rows(d_grad, dtype, rows, vocab, ld_grad, "distill gradient"));
+      if (d_grad == d_logits) {
+        PSSA_RETURN_IF(need(ld_grad == ld, "distill: a gradient in place needs the logits' row stride"));
+      } else {
+        const uintptr_t x = (uintptr_t)d_logits, y = (uintptr_t)d_grad;
+        const size_t nx = ((rows - 1) * ld + vocab) * dtype_size(dtype);
+        const size_t ny = ((rows - 1) * ld_grad + vocab) * dtype_size(dtype);
+        PSSA_RETURN_IF(need(x + nx <= y || y + ny <= x, "distill: the gradient overlaps the logits"));
+      }
+    }
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::DistillArgs a;
+    a.logits = d_logits;
+    a.ld = ld;
+    a.vocab = (int)vocab;
+    a.teacher_ids = d_teacher_ids;
+    a.teacher_logits = d_teacher_logits;
+    a.teacher_k = (int)teacher_k;
+    a.temperature = temperature;
+    a.row_weights = d_row_weights;
+    a.losses = d_losses;
+    a.grad = d_grad;
+    a.ld_grad = ld_grad;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return pssa::launch_distill(ctx->stream, dtype, a, rows);
+  }, err, err_len);
+}
+
+int pssa_hip_batch_token_logprobs(pssa_hip_lanes* L, const uint32_t* targets, size_t n_tokens, float temperature,
+                                  size_t top_k, float* logprobs, float* entropy, uint32_t* top_ids,
+                                  float* top_logprobs, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(L != nullptr, "null lanes"));
+    PSSA_RETURN_IF(need(temperature_ok(temperature), "token logprobs: temperature must be in [1e-6, 1e6]"));
+    PSSA_RETURN_IF(need(top_k <= (size_t)pssa::kMaxAlternatives, "token logprobs: top_k must be at most 64"));
+    std::lock_guard<std::mutex> g(L->ctx->mu);
+    PSSA_RETURN_IF(check_batch(L, n_tokens));
+    PSSA_HIP_TRY(hipSetDevice(L->ctx->device));
+    pssa_hip_ctx* ctx = L->ctx;
+    const size_t V = L->model->cfg.d_vocab;
+    std::vector<uint32_t> target_h;
+    rows_to_device_order(L->tok_row, targets ? targets : L->tok_target.data(), 1, target_h);
+    DevBuf dt, lp, en, id, tl;
+    PSSA_RETURN_IF(upload(ctx, dt, target_h.data(), n_tokens * 4));
+    PSSA_RETURN_IF(lp.alloc(n_tokens * 4, &ctx->pool));
+    PSSA_RETURN_IF(en.alloc(n_tokens * 4, &ctx->pool));
+    PSSA_RETURN_IF(id.alloc(n_tokens * top_k * 4, &ctx->pool));
+    PSSA_RETURN_IF(tl.alloc(n_tokens * top_k * 4, &ctx->pool));
+    pssa::LogprobArgs a;
+    a.logits = L->tok_logits.p;
+    a.ld = V;
+    a.vocab = (int)V;
+    a.targets = dt.as<uint32_t>();
+    a.temperature = temperature;
+    a.top_k = (int)top_k;
+    a.logprobs = lp.as<float>();
+    a.entropy = en.as<float>();
+    a.top_ids = id.as<uint32_t>();
+    a.top_logprobs = tl.as<float>();
+    PSSA_RETURN_IF(pssa::launch_token_logprobs(ctx->stream, PSSA_HIP_F32, a, n_tokens));
+    if (logprobs) PSSA_RETURN_IF(rows_to_host(L, logprobs, lp, 1));
+    if (entropy) PSSA_RETURN_IF(rows_to_host(L, entropy, en, 1));
+    if (top_ids && top_k) PSSA_RETURN_IF(rows_to_host(L, top_ids, id, top_k));
+    if (top_logprobs && top_k) PSSA_RETURN_IF(rows_to_host(L, top_logprobs, tl, top_k));
+    return sync(ctx);
+  }, err, err_len);
+}
+
+int pssa_hip_batch_distill(pssa_hip_lanes* L, const uint32_t* teacher_ids, const float* teacher_logits,
+                           size_t n_tokens, size_t teacher_k, float temperature, const float* row_weights,
+                           float* losses, float* grad_logits, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(L && teacher_ids && teacher_logits && losses, "distill: null buffer"));
+    PSSA_RETURN_IF(need(teacher_k >= 1 && teacher_k <= (size_t)pssa::kMaxTeacher,
+                        "distill: teacher_k must be in 1..=1024"));
+    PSSA_RETURN_IF(need(temperature_ok(temperature), "distill: temperature must be in [1e-6, 1e6]"));
+    std::lock_guard<std::mutex> g(L->ctx->mu);
+    PSSA_RETURN_IF(check_batch(L, n_tokens));
+    pssa_hip_ctx* ctx = L->ctx;
+    const size_t V = L->model->cfg.d_vocab;
+    for (size_t i = 0; i < n_tokens * teacher_k; ++i)
+      if (teacher_ids[i] >= V && teacher_ids[i] != PSSA_HIP_NO_TOKEN)
+        return Status::Invalid("distill: teacher token ID " + std::to_string(teacher_ids[i]) +
+                               " outside model vocabulary");
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    std::vector<uint32_t> ids_h;
+    std::vector<float> t_h, w_h;
+    rows_to_device_order(L->tok_row, teacher_ids, teacher_k, ids_h);
+    rows_to_device_order(L->tok_row, teacher_logits, teacher_k, t_h);
+    if (row_weights) rows_to_device_order(L->tok_row, row_weights, 1, w_h);
+    DevBuf ids, t, w, loss, grad;
+    PSSA_RETURN_IF(upload(ctx, ids, ids_h.data(), ids_h.size() * 4));
+    PSSA_RETURN_IF(upload(ctx, t, t_h.data(), t_h.size() * 4));
+    if (row_weights) PSSA_RETURN_IF(upload(ctx, w, w_h.data(), w_h.size() * 4));
+    PSSA_RETURN_IF(loss.alloc(n_tokens * 4, &ctx->pool));
+    if (grad_logits) PSSA_RETURN_IF(grad.alloc(n_tokens * V * 4, &ctx->pool));
+    pssa::DistillArgs a;
+    a.logits = L->tok_logits.p;
+    a.ld = V;
+    a.vocab = (int)V;
+    a.teacher_ids = ids.as<uint32_t>();
+    a.teacher_logits = t.as<float>();
+    a.teacher_k = (int)teacher_k;
+    a.temperature = temperature;
+    a.row_weights = row_weights ? w.as<float>() : nullptr;
+    a.losses = loss.as<float>();
+    a.grad = grad_logits ? grad.p : nullptr;
+    a.ld_grad = V;
+    PSSA_RETURN_IF(pssa::launch_distill(ctx->stream, PSSA_HIP_F32, a, n_tokens));
+    PSSA_RETURN_IF(rows_to_host(L, losses, loss, 1));
+    if (grad_logits) {
+      // Runs of neighbouring rows go down together, without a second host copy.
+      for (size_t i = 0; i < n_tokens;) {
+        size_t e = i + 1;
+        while (e < n_tokens && L->tok_row[e] == L->tok_row[e - 1] + 1) ++e;
+        PSSA_RETURN_IF(ctx->stage.to_host(grad_logits + i * V, grad.as<float>() + (size_t)L->tok_row[i] * V,
+                                          (e - i) * V * 4, ctx->stream));
+        i = e;
+      }
+    }
+    return sync(ctx);
+  }, err, err_len);
 }
 
 }  // extern "C"

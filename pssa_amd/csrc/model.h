@@ -99,6 +99,9 @@ struct pssa_hip_lanes {
   // packed token index [2, max_tokens], and the per-token losses in packed
   // order [max_tokens].
   pssa::DevBuf tok_logits, tok_meta, tok_loss;
+  // Row of tok_logits of each packed token of the last batch forward, and
+  // its targets (empty: none ran, or the last one failed).
+  std::vector<uint32_t> tok_row, tok_target;
   // Spans, last rows and positions of a ragged call (RaggedRows), allocated
   // on the first one: [4 * lanes + max_tokens] u32.
   pssa::DevBuf row_meta;

@@ -1,0 +1,45 @@
+// Language-model operators on device-resident arrays: log probabilities and
+// distillation over logit rows, linear attention with a decay for each head,
+// products with 4-bit weights.
+#pragma once
+#include "common.h"
+
+namespace pssa {
+
+// Dynamic LDS above the default limit, once for each device.
+Status init_operator_attributes();
+
+// ---------------------------------------------------------------- logit rows
+constexpr int kMaxAlternatives = 64;  // top tokens a row can list: one wave's lanes
+constexpr int kMaxTeacher = 1024;     // teacher entries of a row (held in LDS)
+
+struct LogprobArgs {
+  const void* logits = nullptr;  // row r at logits + r * ld (f32 or bf16)
+  size_t ld = 0;
+  int vocab = 0;
+  const uint32_t* targets = nullptr;  // [rows] or null
+  float temperature = 1.0f;
+  int top_k = 0;
+  float* logprobs = nullptr;      // [rows], with targets
+  float* entropy = nullptr;       // [rows] or null
+  uint32_t* top_ids = nullptr;    // [rows, top_k]
+  float* top_logprobs = nullptr;  // [rows, top_k]
+};
+Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& a, size_t rows);
+
+struct DistillArgs {
+  const void* logits = nullptr;
+  size_t ld = 0;
+  int vocab = 0;
+  const uint32_t* teacher_ids = nullptr;   // [rows, teacher_k]
+  const float* teacher_logits = nullptr;   // [rows, teacher_k]
+  int teacher_k = 0;
+  float temperature = 1.0f;
+  const float* row_weights = nullptr;  // [rows] or null (1)
+  float* losses = nullptr;             // [rows]
+  void* grad = nullptr;                // row r at grad + r * ld_grad, the logits' type, or null
+  size_t ld_grad = 0;
+};
+Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& a, size_t rows);
+
+}  // namespace pssa

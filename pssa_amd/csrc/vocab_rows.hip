@@ -1,0 +1,561 @@
+// Operators over logit rows: log probabilities of given tokens with entropy
+// and top alternatives, and distillation from a teacher's top logits.
+//
+// Both are one pass of a row through the registers of one workgroup: the
+// loads of a whole row are issued at once, its maximum and its sums are
+// reductions over registers, and what needs the finished sums (the gradient,
+// the alternatives) is computed from the registers again.  Rows past the
+// registers go tile by tile, the statistics merged after each tile.
+#include "operators.h"
+
+namespace pssa {
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// 16 bytes at any element's address: rows start anywhere (gfx950 loads and
+// stores them unaligned in one instruction).
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLowest = -3.0e38f;  // stands for differences that overflow: exp of it is 0, products with 0 stay 0
+constexpr uint32_t kNoToken = PSSA_HIP_NO_TOKEN;
+
+struct Bf16 {
+  uint16_t bits;
+};
+template <class T>
+constexpr int vec_n() { return 16 / (int)sizeof(T); }
+
+template <class T>
+__device__ __forceinline__ float elem(const u32x4_t& u, int j);
+template <>
+__device__ __forceinline__ float elem<float>(const u32x4_t& u, int j) { return __uint_as_float(u[j]); }
+template <>
+__device__ __forceinline__ float elem<Bf16>(const u32x4_t& u, int j) {
+  return __uint_as_float(j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
+}
+template <class T>
+__device__ __forceinline__ float load1(const T* p);
+template <>
+__device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+template <>
+__device__ __forceinline__ float load1<Bf16>(const Bf16* p) { return __uint_as_float((uint32_t)p->bits << 16); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(Bf16* p, float v) { p->bits = bf16_bits_dev(v); }
+template <class T>
+__device__ __forceinline__ u32x4_t pack(const float (&v)[vec_n<T>()]);
+template <>
+__device__ __forceinline__ u32x4_t pack<float>(const float (&v)[4]) {
+  return u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+template <>
+__device__ __forceinline__ u32x4_t pack<Bf16>(const float (&v)[8]) {
+  return u32x4_t{bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7])};
+}
+// -inf in one element (the other half of its word kept).
+template <class T>
+__device__ __forceinline__ void mask_elem(u32x4_t& u, int j);
+template <>
+__device__ __forceinline__ void mask_elem<float>(u32x4_t& u, int j) { u[j] = 0xFF800000u; }
+template <>
+__device__ __forceinline__ void mask_elem<Bf16>(u32x4_t& u, int j) {
+  u[j >> 1] = j & 1 ? (u[j >> 1] & 0xFFFFu) | 0xFF800000u : (u[j >> 1] & 0xFFFF0000u) | 0xFF80u;
+}
+
+// Vector i of a row covers elements i*N .. i*N+N-1 and is loaded from
+// vec_start, which moves the row's last, partial vector back to end with the
+// row: every load stays inside the row, and the elements that belong to the
+// vector before (all of them past the row's end) read as -inf.
+template <class T>
+__device__ __forceinline__ int vec_start(int V, int i) {
+  constexpr int N = vec_n<T>();
+  return V < N ? 0 : min(i * N, V - N);
+}
+template <class T>
+__device__ __forceinline__ u32x4_t vec_load(const T* row, int V, int i) {
+  constexpr int N = vec_n<T>();
+  if (V < N) {  // uniform
+    u32x4_t u = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (i == 0 && j < V) {
+        if constexpr (sizeof(T) == 4)
+          u[j] = reinterpret_cast<const uint32_t*>(row)[j];
+        else
+          u[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[j] << (16 * (j & 1));
+      } else {
+        mask_elem<T>(u, j);
+      }
+    }
+    return u;
+  }
+  return *reinterpret_cast<const u32x4_any_t*>(row + vec_start<T>(V, i));
+}
+template <class T>
+__device__ __forceinline__ void vec_mask(u32x4_t& u, int V, int i) {
+  constexpr int N = vec_n<T>();
+  const int lead = i * N - vec_start<T>(V, i);
+  if (V >= N && lead > 0) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < lead) mask_elem<T>(u, j);
+  }
+}
+// The tile's vectors of one thread (vector tile0 + k * 64W + tid); a k past
+// the row is skipped by the whole workgroup.
+template <class T, int W, int NV>
+__device__ __forceinline__ void tile_load(u32x4_t (&u)[NV], const T* row, int V, int tile0) {
+  constexpr int N = vec_n<T>();
+  const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    u[k] = u32x4_t{none, none, none, none};
+    if ((tile0 + k * 64 * W) * N < V) u[k] = vec_load<T>(row, V, tile0 + k * 64 * W + (int)threadIdx.x);
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if ((tile0 + k * 64 * W) * N < V) vec_mask<T>(u[k], V, tile0 + k * 64 * W + (int)threadIdx.x);
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {  // NaN never becomes the maximum
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// ------------------------------------------------------------- ordered keys
+// A token's place in (logit descending, id ascending) order as one whole
+// number: the logit's bits mapped to unsigned order above the complement of
+// the id.  Distinct for every token; 0 is no token.
+__device__ __forceinline__ uint64_t token_key(float v, int id) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 orders as 0
+  return (uint64_t)(b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (uint32_t)~id;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float(b ^ (b >> 31 ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int key_id(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ uint64_t key_step(uint64_t a, int off, bool keep_max) {
+  const uint64_t o = __shfl_xor((unsigned long long)a, off, 64);
+  return (o > a) == keep_max ? o : a;
+}
+// The wave's 64 keys, largest in lane 0 (bitonic, 21 exchanges).
+__device__ __forceinline__ uint64_t wave_sort(uint64_t a, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int off = size >> 1; off >= 1; off >>= 1) a = key_step(a, off, ((lane & off) == 0) == ((lane & size) == 0));
+  return a;
+}
+// The largest 64 of two descending lists, descending; `b` is given reversed.
+__device__ __forceinline__ uint64_t wave_merge(uint64_t a, uint64_t b_reversed, int lane) {
+  a = a > b_reversed ? a : b_reversed;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) a = key_step(a, off, (lane & off) == 0);
+  return a;
+}
+
+// --------------------------------------------------------- log probabilities
+// With m the row's maximum and d_i = (z_i - m) / tau, the log softmax is
+// d_i - log(1 + S) and the entropy log(1 + S) - T / (1 + S), where S and T sum
+// exp(d_i) and exp(d_i) d_i over every token but the first maximum: kept
+// apart from its 1, S carries the small probabilities that a nearly certain
+// row's values consist of.
+//
+// Alternatives: the k-th largest of the threads' maxima bounds the row's k-th
+// largest token from below, and only the k threads whose maximum reaches it
+// can hold tokens above it, so at most k * (tokens of a thread) candidates
+// pass through LDS, whatever the row holds; one wave sorts them.
+template <class T, int W, int NV>
+__global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
+  constexpr int N = vec_n<T>(), TILE = 64 * W * NV;
+  __shared__ uint64_t s_keys[W * 64];
+  __shared__ float s_sum[2 * W];
+  __shared__ uint64_t s_first, s_bound;
+  __shared__ int s_count;
+  extern __shared__ uint64_t s_cand[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab, top = a.top_k;
+  const T* row = static_cast<const T*>(a.logits) + (size_t)blockIdx.x * a.ld;
+  const float inv_tau = 1.0f / a.temperature, c2 = kLog2e * inv_tau;
+  const uint32_t target = a.targets ? a.targets[blockIdx.x] : kNoToken;
+  const float z_target = target < (uint32_t)V ? load1<T>(row + target) : 0.0f;
+
+  float m = -INFINITY, S = 0.0f, Tq = 0.0f;
+  uint64_t best = 0;  // wave 0: the largest keys so far, descending
+  const int vecs = (V + N - 1) / N;
+  for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
+    u32x4_t u[NV];
+    tile_load<T, W, NV>(u, row, V, tile0);
+    float bv = -INFINITY;
+    int bi = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float v = elem<T>(u[k], j);
+        if (v > bv) {
+          bv = v;
+          bi = s + j;
+        }
+      }
+    }
+    const uint64_t mine = bv > -INFINITY ? token_key(bv, bi) : 0;
+    uint64_t first = mine;
+    if (top) {
+      uint64_t key = wave_sort(mine, lane);
+      if constexpr (W > 1) {
+        s_keys[wave * 64 + lane] = key;
+        __syncthreads();
+#pragma unroll
+        for (int half = W / 2; half >= 1; half >>= 1) {
+          if (wave < half) {
+            key = wave_merge(key, s_keys[(wave + half) * 64 + 63 - lane], lane);
+            s_keys[wave * 64 + lane] = key;
+          }
+          __syncthreads();
+        }
+      }
+      if (wave == 0) {
+        if (lane == 0) {
+          s_first = key;
+          s_count = 0;
+        }
+        if (lane == top - 1) s_bound = key > best ? key : best;
+      }
+      __syncthreads();
+      first = s_first;
+      const uint64_t bound = s_bound;
+      // bound 0: fewer than k threads have a token; each takes part with all of its own.
+      if (mine && mine >= bound) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float v = elem<T>(u[k], j);
+            if (v > -INFINITY) {
+              const uint64_t key2 = token_key(v, s + j);
+              if (key2 >= bound) s_cand[atomicAdd(&s_count, 1)] = key2;
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const int n = s_count;
+        for (int c = 0; c < n; c += 64) {
+          const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : 0, lane);
+          best = wave_merge(best, __shfl((unsigned long long)got, 63 - lane, 64), lane);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) first = key_step(first, off, true);
+      if constexpr (W > 1) {
+        if (lane == 0) s_keys[wave] = first;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) first = s_keys[w] > first ? s_keys[w] : first;
+      }
+    }
+
+    // The tile's sums without its first maximum.
+    const bool some = first != 0;
+    const float mt = some ? key_value(first) : 0.0f;
+    const bool own = some && mine == first;
+    float st = 0.0f, tt = 0.0f;
+    auto add = [&](float v) {
+      const float d = v - mt;
+      const float e = __builtin_amdgcn_exp2f(d * c2);
+      st += e;
+      tt = fmaf(e, fmaxf(d, kLowest), tt);
+    };
+    if (__any(own)) {  // one wave
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
+#pragma unroll
+        for (int j = 0; j < N; ++j) add(own && s + j == bi ? -INFINITY : elem<T>(u[k], j));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) add(elem<T>(u[k], j));
+    }
+    st = wave_sum(st);
+    tt = wave_sum(tt);
+    if constexpr (W > 1) {
+      if (lane == 0) {
+        s_sum[wave] = st;
+        s_sum[W + wave] = tt;
+      }
+      __syncthreads();
+      st = s_sum[0];
+      tt = s_sum[W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        st += s_sum[w];
+        tt += s_sum[W + w];
+      }
+      __syncthreads();  // the next tile writes them again
+    }
+    // Joined with the tiles before; the smaller maximum's token becomes a term of the sums.
+    if (!some) {
+      S += st;  // 0, or NaN where the tile holds one
+    } else if (mt > m) {
+      const float d = fmaxf(m - mt, kLowest), f = __builtin_amdgcn_exp2f(d * c2);
+      const float n = m > -INFINITY ? 1.0f : 0.0f;
+      Tq = fmaf(f, Tq, fmaf(f * d, S + n, tt));  // f d first: d alone may be huge where f is 0
+      S = fmaf(f, S + n, st);
+      m = mt;
+    } else {
+      const float d = fmaxf(mt - m, kLowest), f = __builtin_amdgcn_exp2f(d * c2);
+      Tq = fmaf(f, tt, fmaf(f * d, st + 1.0f, Tq));
+      S = fmaf(f, st + 1.0f, S);
+    }
+  }
+
+  // A NaN anywhere makes S NaN, and so does a maximum of +inf (inf - inf).
+  const bool bad = !(S >= 0.0f) || m == INFINITY, empty = m == -INFINITY;
+  const float lse = log1pf(S);
+  if (tid == 0) {
+    if (a.logprobs) {
+      float lp = (z_target - m) * inv_tau - lse;
+      if (empty) lp = -INFINITY;
+      if (bad || target >= (uint32_t)V) lp = NAN;
+      a.logprobs[blockIdx.x] = target == kNoToken ? 0.0f : lp;
+    }
+    if (a.entropy) {
+      const float h = lse - Tq * inv_tau / (1.0f + S);
+      a.entropy[blockIdx.x] = bad ? NAN : empty ? 0.0f : h;
+    }
+  }
+  if (wave == 0 && lane < top) {
+    const size_t at = (size_t)blockIdx.x * top + lane;
+    const bool has = best != 0 && !bad;
+    a.top_ids[at] = has ? (uint32_t)key_id(best) : kNoToken;
+    a.top_logprobs[at] = bad ? NAN : has ? (key_value(best) - m) * inv_tau - lse : -INFINITY;
+  }
+}
+
+// -------------------------------------------------------------- distillation
+// With p the softmax of the student's row and q that of the teacher's entries,
+// both at temperature tau, a row's loss is w tau^2 sum_j q_j (log q_j - log p_j)
+// and its gradient w tau (p - q).  The dense part p is written from the
+// registers that the sums were taken from; the few teacher's tokens are then
+// written again with their q.
+template <class T, int W, int NV>
+__global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
+  constexpr int N = vec_n<T>(), TILE = 64 * W * NV;
+  __shared__ float s_red[2 * W];
+  __shared__ float s_teach[2];  // the teacher's maximum and log of its sum
+  extern __shared__ float s_dyn[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab, K = a.teacher_k;
+  float* s_q = s_dyn;
+  float* s_z = s_dyn + K;  // the student's logits at the teacher's tokens
+  uint32_t* s_id = reinterpret_cast<uint32_t*>(s_dyn + 2 * K);
+  const T* row = static_cast<const T*>(a.logits) + (size_t)blockIdx.x * a.ld;
+  T* grad = a.grad ? static_cast<T*>(a.grad) + (size_t)blockIdx.x * a.ld_grad : nullptr;
+  const float inv_tau = 1.0f / a.temperature, c2 = kLog2e * inv_tau;
+  const float weight = a.row_weights ? a.row_weights[blockIdx.x] : 1.0f;
+  const int vecs = (V + N - 1) / N;
+
+  // The teacher's entries, by the first wave.
+  if (wave == 0) {
+    float mt = -INFINITY;
+    bool bad = false;
+    for (int j = lane; j < K; j += 64) {
+      uint32_t id = a.teacher_ids[(size_t)blockIdx.x * K + j];
+      float t = a.teacher_logits[(size_t)blockIdx.x * K + j];
+      if (id != kNoToken && id >= (uint32_t)V) t = NAN;  // no such token
+      if (id >= (uint32_t)V) id = kNoToken;
+      bad |= id == kNoToken ? t != t && a.teacher_ids[(size_t)blockIdx.x * K + j] != kNoToken : !(t < INFINITY);
+      if (id == kNoToken) t = -INFINITY;
+      s_id[j] = id;
+      s_q[j] = t;
+      s_z[j] = id == kNoToken ? 0.0f : load1<T>(row + id);
+      mt = fmaxf(mt, t);
+    }
+    mt = wave_max(mt);
+    float z = 0.0f;
+    if (mt > -INFINITY)
+      for (int j = lane; j < K; j += 64) z += __builtin_amdgcn_exp2f((s_q[j] - mt) * c2);
+    z = wave_sum(z);
+    if (__any(bad)) mt = NAN;
+    if (lane == 0) {
+      s_teach[0] = mt;
+      s_teach[1] = z;
+    }
+  }
+  __syncthreads();
+  const float t_max = s_teach[0], t_sum = s_teach[1];
+  // A row without weight or without a teacher: zeros, whatever it holds.
+  if (weight == 0.0f || t_max == -INFINITY) {
+    if (tid == 0) a.losses[blockIdx.x] = 0.0f;
+    if (grad) {
+      for (int i = tid; i < vecs; i += 64 * W) {
+        if (i * N + N <= V) {
+          *reinterpret_cast<u32x4_any_t*>(grad + i * N) = u32x4_t{0, 0, 0, 0};
+        } else {
+          for (int e = i * N; e < V; ++e) store1(grad + e, 0.0f);
+        }
+      }
+    }
+    return;
+  }
+
+  float m = -INFINITY, S = 0.0f;
+  u32x4_t u[NV];
+  for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
+    tile_load<T, W, NV>(u, row, V, tile0);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) mt = fmaxf(mt, elem<T>(u[k], j));
+    mt = wave_max(mt);
+    if constexpr (W > 1) {
+      if (lane == 0) s_red[wave] = mt;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) mt = fmaxf(mt, s_red[w]);
+    }
+    const float mn = fmaxf(m, mt), at = mn > -INFINITY ? mn : 0.0f;
+    float st = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) st += __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2);
+    st = wave_sum(st);
+    if constexpr (W > 1) {
+      if (lane == 0) s_red[W + wave] = st;
+      __syncthreads();
+      st = s_red[W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) st += s_red[W + w];
+    }
+    S = (m > -INFINITY ? S * __builtin_amdgcn_exp2f((m - at) * c2) : S) + st;
+    m = mn;
+  }
+  const bool empty = m == -INFINITY;
+  const float at = empty ? 0.0f : m;
+
+  if (wave == 0) {
+    const float log_z = logf(t_sum), log_s = logf(S);
+    float kl = 0.0f;
+    for (int j = lane; j < K; j += 64) {
+      const float t = (s_q[j] - t_max) * inv_tau, q = __builtin_amdgcn_exp2f((s_q[j] - t_max) * c2) / t_sum;
+      if (!(q <= 0.0f)) kl += q * ((t - log_z) - ((s_z[j] - at) * inv_tau - log_s));
+      s_q[j] = q;
+    }
+    kl = wave_sum(kl);
+    if (empty && S == 0.0f) kl = t_max != t_max ? NAN : INFINITY;  // every token masked, yet one is taught
+    if (lane == 0) a.losses[blockIdx.x] = weight * a.temperature * a.temperature * kl;
+  }
+  if (!grad) return;
+  const float scale = weight * a.temperature * (t_max != t_max ? NAN : 1.0f);
+  const float ps = S == 0.0f ? scale * 0.0f : scale / S;
+  auto write = [&](int tile0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = tile0 + k * 64 * W + tid;
+      float g[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) g[j] = __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2) * ps;
+      if (i * N + N <= V) {
+        *reinterpret_cast<u32x4_any_t*>(grad + i * N) = pack<T>(g);
+      } else {
+        const int s = vec_start<T>(V, i);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (s + j >= i * N && s + j < V) store1(grad + s + j, g[j]);
+      }
+    }
+  };
+  if (vecs <= TILE) {
+    write(0);
+  } else {
+    // In place, a partial vector's load also covers its neighbour's elements,
+    // which may be written already: they are masked, as in the sums.
+    for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
+      tile_load<T, W, NV>(u, row, V, tile0);
+      write(tile0);
+    }
+  }
+  // The dense stores have reached the cache before another thread's store to the same token.
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  __syncthreads();
+  for (int j = tid; j < K; j += 64 * W) {
+    const uint32_t id = s_id[j];
+    if (id == kNoToken) continue;
+    float q = 0.0f;
+    bool first = true;
+    for (int i = 0; i < K; ++i) {
+      if (s_id[i] != id) continue;
+      first &= i >= j;
+      q += s_q[i];
+    }
+    if (!first) continue;  // the token's first entry writes it
+    const float p = S == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((s_z[j] - at) * c2) / S;
+    store1(grad + id, scale * (p - q));
+  }
+}
+
+// The smallest workgroup whose registers hold the row.
+template <class T, template <class, int, int> class Launch, class Args>
+Status launch_rows(hipStream_t stream, const Args& a, size_t rows) {
+  const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
+  if (vecs <= 64 * 1 * 4) return Launch<T, 1, 4>::run(stream, a, rows);
+  if (vecs <= 64 * 4 * 4) return Launch<T, 4, 4>::run(stream, a, rows);
+  if (vecs <= 64 * 4 * 8) return Launch<T, 4, 8>::run(stream, a, rows);
+  if (vecs <= 64 * 8 * 8) return Launch<T, 8, 8>::run(stream, a, rows);
+  if (vecs <= 64 * 16 * 8) return Launch<T, 16, 8>::run(stream, a, rows);
+  return Launch<T, 16, 16>::run(stream, a, rows);
+}
+
+template <class T, int W, int NV>
+struct LaunchLogprobs {
+  static Status run(hipStream_t stream, const LogprobArgs& a, size_t rows) {
+    const size_t lds = (size_t)a.top_k * NV * vec_n<T>() * 8;
+    token_logprobs_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, lds, stream>>>(a);
+    PSSA_LAUNCH_CHECK("token_logprobs_kernel");
+    return Status::Ok();
+  }
+};
+template <class T, int W, int NV>
+struct LaunchDistill {
+  static Status run(hipStream_t stream, const DistillArgs& a, size_t rows) {
+    distill_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, (size_t)a.teacher_k * 12, stream>>>(a);
+    PSSA_LAUNCH_CHECK("distill_kernel");
+    return Status::Ok();
+  }
+};
+
+}  // namespace
+
+// 64 alternatives of long rows take 64 KB for their candidates.
+Status init_operator_attributes() {
+  PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&token_logprobs_kernel<Bf16, 16, 16>),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, kMaxAlternatives * 16 * 8 * 8));
+  return Status::Ok();
+}
+
+Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& a, size_t rows) {
+  return dtype == PSSA_HIP_F32 ? launch_rows<float, LaunchLogprobs>(stream, a, rows)
+                               : launch_rows<Bf16, LaunchLogprobs>(stream, a, rows);
+}
+
+Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& a, size_t rows) {
+  return dtype == PSSA_HIP_F32 ? launch_rows<float, LaunchDistill>(stream, a, rows)
+                               : launch_rows<Bf16, LaunchDistill>(stream, a, rows);
+}
+
+}  // namespace pssa

@@ -26,6 +26,12 @@ def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
 
+def _dtype(name: str) -> int:
+    if name not in ("f32", "bf16"):
+        raise ValueError("dtype must be 'f32' or 'bf16'")
+    return _abi.F32 if name == "f32" else _abi.BF16
+
+
 class HipDevice:
     """Device context (CudaContext peer, src/cuda.rs:158-192)."""
 
@@ -292,6 +298,32 @@ class HipDevice:
         dense_scan_resident then runs without allocating."""
         _abi.call(self._lib.pssa_hip_dense_scan_reserve, self.handle, batch, L, s)
 
+    # -- language-model operators on device buffers -----------------------------
+    def token_logprobs_resident(self, logits_ptr: int, dtype: str, rows: int, vocab: int, targets_ptr: int | None = None,
+                                logprobs_ptr: int | None = None, entropy_ptr: int | None = None, top_k: int = 0,
+                                top_ids_ptr: int | None = None, top_logprobs_ptr: int | None = None,
+                                temperature: float = 1.0, ld: int | None = None) -> None:
+        """Log probabilities [rows] of the u32 targets under softmax(logits / temperature), the entropy [rows] and
+        the top_k <= 64 largest tokens [rows, top_k] with theirs (asynchronous on the context stream).  Logits are
+        rows of `ld` (default `vocab`) elements; a target of _abi.NO_TOKEN gives 0."""
+        _abi.call(self._lib.pssa_hip_token_logprobs_resident, self.handle, logits_ptr, _dtype(dtype), rows, vocab,
+                  vocab if ld is None else ld, targets_ptr, temperature, top_k, logprobs_ptr, entropy_ptr, top_ids_ptr,
+                  top_logprobs_ptr)
+
+    def distill_resident(self, logits_ptr: int, dtype: str, rows: int, vocab: int, teacher_ids_ptr: int,
+                         teacher_logits_ptr: int, teacher_k: int, losses_ptr: int, grad_ptr: int | None = None,
+                         temperature: float = 1.0, row_weights_ptr: int | None = None, ld: int | None = None,
+                         ld_grad: int | None = None) -> None:
+        """Distillation loss [rows] from a teacher's top logits (ids u32 and logits f32, both [rows, teacher_k]) and,
+        given grad_ptr, its gradient in the logits' type; grad_ptr may be logits_ptr (asynchronous on the context
+        stream)."""
+        ld = vocab if ld is None else ld
+        if ld_grad is None:
+            ld_grad = ld if grad_ptr == logits_ptr else vocab
+        _abi.call(self._lib.pssa_hip_distill_resident, self.handle, logits_ptr, _dtype(dtype), rows, vocab, ld,
+                  teacher_ids_ptr, teacher_logits_ptr, teacher_k, temperature, row_weights_ptr, losses_ptr, grad_ptr,
+                  ld_grad)
+
 
 class DeviceBuffer:
     """A device allocation made through the C ABI (freed on close/GC)."""
@@ -475,10 +507,12 @@ class PSSALayer:
             arr[i].inputs, arr[i].targets = _abi.ptr(ids, C.c_uint32), _abi.ptr(tg, C.c_uint32)
             tokens += ids.size
         loss = C.c_float()
+        self._batch_tokens = 0
         tl = np.empty(tokens, np.float32) if want_token_losses else None
         lg = np.empty((tokens, self.cfg.d_vocab), np.float32) if want_logits else None
         _abi.call(self._lib.pssa_hip_batch_forward, self.handle, arr, len(seqs), C.byref(loss),
                   _abi.ptr(tl), 0 if tl is None else tl.size, _abi.ptr(lg), 0 if lg is None else lg.size)
+        self._batch_tokens = tokens
         del keep
         out = [float(loss.value)]
         if want_token_losses:
@@ -486,6 +520,40 @@ class PSSALayer:
         if want_logits:
             out.append(lg)
         return out[0] if len(out) == 1 else tuple(out)
+
+    def token_logprobs(self, targets=None, top_k: int = 0, temperature: float = 1.0) -> dict:
+        """Scores the last batch_forward's tokens from the logits it left on the device, in its packed order: the log
+        probability of each target (`targets` [tokens], by default the batch's own; _abi.NO_TOKEN is not scored) and
+        the entropy, plus the top_k <= 64 alternatives' ids and log probabilities [tokens, top_k] when asked."""
+        n = getattr(self, "_batch_tokens", 0)
+        tg = None if targets is None else np.ascontiguousarray(np.asarray(targets).ravel(), dtype=np.uint32)
+        if tg is not None and tg.size != n:
+            raise ValueError("targets must have one id for each token of the last batch_forward")
+        out = {"logprobs": np.empty(n, np.float32), "entropy": np.empty(n, np.float32)}
+        if top_k:
+            out.update(top_ids=np.empty((n, top_k), np.uint32), top_logprobs=np.empty((n, top_k), np.float32))
+        _abi.call(self._lib.pssa_hip_batch_token_logprobs, self.handle, _abi.ptr(tg, C.c_uint32), n, temperature, top_k,
+                  _abi.ptr(out["logprobs"]), _abi.ptr(out["entropy"]), _abi.ptr(out.get("top_ids"), C.c_uint32),
+                  _abi.ptr(out.get("top_logprobs")))
+        return out
+
+    def distill(self, teacher_ids, teacher_logits, temperature: float = 1.0, row_weights=None,
+                want_grad: bool = True):
+        """Distillation of the last batch_forward's tokens from a teacher's top logits (ids and logits [tokens, k], in
+        packed order): the losses [tokens] and, unless want_grad is off, their gradient for the logits [tokens, V]."""
+        ids = np.ascontiguousarray(np.asarray(teacher_ids), dtype=np.uint32)
+        logits = _f32(teacher_logits)
+        n = getattr(self, "_batch_tokens", 0)
+        if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[0] != n:
+            raise ValueError("teacher ids and logits must be [tokens of the last batch_forward, k]")
+        w = None if row_weights is None else _f32(row_weights).ravel()
+        if w is not None and w.size != n:
+            raise ValueError("row_weights must have one weight for each token")
+        losses = np.empty(n, np.float32)
+        grad = np.empty((n, self.cfg.d_vocab), np.float32) if want_grad else None
+        _abi.call(self._lib.pssa_hip_batch_distill, self.handle, _abi.ptr(ids, C.c_uint32), _abi.ptr(logits), n,
+                  ids.shape[1], temperature, _abi.ptr(w), _abi.ptr(losses), _abi.ptr(grad))
+        return (losses, grad) if want_grad else losses
 
     # -- greedy decode (forward_inference + sample, src/pssa.rs:2387-2391,
     #    src/inference.rs:123-127) ------------------------------------------

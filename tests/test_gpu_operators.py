@@ -1,0 +1,441 @@
+"""Language-model operators on the GPU through the C ABI, each against its
+definition in 64 bits.
+
+Tolerances count roundings: u = 2^-24 is half a step of fp32, and an output
+held in bf16 adds its own half step 2^-8 relative.
+"""
+import numpy as np
+import pytest
+
+from pssa_amd import _abi
+from pssa_amd._abi import HipError
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+U16 = 2.0 ** -8  # bf16, relative to the value
+NONE = _abi.NO_TOKEN
+
+
+def say(*a):
+    print("[operators]", *a, flush=True)
+
+
+def to_bf16(x):
+    """(bits, value) of an array rounded to bf16, ties to even; infinities and NaN kept."""
+    x = np.ascontiguousarray(x, np.float32)
+    u = x.view(np.uint32).astype(np.uint64)
+    bits = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    bits = np.where(np.isfinite(x), bits, (u >> 16).astype(np.uint16) | np.where(np.isnan(x), 0x40, 0).astype(np.uint16))
+    bits = bits.astype(np.uint16)
+    return bits, from_bf16(bits)
+
+
+def from_bf16(bits):
+    return (np.ascontiguousarray(bits, np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+class Held:
+    """Device arrays of one test, freed together."""
+
+    def __init__(self, dev):
+        self.dev, self.bufs = dev, []
+
+    def up(self, a):
+        self.bufs.append(self.dev.upload(a))
+        return self.bufs[-1]
+
+    def new(self, shape, dtype, fill):
+        return self.up(np.full(shape, fill, dtype))
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.dev.synchronize()
+        for b in self.bufs:
+            b.close()
+
+
+def typed(x, dtype):
+    """The array in the operator's storage type, and the values it holds."""
+    return (np.ascontiguousarray(x, np.float32),) * 2 if dtype == "f32" else to_bf16(x)
+
+
+# ---------------------------------------------------------------------------
+# Log probabilities
+
+
+def log_softmax64(z, tau):
+    """log softmax in 64 bits, the entropy, and each row's kind: 0 ordinary, 1 empty, 2 not a number."""
+    z = z.astype(np.float64)
+    kind = np.where(np.isnan(z).any(1) | (z == np.inf).any(1), 2, np.where((z == -np.inf).all(1), 1, 0))
+    lp, ent = np.full(z.shape, -np.inf), np.zeros(len(z))
+    for r in range(len(z)):
+        if kind[r] == 2:
+            lp[r], ent[r] = np.nan, np.nan
+        elif kind[r] == 0:
+            d = (z[r] - z[r].max()) / tau
+            e = np.exp(d)
+            i = int(np.argmax(d))
+            lp[r] = d - np.log1p(np.delete(e, i).sum())
+            p = np.exp(lp[r])
+            ent[r] = -np.where(p > 0, p * np.where(p > 0, lp[r], 0.0), 0.0).sum()
+            lp[r][lp[r] < -np.finfo(np.float32).max] = -np.inf  # past fp32's range
+    return lp, ent, kind
+
+
+def top64(z, k):
+    """ids of the k largest logits, equal ones by id; NONE where a token cannot occur."""
+    ids = np.full((len(z), k), NONE, np.uint32)
+    for r, row in enumerate(z):
+        if np.isnan(row).any() or (row == np.inf).any():
+            continue
+        live = np.flatnonzero(row > -np.inf)
+        order = live[np.argsort(-row[live].astype(np.float64), kind="stable")][:k]
+        ids[r, :len(order)] = order
+    return ids
+
+
+def run_logprobs(hip, stored, rows, vocab, ld, targets, tau, k, dtype, offset=0):
+    """`offset`: elements before the first row in its buffer."""
+    with Held(hip) as h:
+        flat = np.concatenate([np.zeros(offset, stored.dtype), stored.ravel()])
+        x, t = h.up(flat), h.up(targets.astype(np.uint32))
+        lp, en = h.new(rows, np.float32, 7.0), h.new(rows, np.float32, 7.0)
+        ids, tl = h.new((rows, max(k, 1)), np.uint32, 7), h.new((rows, max(k, 1)), np.float32, 7.0)
+        hip.token_logprobs_resident(x.ptr + offset * stored.itemsize, dtype, rows, vocab, t.ptr, lp.ptr, en.ptr, k,
+                                    ids.ptr if k else None, tl.ptr if k else None, temperature=tau, ld=ld)
+        hip.synchronize()
+        return lp.to_host(), en.to_host(), ids.to_host()[:, :k], tl.to_host()[:, :k]
+
+
+def check_logprobs(hip, z, targets, tau, k, dtype, pad=0, offset=0):
+    rows, vocab = z.shape
+    wide = np.full((rows, vocab + pad), 1e30, np.float32)  # what lies between the rows is not read as tokens
+    wide[:, :vocab] = z
+    stored, held = typed(wide, dtype)
+    held = held[:, :vocab]
+    lp, en, ids, tl = run_logprobs(hip, stored, rows, vocab, vocab + pad, targets, tau, k, dtype, offset)
+    ref, ent, kind = log_softmax64(held, tau)
+    # A log probability d - log(1 + S): d has three roundings, S at most the sum's depth (64 in a thread, 10 across)
+    # plus the exponential's argument (|d| u relative, weighed by e^-|d| <= 1) and its own last place.
+    fin = np.where(np.isfinite(ref), ref, 0.0)
+    tol = U32 * (4 * np.abs(fin) + 100)
+    given = np.array([0.0 if t == NONE else np.nan if t >= vocab else ref[r, t] for r, t in enumerate(targets)])
+    given = np.where((targets != NONE) & (kind == 2), np.nan, given)
+    gtol = np.array([0.0 if t == NONE or t >= vocab else tol[r, t] for r, t in enumerate(targets)])
+    np.testing.assert_array_equal(np.isnan(lp), np.isnan(given))
+    assert np.all((np.abs(lp - given) <= gtol) | (lp == given) | np.isnan(given)), np.nanmax(np.abs(lp - given) / np.maximum(gtol, 1e-30))
+    # Entropy: every term p log p carries the error of its log p, sum p = 1.
+    span = np.array([(-row[np.isfinite(row)]).max() if np.isfinite(row).any() else 0.0 for row in ref])
+    etol = U32 * (4 * np.minimum(span, 60.0) + 200) * (1 + np.nan_to_num(ent))
+    np.testing.assert_array_equal(np.isnan(en), np.isnan(ent))
+    assert np.all((np.abs(en - ent) <= etol) | np.isnan(ent)), np.nanmax(np.abs(en - ent) / etol)
+    if k:
+        want = top64(held, k)
+        np.testing.assert_array_equal(ids, want)
+        for r in range(rows):
+            for j in range(k):
+                if want[r, j] == NONE:
+                    assert np.isnan(tl[r, j]) if kind[r] == 2 else tl[r, j] == -np.inf
+                else:
+                    assert tl[r, j] == ref[r, want[r, j]] or abs(tl[r, j] - ref[r, want[r, j]]) <= tol[r, want[r, j]]
+
+
+def logits_like(rng, rows, vocab):
+    z = rng.normal(0, 3, (rows, vocab))
+    z[np.arange(rows), rng.integers(0, vocab, rows)] += rng.uniform(0, 25, rows)
+    return z.astype(np.float32)
+
+
+def some_targets(rng, rows, vocab):
+    t = rng.integers(0, vocab, rows).astype(np.uint32)
+    t[rng.random(rows) < 0.2] = NONE
+    return t
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k,pad,tau", [
+    (1, 1, 1, 0, 1.0), (5, 2, 2, 3, 1.0), (3, 3, 3, 0, 2.0), (2, 7, 4, 1, 1.0), (4, 9, 9, 0, 0.5), (7, 64, 64, 0, 1.0),
+    (3, 255, 20, 2, 1.0), (2, 1024, 8, 0, 1.0), (2, 1025, 64, 1, 0.7), (2, 2049, 0, 5, 1.0), (3, 4099, 64, 0, 1.0),
+    (2, 8192, 5, 0, 1.0), (2, 16384, 64, 0, 1.0), (2, 16387, 8, 3, 3.0), (1, 33000, 64, 0, 1.0), (1, 70001, 20, 0, 1.0),
+    (2, 131075, 64, 1, 1.0), (1, 300007, 64, 0, 1.0)])
+def test_logprobs_match_64_bits(hip, dtype, rows, vocab, k, pad, tau):
+    """Every workgroup shape, its borders, and rows past the registers."""
+    say(f"logprobs {rows} x {vocab} (+{pad}) {dtype} top {k} tau {tau}")
+    rng = np.random.default_rng(vocab + k)
+    check_logprobs(hip, logits_like(rng, rows, vocab), some_targets(rng, rows, vocab), tau, k, dtype, pad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_logprobs_rows_at_any_element(hip, dtype, offset):
+    say("logprobs, first row at element", offset, dtype)
+    rng = np.random.default_rng(offset)
+    check_logprobs(hip, logits_like(rng, 5, 1501), some_targets(rng, 5, 1501), 1.0, 8, dtype, pad=offset, offset=offset)
+
+
+@pytest.mark.parametrize("vocab,k", [(50, 64), (3001, 64), (16384, 8), (140000, 64)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logprobs_masks_ties_and_bad_rows(hip, dtype, vocab, k):
+    """Rows with nothing left, with fewer tokens than alternatives, of one value, nearly certain, with signed zeros,
+    with the type's lowest and highest values, and with NaN or +inf."""
+    say("logprobs masks", vocab, k, dtype)
+    rng = np.random.default_rng(vocab)
+    z = logits_like(rng, 12, vocab)
+    z[0] = -np.inf
+    z[1] = -np.inf
+    z[1, [vocab - 1, 3, 4]] = [1.0, 2.0, 2.0]
+    z[2] = 0.25
+    z[3] = np.where(np.arange(vocab) % 2, 0.0, -0.0)
+    z[4, :] = -40.0
+    z[4, vocab // 2] = 20.0
+    low = 3.38e38  # finite in both types
+    z[5, :] = -low
+    z[5, 7] = low
+    z[6, 9] = np.nan
+    z[7, 1] = np.inf
+    z[8] = np.sort(z[8])  # the largest all in one thread's reach or behind it
+    z[9] = np.sort(z[9])[::-1]
+    z[10, rng.random(vocab) < 0.5] = -np.inf
+    z[11] = rng.integers(-2, 3, vocab)  # many equal
+    t = some_targets(rng, 12, vocab)
+    t[[0, 1, 6, 7]] = [0, 3, 9, 2]
+    t[11] = vocab  # no such token
+    check_logprobs(hip, z, t, 1.0, k, dtype)
+
+
+def test_logprobs_outputs_are_optional_and_the_rest_is_untouched(hip):
+    rng = np.random.default_rng(5)
+    z = logits_like(rng, 3, 500)
+    ref, ent, _ = log_softmax64(z, 1.0)
+    with Held(hip) as h:
+        x, en = h.up(z), h.new(4, np.float32, 7.0)
+        hip.token_logprobs_resident(x.ptr, "f32", 3, 500, entropy_ptr=en.ptr)
+        hip.synchronize()
+        got = en.to_host()
+        assert np.all(np.abs(got[:3] - ent) <= U32 * 600 * (1 + ent)) and got[3] == 7.0
+
+
+# ---------------------------------------------------------------------------
+# Distillation
+
+
+def distill64(z, ids, t, tau, w):
+    """Loss and gradient in 64 bits (rows with ordinary values)."""
+    z, t, w = z.astype(np.float64), t.astype(np.float64), w.astype(np.float64)
+    loss, grad = np.zeros(len(z)), np.zeros(z.shape)
+    for r in range(len(z)):
+        live = (ids[r] != NONE) & (t[r] > -np.inf)
+        if not live.any() or w[r] == 0:
+            continue
+        tr = t[r][live] / tau
+        q = np.exp(tr - tr.max())
+        q /= q.sum()
+        with np.errstate(divide="ignore", invalid="ignore"):
+            top = z[r].max()
+            e = np.exp((z[r] - top) / tau) if top > -np.inf else np.zeros_like(z[r])
+            p = e / e.sum() if e.sum() else e
+            lp = (z[r] - top) / tau - np.log(e.sum()) if e.sum() else np.full_like(z[r], -np.inf)
+        at = ids[r][live].astype(np.int64)
+        use = q > 0
+        loss[r] = w[r] * tau * tau * (q[use] * (np.log(q[use]) - lp[at[use]])).sum()
+        np.subtract.at(p, at, q)
+        grad[r] = w[r] * tau * p
+    return loss, grad
+
+
+def run_distill(hip, stored, rows, vocab, ld, ids, t, tau, w, dtype, in_place=False, want_grad=True, ld_grad=None):
+    with Held(hip) as h:
+        x, di, dt = h.up(stored), h.up(ids.astype(np.uint32)), h.up(t.astype(np.float32))
+        dw = None if w is None else h.up(w.astype(np.float32))
+        loss = h.new(rows, np.float32, 7.0)
+        ld_grad = ld if in_place else ld_grad or vocab
+        g = x if in_place else h.new((rows, ld_grad), stored.dtype, 7) if want_grad else None
+        hip.distill_resident(x.ptr, dtype, rows, vocab, di.ptr, dt.ptr, ids.shape[1], loss.ptr, g.ptr if g else None,
+                             temperature=tau, row_weights_ptr=dw.ptr if dw else None, ld=ld, ld_grad=ld_grad)
+        hip.synchronize()
+        grad = g.to_host().reshape(rows, ld_grad) if want_grad else None
+        return loss.to_host(), grad
+
+
+def check_distill(hip, z, ids, t, tau, w, dtype, pad=0, in_place=False, ld_grad=None):
+    rows, vocab = z.shape
+    wide = np.full((rows, vocab + pad), 1e30, np.float32)
+    wide[:, :vocab] = z
+    stored, held = typed(wide, dtype)
+    loss, grad = run_distill(hip, stored, rows, vocab, vocab + pad, ids, t, tau, w, dtype, in_place, True, ld_grad)
+    if in_place or ld_grad:  # what lies behind the rows stays
+        behind = grad[:, vocab:]
+        assert np.all(behind == (stored[:, vocab:] if in_place else 7))
+    grad = grad[:, :vocab]
+    ww = np.ones(rows, np.float32) if w is None else w
+    ref, gref = distill64(held[:, :vocab], ids, t, tau, ww)
+    got = grad if dtype == "f32" else from_bf16(grad)
+    live = (ids != NONE) & (t > -np.inf)
+    zr = np.where(np.isfinite(held[:, :vocab]), held[:, :vocab], 0)
+    span = (zr.max(1) - zr.min(1)) / tau + np.where(live, np.abs(t), 0).max(1) / tau + np.log(vocab)
+    scale = np.abs(ww) * tau
+    # p and q: the exponential's argument (|d| u, against p e^..: at most u once weighed), the sum's depth, two divisions.
+    gtol = (U32 * (100 + 4 * np.minimum(span, 90.0)))[:, None] * (np.abs(gref) + scale[:, None] * 2.0 / 3) + \
+        (U16 * np.abs(gref) if dtype == "bf16" else 0) + 1e-37
+    assert np.all(np.abs(got.astype(np.float64) - gref) <= gtol), np.max(np.abs(got - gref) / gtol)
+    ltol = U32 * (200 + 8 * span) * scale * tau * (1 + span)
+    ok = (np.abs(loss - ref) <= ltol) | (loss == ref)
+    assert ok.all(), (loss[~ok], ref[~ok], ltol[~ok])
+    return loss, got
+
+
+def teacher(rng, rows, vocab, k, dead=0.1):
+    ids = np.stack([rng.choice(vocab, k, replace=k > vocab) for _ in range(rows)]).astype(np.uint32)
+    t = rng.normal(0, 3, (rows, k)).astype(np.float32)
+    ids[rng.random((rows, k)) < dead] = NONE
+    return ids, t
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k,pad,tau", [
+    (1, 1, 1, 0, 1.0), (3, 2, 2, 1, 1.0), (4, 5, 3, 0, 2.0), (2, 9, 9, 0, 1.0), (7, 64, 8, 0, 1.0), (3, 255, 20, 2, 0.7),
+    (2, 1025, 64, 0, 1.0), (3, 2048, 100, 0, 4.0), (3, 4099, 8, 1, 1.0), (2, 8193, 20, 0, 1.0), (2, 16384, 64, 0, 2.0),
+    (2, 33001, 1024, 0, 1.0), (1, 65537, 64, 3, 1.5), (2, 140001, 20, 0, 1.0)])
+def test_distill_matches_64_bits(hip, dtype, rows, vocab, k, pad, tau):
+    say(f"distill {rows} x {vocab} (+{pad}) {dtype} teacher {k} tau {tau}")
+    rng = np.random.default_rng(vocab + k)
+    ids, t = teacher(rng, rows, vocab, k)
+    w = rng.uniform(0.1, 1.0, rows).astype(np.float32)
+    check_distill(hip, logits_like(rng, rows, vocab), ids, t, tau, w, dtype, pad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [37, 5003, 140003])
+def test_distill_in_place_equals_apart(hip, dtype, vocab):
+    say("distill in place", vocab, dtype)
+    rng = np.random.default_rng(vocab)
+    z = logits_like(rng, 4, vocab)
+    ids, t = teacher(rng, 4, vocab, 16)
+    a = check_distill(hip, z, ids, t, 1.5, None, dtype, pad=3, in_place=True)
+    b = check_distill(hip, z, ids, t, 1.5, None, dtype, pad=3, ld_grad=vocab + 5)
+    np.testing.assert_array_equal(a[0], b[0])
+    np.testing.assert_array_equal(a[1], b[1])
+    stored, _ = typed(z, dtype)
+    alone, _ = run_distill(hip, stored, 4, vocab, vocab, ids, t, 1.5, None, dtype, want_grad=False)
+    np.testing.assert_array_equal(alone, a[0])
+
+
+def test_distill_special_rows(hip):
+    """Duplicate entries, frames without entries, rows without weight (whatever they hold), masked student tokens, one
+    certain teacher token, and rows that are not numbers."""
+    say("distill special rows")
+    rng = np.random.default_rng(3)
+    V, K = 3001, 12
+    z = logits_like(rng, 10, V)
+    ids, t = teacher(rng, 10, V, K, dead=0.0)
+    w = rng.uniform(0.5, 1.0, 10).astype(np.float32)
+    ids[0, [3, 7, 11]] = ids[0, 0]  # one token four times
+    ids[1] = NONE
+    t[1] = np.nan  # not read as entries
+    w[2], z[2, 5] = 0.0, np.nan
+    t[3, 1:] = -np.inf
+    z[4, rng.random(V) < 0.5] = -np.inf
+    z[4, ids[4]] = 1.0
+    z[5] = -np.inf
+    z[5, ids[5]] = 0.5
+    good = [0, 1, 3, 4, 5]
+    check_distill(hip, z[good], ids[good], t[good], 1.3, w[good], "f32")
+    z[6, 17] = np.nan
+    z[7, 18] = np.inf
+    t[8, 2] = np.nan
+    ids[9, 4] = V
+    z2, i2, t2, w2 = z[[6, 7, 8, 9, 2]], ids[[6, 7, 8, 9, 2]], t[[6, 7, 8, 9, 2]], w[[6, 7, 8, 9, 2]]
+    loss, grad = run_distill(hip, z2, 5, V, V, i2, t2, 1.0, w2, "f32")
+    assert np.isnan(loss[:4]).all() and np.isnan(grad[:4]).all()
+    assert loss[4] == 0 and not grad[4].any()
+    # A taught token that the student masks: infinite loss, the gradient of what is left finite; a student without
+    # any token likewise.
+    z3 = logits_like(rng, 2, V)
+    i3, t3 = teacher(rng, 2, V, K, dead=0.0)
+    z3[0, i3[0, 0]] = -np.inf
+    z3[1] = -np.inf
+    loss, grad = run_distill(hip, z3, 2, V, V, i3, t3, 1.0, None, "f32")
+    assert np.all(loss == np.inf) and np.isfinite(grad).all()
+    _, gref = distill64(z3, i3, t3, 1.0, np.ones(2))
+    assert np.max(np.abs(grad - gref)) <= U32 * 500
+
+
+def test_distill_gradient_is_the_losses_slope(hip):
+    """Central differences of the loss itself: step h, error h^2/6 |f'''| (third derivatives of a log-sum-exp are at
+    most 1/tau of the row's weight) plus the loss's own rounding over 2h."""
+    rng = np.random.default_rng(9)
+    V, K, tau, h = 40, 6, 1.5, 2.0 ** -4
+    z = rng.normal(0, 1, (1, V)).astype(np.float32)
+    ids, t = teacher(rng, 1, V, K, dead=0.0)
+    _, grad = run_distill(hip, z, 1, V, V, ids, t, tau, None, "f32")
+    up, down = np.repeat(z, V, 0), np.repeat(z, V, 0)
+    up[np.arange(V), np.arange(V)] += np.float32(h)
+    down[np.arange(V), np.arange(V)] -= np.float32(h)
+    step = (up - down).diagonal().astype(np.float64)
+    rep = lambda a: np.repeat(a, V, 0)
+    lu, _ = run_distill(hip, up, V, V, V, rep(ids), rep(t), tau, None, "f32", want_grad=False)
+    ld, _ = run_distill(hip, down, V, V, V, rep(ids), rep(t), tau, None, "f32", want_grad=False)
+    slope = (lu.astype(np.float64) - ld) / step
+    tol = h * h / 6 / tau + U32 * 400 * tau * tau * 8 / h
+    assert np.max(np.abs(slope - grad[0])) <= tol
+
+
+# ---------------------------------------------------------------------------
+# Both on a batch forward's logits
+
+
+def test_batch_scores_and_distillation(hip):
+    """A teacher model scores a ragged batch and keeps each token's top alternatives; a student of the same vocabulary
+    is taught by them: losses and gradients of the packed tokens, in that order."""
+    from pssa_amd import ModelWeights, PSSAConfig, PSSALayer, Sequence
+
+    say("batch scores and distillation")
+    cfg = PSSAConfig(depth=2, d_vocab=517, d_latent=48, d_state=24, d_mem_key=8, mem_capacity=30)
+    rng = np.random.default_rng(4)
+    seqs = [Sequence(lane, rng.integers(0, 517, n, dtype=np.uint32), rng.integers(0, 517, n, dtype=np.uint32), True)
+            for lane, n in ((2, 9), (0, 30), (3, 1), (1, 17))]
+    layers = []
+    for seed in (1, 2):
+        w = ModelWeights.init(cfg, seed, "baseline")
+        w.unembed *= 40.0
+        w.populate_banks(seed + 5, count=27)
+        layers.append(PSSALayer(hip, w, lanes=4, max_tokens=64))
+    teach, learn = layers
+    with pytest.raises((HipError, ValueError)):
+        teach.token_logprobs()
+    K, tau = 10, 2.0
+    loss, token_losses, lg = teach.batch_forward(seqs, want_token_losses=True, want_logits=True)
+    got = teach.token_logprobs(top_k=K)
+    ref, ent, _ = log_softmax64(lg, 1.0)
+    targets = np.concatenate([s.targets for s in seqs])
+    tol = U32 * (4 * np.abs(ref).max() + 200)
+    assert np.max(np.abs(got["logprobs"] - ref[np.arange(len(targets)), targets])) <= tol
+    assert np.max(np.abs(got["logprobs"] + token_losses)) <= 2 * tol + U32 * 400
+    assert np.max(np.abs(got["entropy"] - ent)) <= tol * (1 + ent.max())
+    np.testing.assert_array_equal(got["top_ids"], top64(lg, K))
+    other = targets.copy()
+    other[::3] = NONE
+    again = teach.token_logprobs(targets=other)
+    np.testing.assert_array_equal(again["logprobs"], np.where(other == NONE, 0, got["logprobs"]).astype(np.float32))
+
+    _, slg = learn.batch_forward(seqs, want_logits=True)
+    n = len(targets)
+    weights = np.full(n, 1.0 / n, np.float32)
+    losses, grad = learn.distill(got["top_ids"], got["top_logprobs"], tau, weights)
+    lref, gref = distill64(slg, got["top_ids"], got["top_logprobs"], tau, weights)
+    assert np.max(np.abs(losses - lref)) <= U32 * 2000 * tau * tau / n
+    assert np.max(np.abs(grad - gref)) <= U32 * 400 * tau / n
+    np.testing.assert_array_equal(learn.distill(got["top_ids"], got["top_logprobs"], tau, weights, want_grad=False), losses)
+    # The head's adjoints take the gradient as it is: d logits . unembed and d logits^T . features.
+    back = hip.gemm_nn(grad, w.unembed, n, cfg.d_vocab, cfg.d_latent).reshape(n, -1)
+    want = gref @ w.unembed.astype(np.float64)
+    assert np.max(np.abs(back - want)) <= 1e-4 * np.abs(want).max()
+    with pytest.raises(HipError, match="outside model vocabulary"):
+        bad = got["top_ids"].copy()
+        bad[3, 2] = 517
+        learn.distill(bad, got["top_logprobs"], tau)
+    for layer in layers:
+        layer.close()
