@@ -644,6 +644,39 @@ int pssa_hip_batch_distill(pssa_hip_lanes* lanes, const uint32_t* teacher_ids, c
                            size_t n_tokens, size_t teacher_k, float temperature, const float* row_weights,
                            float* losses, float* grad_logits, char* err, size_t err_len);
 
+/* 4-bit weights of a [n, k] matrix, laid out once for the products:
+ *   W[i][j] = scale[i][j / group] * (code[i][j] - zero[i][j / group]),
+ * codes and zero points 0..15, group 32, 64 or 128 (the last group of a row
+ * may be short).  The handle owns device memory; free it before its context. */
+typedef struct pssa_hip_w4 pssa_hip_w4;
+/* codes [n, k] one byte each (the upper four bits are ignored), scales
+ * [n, ceil(k / group)], zeros likewise or NULL (8 everywhere, so codes stand
+ * for -8..7): device arrays, read before the call returns. */
+int pssa_hip_w4_load_resident(pssa_hip_ctx* ctx, const uint8_t* d_codes, const float* d_scales, const uint8_t* d_zeros,
+                              size_t n, size_t k, size_t group, pssa_hip_w4** out, char* err, size_t err_len);
+/* The same from host arrays. */
+int pssa_hip_w4_load(pssa_hip_ctx* ctx, const uint8_t* codes, size_t codes_len, const float* scales, size_t scales_len,
+                     const uint8_t* zeros, size_t n, size_t k, size_t group, pssa_hip_w4** out, char* err,
+                     size_t err_len);
+void pssa_hip_w4_free(pssa_hip_w4* w);
+/* Codes, scales and (zeros not NULL) zero points of an fp32 matrix, on the
+ * host; no device needed.  Without zero points scale = max |w| / 7; with
+ * them the codes span [min(w, 0), max(w, 0)].  Codes round to nearest, ties to
+ * even; a non-finite weight is PSSA_HIP_EINVAL. */
+int pssa_hip_w4_quantize(const float* w, size_t w_len, size_t n, size_t k, size_t group, uint8_t* codes, float* scales,
+                         uint8_t* zeros, char* err, size_t err_len);
+
+/* y[m, n] = x[m, k] W^T on device arrays: x of x_dtype with rows d_x + i*ld_x
+ * (ld_x >= k), y fp32 with rows d_y + i*ld_y (ld_y >= n), rows at any
+ * element; y must not overlap x.  Products and sums are fp32 (x is not
+ * rounded); a row's values do not depend on the rows beside it.  An infinity or
+ * NaN in a row of x gives values that are not finite in that row. */
+int pssa_hip_matvec_w4_resident(pssa_hip_w4* w, const void* d_x, int x_dtype, size_t m, size_t ld_x, float* d_y,
+                                size_t ld_y, char* err, size_t err_len);
+/* The same on fp32 host arrays x [m, k], y [m, n]. */
+int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, float* y, size_t y_len, char* err,
+                       size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,7 @@ DECODE_GRAPH = 2
 fp = C.POINTER(C.c_float)
 u64p = C.POINTER(C.c_uint64)
 u32p = C.POINTER(C.c_uint32)
+u8p = C.POINTER(C.c_uint8)
 sz = C.c_size_t
 err_t = C.c_char_p
 
@@ -195,6 +196,12 @@ def lib() -> C.CDLL:
         "pssa_hip_distill_resident": ([vp, vp, C.c_int, sz, sz, sz, vp, vp, sz, C.c_float, vp, vp, vp, sz, err_t, sz],
                                       C.c_int),
         "pssa_hip_batch_token_logprobs": ([vp, u32p, sz, C.c_float, sz, fp, fp, u32p, fp, err_t, sz], C.c_int),
+        "pssa_hip_w4_load_resident": ([vp, vp, vp, vp, sz, sz, sz, pp, err_t, sz], C.c_int),
+        "pssa_hip_w4_load": ([vp, u8p, sz, fp, sz, u8p, sz, sz, sz, pp, err_t, sz], C.c_int),
+        "pssa_hip_w4_free": ([vp], None),
+        "pssa_hip_w4_quantize": ([fp, sz, sz, sz, sz, u8p, fp, u8p, err_t, sz], C.c_int),
+        "pssa_hip_matvec_w4_resident": ([vp, vp, C.c_int, sz, sz, vp, sz, err_t, sz], C.c_int),
+        "pssa_hip_matvec_w4": ([vp, fp, sz, sz, fp, sz, err_t, sz], C.c_int),
         "pssa_hip_batch_distill": ([vp, u32p, fp, sz, sz, C.c_float, fp, fp, fp, err_t, sz], C.c_int),
     }
     for name, (args, res) in sig.items():

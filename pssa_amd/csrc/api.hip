@@ -205,6 +205,7 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_decode_attributes());
     PSSA_RETURN_IF(pssa::init_dense_scan_attributes());
     PSSA_RETURN_IF(pssa::init_operator_attributes());
+    PSSA_RETURN_IF(pssa::init_w4_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));
     *out = ctx.release();
     return Status::Ok();
@@ -2023,6 +2024,13 @@ int pssa_hip_dense_scan_reserve(pssa_hip_ctx* ctx, size_t batch, size_t seq_len,
 
 // ------------------------------------------------- language-model operators
 
+// 4-bit weights on the device.
+struct pssa_hip_w4 {
+  pssa_hip_ctx* ctx = nullptr;
+  DevBuf packed, scales, zeros;
+  pssa::W4View view;
+};
+
 namespace {
 
 // Runs an entry point's body; no C++ exception leaves it.
@@ -2074,6 +2082,34 @@ Status rows_to_host(pssa_hip_lanes* L, T* out, const DevBuf& buf, size_t width) 
 Status check_batch(const pssa_hip_lanes* L, size_t n_tokens) {
   PSSA_RETURN_IF(need(!L->tok_row.empty(), "no batch forward has left logits on these lanes"));
   return need(n_tokens == L->tok_row.size(), "token count must be the last batch forward's");
+}
+
+Status check_w4(size_t n, size_t k, size_t group) {
+  PSSA_RETURN_IF(need(n && k, "4-bit weights: dimensions must be positive"));
+  PSSA_RETURN_IF(need(group == 32 || group == 64 || group == 128, "4-bit weights: group must be 32, 64 or 128"));
+  // Tiles and columns are counted in 32 bits, the packed bytes in the grid of the layout's kernel.
+  return need(n <= ((size_t)1 << 30) && k <= ((size_t)1 << 24) && n <= ((size_t)1 << 38) / k,
+              "4-bit weights: too large");
+}
+
+// Lays device arrays out into a new handle; the caller waits for the stream.
+Status load_w4(pssa_hip_ctx* ctx, const uint8_t* codes, const float* scales, const uint8_t* zeros, size_t n, size_t k,
+               size_t group, std::unique_ptr<pssa_hip_w4>& w) {
+  w = std::make_unique<pssa_hip_w4>();
+  w->ctx = ctx;
+  const size_t held = pssa::w4_groups_held(n, k, group);
+  PSSA_RETURN_IF(w->packed.alloc(pssa::w4_packed_bytes(n, k)));
+  PSSA_RETURN_IF(w->scales.alloc(held * 4));
+  if (zeros) PSSA_RETURN_IF(w->zeros.alloc(held));
+  PSSA_RETURN_IF(pssa::launch_w4_pack(ctx->stream, codes, scales, zeros, (int)n, (int)k, (int)group, w->packed.p,
+                                      w->scales.as<float>(), w->zeros.as<uint8_t>()));
+  w->view.packed = w->packed.p;
+  w->view.scales = w->scales.as<float>();
+  w->view.zeros = zeros ? w->zeros.as<uint8_t>() : nullptr;
+  w->view.n = (int)n;
+  w->view.k = (int)k;
+  w->view.group = (int)group;
+  return Status::Ok();
 }
 
 }  // namespace
@@ -2248,6 +2284,102 @@ int pssa_hip_batch_distill(pssa_hip_lanes* L, const uint32_t* teacher_ids, const
         i = e;
       }
     }
+    return sync(ctx);
+  }, err, err_len);
+}
+
+int pssa_hip_w4_load_resident(pssa_hip_ctx* ctx, const uint8_t* d_codes, const float* d_scales, const uint8_t* d_zeros,
+                              size_t n, size_t k, size_t group, pssa_hip_w4** out, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(out != nullptr, "null output handle"));
+    *out = nullptr;
+    PSSA_RETURN_IF(need(d_codes && d_scales, "4-bit weights: null buffer"));
+    PSSA_RETURN_IF(check_w4(n, k, group));
+    PSSA_RETURN_IF(need(aligned_to(d_scales, 4), "4-bit weights: misaligned buffer"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    std::unique_ptr<pssa_hip_w4> w;
+    PSSA_RETURN_IF(load_w4(ctx, d_codes, d_scales, d_zeros, n, k, group, w));
+    PSSA_RETURN_IF(sync(ctx));
+    *out = w.release();
+    return Status::Ok();
+  }, err, err_len);
+}
+
+int pssa_hip_w4_load(pssa_hip_ctx* ctx, const uint8_t* codes, size_t codes_len, const float* scales, size_t scales_len,
+                     const uint8_t* zeros, size_t n, size_t k, size_t group, pssa_hip_w4** out, char* err,
+                     size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(out != nullptr, "null output handle"));
+    *out = nullptr;
+    PSSA_RETURN_IF(need(codes && scales, "4-bit weights: null buffer"));
+    PSSA_RETURN_IF(check_w4(n, k, group));
+    const size_t groups = n * ((k + group - 1) / group);
+    PSSA_RETURN_IF(need(codes_len == n * k && scales_len == groups,
+                        "4-bit weights: codes must be [n, k] and scales [n, ceil(k / group)]"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    DevBuf dc, ds, dz;
+    PSSA_RETURN_IF(upload(ctx, dc, codes, codes_len));
+    PSSA_RETURN_IF(upload(ctx, ds, scales, groups * 4));
+    if (zeros) PSSA_RETURN_IF(upload(ctx, dz, zeros, groups));
+    std::unique_ptr<pssa_hip_w4> w;
+    PSSA_RETURN_IF(load_w4(ctx, dc.as<uint8_t>(), ds.as<float>(), zeros ? dz.as<uint8_t>() : nullptr, n, k, group, w));
+    PSSA_RETURN_IF(sync(ctx));
+    *out = w.release();
+    return Status::Ok();
+  }, err, err_len);
+}
+
+void pssa_hip_w4_free(pssa_hip_w4* w) {
+  if (!w) return;
+  {
+    std::lock_guard<std::mutex> g(w->ctx->mu);
+    (void)hipSetDevice(w->ctx->device);
+    (void)hipStreamSynchronize(w->ctx->stream);
+  }
+  delete w;
+}
+
+int pssa_hip_matvec_w4_resident(pssa_hip_w4* w, const void* d_x, int x_dtype, size_t m, size_t ld_x, float* d_y,
+                                size_t ld_y, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(w && d_x && d_y, "4-bit product: null weights or buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(x_dtype), "unknown dtype"));
+    PSSA_RETURN_IF(need(m >= 1, "4-bit product: dimensions must be positive"));
+    PSSA_RETURN_IF(need(m <= 65535, "4-bit product: at most 65535 rows"));
+    const size_t n = (size_t)w->view.n, k = (size_t)w->view.k;
+    PSSA_RETURN_IF(need(ld_x >= k && ld_y >= n, "4-bit product: row stride below the row"));
+    size_t nx = 0, ny = 0;
+    PSSA_RETURN_IF(pssa::checked_count({m, ld_x}, &nx, "4-bit product input"));
+    PSSA_RETURN_IF(pssa::checked_count({m, ld_y}, &ny, "4-bit product output"));
+    PSSA_RETURN_IF(need(aligned_to(d_x, dtype_size(x_dtype)) && aligned_to(d_y, 4), "4-bit product: misaligned buffer"));
+    const uintptr_t x = (uintptr_t)d_x, y = (uintptr_t)d_y;
+    PSSA_RETURN_IF(need(x + ((m - 1) * ld_x + k) * dtype_size(x_dtype) <= y || y + ((m - 1) * ld_y + n) * 4 <= x,
+                        "4-bit product: the output overlaps the input"));
+    std::lock_guard<std::mutex> g(w->ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(w->ctx->device));
+    return pssa::launch_matvec_w4(w->ctx->stream, x_dtype, d_x, ld_x, (int)m, w->view, d_y, ld_y);
+  }, err, err_len);
+}
+
+int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, float* y, size_t y_len, char* err,
+                       size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(w && x && y, "4-bit product: null weights or buffer"));
+    PSSA_RETURN_IF(need(m >= 1 && m <= 65535, "4-bit product: rows must be in 1..=65535"));
+    const size_t n = (size_t)w->view.n, k = (size_t)w->view.k;
+    PSSA_RETURN_IF(need(x_len == m * k && y_len == m * n, "4-bit product: x must be [m, k] and y [m, n]"));
+    pssa_hip_ctx* ctx = w->ctx;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    DevBuf dx, dy;
+    PSSA_RETURN_IF(upload(ctx, dx, x, x_len * 4));
+    PSSA_RETURN_IF(dy.alloc(y_len * 4, &ctx->pool));
+    PSSA_RETURN_IF(pssa::launch_matvec_w4(ctx->stream, PSSA_HIP_F32, dx.p, k, (int)m, w->view, dy.as<float>(), n));
+    PSSA_RETURN_IF(download(ctx, y, dy, y_len * 4));
     return sync(ctx);
   }, err, err_len);
 }

@@ -276,3 +276,40 @@ extern "C" int pssa_hip_weights_set_value_cap(const pssa_hip_weights* w, float c
   }
   return PSSA_HIP_OK;
 }
+
+extern "C" int pssa_hip_w4_quantize(const float* w, size_t w_len, size_t n, size_t k, size_t group, uint8_t* codes,
+                                    float* scales, uint8_t* zeros, char* err, size_t err_len) {
+  if (!w || !codes || !scales) {
+    set_err(err, err_len, "4-bit weights: null buffer");
+    return PSSA_HIP_EINVAL;
+  }
+  if (!n || !k || (group != 32 && group != 64 && group != 128) || n > ((size_t)1 << 38) / k || w_len != n * k) {
+    set_err(err, err_len, "4-bit weights: w must be [n, k], group 32, 64 or 128");
+    return PSSA_HIP_EINVAL;
+  }
+  for (size_t i = 0; i < w_len; i++)
+    if (!std::isfinite(w[i])) {
+      set_err(err, err_len, "4-bit weights: weights must be finite");
+      return PSSA_HIP_EINVAL;
+    }
+  const size_t groups = (k + group - 1) / group;
+  for (size_t r = 0; r < n; r++)
+    for (size_t g = 0; g < groups; g++) {
+      const float* p = w + r * k + g * group;
+      uint8_t* q = codes + r * k + g * group;
+      const size_t len = std::min(group, k - g * group);
+      double lo = 0.0, hi = 0.0;
+      for (size_t i = 0; i < len; i++) {
+        lo = std::min(lo, (double)p[i]);
+        hi = std::max(hi, (double)p[i]);
+      }
+      const float s = (float)(zeros ? (hi - lo) / 15.0 : std::max(hi, -lo) / 7.0);
+      const double zero = !zeros ? 8.0 : s > 0.0f ? std::min(15.0, std::nearbyint(-lo / s)) : 0.0;
+      scales[r * groups + g] = s;
+      if (zeros) zeros[r * groups + g] = (uint8_t)zero;
+      for (size_t i = 0; i < len; i++)
+        q[i] = (uint8_t)(s > 0.0f ? std::min(15.0, std::max(0.0, std::nearbyint(p[i] / (double)s) + zero)) : zero);
+    }
+  if (err && err_len) err[0] = 0;
+  return PSSA_HIP_OK;
+}

@@ -8,6 +8,7 @@ namespace pssa {
 
 // Dynamic LDS above the default limit, once for each device.
 Status init_operator_attributes();
+Status init_w4_attributes();
 
 // ---------------------------------------------------------------- logit rows
 constexpr int kMaxAlternatives = 64;  // top tokens a row can list: one wave's lanes
@@ -41,5 +42,19 @@ struct DistillArgs {
   size_t ld_grad = 0;
 };
 Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& a, size_t rows);
+
+// -------------------------------------------------------------- 4-bit weights
+struct W4View {
+  const void* packed = nullptr;
+  const float* scales = nullptr;   // half of each group's scale, [tile][group][16]
+  const uint8_t* zeros = nullptr;  // [tile][group][16], null: 8 everywhere
+  int n = 0, k = 0, group = 0;
+};
+size_t w4_packed_bytes(size_t n, size_t k);
+size_t w4_groups_held(size_t n, size_t k, size_t group);
+Status launch_w4_pack(hipStream_t stream, const uint8_t* codes, const float* scales, const uint8_t* zeros, int n, int k,
+                      int group, void* packed, float* out_scales, uint8_t* out_zeros);
+Status launch_matvec_w4(hipStream_t stream, int x_dtype, const void* x, size_t ld_x, int m, const W4View& w, float* y,
+                        size_t ld_y);
 
 }  // namespace pssa

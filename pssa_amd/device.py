@@ -324,6 +324,77 @@ class HipDevice:
                   teacher_ids_ptr, teacher_logits_ptr, teacher_k, temperature, row_weights_ptr, losses_ptr, grad_ptr,
                   ld_grad)
 
+    def w4_matrix_resident(self, codes_ptr: int, scales_ptr: int, n: int, k: int, group: int,
+                           zeros_ptr: int | None = None) -> "W4Matrix":
+        """4-bit weights from device arrays: u8 codes [n, k], f32 scales [n, ceil(k / group)] and u8 zero points
+        likewise (8 everywhere when None), laid out for matvec_w4 before the call returns."""
+        h = C.c_void_p()
+        _abi.call(self._lib.pssa_hip_w4_load_resident, self.handle, codes_ptr, scales_ptr, zeros_ptr, n, k, group,
+                  C.byref(h))
+        return W4Matrix(self, h, n, k, group)
+
+    def w4_matrix(self, codes, scales, group: int, zeros=None) -> "W4Matrix":
+        """The same from host arrays (quantize_w4 makes them of an fp32 matrix)."""
+        codes = np.ascontiguousarray(codes, np.uint8)
+        scales = _f32(scales)
+        n, k = codes.shape
+        if zeros is not None:
+            zeros = np.ascontiguousarray(zeros, np.uint8)
+            if zeros.shape != scales.shape:
+                raise ValueError("zero points must have the scales' shape")
+        h = C.c_void_p()
+        _abi.call(self._lib.pssa_hip_w4_load, self.handle, _abi.ptr(codes, C.c_uint8), codes.size, _abi.ptr(scales),
+                  scales.size, _abi.ptr(zeros, C.c_uint8), n, k, group, C.byref(h))
+        return W4Matrix(self, h, n, k, group)
+
+    def matvec_w4_resident(self, x_ptr: int, x_dtype: str, m: int, w: "W4Matrix", y_ptr: int, ld_x: int | None = None,
+                           ld_y: int | None = None) -> None:
+        """y[m, n] (f32) = x[m, k] W^T on device arrays, m few rows of f32 or bf16 (asynchronous on the context
+        stream of the weights' device)."""
+        _abi.call(self._lib.pssa_hip_matvec_w4_resident, w.handle, x_ptr, _dtype(x_dtype), m,
+                  w.k if ld_x is None else ld_x, y_ptr, w.n if ld_y is None else ld_y)
+
+    def matvec_w4(self, x, w: "W4Matrix") -> np.ndarray:
+        """y[m, n] = x[m, k] W^T for f32 host rows (one row may be given as [k])."""
+        x = np.atleast_2d(_f32(x))
+        if x.ndim != 2 or x.shape[1] != w.k:
+            raise ValueError(f"x must be [m, {w.k}]")
+        y = np.empty((x.shape[0], w.n), np.float32)
+        _abi.call(self._lib.pssa_hip_matvec_w4, w.handle, _abi.ptr(x), x.size, x.shape[0], _abi.ptr(y), y.size)
+        return y
+
+
+def quantize_w4(w, group: int, zeros: bool = False):
+    """Codes u8 [n, k], scales f32 [n, ceil(k / group)] and zero points u8 (None unless asked) of an fp32 matrix, on
+    the host: W = scale * (code - zero), zero 8 where there are no zero points."""
+    w = _f32(w)
+    n, k = w.shape
+    groups = -(-k // max(group, 1))
+    codes, scales = np.empty((n, k), np.uint8), np.empty((n, groups), np.float32)
+    zp = np.empty((n, groups), np.uint8) if zeros else None
+    _abi.call(_abi.lib().pssa_hip_w4_quantize, _abi.ptr(w), w.size, n, k, group, _abi.ptr(codes, C.c_uint8),
+              _abi.ptr(scales), _abi.ptr(zp, C.c_uint8))
+    return codes, scales, zp
+
+
+class W4Matrix:
+    """4-bit weights [n, k] in the products' layout on a device (freed on close/GC)."""
+
+    def __init__(self, device: HipDevice, handle, n: int, k: int, group: int):
+        self.device, self.handle, self.n, self.k, self.group = device, handle, n, k, group
+        device._children.add(self)
+
+    def close(self) -> None:
+        if self.handle and self.device.handle:
+            self.device._lib.pssa_hip_w4_free(self.handle)
+        self.handle = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
 
 class DeviceBuffer:
     """A device allocation made through the C ABI (freed on close/GC)."""

@@ -439,3 +439,105 @@ def test_batch_scores_and_distillation(hip):
         learn.distill(bad, got["top_logprobs"], tau)
     for layer in layers:
         layer.close()
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights
+
+
+def w4_inputs(rng, n, k, group, zeros):
+    codes = rng.integers(0, 16, (n, k), dtype=np.uint8)
+    scales = (rng.uniform(0.5, 1.5, (n, -(-k // group))) * 0.1).astype(np.float32)
+    zp = rng.integers(0, 16, scales.shape, dtype=np.uint8) if zeros else None
+    at = np.arange(k) // group
+    w = (codes - (zp[:, at].astype(np.float64) if zeros else 8.0)) * scales[:, at].astype(np.float64)
+    return codes, scales, zp, w
+
+
+def w4_tolerance(x, codes, scales, zp, group):
+    """Exact products; sums of 32 in the matrix instruction, of a group's four, of the groups and of the waves: at most
+    32 + 4 + k / group + 8 roundings of partial sums that sum |x| (|2q - 15| + |15 - 2z|) s / 2 bounds."""
+    at = np.arange(codes.shape[1]) // group
+    z = zp[:, at].astype(np.float64) if zp is not None else 8.0
+    mag = (np.abs(2.0 * codes - 15) + np.abs(15 - 2 * z)) * scales[:, at] / 2
+    return U32 * (44 + codes.shape[1] / group) * (np.abs(x.astype(np.float64)) @ mag.T) + 1e-37
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k,group,zeros", [
+    (1, 1, 1, 32, False), (1, 16, 128, 32, True), (2, 17, 129, 64, False), (1, 100, 768, 64, False),
+    (5, 33, 100, 32, True), (6, 48, 300, 128, True), (10, 64, 257, 64, True), (11, 20, 500, 32, False),
+    (16, 31, 640, 128, False), (17, 40, 333, 32, True), (33, 70, 1030, 64, True), (3, 5000, 96, 32, True),
+    (1, 40, 8192, 128, True), (4, 70000, 130, 64, False), (70, 24, 128, 128, True)])
+def test_matvec_w4_matches_64_bits(hip, dtype, m, n, k, group, zeros):
+    say(f"w4 {m} x {n} x {k} group {group} {dtype} zeros {zeros}")
+    rng = np.random.default_rng(n + k)
+    codes, scales, zp, w = w4_inputs(rng, n, k, group, zeros)
+    pad_x, pad_y = 3, 5
+    stored, held = typed(rng.normal(0, 1, (m, k + pad_x)).astype(np.float32), dtype)
+    mat = hip.w4_matrix(codes, scales, group, zp)
+    with Held(hip) as h:
+        x, y = h.up(stored), h.new((m, n + pad_y), np.float32, 7.0)
+        hip.matvec_w4_resident(x.ptr, dtype, m, mat, y.ptr, ld_x=k + pad_x, ld_y=n + pad_y)
+        hip.synchronize()
+        got = y.to_host()
+        assert np.all(got[:, n:] == 7.0)
+        ref = held[:, :k].astype(np.float64) @ w.T
+        tol = w4_tolerance(held[:, :k], codes, scales, zp, group)
+        assert np.all(np.abs(got[:, :n] - ref) <= tol), np.max(np.abs(got[:, :n] - ref) / tol)
+        # A row alone has the same bits.
+        i = m // 2
+        hip.matvec_w4_resident(x.ptr + i * (k + pad_x) * stored.itemsize, dtype, 1, mat, y.ptr)
+        hip.synchronize()
+        np.testing.assert_array_equal(y.to_host().ravel()[:n].view(np.uint32), got[i, :n].view(np.uint32))
+    if dtype == "f32":
+        np.testing.assert_array_equal(hip.matvec_w4(held[:, :k], mat), got[:, :n])
+    mat.close()
+
+
+def test_matvec_w4_takes_any_fp32_value(hip):
+    """Rows of very large, very small and mixed values (nothing of x is rounded away), of one sign, of zeros, and rows
+    that are not numbers, which leave the rows beside them alone."""
+    say("w4 values")
+    rng = np.random.default_rng(8)
+    n, k, group = 50, 300, 64
+    codes, scales, zp, w = w4_inputs(rng, n, k, group, True)
+    x = rng.normal(0, 1, (8, k)).astype(np.float32)
+    x[0] *= np.float32(1e35)
+    x[1] *= np.float32(1e-30)
+    x[2] *= np.exp2(rng.integers(-30, 30, k)).astype(np.float32)
+    x[3] = np.abs(x[3])
+    x[4] = 0
+    x[5, 7] = np.inf
+    x[6, 8] = np.nan
+    x[7] = np.float32(1) + np.float32(2) ** -23
+    mat = hip.w4_matrix(codes, scales, group, zp)
+    got = hip.matvec_w4(x, mat)
+    good = [0, 1, 2, 3, 4, 7]
+    tol = w4_tolerance(x[good], codes, scales, zp, group)
+    assert np.all(np.abs(got[good] - x[good].astype(np.float64) @ w.T) <= tol)
+    assert not np.isfinite(got[[5, 6]]).any()
+    mat.close()
+
+
+def test_matvec_w4_refuses_on_a_handle(hip):
+    codes, scales, _, _ = w4_inputs(np.random.default_rng(0), 16, 64, 32, False)
+    with pytest.raises(HipError, match="codes must be"):
+        hip.w4_matrix(codes, scales[:, :1], 32)
+    mat = hip.w4_matrix(codes, scales, 32)
+    buf = hip.empty((4096,), np.float32)
+    for args, message in (((buf.ptr, "f32", 0, mat, buf.ptr + 8192), "positive"),
+                          ((buf.ptr, "f32", 1, mat, buf.ptr + 128), "overlaps"),
+                          ((buf.ptr, "f32", 70000, mat, buf.ptr + 8192), "65535"),
+                          ((buf.ptr, "f32", 1, mat, buf.ptr + 8192, 63), "row stride"),
+                          ((buf.ptr, "f32", 1, mat, buf.ptr + 8192, 64, 15), "row stride"),
+                          ((buf.ptr + 2, "f32", 1, mat, buf.ptr + 8192), "misaligned"),
+                          ((0, "f32", 1, mat, buf.ptr), "null")):
+        with pytest.raises(HipError, match=message):
+            hip.matvec_w4_resident(*args)
+    with pytest.raises(ValueError, match="m, 64"):
+        hip.matvec_w4(np.ones((2, 65), np.float32), mat)
+    mat.close()
+    with pytest.raises(HipError, match="null weights"):
+        hip.matvec_w4_resident(buf.ptr, "f32", 1, mat, buf.ptr + 8192)
+    buf.close()

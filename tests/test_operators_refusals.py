@@ -60,3 +60,56 @@ def test_batch_forms_refuse_null_lanes_and_python_forms_refuse_types():
     with pytest.raises(ValueError, match="f32"):
         _dtype("f64")
     assert np.uint32(_abi.NO_TOKEN) == 0xFFFFFFFF
+
+
+def codes_of(w, group, zeros):
+    from pssa_amd import quantize_w4
+
+    return quantize_w4(w, group, zeros)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 31, 32), (2, 64, 64), (5, 129, 128), (4, 200, 64)])
+def test_w4_quantize_rounds_to_the_nearest_code(n, k, group, zeros):
+    """Every weight is within half a step of the code it got (the zero point's rounding can push one end past the last
+    code: another half step there)."""
+    rng = np.random.default_rng(n * k)
+    w = rng.normal(0, 1, (n, k)).astype(np.float32)
+    w[0] = np.abs(w[0])  # a row on one side of zero
+    codes, scales, zp = codes_of(w, group, zeros)
+    assert codes.max() <= 15 and scales.shape == (n, -(-k // group))
+    at = np.arange(k) // group
+    z = zp[:, at].astype(np.float64) if zeros else 8.0
+    back = (codes - z) * scales[:, at].astype(np.float64)
+    assert np.all(np.abs(back - w) <= scales[:, at] * (1.0 if zeros else 0.5) * (1 + 1e-6))
+    if not zeros:
+        assert codes.min() >= 1  # symmetric: -7..7
+
+
+def test_w4_quantize_zero_rows_and_refusals():
+    codes, scales, _ = codes_of(np.zeros((2, 40), np.float32), 32, False)
+    assert not scales.any() and np.all(codes == 8)
+    codes, scales, zp = codes_of(np.zeros((2, 40), np.float32), 32, True)
+    assert not scales.any() and np.all(codes == zp[0, 0])
+    for bad, group in ((np.full((1, 4), np.nan, np.float32), 32), (np.ones((1, 4), np.float32), 48)):
+        with pytest.raises(_abi.HipError):
+            codes_of(bad, group, False)
+
+
+W4 = dict(ctx=None, codes=P, scales=P, zeros=None, n=16, k=64, group=32)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "null context"), ({"codes": None}, "null buffer"), ({"n": 0}, "positive"), ({"k": 0}, "positive"),
+    ({"group": 16}, "32, 64 or 128"), ({"group": 0}, "32, 64 or 128"), ({"scales": P + 2}, "misaligned"),
+    ({"n": 1 << 31}, "too large"), ({"k": 1 << 25}, "too large"), ({"n": 1 << 30, "k": 1 << 20}, "too large")])
+def test_w4_load_refuses(change, message):
+    out = C.c_void_p(1)
+    refused(_abi.lib().pssa_hip_w4_load_resident, changed(W4, **change) + [C.byref(out)], message)
+    assert not out.value
+
+
+def test_w4_products_refuse_null_weights():
+    refused(_abi.lib().pssa_hip_matvec_w4_resident, [None, P, 0, 1, 64, P, 16], "null weights")
+    refused(_abi.lib().pssa_hip_matvec_w4, [None, None, 0, 1, None, 0], "null weights")
+    refused(_abi.lib().pssa_hip_w4_load, [None, None, 0, None, 0, None, 1, 1, 32, C.byref(C.c_void_p())], "null buffer")
