@@ -677,6 +677,33 @@ int pssa_hip_matvec_w4_resident(pssa_hip_w4* w, const void* d_x, int x_dtype, si
 int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, float* y, size_t y_len, char* err,
                        size_t err_len);
 
+/* Linear attention with a decay for each head, the recurrence
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
+ * over n_seqs sequences packed one after another: lens [n_seqs] (a host array)
+ * holds their lengths, 0 allowed, or is NULL where every sequence has seq_len
+ * tokens.  q [tokens, heads, d_key], k [tokens, kv_heads, d_key], v [tokens,
+ * kv_heads, d_val], out [tokens, heads, d_val], all of `dtype`: token t of q
+ * starts at d_q + t*ld_q elements, its heads follow one another (likewise the
+ * others, so the columns of one projection's output can be passed).  Query
+ * head h reads key and value head h / (heads / kv_heads).  log_decay [heads]
+ * is <= 0 (0: no decay; -inf: only the token itself).  States are fp32
+ * [n_seqs, heads, d_key, d_val]: d_state_in NULL starts from zeros,
+ * d_state_out (NULL: not kept) receives the states behind the last tokens and
+ * may be d_state_in.  out may lie in the buffer of q, k and v in columns of its own (same row stride) and must
+ * not overlap them otherwise.  d_key <= 128, d_val <= 4096, n_seqs and heads
+ * <= 65535.  bf16 outputs round once; every sum and the states are fp32.  A
+ * value that is not finite reaches the outputs from its own token on and no
+ * earlier one. */
+int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
+                                       size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
+                                       const float* d_state_in, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                       size_t heads, size_t kv_heads, size_t d_key, size_t d_val, float scale,
+                                       void* d_out, size_t ld_out, float* d_state_out, char* err, size_t err_len);
+/* Grows the context's scratch (synchronously) to what such a call needs, so
+ * that it then allocates nothing and stays asynchronous. */
+int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                      size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

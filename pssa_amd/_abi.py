@@ -202,6 +202,9 @@ def lib() -> C.CDLL:
         "pssa_hip_w4_quantize": ([fp, sz, sz, sz, sz, u8p, fp, u8p, err_t, sz], C.c_int),
         "pssa_hip_matvec_w4_resident": ([vp, vp, C.c_int, sz, sz, vp, sz, err_t, sz], C.c_int),
         "pssa_hip_matvec_w4": ([vp, fp, sz, sz, fp, sz, err_t, sz], C.c_int),
+        "pssa_hip_linear_attention_resident": ([vp, C.c_int, vp, sz, vp, sz, vp, sz, vp, vp, u64p, sz, sz, sz, sz, sz, sz,
+                                                C.c_float, vp, sz, vp, err_t, sz], C.c_int),
+        "pssa_hip_linear_attention_reserve": ([vp, C.c_int, u64p, sz, sz, sz, sz, sz, err_t, sz], C.c_int),
         "pssa_hip_batch_distill": ([vp, u32p, fp, sz, sz, C.c_float, fp, fp, fp, err_t, sz], C.c_int),
     }
     for name, (args, res) in sig.items():

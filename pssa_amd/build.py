@@ -17,7 +17,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpssa_hip.so")
 
 HIP_SOURCES = ["api.hip", "gemm.hip", "ssm.hip", "memory.hip", "model.hip", "decode.hip", "dense_scan.hip",
-               "vocab_rows.hip", "matvec_w4.hip"]
+               "vocab_rows.hip", "matvec_w4.hip", "linear_attention.hip"]
 HOST_SOURCES = ["host_weights.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -206,6 +206,7 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_dense_scan_attributes());
     PSSA_RETURN_IF(pssa::init_operator_attributes());
     PSSA_RETURN_IF(pssa::init_w4_attributes());
+    PSSA_RETURN_IF(pssa::init_linear_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));
     *out = ctx.release();
     return Status::Ok();
@@ -2112,6 +2113,58 @@ Status load_w4(pssa_hip_ctx* ctx, const uint8_t* codes, const float* scales, con
   return Status::Ok();
 }
 
+bool disjoint(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x + na <= y || y + nb <= x;
+}
+
+// Token rows `w` wide at stride ld apart from rows `wo` wide at stride ldo:
+// in memory, or as other columns of the same rows.
+bool rows_disjoint(const void* p, size_t ld, size_t w, const void* o, size_t ldo, size_t wo, size_t rows, size_t size) {
+  if (!rows || disjoint(p, ((rows - 1) * ld + w) * size, o, ((rows - 1) * ldo + wo) * size)) return true;
+  const intptr_t d = (intptr_t)o - (intptr_t)p;
+  if (ld != ldo || d % (intptr_t)size) return false;
+  const intptr_t row = (intptr_t)ld;
+  const size_t at = (size_t)((d / (intptr_t)size % row + row) % row);
+  return at >= w && at + wo <= ld;
+}
+
+// The sequences of a linear attention call: offsets, or one length for all.
+Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, pssa::LinearArgs& a,
+                      std::vector<uint32_t>& table, size_t* tokens, size_t* longest) {
+  PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "linear attention: sequences must be in 1..=65535"));
+  a.n_seqs = (int)n_seqs;
+  const size_t most = INT32_MAX;
+  bool same = true;
+  *tokens = 0;
+  *longest = 0;
+  for (size_t i = 0; i < n_seqs; ++i) {
+    const size_t len = lens ? lens[i] : seq_len;
+    PSSA_RETURN_IF(need(len <= most && *tokens + len <= most, "linear attention: too many tokens"));
+    *tokens += len;
+    *longest = std::max(*longest, len);
+    same &= !lens || lens[i] == lens[0];
+  }
+  a.uniform_len = same ? (int)*longest : -1;
+  if (same) return Status::Ok();
+  uint32_t at = 0;
+  if (n_seqs > (size_t)pssa::kLinearInline) table.resize(n_seqs + 1);
+  uint32_t* out = table.empty() ? a.inline_table : table.data();
+  for (size_t i = 0; i < n_seqs; ++i) {
+    out[i] = at;
+    at += (uint32_t)lens[i];
+  }
+  out[n_seqs] = at;
+  return Status::Ok();
+}
+
+Status check_heads(size_t heads, size_t d_key, size_t d_val) {
+  PSSA_RETURN_IF(need(heads && d_key && d_val, "linear attention: dimensions must be positive"));
+  PSSA_RETURN_IF(need(heads <= 65535, "linear attention: at most 65535 heads"));
+  PSSA_RETURN_IF(need(d_key <= (size_t)pssa::kLinearMaxKey, "linear attention: d_key above 128 is not supported"));
+  return need(d_val <= 4096, "linear attention: d_val above 4096 is not supported");
+}
+
 }  // namespace
 
 extern "C" {
@@ -2381,6 +2434,84 @@ int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, f
     PSSA_RETURN_IF(pssa::launch_matvec_w4(ctx->stream, PSSA_HIP_F32, dx.p, k, (int)m, w->view, dy.as<float>(), n));
     PSSA_RETURN_IF(download(ctx, y, dy, y_len * 4));
     return sync(ctx);
+  }, err, err_len);
+}
+
+int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
+                                       size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
+                                       const float* d_state_in, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                       size_t heads, size_t kv_heads, size_t d_key, size_t d_val, float scale,
+                                       void* d_out, size_t ld_out, float* d_state_out, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_q && d_k && d_v && d_log_decay && d_out, "linear attention: null buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(check_heads(heads, d_key, d_val));
+    PSSA_RETURN_IF(need(kv_heads && heads % kv_heads == 0, "linear attention: kv_heads must divide heads"));
+    PSSA_RETURN_IF(need(std::isfinite(scale), "linear attention: scale must be finite"));
+    const size_t size = dtype_size(dtype), wq = heads * d_key, wk = kv_heads * d_key, wv = kv_heads * d_val,
+                 wo = heads * d_val;
+    PSSA_RETURN_IF(need(ld_q >= wq && ld_k >= wk && ld_v >= wv && ld_out >= wo,
+                        "linear attention: row stride below the heads' width"));
+    PSSA_RETURN_IF(need(aligned_to(d_q, size) && aligned_to(d_k, size) && aligned_to(d_v, size) &&
+                            aligned_to(d_out, size) && aligned_to(d_log_decay, 4) && aligned_to(d_state_in, 4) &&
+                            aligned_to(d_state_out, 4),
+                        "linear attention: misaligned buffer"));
+    pssa::LinearArgs a;
+    std::vector<uint32_t> table;
+    size_t tokens = 0, longest = 0, n = 0;
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, a, table, &tokens, &longest));
+    for (size_t ld : {ld_q, ld_k, ld_v, ld_out}) PSSA_RETURN_IF(pssa::checked_count({tokens, ld}, &n, "linear attention"));
+    PSSA_RETURN_IF(pssa::checked_count({n_seqs, heads, d_key, d_val}, &n, "linear attention states"));
+    PSSA_RETURN_IF(need(rows_disjoint(d_q, ld_q, wq, d_out, ld_out, wo, tokens, size) &&
+                            rows_disjoint(d_k, ld_k, wk, d_out, ld_out, wo, tokens, size) &&
+                            rows_disjoint(d_v, ld_v, wv, d_out, ld_out, wo, tokens, size),
+                        "linear attention: the output overlaps its inputs"));
+    if (d_state_out) {
+      PSSA_RETURN_IF(need(!d_state_in || d_state_in == d_state_out || disjoint(d_state_in, n * 4, d_state_out, n * 4),
+                          "linear attention: the states overlap"));
+      if (tokens)
+        for (auto [p, ld, w] : {std::tuple{d_q, ld_q, wq}, {d_k, ld_k, wk}, {d_v, ld_v, wv}, {(const void*)d_out, ld_out, wo}})
+          PSSA_RETURN_IF(need(disjoint(p, ((tokens - 1) * ld + w) * size, d_state_out, n * 4),
+                              "linear attention: the states overlap"));
+    }
+    PSSA_RETURN_IF(check_ctx(ctx));
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.ld_q = ld_q;
+    a.ld_k = ld_k;
+    a.ld_v = ld_v;
+    a.ld_out = ld_out;
+    a.log_decay = d_log_decay;
+    a.state_in = d_state_in;
+    a.state_out = d_state_out;
+    a.out = d_out;
+    a.scale = scale;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv_heads;
+    a.dk = (int)d_key;
+    a.dv = (int)d_val;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    DevBuf dt;
+    if (!table.empty()) {
+      PSSA_RETURN_IF(upload(ctx, dt, table.data(), table.size() * 4));
+      a.table = dt.as<uint32_t>();
+    }
+    return pssa::launch_linear_attention(ctx->stream, dtype, a, (int)longest);
+  }, err, err_len);
+}
+
+int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                      size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(check_heads(heads, d_key, d_val));
+    pssa::LinearArgs a;
+    std::vector<uint32_t> table;
+    size_t tokens = 0, longest = 0;
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, a, table, &tokens, &longest));
+    return check_ctx(ctx);
   }, err, err_len);
 }
 

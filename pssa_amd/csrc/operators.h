@@ -57,4 +57,25 @@ Status launch_w4_pack(hipStream_t stream, const uint8_t* codes, const float* sca
 Status launch_matvec_w4(hipStream_t stream, int x_dtype, const void* x, size_t ld_x, int m, const W4View& w, float* y,
                         size_t ld_y);
 
+// ------------------------------------------------------------ linear attention
+constexpr int kLinearMaxKey = 128;      // d_key held in a workgroup's tiles
+constexpr int kLinearSteps = 4;         // up to this length a sequence runs token by token
+constexpr int kLinearInline = 256;      // sequences whose offsets travel with the kernel's arguments
+
+struct LinearArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // token t, head h at t * ld + h * width
+  size_t ld_q = 0, ld_k = 0, ld_v = 0, ld_out = 0;
+  const float* log_decay = nullptr;  // [heads]
+  const float* state_in = nullptr;   // [n_seqs, heads, dk, dv] or null (zeros)
+  float* state_out = nullptr;        // likewise, or null
+  void* out = nullptr;
+  float scale = 1.0f;
+  int n_seqs = 0, heads = 0, kv_heads = 0, dk = 0, dv = 0;
+  int uniform_len = -1;             // every sequence's length, or -1: the table
+  const uint32_t* table = nullptr;  // [n_seqs + 1] first tokens on the device, or null: the next
+  uint32_t inline_table[kLinearInline + 1] = {};
+};
+Status init_linear_attributes();
+Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int max_len);
+
 }  // namespace pssa

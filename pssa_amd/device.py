@@ -32,6 +32,15 @@ def _dtype(name: str) -> int:
     return _abi.F32 if name == "f32" else _abi.BF16
 
 
+def _lens(lens):
+    """Sequence lengths as a u64 C array."""
+    if isinstance(lens, C.Array):
+        return lens
+    if min(lens, default=0) < 0:
+        raise ValueError("sequence lengths must not be negative")
+    return (C.c_uint64 * len(lens))(*lens)
+
+
 class HipDevice:
     """Device context (CudaContext peer, src/cuda.rs:158-192)."""
 
@@ -323,6 +332,32 @@ class HipDevice:
         _abi.call(self._lib.pssa_hip_distill_resident, self.handle, logits_ptr, _dtype(dtype), rows, vocab, ld,
                   teacher_ids_ptr, teacher_logits_ptr, teacher_k, temperature, row_weights_ptr, losses_ptr, grad_ptr,
                   ld_grad)
+
+    def linear_attention_resident(self, q_ptr: int, k_ptr: int, v_ptr: int, log_decay_ptr: int, dtype: str, heads: int,
+                                  d_key: int, d_val: int, out_ptr: int, lens=None, n_seqs: int = 1, seq_len: int = 1,
+                                  kv_heads: int | None = None, scale: float = 1.0, state_in_ptr: int | None = None,
+                                  state_out_ptr: int | None = None, ld_q: int | None = None, ld_k: int | None = None,
+                                  ld_v: int | None = None, ld_out: int | None = None) -> None:
+        """Linear attention S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, out_t = scale q_t S_t over packed sequences
+        of `lens` tokens (or n_seqs of seq_len), on device arrays: q [tokens, heads, d_key], k and v [tokens, kv_heads,
+        .], out [tokens, heads, d_val] with row strides ld_*, f32 states [n_seqs, heads, d_key, d_val]
+        (asynchronous on the context stream)."""
+        kv = heads if kv_heads is None else kv_heads
+        if lens is not None:
+            lens, n_seqs = _lens(lens), len(lens)
+        _abi.call(self._lib.pssa_hip_linear_attention_resident, self.handle, _dtype(dtype), q_ptr,
+                  heads * d_key if ld_q is None else ld_q, k_ptr, kv * d_key if ld_k is None else ld_k, v_ptr,
+                  kv * d_val if ld_v is None else ld_v, log_decay_ptr, state_in_ptr, lens, n_seqs, seq_len, heads, kv,
+                  d_key, d_val, scale, out_ptr, heads * d_val if ld_out is None else ld_out, state_out_ptr)
+
+    def linear_attention_reserve(self, dtype: str, heads: int, d_key: int, d_val: int, lens=None, n_seqs: int = 1,
+                                 seq_len: int = 1) -> None:
+        """Sizes the context's scratch for linear_attention_resident calls of this shape, so that they allocate
+        nothing."""
+        if lens is not None:
+            lens, n_seqs = _lens(lens), len(lens)
+        _abi.call(self._lib.pssa_hip_linear_attention_reserve, self.handle, _dtype(dtype), lens, n_seqs, seq_len, heads,
+                  d_key, d_val)
 
     def w4_matrix_resident(self, codes_ptr: int, scales_ptr: int, n: int, k: int, group: int,
                            zeros_ptr: int | None = None) -> "W4Matrix":

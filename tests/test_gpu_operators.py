@@ -541,3 +541,192 @@ def test_matvec_w4_refuses_on_a_handle(hip):
     with pytest.raises(HipError, match="null weights"):
         hip.matvec_w4_resident(buf.ptr, "f32", 1, mat, buf.ptr + 8192)
     buf.close()
+
+
+# ---------------------------------------------------------------------------
+# Linear attention
+
+
+def linear64(q, k, v, log_decay, lens, scale, state):
+    """The recurrence in 64 bits; q [tokens, h, dk], k and v [tokens, hk, .]."""
+    h, dk, dv, rep = q.shape[1], q.shape[2], v.shape[2], q.shape[1] // k.shape[1]
+    q, k, v = (a.astype(np.float64) for a in (q, np.repeat(k, rep, 1), np.repeat(v, rep, 1)))
+    lam = np.exp(log_decay.astype(np.float64))[:, None, None]
+    out, last, at = np.zeros((len(q), h, dv)), np.zeros((len(lens), h, dk, dv)), 0
+    size = np.zeros_like(out), np.zeros_like(last)  # the same sums of magnitudes: what roundings are relative to
+    for i, n in enumerate(lens):
+        s = np.zeros((h, dk, dv)) if state is None else state[i].astype(np.float64)
+        m = np.abs(s)
+        for t in range(at, at + n):
+            s = lam * s + k[t][:, :, None] * v[t][:, None, :]
+            m = lam * m + np.abs(k[t][:, :, None] * v[t][:, None, :])
+            out[t] = scale * np.einsum("hd,hdv->hv", q[t], s)
+            size[0][t] = abs(scale) * np.einsum("hd,hdv->hv", np.abs(q[t]), m)
+        last[i], size[1][i], at = s, m, at + n
+    return out, last, size
+
+
+def run_linear(hip, q, k, v, g, lens, scale, state, dtype, gap=0, out_gap=0, in_place=False, keep=True):
+    """Through one row buffer of q | k | v with `gap` elements behind each row."""
+    n, h, dk = q.shape
+    hk, dv = v.shape[1], v.shape[2]
+    row = np.concatenate([q.reshape(n, h * dk), k.reshape(n, hk * dk), v.reshape(n, hk * dv), np.full((n, gap), 1e30)], 1)
+    stored, held = typed(row.astype(np.float32), dtype)
+    wide = row.shape[1]
+    with Held(hip) as b:
+        x, d = b.up(stored if n else np.zeros(8, stored.dtype)), b.up(g)
+        o = b.new((n + 1, h * dv + out_gap), stored.dtype, 7)
+        s_in = None if state is None else b.up(state)
+        s_out = s_in if in_place else b.new((len(lens), h, dk, dv), np.float32, 7.0) if keep else None
+        size = stored.itemsize
+        hip.linear_attention_resident(x.ptr, x.ptr + h * dk * size, x.ptr + (h + hk) * dk * size, d.ptr, dtype, h, dk, dv,
+                                      o.ptr, lens, kv_heads=hk, scale=scale, state_in_ptr=s_in.ptr if s_in else None,
+                                      state_out_ptr=s_out.ptr if s_out else None, ld_q=wide, ld_k=wide, ld_v=wide,
+                                      ld_out=h * dv + out_gap)
+        hip.synchronize()
+        out = o.to_host()
+        assert np.all(out[n] == 7) and np.all(out[:, h * dv:] == 7)  # behind the last token and between the rows
+        out = out[:n, :h * dv].reshape(n, h, dv)
+        out = out if dtype == "f32" else from_bf16(out)
+        parts = np.split(held, [h * dk, (h + hk) * dk, (h + hk) * dk + hk * dv], 1)[:3]
+        return out, s_out.to_host() if s_out else None, [p.reshape(n, c, d) for p, c, d in zip(parts, (h, hk, hk), (dk, dk, dv))]
+
+
+def check_linear(hip, lens, h, hk, dk, dv, dtype, with_state, gap=0, out_gap=0, decays=None, in_place=False, seed=0):
+    rng = np.random.default_rng([seed, sum(lens), dk, dv])
+    n = sum(lens)
+    q, k, v = (rng.normal(0, 1, s) for s in ((n, h, dk), (n, hk, dk), (n, hk, dv)))
+    g = np.log(rng.uniform(0.5, 0.999, h)) if decays is None else np.asarray(decays)
+    g = g.astype(np.float32)
+    state = rng.normal(0, 1, (len(lens), h, dk, dv)).astype(np.float32) if with_state else None
+    out, last, held = run_linear(hip, q, k, v, g, lens, 0.37, state, dtype, gap, out_gap, in_place)
+    ref, rlast, (so, ss) = linear64(*held, g, lens, 0.37, state)
+    # Roundings of a path through the sums: d_key + 64 terms in a product, one for each chunk's state, six for a decay's
+    # power (its exponent's own, weighed by |x| e^-|x|) and the products; bf16 operands of two parts carry 2^-17 each.
+    chunks = max(lens, default=0) // 64 + 1
+    part = U32 * (dk + 64 + 2 * min(chunks, 40) + 12)
+    low = 3 * 2.0 ** -17 if dtype == "bf16" else 0.0
+    otol = (part + low) * so + (U16 * np.abs(ref) if dtype == "bf16" else 0)
+    assert np.all(np.abs(out - ref) <= otol + 1e-30), np.max(np.abs(out - ref) / (otol + 1e-30))
+    assert np.all(np.abs(last - rlast) <= part * ss + 1e-30), np.max(np.abs(last - rlast) / (part * ss + 1e-30))
+    return out, last
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,h,hk,dk,dv,with_state", [
+    ([1], 1, 1, 1, 1, False), ([1], 2, 1, 16, 32, True), ([1] * 9, 3, 3, 64, 64, True), ([1, 0, 1], 2, 2, 128, 72, True),
+    ([2, 4, 3], 2, 1, 100, 5, True), ([0], 1, 1, 8, 8, True), ([0, 0], 1, 1, 8, 8, False), ([5], 1, 1, 7, 9, False),
+    ([63], 1, 1, 32, 64, False), ([64], 2, 2, 64, 64, True), ([65], 1, 1, 128, 128, True), ([127, 1, 0, 129], 2, 1, 33, 70, True),
+    ([200], 3, 1, 100, 192, False), ([300, 17], 1, 1, 128, 64, True), ([7] * 300, 1, 1, 16, 16, True),
+    (list(range(300)), 1, 1, 16, 24, False), ([1500], 2, 2, 64, 32, True)])
+def test_linear_attention_matches_the_recurrence(hip, dtype, lens, h, hk, dk, dv, with_state):
+    say(f"linear {len(lens)} sequences, {sum(lens)} tokens, {h}/{hk} heads {dk} x {dv} {dtype}")
+    check_linear(hip, lens, h, hk, dk, dv, dtype, with_state)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gap,out_gap", [(1, 3), (2, 0), (3, 1), (8, 8)])
+def test_linear_attention_strides_and_states_in_place(hip, dtype, gap, out_gap):
+    say("linear strides", gap, out_gap, dtype)
+    check_linear(hip, [70, 1, 130], 2, 1, 36, 40, dtype, True, gap, out_gap, in_place=True)
+    check_linear(hip, [1] * 5, 2, 1, 36, 40, dtype, True, gap, out_gap, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[1, 1], [3, 2], [64], [131, 70]])
+def test_linear_attention_decays(hip, dtype, lens):
+    """No decay, hardly any, one that leaves nothing within a chunk, and none of the past at all (-inf)."""
+    say("linear decays", lens, dtype)
+    check_linear(hip, lens, 5, 1, 32, 48, dtype, True, decays=[0.0, -1e-6, -3.0, -200.0, -np.inf])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_attention_long_sums(hip, dtype):
+    """Thousands of tokens without decay: the state only grows."""
+    say("linear long", dtype)
+    check_linear(hip, [4100], 1, 1, 16, 16, dtype, False, decays=[0.0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("length,at", [(150, 100), (150, 64), (4, 2), (70, 69)])
+def test_linear_attention_keeps_what_is_not_finite_to_later_tokens(hip, dtype, length, at):
+    """A NaN, an infinity in v, k or q: earlier tokens and other sequences are as without it."""
+    say("linear not finite", length, at, dtype)
+    rng = np.random.default_rng(at)
+    lens, h, dk, dv = [length, 20], 2, 32, 40
+    n = sum(lens)
+    q, k, v = (rng.normal(0, 1, s) for s in ((n, h, dk), (n, h, dk), (n, h, dv)))
+    g = np.log(np.array([0.9, 0.99])).astype(np.float32)
+    clean, _, _ = run_linear(hip, q, k, v, g, lens, 1.0, None, dtype)
+    for which, value in (("v", np.nan), ("v", np.inf), ("k", np.inf), ("k", np.nan), ("q", np.nan)):
+        x = {"q": q.copy(), "k": k.copy(), "v": v.copy()}
+        x[which][at, 1, 3] = value
+        out, _, held = run_linear(hip, x["q"], x["k"], x["v"], g, lens, 1.0, None, dtype)
+        with np.errstate(invalid="ignore"):
+            ref, _, (size, _) = linear64(*held, g, lens, 1.0, None)
+        fine = np.isfinite(ref)
+        assert fine[:at].all() and fine[length:].all() and not fine.all()
+        assert np.isfinite(out[fine]).all() and not np.isfinite(out[~fine]).any(), which
+        tol = (U32 * 200 + 3 * 2.0 ** -17) * size[fine] + U16 * np.abs(ref[fine])
+        assert np.all(np.abs(out[fine] - ref[fine]) <= tol)
+    assert np.isfinite(clean).all()
+
+
+def test_linear_attention_prompt_then_tokens_equals_the_whole(hip):
+    """A prompt's state carried on by single tokens gives the outputs of the longer prompt."""
+    say("linear prompt then tokens")
+    rng = np.random.default_rng(6)
+    lens, h, dk, dv, more = [90, 33], 2, 64, 64, 6
+    g = np.log(np.array([0.95, 0.999])).astype(np.float32)
+    whole = [rng.normal(0, 1, (n + more, 3, h, 64)) for n in lens]
+    cut = lambda f: [np.concatenate([f(w, n) for w, n in zip(whole, lens)])[:, i] for i in range(3)]
+    full, fstate, _ = run_linear(hip, *cut(lambda w, n: w), g, [n + more for n in lens], 0.5, None, "f32")
+    part, state, _ = run_linear(hip, *cut(lambda w, n: w[:n]), g, lens, 0.5, None, "f32")
+    outs = [part]
+    for t in range(more):
+        out, state, _ = run_linear(hip, *cut(lambda w, n: w[n + t:n + t + 1]), g, [1, 1], 0.5, state, "f32")
+        outs.append(out)
+    ends = np.cumsum([n + more for n in lens])
+    for i, n in enumerate(lens):
+        start, first = ends[i] - n - more, sum(lens[:i])
+        got = np.concatenate([part[first:first + n]] + [o[i:i + 1] for o in outs[1:]])
+        scale = np.abs(full).max()
+        assert np.max(np.abs(got - full[start:ends[i]])) <= U32 * 400 * scale * 8
+    assert np.max(np.abs(state - fstate)) <= U32 * 400 * np.abs(fstate).max() * 8
+
+
+def test_a_step_of_a_served_model_runs_through_the_operators(hip):
+    """As they are used together: a token of each stream through linear attention, a 4-bit head, and the next token's
+    log probabilities and alternatives, on the context's stream without a wait between."""
+    say("served step")
+    rng = np.random.default_rng(12)
+    streams, h, d, V, K = 3, 2, 64, 997, 6
+    codes, scales, zp, w = w4_inputs(rng, V, h * d, 64, True)
+    mat = hip.w4_matrix(codes, scales, 64, zp)
+    row = rng.normal(0, 1, (streams, 3 * h * d)).astype(np.float32)
+    state = rng.normal(0, 1, (streams, h, d, d)).astype(np.float32)
+    g = np.log(np.array([0.9, 0.99])).astype(np.float32)
+    targets = rng.integers(0, V, streams).astype(np.uint32)
+    with Held(hip) as b:
+        x, s, dg, t = b.up(row), b.up(state), b.up(g), b.up(targets)
+        o, logits = b.new((streams, h * d), np.float32, 0), b.new((streams, V), np.float32, 0)
+        lp, en = b.new(streams, np.float32, 0), b.new(streams, np.float32, 0)
+        ids, tl = b.new((streams, K), np.uint32, 0), b.new((streams, K), np.float32, 0)
+        ld = 3 * h * d
+        hip.linear_attention_resident(x.ptr, x.ptr + 4 * h * d, x.ptr + 8 * h * d, dg.ptr, "f32", h, d, d, o.ptr,
+                                      n_seqs=streams, scale=0.125, state_in_ptr=s.ptr, state_out_ptr=s.ptr, ld_q=ld,
+                                      ld_k=ld, ld_v=ld)
+        hip.matvec_w4_resident(o.ptr, "f32", streams, mat, logits.ptr)
+        hip.token_logprobs_resident(logits.ptr, "f32", streams, V, t.ptr, lp.ptr, en.ptr, K, ids.ptr, tl.ptr)
+        hip.synchronize()
+        got = [a.to_host() for a in (o, s, logits, lp, ids)]
+    q, k, v = (row.reshape(streams, 3, h, d)[:, i] for i in range(3))
+    ref, rs, (so, ss) = linear64(q, k, v, g, [1] * streams, 0.125, state)
+    assert np.all(np.abs(got[0].reshape(ref.shape) - ref) <= U32 * 200 * so)
+    assert np.all(np.abs(got[1] - rs) <= U32 * 20 * ss)
+    # The later stages against 64 bits from what the stage before handed on.
+    assert np.all(np.abs(got[2] - got[0].astype(np.float64) @ w.T) <= w4_tolerance(got[0], codes, scales, zp, 64))
+    lref, _, _ = log_softmax64(got[2], 1.0)
+    assert np.max(np.abs(got[3] - lref[np.arange(streams), targets])) <= U32 * (4 * np.abs(lref).max() + 100)
+    np.testing.assert_array_equal(got[4], top64(got[2], K))
+    mat.close()

@@ -113,3 +113,37 @@ def test_w4_products_refuse_null_weights():
     refused(_abi.lib().pssa_hip_matvec_w4_resident, [None, P, 0, 1, 64, P, 16], "null weights")
     refused(_abi.lib().pssa_hip_matvec_w4, [None, None, 0, 1, None, 0], "null weights")
     refused(_abi.lib().pssa_hip_w4_load, [None, None, 0, None, 0, None, 1, 1, 32, C.byref(C.c_void_p())], "null buffer")
+
+
+LINEAR = dict(ctx=None, dtype=_abi.F32, q=P, ld_q=64, k=P + 0x10000, ld_k=32, v=P + 0x20000, ld_v=48, decay=P,
+              state_in=None, lens=None, n_seqs=2, seq_len=8, heads=4, kv_heads=2, d_key=16, d_val=24, scale=1.0,
+              out=P + 0x30000, ld_out=96, state_out=P + 0x40000)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({}, "null context"), ({"v": None}, "null buffer"), ({"decay": None}, "null buffer"), ({"dtype": 3}, "unknown dtype"),
+    ({"heads": 0}, "positive"), ({"d_val": 0}, "positive"), ({"kv_heads": 0}, "divide"), ({"kv_heads": 3}, "divide"),
+    ({"d_key": 129}, "128"), ({"d_val": 4097}, "4096"), ({"heads": 65536, "kv_heads": 65536}, "65535"),
+    ({"n_seqs": 0}, "sequences"), ({"n_seqs": 65536}, "sequences"), ({"seq_len": 1 << 31}, "too many tokens"),
+    ({"n_seqs": 60000, "seq_len": 1 << 20}, "too many tokens"), ({"ld_q": 63}, "row stride"), ({"ld_out": 95}, "row stride"),
+    ({"scale": float("inf")}, "scale"), ({"q": P + 2}, "misaligned"), ({"state_out": P + 0x40002}, "misaligned"),
+    ({"out": P}, "overlaps"), ({"out": P + 0x10000 + 4, "ld_out": 96}, "overlaps"), ({"state_out": P + 0x30000}, "states"),
+    ({"state_in": P + 0x40004}, "states"), ({"state_in": P + 0x40000}, "null context"), ({"seq_len": 0}, "null context"),
+    # One row buffer of q | k | v | out: the columns are apart; one element less and they are not.
+    ({"ld_q": 240, "k": P + 256, "ld_k": 240, "v": P + 384, "ld_v": 240, "out": P + 576, "ld_out": 240}, "null context"),
+    ({"ld_q": 240, "k": P + 256, "ld_k": 240, "v": P + 384, "ld_v": 240, "out": P + 572, "ld_out": 240}, "overlaps"),
+    ({"ld_q": 239, "k": P + 256, "ld_k": 239, "v": P + 384, "ld_v": 239, "out": P + 576, "ld_out": 239}, "overlaps")])
+def test_linear_attention_refuses(change, message):
+    refused(_abi.lib().pssa_hip_linear_attention_resident, changed(LINEAR, **change), message)
+
+
+def test_linear_attention_reserve_and_lens_refuse():
+    fn = _abi.lib().pssa_hip_linear_attention_reserve
+    refused(fn, [None, 0, None, 2, 8, 4, 16, 24], "null context")
+    refused(fn, [None, 5, None, 2, 8, 4, 16, 24], "unknown dtype")
+    refused(fn, [None, 0, None, 2, 8, 4, 130, 24], "128")
+    from pssa_amd.device import _lens
+
+    assert list(_lens([3, 0, 5])) == [3, 0, 5]
+    with pytest.raises(ValueError, match="negative"):
+        _lens([3, -1])
