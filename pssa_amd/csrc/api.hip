@@ -2129,33 +2129,51 @@ bool rows_disjoint(const void* p, size_t ld, size_t w, const void* o, size_t ldo
   return at >= w && at + wo <= ld;
 }
 
-// The sequences of a linear attention call: offsets, or one length for all.
-Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, pssa::LinearArgs& a,
-                      std::vector<uint32_t>& table, size_t* tokens, size_t* longest) {
+// The sequences of a linear attention call and their split into work items.
+struct LinearPlan {
+  std::vector<uint32_t> table;  // first tokens and items, where the arguments do not hold them
+  size_t tokens = 0, longest = 0;
+};
+Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_val,
+                      pssa::LinearArgs& a, LinearPlan& p) {
   PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "linear attention: sequences must be in 1..=65535"));
   a.n_seqs = (int)n_seqs;
   const size_t most = INT32_MAX;
   bool same = true;
-  *tokens = 0;
-  *longest = 0;
   for (size_t i = 0; i < n_seqs; ++i) {
     const size_t len = lens ? lens[i] : seq_len;
-    PSSA_RETURN_IF(need(len <= most && *tokens + len <= most, "linear attention: too many tokens"));
-    *tokens += len;
-    *longest = std::max(*longest, len);
+    PSSA_RETURN_IF(need(len <= most && p.tokens + len <= most, "linear attention: too many tokens"));
+    p.tokens += len;
+    p.longest = std::max(p.longest, len);
     same &= !lens || lens[i] == lens[0];
   }
-  a.uniform_len = same ? (int)*longest : -1;
-  if (same) return Status::Ok();
-  uint32_t at = 0;
-  if (n_seqs > (size_t)pssa::kLinearInline) table.resize(n_seqs + 1);
-  uint32_t* out = table.empty() ? a.inline_table : table.data();
-  for (size_t i = 0; i < n_seqs; ++i) {
-    out[i] = at;
-    at += (uint32_t)lens[i];
+  const size_t seg = (size_t)pssa::linear_segment(n_seqs, p.longest, p.tokens, heads, d_val);
+  a.seg_len = (int)(seg ? seg : std::max<size_t>(p.longest, 1));
+  a.uniform_len = same ? (int)p.longest : -1;
+  a.uniform_segs = (int)std::max<size_t>(1, (p.longest + a.seg_len - 1) / a.seg_len);
+  if (same) {
+    a.items = (int)n_seqs * a.uniform_segs;
+  } else {
+    const bool inside = n_seqs <= (size_t)pssa::kLinearInline;
+    if (!inside) p.table.resize(2 * (n_seqs + 1));
+    uint32_t* tok = inside ? a.inline_tokens : p.table.data();
+    uint32_t* item = inside ? a.inline_items : p.table.data() + n_seqs + 1;
+    uint32_t t = 0, w = 0;
+    for (size_t i = 0; i < n_seqs; ++i) {
+      tok[i] = t;
+      item[i] = w;
+      t += (uint32_t)lens[i];
+      w += (uint32_t)std::max<size_t>(1, (lens[i] + a.seg_len - 1) / a.seg_len);
+    }
+    tok[n_seqs] = t;
+    item[n_seqs] = w;
+    a.items = (int)w;
   }
-  out[n_seqs] = at;
   return Status::Ok();
+}
+// Scratch of a split call: a state for each item.
+size_t linear_scratch_bytes(const pssa::LinearArgs& a, size_t heads, size_t d_key, size_t d_val) {
+  return a.items > a.n_seqs ? (size_t)a.items * heads * d_key * d_val * 4 : 0;
 }
 
 Status check_heads(size_t heads, size_t d_key, size_t d_val) {
@@ -2457,9 +2475,10 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
                             aligned_to(d_state_out, 4),
                         "linear attention: misaligned buffer"));
     pssa::LinearArgs a;
-    std::vector<uint32_t> table;
-    size_t tokens = 0, longest = 0, n = 0;
-    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, a, table, &tokens, &longest));
+    LinearPlan plan;
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_val, a, plan));
+    const size_t tokens = plan.tokens;
+    size_t n = 0;
     for (size_t ld : {ld_q, ld_k, ld_v, ld_out}) PSSA_RETURN_IF(pssa::checked_count({tokens, ld}, &n, "linear attention"));
     PSSA_RETURN_IF(pssa::checked_count({n_seqs, heads, d_key, d_val}, &n, "linear attention states"));
     PSSA_RETURN_IF(need(rows_disjoint(d_q, ld_q, wq, d_out, ld_out, wo, tokens, size) &&
@@ -2494,11 +2513,15 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     DevBuf dt;
-    if (!table.empty()) {
-      PSSA_RETURN_IF(upload(ctx, dt, table.data(), table.size() * 4));
+    if (!plan.table.empty()) {
+      PSSA_RETURN_IF(upload(ctx, dt, plan.table.data(), plan.table.size() * 4));
       a.table = dt.as<uint32_t>();
     }
-    return pssa::launch_linear_attention(ctx->stream, dtype, a, (int)longest);
+    if (const size_t bytes = linear_scratch_bytes(a, heads, d_key, d_val)) {
+      PSSA_RETURN_IF(grow_scratch(ctx, bytes, false));
+      a.seg_state = static_cast<float*>(ctx->scratch);
+    }
+    return pssa::launch_linear_attention(ctx->stream, dtype, a, (int)plan.longest);
   }, err, err_len);
 }
 
@@ -2508,10 +2531,12 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
     PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
     PSSA_RETURN_IF(check_heads(heads, d_key, d_val));
     pssa::LinearArgs a;
-    std::vector<uint32_t> table;
-    size_t tokens = 0, longest = 0;
-    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, a, table, &tokens, &longest));
-    return check_ctx(ctx);
+    LinearPlan plan;
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_val, a, plan));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return grow_scratch(ctx, linear_scratch_bytes(a, heads, d_key, d_val), false);
   }, err, err_len);
 }
 

@@ -71,11 +71,19 @@ struct LinearArgs {
   void* out = nullptr;
   float scale = 1.0f;
   int n_seqs = 0, heads = 0, kv_heads = 0, dk = 0, dv = 0;
-  int uniform_len = -1;             // every sequence's length, or -1: the table
-  const uint32_t* table = nullptr;  // [n_seqs + 1] first tokens on the device, or null: the next
-  uint32_t inline_table[kLinearInline + 1] = {};
+  // The work items: whole sequences, or (split) their segments of seg_len tokens.
+  int items = 0, seg_len = 0;
+  float* seg_state = nullptr;       // [items, heads, dk, dv] of a split call
+  int uniform_len = -1;             // every sequence's length, or -1: the tables
+  int uniform_segs = 1;             // its segments
+  // [n_seqs + 1] first tokens, then as many first items: on the device, or null and here.
+  const uint32_t* table = nullptr;
+  uint32_t inline_tokens[kLinearInline + 1] = {};
+  uint32_t inline_items[kLinearInline + 1] = {};
 };
 Status init_linear_attributes();
-Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int max_len);
+// Tokens of a segment where a call of these sizes is split, else 0.
+int linear_segment(size_t n_seqs, size_t longest, size_t tokens, size_t heads, size_t d_val);
+Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int longest);
 
 }  // namespace pssa

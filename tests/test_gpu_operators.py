@@ -618,7 +618,9 @@ def check_linear(hip, lens, h, hk, dk, dv, dtype, with_state, gap=0, out_gap=0, 
     ([2, 4, 3], 2, 1, 100, 5, True), ([0], 1, 1, 8, 8, True), ([0, 0], 1, 1, 8, 8, False), ([5], 1, 1, 7, 9, False),
     ([63], 1, 1, 32, 64, False), ([64], 2, 2, 64, 64, True), ([65], 1, 1, 128, 128, True), ([127, 1, 0, 129], 2, 1, 33, 70, True),
     ([200], 3, 1, 100, 192, False), ([300, 17], 1, 1, 128, 64, True), ([7] * 300, 1, 1, 16, 16, True),
-    (list(range(300)), 1, 1, 16, 24, False), ([1500], 2, 2, 64, 32, True)])
+    (list(range(300)), 1, 1, 16, 24, False), ([1500], 2, 2, 64, 32, True),
+    # Split into segments: ragged ends, sequences of one segment and of none, one end on a segment's border.
+    ([900, 0, 3, 513, 256, 512], 2, 1, 24, 72, True), ([1029], 1, 1, 128, 130, True), ([640, 640], 3, 3, 40, 8, False)])
 def test_linear_attention_matches_the_recurrence(hip, dtype, lens, h, hk, dk, dv, with_state):
     say(f"linear {len(lens)} sequences, {sum(lens)} tokens, {h}/{hk} heads {dk} x {dv} {dtype}")
     check_linear(hip, lens, h, hk, dk, dv, dtype, with_state)
@@ -648,7 +650,7 @@ def test_linear_attention_long_sums(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("length,at", [(150, 100), (150, 64), (4, 2), (70, 69)])
+@pytest.mark.parametrize("length,at", [(150, 100), (150, 64), (4, 2), (70, 69), (700, 300)])
 def test_linear_attention_keeps_what_is_not_finite_to_later_tokens(hip, dtype, length, at):
     """A NaN, an infinity in v, k or q: earlier tokens and other sequences are as without it."""
     say("linear not finite", length, at, dtype)
