@@ -204,7 +204,6 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_retrieve_attributes());
     PSSA_RETURN_IF(pssa::init_decode_attributes());
     PSSA_RETURN_IF(pssa::init_dense_scan_attributes());
-    PSSA_RETURN_IF(pssa::init_operator_attributes());
     PSSA_RETURN_IF(pssa::init_w4_attributes());
     PSSA_RETURN_IF(pssa::init_linear_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));

@@ -7,7 +7,6 @@
 namespace pssa {
 
 // Dynamic LDS above the default limit, once for each device.
-Status init_operator_attributes();
 Status init_w4_attributes();
 
 // ---------------------------------------------------------------- logit rows

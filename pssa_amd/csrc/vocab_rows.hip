@@ -102,19 +102,51 @@ __device__ __forceinline__ void vec_mask(u32x4_t& u, int V, int i) {
   }
 }
 // The tile's vectors of one thread (vector tile0 + k * 64W + tid); a k past
-// the row is skipped by the whole workgroup.
+// the row is skipped, and one that lies inside it loaded plainly, by the
+// whole workgroup.
 template <class T, int W, int NV>
 __device__ __forceinline__ void tile_load(u32x4_t (&u)[NV], const T* row, int V, int tile0) {
   constexpr int N = vec_n<T>();
   const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+  const T* mine = row + (size_t)(tile0 + (int)threadIdx.x) * N;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     u[k] = u32x4_t{none, none, none, none};
-    if ((tile0 + k * 64 * W) * N < V) u[k] = vec_load<T>(row, V, tile0 + k * 64 * W + (int)threadIdx.x);
+    if ((tile0 + (k + 1) * 64 * W) * N <= V)
+      u[k] = *reinterpret_cast<const u32x4_any_t*>(mine + k * 64 * W * N);
+    else if ((tile0 + k * 64 * W) * N < V)
+      u[k] = vec_load<T>(row, V, tile0 + k * 64 * W + (int)threadIdx.x);
   }
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if ((tile0 + k * 64 * W) * N < V) vec_mask<T>(u[k], V, tile0 + k * 64 * W + (int)threadIdx.x);
+    if ((tile0 + (k + 1) * 64 * W) * N > V && (tile0 + k * 64 * W) * N < V)
+      vec_mask<T>(u[k], V, tile0 + k * 64 * W + (int)threadIdx.x);
+}
+// Between two uses of a tile: what one computed of it (bf16 values widened,
+// twice the registers) is not kept for the next.
+template <int NV>
+__device__ __forceinline__ void tile_again(u32x4_t (&u)[NV]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) asm volatile("" : "+v"(u[k]));
+}
+// The largest of three; a NaN is passed over.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <class T, int NV>
+__device__ __forceinline__ float tile_max(const u32x4_t (&u)[NV]) {
+  constexpr int N = vec_n<T>();
+  float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      m0 = max3(m0, elem<T>(u[k], j), elem<T>(u[k], j + 1));
+      m1 = max3(m1, elem<T>(u[k], j + 2), elem<T>(u[k], j + 3));
+    }
+  return fmaxf(m0, m1);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -145,8 +177,14 @@ __device__ __forceinline__ uint64_t key_step(uint64_t a, int off, bool keep_max)
   const uint64_t o = __shfl_xor((unsigned long long)a, off, 64);
   return (o > a) == keep_max ? o : a;
 }
+__device__ __forceinline__ uint32_t value_key(float v) { return (uint32_t)(token_key(v, 0) >> 32); }
+__device__ __forceinline__ uint32_t key_step(uint32_t a, int off, bool keep_max) {
+  const uint32_t o = __shfl_xor(a, off, 64);
+  return keep_max ? max(o, a) : min(o, a);
+}
 // The wave's 64 keys, largest in lane 0 (bitonic, 21 exchanges).
-__device__ __forceinline__ uint64_t wave_sort(uint64_t a, int lane) {
+template <class Key>
+__device__ __forceinline__ Key wave_sort(Key a, int lane) {
 #pragma unroll
   for (int size = 2; size <= 64; size <<= 1)
 #pragma unroll
@@ -154,7 +192,8 @@ __device__ __forceinline__ uint64_t wave_sort(uint64_t a, int lane) {
   return a;
 }
 // The largest 64 of two descending lists, descending; `b` is given reversed.
-__device__ __forceinline__ uint64_t wave_merge(uint64_t a, uint64_t b_reversed, int lane) {
+template <class Key>
+__device__ __forceinline__ Key wave_merge(Key a, Key b_reversed, int lane) {
   a = a > b_reversed ? a : b_reversed;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) a = key_step(a, off, (lane & off) == 0);
@@ -168,17 +207,22 @@ __device__ __forceinline__ uint64_t wave_merge(uint64_t a, uint64_t b_reversed, 
 // apart from its 1, S carries the small probabilities that a nearly certain
 // row's values consist of.
 //
-// Alternatives: the k-th largest of the threads' maxima bounds the row's k-th
-// largest token from below, and only the k threads whose maximum reaches it
-// can hold tokens above it, so at most k * (tokens of a thread) candidates
-// pass through LDS, whatever the row holds; one wave sorts them.
+// Alternatives: the k-th largest of the maxima of some groups of threads (64
+// groups, or every thread for itself where k is large) bounds the row's k-th
+// largest token from below.  The tokens that reach the bound, hardly more
+// than k of them, pass through LDS to one wave that sorts them by value and
+// id.  A row where they are too many (all logits equal, say) takes its
+// tokens one by one, each round the largest behind the one before.
+constexpr int kCandidates = 1024;
+
 template <class T, int W, int NV>
 __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int N = vec_n<T>(), TILE = 64 * W * NV;
-  __shared__ uint64_t s_keys[W * 64];
+  __shared__ uint32_t s_keys[W * 64];
+  __shared__ uint64_t s_round[W];
   __shared__ float s_sum[2 * W];
-  __shared__ uint64_t s_first, s_bound;
-  __shared__ int s_count;
+  __shared__ uint32_t s_bound, s_kth;
+  __shared__ int s_count, s_owner;
   extern __shared__ uint64_t s_cand[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab, top = a.top_k;
   const T* row = static_cast<const T*>(a.logits) + (size_t)blockIdx.x * a.ld;
@@ -192,84 +236,106 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
   for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
     u32x4_t u[NV];
     tile_load<T, W, NV>(u, row, V, tile0);
-    float bv = -INFINITY;
-    int bi = 0;
+    const float bv = tile_max<T, NV>(u);
+    tile_again(u);
+    // The groups' maxima, the tile's, and the bound.
+    float mt;
+    {
+      const bool fine = top > 24;  // every thread a group
+      float gm = bv;
+      if (!fine) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float v = elem<T>(u[k], j);
-        if (v > bv) {
-          bv = v;
-          bi = s + j;
+        for (int off = 1; off < W; off <<= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
+      }
+      uint32_t key = value_key(gm);
+      if constexpr (W > 1) {
+        if (fine) {
+          key = wave_sort(key, lane);
+          s_keys[tid] = key;
+        } else if (lane % W == 0) {
+          s_keys[tid / W] = key;
         }
       }
-    }
-    const uint64_t mine = bv > -INFINITY ? token_key(bv, bi) : 0;
-    uint64_t first = mine;
-    if (top) {
-      uint64_t key = wave_sort(mine, lane);
+      if (tid == 0) {
+        s_count = 0;
+        s_owner = 64 * W;
+      }
+      __syncthreads();
       if constexpr (W > 1) {
-        s_keys[wave * 64 + lane] = key;
-        __syncthreads();
+        if (fine) {
 #pragma unroll
-        for (int half = W / 2; half >= 1; half >>= 1) {
-          if (wave < half) {
-            key = wave_merge(key, s_keys[(wave + half) * 64 + 63 - lane], lane);
-            s_keys[wave * 64 + lane] = key;
+          for (int half = W / 2; half >= 1; half >>= 1) {
+            if (wave < half) {
+              key = wave_merge(key, s_keys[(wave + half) * 64 + 63 - lane], lane);
+              s_keys[tid] = key;
+            }
+            __syncthreads();
           }
-          __syncthreads();
         }
       }
       if (wave == 0) {
-        if (lane == 0) {
-          s_first = key;
-          s_count = 0;
-        }
-        if (lane == top - 1) s_bound = key > best ? key : best;
+        if (W == 1 || !fine) key = wave_sort(W == 1 ? key : s_keys[lane], lane);
+        if (lane == 0) s_bound = key;
+        if (top && lane == top - 1) s_kth = max(key, (uint32_t)(best >> 32));
       }
       __syncthreads();
-      first = s_first;
-      const uint64_t bound = s_bound;
-      // bound 0: fewer than k threads have a token; each takes part with all of its own.
-      if (mine && mine >= bound) {
+      mt = key_value((uint64_t)s_bound << 32);
+    }
+    const bool some = mt > -INFINITY;
+    if (bv == mt && some) atomicMin(&s_owner, tid);  // this thread's first maximum is left out of the sums
+    if (top) {
+      const float bound = key_value((uint64_t)s_kth << 32);
+      if (bv >= bound) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             const float v = elem<T>(u[k], j);
-            if (v > -INFINITY) {
-              const uint64_t key2 = token_key(v, s + j);
-              if (key2 >= bound) s_cand[atomicAdd(&s_count, 1)] = key2;
+            if (v >= bound && v > -INFINITY) {
+              const int at = atomicAdd(&s_count, 1);
+              if (at < kCandidates) s_cand[at] = token_key(v, vec_start<T>(V, tile0 + k * 64 * W + tid) + j);
             }
           }
-        }
       }
-      __syncthreads();
-      if (wave == 0) {
-        const int n = s_count;
-        for (int c = 0; c < n; c += 64) {
-          const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : 0, lane);
-          best = wave_merge(best, __shfl((unsigned long long)got, 63 - lane, 64), lane);
+      tile_again(u);
+    }
+    __syncthreads();
+    if (top) {
+      const int n = s_count;
+      if (n <= kCandidates) {
+        if (wave == 0) {
+          for (int c = 0; c < n; c += 64) {
+            const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : (uint64_t)0, lane);
+            best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
+          }
         }
-      }
-    } else {
+      } else {
+        uint64_t last = ~(uint64_t)0, list = 0;
+        for (int i = 0; i < top; ++i) {
+          uint64_t mine = 0;
+          for (int e = tile0 * N + tid; e < min(V, (tile0 + TILE) * N); e += 64 * W) {  // from the cache: rare
+            const float v = load1<T>(row + e);
+            const uint64_t key = v > -INFINITY ? token_key(v, e) : 0;
+            if (key < last && key > mine) mine = key;
+          }
 #pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) first = key_step(first, off, true);
-      if constexpr (W > 1) {
-        if (lane == 0) s_keys[wave] = first;
-        __syncthreads();
+          for (int off = 32; off >= 1; off >>= 1) mine = key_step(mine, off, true);
+          if (lane == 0) s_round[wave] = mine;
+          __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) first = s_keys[w] > first ? s_keys[w] : first;
+          for (int w = 0; w < W; ++w) mine = s_round[w] > mine ? s_round[w] : mine;
+          __syncthreads();
+          last = mine;
+          if (lane == i) list = mine;
+          if (!mine) break;  // uniform
+        }
+        if (wave == 0) best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
       }
     }
 
     // The tile's sums without its first maximum.
-    const bool some = first != 0;
-    const float mt = some ? key_value(first) : 0.0f;
-    const bool own = some && mine == first;
+    bool left_out = s_owner != tid;
+    if (!some) mt = 0.0f;
     float st = 0.0f, tt = 0.0f;
     auto add = [&](float v) {
       const float d = v - mt;
@@ -277,13 +343,16 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
       st += e;
       tt = fmaf(e, fmaxf(d, kLowest), tt);
     };
-    if (__any(own)) {  // one wave
+    if (__any(!left_out)) {  // one wave
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int s = vec_start<T>(V, tile0 + k * 64 * W + tid);
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int j = 0; j < N; ++j) add(own && s + j == bi ? -INFINITY : elem<T>(u[k], j));
-      }
+        for (int j = 0; j < N; ++j) {
+          const float v = elem<T>(u[k], j);
+          const bool now = !left_out && v == mt;
+          left_out |= now;
+          add(now ? -INFINITY : v);
+        }
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -305,8 +374,8 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
         st += s_sum[w];
         tt += s_sum[W + w];
       }
-      __syncthreads();  // the next tile writes them again
     }
+    __syncthreads();  // the next tile writes LDS again
     // Joined with the tiles before; the smaller maximum's token becomes a term of the sums.
     if (!some) {
       S += st;  // 0, or NaN where the tile holds one
@@ -416,11 +485,8 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   u32x4_t u[NV];
   for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
     tile_load<T, W, NV>(u, row, V, tile0);
-    float mt = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < N; ++j) mt = fmaxf(mt, elem<T>(u[k], j));
+    float mt = tile_max<T, NV>(u);
+    tile_again(u);
     mt = wave_max(mt);
     if constexpr (W > 1) {
       if (lane == 0) s_red[wave] = mt;
@@ -431,9 +497,12 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
     const float mn = fmaxf(m, mt), at = mn > -INFINITY ? mn : 0.0f;
     float st = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      if constexpr (NV > 8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < N; ++j) st += __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2);
+    }
+    tile_again(u);
     st = wave_sum(st);
     if constexpr (W > 1) {
       if (lane == 0) s_red[W + wave] = st;
@@ -464,14 +533,17 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   const float scale = weight * a.temperature * (t_max != t_max ? NAN : 1.0f);
   const float ps = S == 0.0f ? scale * 0.0f : scale / S;
   auto write = [&](int tile0) {
+    T* mine = grad + (size_t)(tile0 + tid) * N;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      if ((tile0 + k * 64 * W) * N >= V) continue;
+      if constexpr (NV > 8) __builtin_amdgcn_sched_barrier(0);  // one vector's exponentials at a time: registers
       const int i = tile0 + k * 64 * W + tid;
       float g[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) g[j] = __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2) * ps;
       if (i * N + N <= V) {
-        *reinterpret_cast<u32x4_any_t*>(grad + i * N) = pack<T>(g);
+        *reinterpret_cast<u32x4_any_t*>(mine + k * 64 * W * N) = pack<T>(g);
       } else {
         const int s = vec_start<T>(V, i);
 #pragma unroll
@@ -524,7 +596,7 @@ Status launch_rows(hipStream_t stream, const Args& a, size_t rows) {
 template <class T, int W, int NV>
 struct LaunchLogprobs {
   static Status run(hipStream_t stream, const LogprobArgs& a, size_t rows) {
-    const size_t lds = (size_t)a.top_k * NV * vec_n<T>() * 8;
+    const size_t lds = a.top_k ? kCandidates * 8 : 0;
     token_logprobs_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, lds, stream>>>(a);
     PSSA_LAUNCH_CHECK("token_logprobs_kernel");
     return Status::Ok();
@@ -540,13 +612,6 @@ struct LaunchDistill {
 };
 
 }  // namespace
-
-// 64 alternatives of long rows take 64 KB for their candidates.
-Status init_operator_attributes() {
-  PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&token_logprobs_kernel<Bf16, 16, 16>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, kMaxAlternatives * 16 * 8 * 8));
-  return Status::Ok();
-}
 
 Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& a, size_t rows) {
   return dtype == PSSA_HIP_F32 ? launch_rows<float, LaunchLogprobs>(stream, a, rows)
