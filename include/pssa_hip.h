@@ -691,7 +691,7 @@ int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, f
  * d_state_out (NULL: not kept) receives the states behind the last tokens and
  * may be d_state_in.  out may lie in the buffer of q, k and v in columns of its own (same row stride) and must
  * not overlap them otherwise.  d_key <= 128, d_val <= 4096, n_seqs and heads
- * <= 65535.  bf16 outputs round once; every sum and the states are fp32.  A
+ * <= 65535, row strides below 2^24.  bf16 outputs round once; every sum and the states are fp32.  A
  * value that is not finite reaches the outputs from its own token on and no
  * earlier one. */
 int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,

@@ -2469,6 +2469,8 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
                  wo = heads * d_val;
     PSSA_RETURN_IF(need(ld_q >= wq && ld_k >= wk && ld_v >= wv && ld_out >= wo,
                         "linear attention: row stride below the heads' width"));
+    PSSA_RETURN_IF(need(std::max(std::max(ld_q, ld_k), std::max(ld_v, ld_out)) < ((size_t)1 << 24),
+                        "linear attention: row strides must be below 2^24"));
     PSSA_RETURN_IF(need(aligned_to(d_q, size) && aligned_to(d_k, size) && aligned_to(d_v, size) &&
                             aligned_to(d_out, size) && aligned_to(d_log_decay, 4) && aligned_to(d_state_in, 4) &&
                             aligned_to(d_state_out, 4),

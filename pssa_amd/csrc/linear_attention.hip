@@ -300,25 +300,17 @@ __global__ __launch_bounds__(256) void linear_chunks_f32_kernel(LinearArgs a) {
 //
 // A 32-deep operand's lane holds eight places: 4 quad + r of one 16-row tile
 // and of the next, the order in which two accumulators lie in the lane's
-// registers.  Everything that meets an accumulator is kept in that order
-// (columns of q and k, tokens of the transposed k and v), so S and P are
-// operands without a move; P passes through LDS as ready fragments because
-// one wave computes 16 rows of it and every wave needs all.
+// registers.  So S and P are operands without a move (P passes through LDS as
+// ready fragments because one wave computes 16 rows of it and every wave
+// needs all), and what meets them is read in that order: rows of q in two
+// halves, columns of k and v (their tokens) by ds_read_b64_tr_b16, which gives
+// a lane four rows of its column.  Rows go from memory straight into one of
+// two LDS buffers while the other one's chunk is worked on.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 
-// 8 neighbouring elements, zeros past `left`.
-__device__ __forceinline__ u32x4_t load8(const uint16_t* p, int left) {
-  if (left >= 8) return *reinterpret_cast<const u32x4_any_t*>(p);
-  u32x4_t v = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 7; ++i)
-    if (i < left) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-  return v;
-}
-// Lower or upper halves of two words side by side.
-__device__ __forceinline__ uint32_t lower2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+// Upper halves of two words side by side.
 __device__ __forceinline__ uint32_t upper2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 // Two fp32 values as bf16 parts: v = hi + lo to 2^-17 of it.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -338,290 +330,411 @@ __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, cons
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// LDS in 16-byte units; a row has one more than it needs, so that 16 rows
-// read at one unit lie in 16 different places.
+// Token rows of W columns lie in LDS as W / 8 units of 16 bytes, a row's units
+// exchanged (twice is none) so that rows read at one unit hit different banks.
 template <int W>
-__device__ __forceinline__ int row_at(int row, int u) { return row * (W / 8 + 1) + u; }
-// Rows of 64 tokens.
-__device__ __forceinline__ int tok_at(int row, int u) { return row * 9 + u; }
-// The unit and half of columns (or tokens) c .. c + 3 in operand order.
-__device__ __forceinline__ int order_unit(int c) { return (c >> 5) * 4 + ((c >> 2) & 3); }
-__device__ __forceinline__ int order_half(int c) { return (c >> 4) & 1; }
+__device__ __forceinline__ int row_unit(int row, int u) {
+  return W == 32 ? u ^ ((row >> 1) & 3) : u ^ (row & 7);
+}
+// Columns 8 u .. of a row: an operand in the rows' own order.
+template <int W>
+__device__ __forceinline__ u32x4_t row_frag(const u32x4_t* s, int row, int u) {
+  return s[row * (W / 8) + row_unit<W>(row, u)];
+}
+// Columns c .. c + 3 (c in fours) of a row.
+template <int W>
+__device__ __forceinline__ u32x2_t four_of(const u32x4_t* s, int row, int c) {
+  return reinterpret_cast<const u32x2_t*>(s + row * (W / 8) + row_unit<W>(row, c >> 3))[(c >> 2) & 1];
+}
+// Columns 32 kp + 4 quad .. + 3 and 16 more of a row: an operand in the accumulators' order.
+template <int W>
+__device__ __forceinline__ u32x4_t order_frag(const u32x4_t* s, int row, int kp, int quad) {
+  const u32x2_t x = four_of<W>(s, row, 32 * kp + 4 * quad), y = four_of<W>(s, row, 32 * kp + 16 + 4 * quad);
+  return u32x4_t{x[0], x[1], y[0], y[1]};
+}
+// Rows row0 + 4 quad .. + 3 and 16 more at column c0 + col (c0 in sixteens):
+// 16 lanes read a 4 x 16 block, 4 columns each, and are handed its columns.
+// The LDS address of the lane's part; the next sixteen columns are 32 bytes
+// further but for the exchange, so theirs is an exclusive or.
+template <int W>
+__device__ __forceinline__ uint32_t turned_at(const u32x4_t* s, int row0, int c0, int lane) {
+  const int row = row0 + 4 * (lane >> 4) + ((lane >> 2) & 3), c = c0 + 4 * (lane & 3);
+  const u32x4_t* unit = s + row * (W / 8) + row_unit<W>(row, c >> 3);
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)unit + 8 * ((c >> 2) & 1);
+}
+// One fragment of v and N neighbouring ones of k.  Written out, with their
+// wait, because the compiler would let the builtin wait for the loads that
+// are on their way into the other buffer.
+template <int WV, int WK, int N>
+__device__ __forceinline__ void turned_frags(uint32_t av, u32x4_t& v, uint32_t ak, u32x4_t (&k)[N]) {
+  static_assert(N == 2 || N == 4, "fragments of k");
+  u32x2_t v0, v1, k0[N], k1[N];
+  if constexpr (N == 4) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %10\n\tds_read_b64_tr_b16 %1, %10 offset:%c15\n\t"
+        "ds_read_b64_tr_b16 %2, %11\n\tds_read_b64_tr_b16 %3, %11 offset:%c16\n\t"
+        "ds_read_b64_tr_b16 %4, %12\n\tds_read_b64_tr_b16 %5, %12 offset:%c16\n\t"
+        "ds_read_b64_tr_b16 %6, %13\n\tds_read_b64_tr_b16 %7, %13 offset:%c16\n\t"
+        "ds_read_b64_tr_b16 %8, %14\n\tds_read_b64_tr_b16 %9, %14 offset:%c16\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v0), "=&v"(v1), "=&v"(k0[0]), "=&v"(k1[0]), "=&v"(k0[1]), "=&v"(k1[1]), "=&v"(k0[2]), "=&v"(k1[2]),
+          "=&v"(k0[3]), "=&v"(k1[3])
+        : "v"(av), "v"(ak), "v"(ak ^ 32), "v"(ak ^ 64), "v"(ak ^ 96), "i"(32 * WV), "i"(32 * WK)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %6\n\tds_read_b64_tr_b16 %1, %6 offset:%c9\n\t"
+        "ds_read_b64_tr_b16 %2, %7\n\tds_read_b64_tr_b16 %3, %7 offset:%c10\n\t"
+        "ds_read_b64_tr_b16 %4, %8\n\tds_read_b64_tr_b16 %5, %8 offset:%c10\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v0), "=&v"(v1), "=&v"(k0[0]), "=&v"(k1[0]), "=&v"(k0[1]), "=&v"(k1[1])
+        : "v"(av), "v"(ak), "v"(ak ^ 32), "i"(32 * WV), "i"(32 * WK)
+        : "memory");
+  }
+  v = u32x4_t{v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+  for (int i = 0; i < N; ++i) k[i] = u32x4_t{k0[i][0], k0[i][1], k1[i][0], k1[i][1]};
+}
 
-// Place of query tile t's keys 32 h ..: none behind the queries.
-constexpr int pair_at(int t, int h) { return t < 2 ? t : 2 * t - 2 + h; }
+// Four more of k.
+template <int WK>
+__device__ __forceinline__ void turned_frags(uint32_t ak, u32x4_t (&k)[4]) {
+  u32x2_t k0[4], k1[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%c12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(k0[0]), "=&v"(k1[0]), "=&v"(k0[1]), "=&v"(k1[1]), "=&v"(k0[2]), "=&v"(k1[2]), "=&v"(k0[3]), "=&v"(k1[3])
+      : "v"(ak), "v"(ak ^ 32), "v"(ak ^ 64), "v"(ak ^ 96), "i"(32 * WK)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = u32x4_t{k0[i][0], k0[i][1], k1[i][0], k1[i][1]};
+}
 
-template <int DKP, int NC, int MODE>
-__global__ __launch_bounds__(256, NC == 2 || DKP == 128 ? 1 : 2) void linear_chunks_bf16_kernel(LinearArgs a) {
-  constexpr int DVT = 64 * NC, NB = DKP / 16, KP = DKP / 32;
-  constexpr int QV = LA_C * DKP / 8 / 256;              // 16-byte pieces of q for a thread (DKP = 32: one)
-  constexpr int TASKS = 16 * (DKP / 8 + DVT / 8);       // 4 tokens x 8 columns of k, then of v
-  constexpr int TV = (TASKS + 255) / 256;
-  extern __shared__ u32x4_t s_bf[];
-  u32x4_t* sQ = s_bf;                       // [64][DKP], operand order
-  u32x4_t* sK = sQ + (MODE == LA_LOCAL ? 0 : LA_C * (DKP / 8 + 1));
-  u32x4_t* sKT = sK + (MODE == LA_LOCAL ? 0 : LA_C * (DKP / 8 + 1));  // [DKP][64 tokens]
-  u32x4_t* sVT = sKT + DKP * 9;  // [DVT][64 tokens]
-  u32x4_t* sP = sVT + DVT * 9;   // [6 pairs of a query tile and a key half][2 parts][64 lanes]
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, quad = lane >> 4;
+// Element i of bf16 values in a register or LDS.
+template <class V>
+__device__ __forceinline__ float bf16_at(const V* p, int i) {
+  return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
+}
+
+// Of a chunk's P the pairs of a query tile and a key half that hold anything,
+// the largest first: a wave computes one or two.
+constexpr int kLdsOnly = 0xF | (0x3 << 14) | (0x7 << 4);  // s_waitcnt lgkmcnt(0)
+constexpr int kPairs = 6;
+__device__ __forceinline__ int pair_query(int p) { return (0x201233 >> (4 * p)) & 3; }
+__device__ __forceinline__ int pair_half(int p) { return (0x100010 >> (4 * p)) & 1; }
+constexpr int pair_of(int t, int h) { return t == 3 ? h : t == 2 ? (h ? 5 : 2) : t == 1 ? 3 : 4; }
+
+// What stands in for rows and columns that are not there.
+__device__ uint32_t g_nothing[4];
+
+// LDS units (16 bytes) of the kernel: two buffers of q | k | v, then P.
+template <int DKP, int WAVES, bool LOCAL>
+struct ChunkLds {
+  static constexpr int kQ = LOCAL ? 0 : LA_C * DKP / 8, kK = LA_C * DKP / 8, kV = LA_C * 2 * WAVES;
+  static constexpr int kBuffer = kQ + kK + kV;
+  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + (LOCAL ? 0 : kPairs * 128));
+};
+
+// LB: bytes of one load, 16 where every row and head is so aligned, else 4.
+template <int DKP, int WAVES, int MODE, int LB>
+__global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(LinearArgs a) {
+  constexpr bool LOCAL = MODE == LA_LOCAL;
+  using Lds = ChunkLds<DKP, WAVES, LOCAL>;
+  constexpr int DVT = 16 * WAVES, NB = DKP / 16, KP = DKP / 32;
+  constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + WAVES - 1) / WAVES;  // instructions of a chunk, of a wave
+  constexpr int SLOTS = (kPairs + WAVES - 1) / WAVES;
+  extern __shared__ __attribute__((aligned(256))) u32x4_t s_bf[];
+  u32x4_t* sP = s_bf + 2 * Lds::kBuffer;  // [pairs][2 parts][64 lanes]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int dv0 = blockIdx.x * DVT, head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
   const Span sp = span_of(a, blockIdx.z);
   const float g = a.log_decay[head], g2 = g * kLog2e;
-  const uint16_t* q0 = static_cast<const uint16_t*>(a.q) + (size_t)head * a.dk;
-  const uint16_t* k0 = static_cast<const uint16_t*>(a.k) + (size_t)kv_head * a.dk;
-  const uint16_t* v0 = static_cast<const uint16_t*>(a.v) + (size_t)kv_head * a.dv + dv0;
-  uint16_t* o0 = static_cast<uint16_t*>(a.out) + (size_t)head * a.dv;
   const size_t state0 = ((size_t)(MODE == LA_WHOLE ? sp.seq : sp.item) * a.heads + head) * a.dk * a.dv;
-  const float* state_in = MODE == LA_WHOLE ? a.state_in : MODE == LA_LOCAL ? nullptr : a.seg_state;
-  float* state_out = MODE == LA_WHOLE ? a.state_out : MODE == LA_LOCAL ? a.seg_state : nullptr;
+  const float* state_in = MODE == LA_WHOLE ? a.state_in : LOCAL ? nullptr : a.seg_state;
+  float* state_out = MODE == LA_WHOLE ? a.state_out : LOCAL ? a.seg_state : nullptr;
 
-  // S: rows 16 b + 4 quad + r, column dv0 + 16 NC wave + 16 c + col.
-  f32x4_t S[NB][NC];
+  // The n tokens from pos on into a buffer, straight from memory.  A load's 64
+  // lanes fill 64 neighbouring places, so each lane looks up what belongs in
+  // its own: rows swizzled by row_unit, zeros where nothing is.
+  struct Piece {
+    const uint16_t* base;  // of the chunk's first row
+    size_t ld;
+    int row, c, width;
+  };
+  auto piece = [&](int i, int ln) {
+    const int at = (wave * PER + i) * 64 / (16 / LB);  // first unit
+    const bool is_q = at < Lds::kQ, is_k = !is_q && at < Lds::kQ + Lds::kK;
+    const int unit = at - (is_q ? 0 : is_k ? Lds::kQ : Lds::kQ + Lds::kK) + ln / (16 / LB);
+    const int units = is_q || is_k ? DKP / 8 : DVT / 8;
+    Piece p;
+    p.row = unit / units;
+    const int here = unit % units;
+    p.c = 8 * (is_q || is_k ? row_unit<DKP>(p.row, here) : row_unit<DVT>(p.row, here)) + ln % (16 / LB) * (LB / 2);
+    p.ld = is_q ? a.ld_q : is_k ? a.ld_k : a.ld_v;
+    p.width = is_q || is_k ? a.dk : a.dv - dv0;
+    p.base = is_q   ? static_cast<const uint16_t*>(a.q) + (size_t)head * a.dk
+             : is_k ? static_cast<const uint16_t*>(a.k) + (size_t)kv_head * a.dk
+                    : static_cast<const uint16_t*>(a.v) + (size_t)kv_head * a.dv + dv0;
+    return p;
+  };
+  constexpr bool KEEP = LB == 16;  // the places of a whole chunk's pieces stay in registers
+  uint32_t place[KEEP ? PER : 1];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const Piece p = piece(i, lane);
+      place[i] = __umul24(p.row, (uint32_t)p.ld) + p.c;
+    }
+  }
+  const bool heads_fill = a.dk == DKP && a.dv - dv0 >= DVT;
+  auto issue = [&](int pos, int n, u32x4_t* buffer, int ln) {
+    const size_t tok = sp.tok + pos;
+    const bool plain = KEEP && heads_fill && n == LA_C;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (LOADS % WAVES != 0 && wave * PER + i >= LOADS) continue;
+      auto* dst = (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(buffer) + (wave * PER + i) * 64 * LB);
+      const Piece p = piece(i, ln);
+      const uint16_t* base = p.base + tok * p.ld;
+      const void* src;
+      if (plain)
+        src = base + place[KEEP ? i : 0];
+      else
+        src = p.row < n && p.c < p.width ? static_cast<const void*>(base + (__umul24(p.row, (uint32_t)p.ld) + p.c)) : g_nothing;
+      if constexpr (LB == 16)
+        __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+      else
+        __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0);
+    }
+  };
+
+  int n = min(LA_C, sp.len);
+  if (n > 0) issue(0, n, s_bf, lane);
+  // S: rows 16 b + 4 quad + r, column dv0 + 16 wave + col.
+  f32x4_t S[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * b + 4 * quad + r, j = dv0 + 16 * NC * wave + 16 * c + col;
-        S[b][c][r] = state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
-      }
-  const float full = decay_pow_exact(g, LA_C);
-  float first[4];  // lambda^(i+1) of the lane's query in each tile
-#pragma unroll
-  for (int t = 0; t < 4; ++t) first[t] = decay_pow(g2, 16 * t + col + 1);
-
-  u32x4_t rq[QV > 0 ? QV : 1], rt[TV][4];
-  auto fetch = [&](int pos, int n) {
-    if constexpr (MODE != LA_LOCAL) {
-#pragma unroll
-      for (int i = 0; i < QV; ++i) {
-        const int at = tid + 256 * i, row = at / (DKP / 8), c = at % (DKP / 8) * 8;
-        rq[i] = row < n && c < a.dk ? load8(q0 + (sp.tok + pos + row) * a.ld_q + c, a.dk - c) : u32x4_t{0, 0, 0, 0};
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      S[b][r] = state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
     }
+  // The state's loads end here: waited for in the loop, they would be waited
+  // for together with the loads of every next chunk.
 #pragma unroll
-    for (int i = 0; i < TV; ++i) {
-      const int task = tid + 256 * i;
-      const bool is_k = task < 16 * (DKP / 8);
-      const int row = (task & 15) * 4, c = (is_k ? task >> 4 : (task >> 4) - DKP / 8) * 8;
-      const int left = task < TASKS ? (is_k ? a.dk : a.dv - dv0) - c : 0;
-      const uint16_t* src = is_k ? k0 : v0;
-      const size_t ld = is_k ? a.ld_k : a.ld_v;
+  for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(S[b]));
+  // Powers of the decay, as products of a lane's and a uniform one, every
+  // exponent >= 0: scale lambda^(i+1) for the lane's queries; lambda^(i-j) in
+  // P's diagonal tiles and 15 more for the others; lambda^(n-1-j) for a half
+  // chunk's tokens of v and lambda^n for the state.
+  float first[4], diag[4], off[4], left[8], fs = 1.0f, tile_pow[4];
+  int n_left = -1;  // what `left` and `fs` are for
+  if constexpr (!LOCAL) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        rt[i][t] = row + t < n && left > 0 ? load8(src + (sp.tok + pos + row + t) * ld + c, left) : u32x4_t{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) {
+      const int col = lane & 15, quad = lane >> 4;
+      first[t] = a.scale * decay_pow(g2, 16 * t + col + 1);
+      diag[t] = a.scale * decay_pow(g2, col - 4 * quad - t);
+      off[t] = decay_pow(g2, col - 4 * quad - t + 15);
+      tile_pow[t] = a.scale * decay_pow(g2, 16 * t - 15);
+    }
+  }
+  // A chunk's outputs are stored in the next one's course, before which every
+  // memory operation of the chunk before has to have ended.
+  u32x2_t out[4];
+  auto put = [&](int pos, int n, int ln) {
+    const int j = dv0 + 16 * wave + 4 * (ln >> 4);
+    uint16_t* base = static_cast<uint16_t*>(a.out) + (size_t)head * a.dv + (sp.tok + pos) * a.ld_out;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int i = 16 * t + (ln & 15);
+      if (i >= n || j >= a.dv) continue;
+      uint16_t* dst = base + (__umul24(i, (uint32_t)a.ld_out) + j);
+      if (LB == 16 || j + 4 <= a.dv) {
+        *reinterpret_cast<u32x2_any_t*>(dst) = out[t];
+      } else {  // heads are whole in pairs
+        dst[0] = (uint16_t)out[t][0];
+        dst[1] = (uint16_t)(out[t][0] >> 16);
+      }
     }
   };
-  // The fetched chunk into LDS; whether a value of v is not finite.
-  auto place = [&]() {
-    u32x2_t* q8 = reinterpret_cast<u32x2_t*>(sQ);
-    u32x2_t* k8 = reinterpret_cast<u32x2_t*>(sK);
-    bool odd = false;
-    if constexpr (MODE != LA_LOCAL) {
-#pragma unroll
-      for (int i = 0; i < QV; ++i) {
-        const int at = tid + 256 * i, row = at / (DKP / 8), c = at % (DKP / 8) * 8;
-        q8[2 * row_at<DKP>(row, order_unit(c)) + order_half(c)] = u32x2_t{rq[i][0], rq[i][1]};
-        q8[2 * row_at<DKP>(row, order_unit(c + 4)) + order_half(c)] = u32x2_t{rq[i][2], rq[i][3]};
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < TV; ++i) {
-      const int task = tid + 256 * i;
-      if (task >= TASKS) continue;
-      const bool is_k = task < 16 * (DKP / 8);
-      const int row = (task & 15) * 4, c = (is_k ? task >> 4 : (task >> 4) - DKP / 8) * 8;
-      if constexpr (MODE != LA_LOCAL) {
-        if (is_k) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            k8[2 * row_at<DKP>(row + t, order_unit(c)) + order_half(c)] = u32x2_t{rt[i][t][0], rt[i][t][1]};
-            k8[2 * row_at<DKP>(row + t, order_unit(c + 4)) + order_half(c)] = u32x2_t{rt[i][t][2], rt[i][t][3]};
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              odd |= (rt[i][t][e] & 0x7F80u) == 0x7F80u || (rt[i][t][e] & 0x7F800000u) == 0x7F800000u;
-        }
-      }
-      u32x2_t* t8 = reinterpret_cast<u32x2_t*>(is_k ? sKT : sVT);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        t8[2 * tok_at(c + 2 * e, order_unit(row)) + order_half(row)] =
-            u32x2_t{lower2(rt[i][0][e], rt[i][1][e]), lower2(rt[i][2][e], rt[i][3][e])};
-        t8[2 * tok_at(c + 2 * e + 1, order_unit(row)) + order_half(row)] =
-            u32x2_t{upper2(rt[i][0][e], rt[i][1][e]), upper2(rt[i][2][e], rt[i][3][e])};
-      }
-    }
-    return odd;
-  };
 
-  int singles = 0;  // tokens left of a chunk that runs one by one
-  if (sp.len > 0) fetch(0, min(LA_C, sp.len));
-  for (int pos = 0; pos < sp.len;) {
-    int n = singles ? 1 : min(LA_C, sp.len - pos);
-    __syncthreads();  // the chunk before is read
-    const bool odd = place();
-    // A value that is not finite would reach the rows before it (0 times it is
-    // NaN): such a chunk's tokens run one at a time.
-    if (MODE != LA_LOCAL) {
-      if (__syncthreads_or(odd) && n > 1) {
-        singles = n;
-        n = 1;
-        fetch(pos, 1);
-        place();
-        __syncthreads();
-      }
-    } else {
-      __syncthreads();
+  u32x4_t* buffer = s_bf;
+  for (int pos = 0, before = 0; pos < sp.len; pos += n, before = n) {
+    n = min(LA_C, sp.len - pos);
+    // The lane's number, new for the compiler in each chunk: what follows from
+    // it is worked out again, as kept it would take more registers than the
+    // kernel's work.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int col = ln & 15, quad = ln >> 4;
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    __syncthreads();  // the chunk is there, and the one before is read
+    u32x4_t* other = buffer == s_bf ? s_bf + Lds::kBuffer : s_bf;
+    if (pos + n < sp.len) issue(pos + n, min(LA_C, sp.len - pos - n), other, ln);
+    if constexpr (!LOCAL) {
+      if (before) put(pos - before, before, ln);
     }
-    const int next = pos + n;
-    if (next < sp.len) fetch(next, singles > 1 ? 1 : min(LA_C, sp.len - next));
+    const u32x4_t *sQ = buffer, *sK = buffer + Lds::kQ, *sV = sK + Lds::kK;
+    buffer = other;
 
-    f32x4_t o[4][NC];
-    if constexpr (MODE != LA_LOCAL) {
-      // P^T = (k q^T) lambda^(i-j), j <= i, of query tile `wave`.
-      f32x4_t p[4];
+    f32x4_t o[4];
+    if constexpr (!LOCAL) {
+      // P^T = scale (k q^T) lambda^(i-j), j <= i, of the wave's pairs.
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        p[jt] = f32x4_t{0, 0, 0, 0};
-        if (jt > wave) continue;  // uniform
+      for (int s = 0; s < SLOTS; ++s) {
+        const int p = wave + WAVES * s, qt = pair_query(p), half = pair_half(p);
+        if (p >= kPairs) continue;  // uniform
+        f32x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int kp = 0; kp < KP; ++kp)
-          p[jt] = mfma(sK[row_at<DKP>(16 * jt + col, 4 * kp + quad)], sQ[row_at<DKP>(16 * wave + col, 4 * kp + quad)], p[jt]);
+        for (int kp = 0; kp < KP; ++kp) {
+          const u32x4_t qf = row_frag<DKP>(sQ, 16 * qt + col, 4 * kp + quad);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * wave + col, j = 16 * jt + 4 * quad + r;
-          p[jt][r] = j <= i ? p[jt][r] * decay_pow(g2, i - j) : 0.0f;
+          for (int x = 0; x < 2; ++x) acc[x] = mfma(row_frag<DKP>(sK, 32 * half + 16 * x + col, 4 * kp + quad), qf, acc[x]);
         }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (2 * h > wave) continue;
         u32x4_t hi, lo;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int ahead = qt - 2 * half - x;  // tiles from the keys to the queries
+          const float u = ahead == 1 ? tile_pow[1] : ahead == 2 ? tile_pow[2] : tile_pow[3];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float d = ahead == 0 ? diag[r] : off[r] * u;
+            acc[x][r] = 16 * ahead + col >= 4 * quad + r ? acc[x][r] * d : 0.0f;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t h, l;
+            split2(acc[x][2 * e], acc[x][2 * e + 1], h, l);
+            hi[2 * x + e] = h;
+            lo[2 * x + e] = l;
+          }
+        }
+        sP[(2 * p) * 64 + ln] = hi;
+        sP[(2 * p + 1) * 64 + ln] = lo;
+      }
+      // (q S)^T, each query's column times scale lambda^(i+1).
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) {
+        u32x4_t hi, lo, qf[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) qf[t] = order_frag<DKP>(sQ, 16 * t + col, kp, quad);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t x, y;
-          split2(p[2 * h + (e >> 1)][2 * (e & 1)], p[2 * h + (e >> 1)][2 * (e & 1) + 1], x, y);
+          split2(S[2 * kp + (e >> 1)][2 * (e & 1)], S[2 * kp + (e >> 1)][2 * (e & 1) + 1], x, y);
           hi[e] = x;
           lo[e] = y;
         }
-        sP[(pair_at(wave, h) * 2 + 0) * 64 + lane] = hi;
-        sP[(pair_at(wave, h) * 2 + 1) * 64 + lane] = lo;
-      }
-      // (q S)^T, each query's column times lambda^(i+1).
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) o[t] = mfma(lo, qf[t], o[t]);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) o[t][c] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int kp = 0; kp < KP; ++kp) {
-        u32x4_t hi[NC], lo[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t x, y;
-            split2(S[2 * kp + (e >> 1)][c][2 * (e & 1)], S[2 * kp + (e >> 1)][c][2 * (e & 1) + 1], x, y);
-            hi[c][e] = x;
-            lo[c][e] = y;
-          }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const u32x4_t qf = sQ[row_at<DKP>(16 * t + col, 4 * kp + quad)];
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            o[t][c] = mfma(lo[c], qf, o[t][c]);
-            o[t][c] = mfma(hi[c], qf, o[t][c]);
-          }
-        }
+        for (int t = 0; t < 4; ++t) o[t] = mfma(hi, qf[t], o[t]);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) o[t][c] *= first[t];
-      __syncthreads();  // P is there
+      for (int t = 0; t < 4; ++t) o[t] *= first[t];
+      // P is there; the next chunk's loads stay in flight (__syncthreads would wait for them).
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(kLdsOnly);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
     }
 
-    // (P v)^T, and S = lambda^n S + k^T (lambda^(n-1-j) v).
-    const float fs = n == LA_C ? full : decay_pow_exact(g, n);
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) S[b][c] *= fs;
+    // (P v)^T, and S = lambda^n S + k^T (lambda^(n-1-j) v), 32 tokens at a time.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4_t w0[NC], w1[NC], w2[NC];
+      const int nh = min(max(n - 32 * h, 0), 32);
+      if (nh != n_left) {
+        n_left = nh;
+        fs = decay_pow_exact(g, nh);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const u32x4_t vf = sVT[tok_at(16 * NC * wave + 16 * c + col, 4 * h + quad)];
-        if constexpr (MODE != LA_LOCAL) {
+        for (int e = 0; e < 8; ++e) left[e] = decay_pow(g2, nh - 1 - (16 * (e >> 2) + 4 * quad + (e & 3)));
+      }
+      constexpr int BG = NB < 4 ? NB : 4;  // tiles whose sums run beside each other
+      u32x4_t vf, kf[BG];
+      turned_frags<DVT, DKP, BG>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf, turned_at<DKP>(sK, 32 * h, 0, ln), kf);
+      if constexpr (!LOCAL) {
+        u32x4_t hi[4], lo[4];
 #pragma unroll
-          for (int t = 2 * h; t < 4; ++t) {
-            o[t][c] = mfma(vf, sP[(pair_at(t, h) * 2 + 1) * 64 + lane], o[t][c]);
-            o[t][c] = mfma(vf, sP[(pair_at(t, h) * 2 + 0) * 64 + lane], o[t][c]);
+        for (int t = 2 * h; t < 4; ++t) {
+          hi[t] = sP[(2 * pair_of(t, h)) * 64 + ln];
+          lo[t] = sP[(2 * pair_of(t, h) + 1) * 64 + ln];
+        }
+        // An exponent of ones carries into the bit above it.
+        uint32_t odd = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (vf[e] & 0x7F807F80u) + 0x00800080u;
+        u32x4_t fine = vf;
+        if (__any((odd & 0x80008000u) != 0)) {
+          // Values that are not finite leave the product, where 0 times one
+          // would reach the queries before it, and are added one by one.
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t carry = ((vf[e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+            fine[e] = vf[e] & ~((carry >> 15) * 0xFFFFu);
+          }
+          for (int j = 0; j < 32; ++j) {
+            const u32x2_t v4 = four_of<DVT>(sV, 32 * h + j, 16 * wave + 4 * quad);
+#pragma unroll
+            for (int t = 2 * h; t < 4; ++t) {
+              const int i = 16 * t + col, place = (2 * pair_of(t, h)) * 64 + 16 * ((j & 15) >> 2) + col;
+              const float p = bf16_at(&sP[place], 4 * (j >> 4) + (j & 3));
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float v = bf16_at(&v4, r);
+                if (i >= 32 * h + j && !(fabsf(v) < INFINITY)) o[t][r] += p * v;
+              }
+            }
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 32 * h + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);  // of the word's first token
-          uint32_t x, y, z;
-          split3(__uint_as_float(vf[e] << 16) * decay_pow(g2, n - 1 - j),
-                 __uint_as_float(vf[e] & 0xFFFF0000u) * decay_pow(g2, n - 2 - j), x, y, z);
-          w0[c][e] = x;
-          w1[c][e] = y;
-          w2[c][e] = z;
-        }
+        for (int t = 2 * h; t < 4; ++t) o[t] = mfma(fine, lo[t], o[t]);
+#pragma unroll
+        for (int t = 2 * h; t < 4; ++t) o[t] = mfma(fine, hi[t], o[t]);
+      }
+      u32x4_t w[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t x, y, z;
+        split3(__uint_as_float(vf[e] << 16) * left[2 * e], __uint_as_float(vf[e] & 0xFFFF0000u) * left[2 * e + 1], x, y, z);
+        w[0][e] = x;
+        w[1][e] = y;
+        w[2][e] = z;
       }
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const u32x4_t kf = sKT[tok_at(16 * b + col, 4 * h + quad)];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          S[b][c] = mfma(kf, w2[c], S[b][c]);
-          S[b][c] = mfma(kf, w1[c], S[b][c]);
-          S[b][c] = mfma(kf, w0[c], S[b][c]);
+      for (int b0 = 0; b0 < NB; b0 += BG) {
+        if constexpr (NB > 4) {
+          if (b0) turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, ln), kf);
         }
-      }
-    }
-    if constexpr (MODE != LA_LOCAL) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int i = 16 * t + col;
-        if (i >= n) continue;
-        uint16_t* dst = o0 + (sp.tok + pos + i) * a.ld_out;
+        for (int b = 0; b < BG; ++b) S[b0 + b] *= fs;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int j = dv0 + 16 * NC * wave + 16 * c + 4 * quad;
-          const u32x2_t v = {bf16x2_bits(o[t][c][0] * a.scale, o[t][c][1] * a.scale),
-                             bf16x2_bits(o[t][c][2] * a.scale, o[t][c][3] * a.scale)};
-          if (j + 4 <= a.dv) {
-            *reinterpret_cast<u32x2_any_t*>(dst + j) = v;
-          } else {
+        for (int p = 2; p >= 0; --p)
 #pragma unroll
-            for (int e = 0; e < 3; ++e)
-              if (j + e < a.dv) dst[j + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-          }
-        }
+          for (int b = 0; b < BG; ++b) S[b0 + b] = mfma(kf[b], w[p], S[b0 + b]);
       }
     }
-    pos = next;
-    if (singles) --singles;
+    if constexpr (!LOCAL) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) out[t] = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
+    }
+  }
+  if constexpr (!LOCAL) {
+    if (sp.len > 0) put(sp.len - n, n, lane);
   }
   if (!state_out) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * b + 4 * quad + r, j = dv0 + 16 * NC * wave + 16 * c + col;
-        if (i < a.dk && j < a.dv) state_out[state0 + (size_t)i * a.dv + j] = S[b][c][r];
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      if (i < a.dk && j < a.dv) state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
+    }
 }
 
 // The scan over the segments of a sequence: every segment's own state becomes
@@ -734,38 +847,57 @@ Status launch_steps(hipStream_t stream, const LinearArgs& a) {
   return Status::Ok();
 }
 
-template <class T, int DKP, int NC, int MODE>
+// The kernel of a call: the bf16 kernel with loads of LB bytes, or (0) the
+// fp32 products, which take any width and alignment.
+template <class T, int DKP, int NC, int MODE, int LB>
 struct Chunks {
   static constexpr size_t kLds = (size_t)(2 * LA_C * (DKP + 4) + LA_C * (64 * NC + 4) + LA_C * 68) * 4;
+  static constexpr int kThreads = 256;
   static constexpr auto kKernel = &linear_chunks_f32_kernel<T, DKP, NC, MODE>;
 };
-template <int DKP, int NC, int MODE>
-struct Chunks<Bf16, DKP, NC, MODE> {
-  static constexpr size_t kLds = (MODE == LA_LOCAL ? 0 : 2 * LA_C * (DKP * 2 + 16) + 12288) + (DKP + 64 * NC) * 144;
-  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, NC, MODE>;
+template <int DKP, int NC, int MODE, int LB>
+struct ChunksBf16 {
+  static constexpr size_t kLds = ChunkLds<DKP, 4 * NC, MODE == LA_LOCAL>::kBytes;
+  static constexpr int kThreads = 256 * NC;
+  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4 * NC, MODE, LB>;
 };
+template <int DKP, int NC, int MODE>
+struct Chunks<Bf16, DKP, NC, MODE, 16> : ChunksBf16<DKP, NC, MODE, 16> {};
+template <int DKP, int NC, int MODE>
+struct Chunks<Bf16, DKP, NC, MODE, 4> : ChunksBf16<DKP, NC, MODE, 4> {};
 
-// Calls f with the kernel choice for a call's head widths and type.
+// Calls f with the kernel for a call's type, head widths and loads.
 template <int MODE, class F>
-Status with_chunks(int dtype, int dk, int dv, F f) {
-  auto typed = [&](auto t) {
+Status with_chunks(int dtype, int dk, int dv, int load, F f) {
+  auto typed = [&](auto t, auto lb) {
     using T = decltype(t);
+    constexpr int LB = decltype(lb)::value;
     auto wide = [&](auto dkp) {
       constexpr int D = decltype(dkp)::value;
-      return dv > 64 ? f(Chunks<T, D, 2, MODE>{}, 2) : f(Chunks<T, D, 1, MODE>{}, 1);
+      return dv > 64 ? f(Chunks<T, D, 2, MODE, LB>{}, 2) : f(Chunks<T, D, 1, MODE, LB>{}, 1);
     };
     if (dk <= 32) return wide(std::integral_constant<int, 32>{});
     if (dk <= 64) return wide(std::integral_constant<int, 64>{});
     return wide(std::integral_constant<int, 128>{});
   };
-  return dtype == PSSA_HIP_F32 ? typed(0.0f) : typed(Bf16{});
+  if (dtype == PSSA_HIP_F32) return typed(0.0f, std::integral_constant<int, 0>{});
+  if (load == 16) return typed(Bf16{}, std::integral_constant<int, 16>{});
+  if (load == 4) return typed(Bf16{}, std::integral_constant<int, 4>{});
+  return typed(Bf16{}, std::integral_constant<int, 0>{});
+}
+
+// The largest load that every row's and head's start is aligned to.
+int load_bytes(const LinearArgs& a) {
+  const size_t all = (size_t)a.q | (size_t)a.k | (size_t)a.v |
+                     2 * (a.ld_q | a.ld_k | a.ld_v | (size_t)a.dk | (size_t)a.dv);
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 0;
 }
 
 template <int MODE>
 Status launch_chunks(hipStream_t stream, int dtype, const LinearArgs& a) {
-  return with_chunks<MODE>(dtype, a.dk, a.dv, [&](auto c, int nc) -> Status {
+  return with_chunks<MODE>(dtype, a.dk, a.dv, load_bytes(a), [&](auto c, int nc) -> Status {
     const dim3 grid((a.dv + 64 * nc - 1) / (64 * nc), a.heads, a.items);
-    c.kKernel<<<grid, 256, c.kLds, stream>>>(a);
+    c.kKernel<<<grid, c.kThreads, c.kLds, stream>>>(a);
     PSSA_LAUNCH_CHECK("linear_chunks_kernel");
     return Status::Ok();
   });
@@ -776,11 +908,12 @@ Status chunks_attributes() {
   for (int dtype : {PSSA_HIP_F32, PSSA_HIP_BF16})
     for (int dk : {32, 64, 128})
       for (int dv : {64, 128})
-        PSSA_RETURN_IF(with_chunks<MODE>(dtype, dk, dv, [&](auto c, int) -> Status {
-          PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(c.kKernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)c.kLds));
-          return Status::Ok();
-        }));
+        for (int load : {16, 4, 0})
+          PSSA_RETURN_IF(with_chunks<MODE>(dtype, dk, dv, load, [&](auto c, int) -> Status {
+            PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(c.kKernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)c.kLds));
+            return Status::Ok();
+          }));
   return Status::Ok();
 }
 

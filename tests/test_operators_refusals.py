@@ -125,7 +125,7 @@ LINEAR = dict(ctx=None, dtype=_abi.F32, q=P, ld_q=64, k=P + 0x10000, ld_k=32, v=
     ({"heads": 0}, "positive"), ({"d_val": 0}, "positive"), ({"kv_heads": 0}, "divide"), ({"kv_heads": 3}, "divide"),
     ({"d_key": 129}, "128"), ({"d_val": 4097}, "4096"), ({"heads": 65536, "kv_heads": 65536}, "65535"),
     ({"n_seqs": 0}, "sequences"), ({"n_seqs": 65536}, "sequences"), ({"seq_len": 1 << 31}, "too many tokens"),
-    ({"n_seqs": 60000, "seq_len": 1 << 20}, "too many tokens"), ({"ld_q": 63}, "row stride"), ({"ld_out": 95}, "row stride"),
+    ({"n_seqs": 60000, "seq_len": 1 << 20}, "too many tokens"), ({"ld_q": 63}, "row stride"), ({"ld_out": 95}, "row stride"), ({"ld_k": 1 << 24}, "2^24"),
     ({"scale": float("inf")}, "scale"), ({"q": P + 2}, "misaligned"), ({"state_out": P + 0x40002}, "misaligned"),
     ({"out": P}, "overlaps"), ({"out": P + 0x10000 + 4, "ld_out": 96}, "overlaps"), ({"state_out": P + 0x30000}, "states"),
     ({"state_in": P + 0x40004}, "states"), ({"state_in": P + 0x40000}, "null context"), ({"seq_len": 0}, "null context"),
