@@ -2146,7 +2146,7 @@ Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_
     p.longest = std::max(p.longest, len);
     same &= !lens || lens[i] == lens[0];
   }
-  const size_t seg = (size_t)pssa::linear_segment(n_seqs, p.longest, p.tokens, heads, d_val);
+  const size_t seg = (size_t)pssa::linear_segment(lens, n_seqs, p.longest, heads, d_val);
   a.seg_len = (int)(seg ? seg : std::max<size_t>(p.longest, 1));
   a.uniform_len = same ? (int)p.longest : -1;
   a.uniform_segs = (int)std::max<size_t>(1, (p.longest + a.seg_len - 1) / a.seg_len);

@@ -2,16 +2,17 @@
 //   S_t = lambda_h S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
 // over packed sequences, from one token to long prompts.
 //
-// Prompts run in chunks of 64 tokens.  Within a chunk entered with state S
+// Prompts run in chunks of 64 tokens (32 in fp32).  Within a chunk entered with state S
 // (i, j count its tokens, n of them)
 //   o_i = scale (lambda^(i+1) q_i S + sum_{j<=i} lambda^(i-j) (q_i k_j) v_j)
 //   S'  = lambda^n S + sum_j k_j (lambda^(n-1-j) v_j)^T,
-// four matrix products.  A workgroup of four waves walks one sequence's (or
-// segment's) chunks for one head and a tile of value columns; a wave owns 16
-// or 32 of the columns, its part of S stays in its accumulators, and these
-// are the product q S's operand as they stand: the accumulator layout (lane l
-// holds column l % 16, rows 4 (l / 16) + r) is the matrix instruction's
-// operand layout once q's columns are read in the same order.
+// four matrix products.  A workgroup walks one sequence's (or segment's)
+// chunks for one head and a tile of value columns, of which a wave owns 16;
+// its part of S stays in its accumulators, and these are the product q S's
+// operand as they stand: the accumulator layout (lane l holds column l % 16,
+// rows 4 (l / 16) + r) is the matrix instruction's operand layout once q's
+// columns are read in the same order.  The next chunk's rows go straight into
+// the other of two LDS buffers meanwhile.
 //
 // Few long sequences are split into segments: the segments' own states (the
 // second product alone, from zero), a scan over them that leaves every
@@ -119,9 +120,9 @@ __device__ __forceinline__ Span span_of(const LinearArgs& a, int item) {
 // state, or a segment's outputs from its entry state.
 enum { LA_WHOLE, LA_LOCAL, LA_SEGMENT };
 
-// fp32 matrix products (v_mfma_f32_16x16x4_f32); bf16 inputs widened.
+// Any widths and alignment: bf16 inputs widened for fp32 products.
 template <class T, int DKP, int NC, int MODE>
-__global__ __launch_bounds__(256) void linear_chunks_f32_kernel(LinearArgs a) {
+__global__ __launch_bounds__(256) void linear_chunks_any_kernel(LinearArgs a) {
   constexpr int LDK = DKP + 4, LDV = 64 * NC + 4, LDP = 68, NB = DKP / 16;
   extern __shared__ float s_lin[];
   float* sQ = s_lin;
@@ -362,9 +363,19 @@ __device__ __forceinline__ uint32_t turned_at(const u32x4_t* s, int row0, int c0
   const u32x4_t* unit = s + row * (W / 8) + row_unit<W>(row, c >> 3);
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)unit + 8 * ((c >> 2) & 1);
 }
-// One fragment of v and N neighbouring ones of k.  Written out, with their
+// One fragment.  Written out, with their
 // wait, because the compiler would let the builtin wait for the loads that
 // are on their way into the other buffer.
+template <int W>
+__device__ __forceinline__ void turned_frag(uint32_t at, u32x4_t& v) {
+  u32x2_t x, y;
+  asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x), "=&v"(y)
+               : "v"(at), "i"(32 * W)
+               : "memory");
+  v = u32x4_t{x[0], x[1], y[0], y[1]};
+}
+// One of v and N neighbouring ones of k.
 template <int WV, int WK, int N>
 __device__ __forceinline__ void turned_frags(uint32_t av, u32x4_t& v, uint32_t ak, u32x4_t (&k)[N]) {
   static_assert(N == 2 || N == 4, "fragments of k");
@@ -430,25 +441,35 @@ constexpr int pair_of(int t, int h) { return t == 3 ? h : t == 2 ? (h ? 5 : 2) :
 // What stands in for rows and columns that are not there.
 __device__ uint32_t g_nothing[4];
 
-// LDS units (16 bytes) of the kernel: two buffers of q | k | v, then P.
+// LDS units (16 bytes) of the kernel: two buffers of q | k | v, P, and q S.
 template <int DKP, int WAVES, bool LOCAL>
 struct ChunkLds {
   static constexpr int kQ = LOCAL ? 0 : LA_C * DKP / 8, kK = LA_C * DKP / 8, kV = LA_C * 2 * WAVES;
   static constexpr int kBuffer = kQ + kK + kV;
-  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + (LOCAL ? 0 : kPairs * 128));
+  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + (LOCAL ? 0 : kPairs * 128 + WAVES * 256));
 };
 
+// A tile of 16 WAVES value columns takes two groups of as many waves: one
+// computes P and P v and stores the outputs, the other keeps S, computes q S
+// (handed over through LDS) and the next S.  Both halves of a chunk's work
+// are about as long, and every SIMD has a wave of each.  (One group doing
+// both in turn took 7000 cycles a chunk at heads of 64, two of them with
+// two workgroups' state passes in between.)
 // LB: bytes of one load, 16 where every row and head is so aligned, else 4.
 template <int DKP, int WAVES, int MODE, int LB>
-__global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(LinearArgs a) {
+__global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA_LOCAL || DKP == 128 ? 2 : 4) void linear_chunks_bf16_kernel(LinearArgs a) {
   constexpr bool LOCAL = MODE == LA_LOCAL;
+  constexpr int ALL = LOCAL ? WAVES : 2 * WAVES;
   using Lds = ChunkLds<DKP, WAVES, LOCAL>;
   constexpr int DVT = 16 * WAVES, NB = DKP / 16, KP = DKP / 32;
-  constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + WAVES - 1) / WAVES;  // instructions of a chunk, of a wave
+  constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;  // instructions of a chunk, of a wave
   constexpr int SLOTS = (kPairs + WAVES - 1) / WAVES;
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_bf[];
   u32x4_t* sP = s_bf + 2 * Lds::kBuffer;  // [pairs][2 parts][64 lanes]
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x4_t* sO = reinterpret_cast<f32x4_t*>(sP + kPairs * 128);  // [column group][query tile][64 lanes]
+  const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool keeps_state = LOCAL || in_all >= WAVES;
+  const int wave = LOCAL ? in_all : in_all % WAVES;  // of its group: its 16 columns
   const int dv0 = blockIdx.x * DVT, head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
   const Span sp = span_of(a, blockIdx.z);
   const float g = a.log_decay[head], g2 = g * kLog2e;
@@ -465,8 +486,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
     int row, c, width;
   };
   auto piece = [&](int i, int ln) {
-    const int at = (wave * PER + i) * 64 / (16 / LB);  // first unit
-    const bool is_q = at < Lds::kQ, is_k = !is_q && at < Lds::kQ + Lds::kK;
+    const int at = (i * ALL + in_all) * 64 / (16 / LB);  // first unit
+    // Where all waves load from the same array the compiler sees which.
+    constexpr int STEP = ALL * 64 / (16 / LB);
+    const bool even = Lds::kQ % STEP == 0 && Lds::kK % STEP == 0;
+    const int by = even ? i * STEP : at;
+    const bool is_q = by < Lds::kQ, is_k = !is_q && by < Lds::kQ + Lds::kK;
     const int unit = at - (is_q ? 0 : is_k ? Lds::kQ : Lds::kQ + Lds::kK) + ln / (16 / LB);
     const int units = is_q || is_k ? DKP / 8 : DVT / 8;
     Piece p;
@@ -495,8 +520,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
     const bool plain = KEEP && heads_fill && n == LA_C;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (LOADS % WAVES != 0 && wave * PER + i >= LOADS) continue;
-      auto* dst = (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(buffer) + (wave * PER + i) * 64 * LB);
+      if (LOADS % ALL != 0 && i * ALL + in_all >= LOADS) continue;
+      auto* dst = (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(buffer) + (i * ALL + in_all) * 64 * LB);
       const Piece p = piece(i, ln);
       const uint16_t* base = p.base + tok * p.ld;
       const void* src;
@@ -520,31 +545,30 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
-      S[b][r] = state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
+      S[b][r] = keeps_state && state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
     }
   // The state's loads end here: waited for in the loop, they would be waited
   // for together with the loads of every next chunk.
 #pragma unroll
   for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(S[b]));
   // Powers of the decay, as products of a lane's and a uniform one, every
-  // exponent >= 0: scale lambda^(i+1) for the lane's queries; lambda^(i-j) in
-  // P's diagonal tiles and 15 more for the others; lambda^(n-1-j) for a half
-  // chunk's tokens of v and lambda^n for the state.
-  float first[4], diag[4], off[4], left[8], fs = 1.0f, tile_pow[4];
-  int n_left = -1;  // what `left` and `fs` are for
-  if constexpr (!LOCAL) {
+  // exponent >= 0.  The first group of waves: scale lambda^(i-j) in P's
+  // diagonal tiles, lambda^(i-j+15) for the others.  The second: scale
+  // lambda^(i+1) for the lane's queries, lambda^(n-1-j) for its tokens of a
+  // half chunk (n_left and fs = lambda^n say which).
+  float pw[12], fs = 1.0f;
+  int n_left = -1;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int col = lane & 15, quad = lane >> 4;
-      first[t] = a.scale * decay_pow(g2, 16 * t + col + 1);
-      diag[t] = a.scale * decay_pow(g2, col - 4 * quad - t);
-      off[t] = decay_pow(g2, col - 4 * quad - t + 15);
-      tile_pow[t] = a.scale * decay_pow(g2, 16 * t - 15);
-    }
+  for (int t = 0; t < 4; ++t) {
+    const int col = lane & 15, quad = lane >> 4;
+    pw[t] = LOCAL ? 0.0f : a.scale * decay_pow(g2, keeps_state ? 16 * t + col + 1 : col - 4 * quad - t);
+    pw[4 + t] = LOCAL ? 0.0f : decay_pow(g2, col - 4 * quad - t + 15);
+    pw[8 + t] = 0.0f;
   }
+  const float tile_pow[4] = {0.0f, a.scale * decay_pow(g2, 1), a.scale * decay_pow(g2, 17), a.scale * decay_pow(g2, 33)};
   // A chunk's outputs are stored in the next one's course, before which every
-  // memory operation of the chunk before has to have ended.
-  u32x2_t out[4];
+  // memory operation of the chunk before has to have ended.  The waves that
+  // store have no state: the outputs lie in its registers.
   auto put = [&](int pos, int n, int ln) {
     const int j = dv0 + 16 * wave + 4 * (ln >> 4);
     uint16_t* base = static_cast<uint16_t*>(a.out) + (size_t)head * a.dv + (sp.tok + pos) * a.ld_out;
@@ -552,12 +576,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
     for (int t = 0; t < 4; ++t) {
       const int i = 16 * t + (ln & 15);
       if (i >= n || j >= a.dv) continue;
+      const u32x2_t v = {__float_as_uint(S[t >> 1][2 * (t & 1)]), __float_as_uint(S[t >> 1][2 * (t & 1) + 1])};
       uint16_t* dst = base + (__umul24(i, (uint32_t)a.ld_out) + j);
       if (LB == 16 || j + 4 <= a.dv) {
-        *reinterpret_cast<u32x2_any_t*>(dst) = out[t];
+        *reinterpret_cast<u32x2_any_t*>(dst) = v;
       } else {  // heads are whole in pairs
-        dst[0] = (uint16_t)out[t][0];
-        dst[1] = (uint16_t)(out[t][0] >> 16);
+        dst[0] = (uint16_t)v[0];
+        dst[1] = (uint16_t)(v[0] >> 16);
       }
     }
   };
@@ -570,19 +595,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
     // kernel's work.
     int ln = lane;
     asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int i = 0; i < 12; ++i) asm volatile("" : "+v"(pw[i]));
     const int col = ln & 15, quad = ln >> 4;
     __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
     __syncthreads();  // the chunk is there, and the one before is read
     u32x4_t* other = buffer == s_bf ? s_bf + Lds::kBuffer : s_bf;
     if (pos + n < sp.len) issue(pos + n, min(LA_C, sp.len - pos - n), other, ln);
     if constexpr (!LOCAL) {
-      if (before) put(pos - before, before, ln);
+      if (before && !keeps_state) put(pos - before, before, ln);
     }
     const u32x4_t *sQ = buffer, *sK = buffer + Lds::kQ, *sV = sK + Lds::kK;
     buffer = other;
 
-    f32x4_t o[4];
-    if constexpr (!LOCAL) {
+    if (!LOCAL && !keeps_state) {
       // P^T = scale (k q^T) lambda^(i-j), j <= i, of the wave's pairs.
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) {
@@ -602,7 +628,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
           const float u = ahead == 1 ? tile_pow[1] : ahead == 2 ? tile_pow[2] : tile_pow[3];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float d = ahead == 0 ? diag[r] : off[r] * u;
+            const float d = ahead == 0 ? pw[r] : pw[4 + r] * u;
             acc[x][r] = 16 * ahead + col >= 4 * quad + r ? acc[x][r] * d : 0.0f;
           }
 #pragma unroll
@@ -616,7 +642,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
         sP[(2 * p) * 64 + ln] = hi;
         sP[(2 * p + 1) * 64 + ln] = lo;
       }
+    } else if (!LOCAL) {
       // (q S)^T, each query's column times scale lambda^(i+1).
+      f32x4_t o[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
@@ -637,97 +665,364 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_chunks_bf16_kernel(Linea
         for (int t = 0; t < 4; ++t) o[t] = mfma(hi, qf[t], o[t]);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) o[t] *= first[t];
-      // P is there; the next chunk's loads stay in flight (__syncthreads would wait for them).
+      for (int t = 0; t < 4; ++t) sO[(4 * wave + t) * 64 + ln] = o[t] * pw[t];
+    }
+    if constexpr (!LOCAL) {
+      // P and q S are there; the next chunk's loads stay in flight (__syncthreads would wait for them).
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_waitcnt(kLdsOnly);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
 
-    // (P v)^T, and S = lambda^n S + k^T (lambda^(n-1-j) v), 32 tokens at a time.
+    if (!LOCAL && !keeps_state) {
+      // + (P v)^T, 32 tokens at a time.
+      u32x4_t vf[2];
+      uint32_t odd = 0;  // an exponent of ones carries into the bit above it
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int nh = min(max(n - 32 * h, 0), 32);
-      if (nh != n_left) {
-        n_left = nh;
-        fs = decay_pow_exact(g, nh);
+      for (int h = 0; h < 2; ++h) {
+        turned_frag<DVT>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf[h]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) left[e] = decay_pow(g2, nh - 1 - (16 * (e >> 2) + 4 * quad + (e & 3)));
+        for (int e = 0; e < 4; ++e) odd |= (vf[h][e] & 0x7F807F80u) + 0x00800080u;
       }
-      constexpr int BG = NB < 4 ? NB : 4;  // tiles whose sums run beside each other
-      u32x4_t vf, kf[BG];
-      turned_frags<DVT, DKP, BG>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf, turned_at<DKP>(sK, 32 * h, 0, ln), kf);
-      if constexpr (!LOCAL) {
-        u32x4_t hi[4], lo[4];
+      if (__any((odd & 0x80008000u) != 0)) {
+        // Values that are not finite leave the product, where 0 times one
+        // would reach the queries before it, and are added one by one.
 #pragma unroll
-        for (int t = 2 * h; t < 4; ++t) {
-          hi[t] = sP[(2 * pair_of(t, h)) * 64 + ln];
-          lo[t] = sP[(2 * pair_of(t, h) + 1) * 64 + ln];
-        }
-        // An exponent of ones carries into the bit above it.
-        uint32_t odd = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= (vf[e] & 0x7F807F80u) + 0x00800080u;
-        u32x4_t fine = vf;
-        if (__any((odd & 0x80008000u) != 0)) {
-          // Values that are not finite leave the product, where 0 times one
-          // would reach the queries before it, and are added one by one.
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t carry = ((vf[e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-            fine[e] = vf[e] & ~((carry >> 15) * 0xFFFFu);
+            const uint32_t carry = ((vf[h][e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+            vf[h][e] &= ~((carry >> 15) * 0xFFFFu);
           }
-          for (int j = 0; j < 32; ++j) {
-            const u32x2_t v4 = four_of<DVT>(sV, 32 * h + j, 16 * wave + 4 * quad);
+#pragma unroll 1
+        for (int j = 0; j < LA_C; ++j) {
+          const u32x2_t v4 = four_of<DVT>(sV, j, 16 * wave + 4 * quad);
+#pragma unroll 1
+          for (int t = j >> 4; t < 4; ++t) {
+            const int pair = t == 3 ? j >> 5 : t == 2 ? (j >> 5 ? 5 : 2) : t == 1 ? 3 : 4;
+            const float p = bf16_at(&sP[2 * pair * 64 + 16 * ((j & 15) >> 2) + col], 4 * ((j >> 4) & 1) + (j & 3));
+            f32x4_t& o = sO[(4 * wave + t) * 64 + ln];
 #pragma unroll
-            for (int t = 2 * h; t < 4; ++t) {
-              const int i = 16 * t + col, place = (2 * pair_of(t, h)) * 64 + 16 * ((j & 15) >> 2) + col;
-              const float p = bf16_at(&sP[place], 4 * (j >> 4) + (j & 3));
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float v = bf16_at(&v4, r);
-                if (i >= 32 * h + j && !(fabsf(v) < INFINITY)) o[t][r] += p * v;
-              }
+            for (int r = 0; r < 4; ++r) {
+              const float v = __uint_as_float(r & 1 ? v4[r >> 1] & 0xFFFF0000u : v4[r >> 1] << 16);
+              if (16 * t + col >= j && !(fabsf(v) < INFINITY)) o[r] += p * v;
             }
           }
         }
-#pragma unroll
-        for (int t = 2 * h; t < 4; ++t) o[t] = mfma(fine, lo[t], o[t]);
-#pragma unroll
-        for (int t = 2 * h; t < 4; ++t) o[t] = mfma(fine, hi[t], o[t]);
       }
-      u32x4_t w[3];
+      f32x4_t o[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t x, y, z;
-        split3(__uint_as_float(vf[e] << 16) * left[2 * e], __uint_as_float(vf[e] & 0xFFFF0000u) * left[2 * e + 1], x, y, z);
-        w[0][e] = x;
-        w[1][e] = y;
-        w[2][e] = z;
+      for (int t = 0; t < 4; ++t) o[t] = sO[(4 * wave + t) * 64 + ln];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int part = 1; part >= 0; --part)
+#pragma unroll
+          for (int t = 2 * h; t < 4; ++t) o[t] = mfma(vf[h], sP[(2 * pair_of(t, h) + part) * 64 + ln], o[t]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        S[t >> 1][2 * (t & 1)] = __uint_as_float(bf16x2_bits(o[t][0], o[t][1]));
+        S[t >> 1][2 * (t & 1) + 1] = __uint_as_float(bf16x2_bits(o[t][2], o[t][3]));
       }
+    } else {
+      // S = lambda^n S + k^T (lambda^(n-1-j) v), 32 tokens at a time.
 #pragma unroll
-      for (int b0 = 0; b0 < NB; b0 += BG) {
-        if constexpr (NB > 4) {
-          if (b0) turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, ln), kf);
+      for (int h = 0; h < 2; ++h) {
+        const int nh = min(max(n - 32 * h, 0), 32);
+        if (nh != n_left) {
+          n_left = nh;
+          fs = decay_pow_exact(g, nh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pw[4 + e] = decay_pow(g2, nh - 1 - (16 * (e >> 2) + 4 * quad + (e & 3)));
+        }
+        constexpr int BG = NB < 4 ? NB : 4;  // tiles whose sums run beside each other
+        u32x4_t vf, kf[BG];
+        turned_frags<DVT, DKP, BG>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf, turned_at<DKP>(sK, 32 * h, 0, ln), kf);
+        u32x4_t w[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t x, y, z;
+          split3(__uint_as_float(vf[e] << 16) * pw[4 + 2 * e], __uint_as_float(vf[e] & 0xFFFF0000u) * pw[5 + 2 * e], x, y, z);
+          w[0][e] = x;
+          w[1][e] = y;
+          w[2][e] = z;
         }
 #pragma unroll
-        for (int b = 0; b < BG; ++b) S[b0 + b] *= fs;
+        for (int b0 = 0; b0 < NB; b0 += BG) {
+          if constexpr (NB > 4) {
+            if (b0) turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, ln), kf);
+          }
 #pragma unroll
-        for (int p = 2; p >= 0; --p)
+          for (int b = 0; b < BG; ++b) S[b0 + b] *= fs;
 #pragma unroll
-          for (int b = 0; b < BG; ++b) S[b0 + b] = mfma(kf[b], w[p], S[b0 + b]);
+          for (int p = 2; p >= 0; --p)
+#pragma unroll
+            for (int b = 0; b < BG; ++b) S[b0 + b] = mfma(kf[b], w[p], S[b0 + b]);
+        }
       }
-    }
-    if constexpr (!LOCAL) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) out[t] = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
     }
   }
   if constexpr (!LOCAL) {
-    if (sp.len > 0) put(sp.len - n, n, lane);
+    if (sp.len > 0 && !keeps_state) put(sp.len - n, n, lane);
   }
-  if (!state_out) return;
+  if (!state_out || !keeps_state) return;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      if (i < a.dk && j < a.dv) state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
+    }
+}
+
+// ---------------------------------------------------------------- fp32 inputs
+// The same walk on v_mfma_f32_16x16x4_f32, exact fp32 products, in chunks of
+// 32 tokens: the instruction has a sixteenth of the bf16 one's rate, so a
+// shorter chunk's smaller triangle of P saves more than its barriers cost.
+// Its operands are single elements, four of which follow one another in an
+// accumulator's rows, so rows of q and k are read 16 bytes at a time and
+// columns of k and v element by element.  9 prompts of 5 to 1000 tokens, 12
+// heads of 64, not split: 89 us, against 173 us of the kernel for any widths
+// in chunks of 64.
+constexpr int LA_C32 = 32;
+
+template <int DKP, bool LOCAL>
+struct ChunkLds32 {
+  static constexpr int kQ = LOCAL ? 0 : LA_C32 * DKP / 4, kK = LA_C32 * DKP / 4, kV = LA_C32 * 16;
+  static constexpr int kBuffer = kQ + kK + kV;
+  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + (LOCAL ? 0 : 3 * 64 + 4 * 128));
+};
+// Units of a row of W fp32 columns, exchanged like the bf16 ones.
+__device__ __forceinline__ int row_unit32(int row, int u) { return u ^ (row & 7); }
+template <int W>
+__device__ __forceinline__ f32x4_t row_frag32(const f32x4_t* s, int row, int u) {
+  return s[row * (W / 4) + row_unit32(row, u)];
+}
+template <int W>
+__device__ __forceinline__ float element32(const f32x4_t* s, int row, int c) {
+  return reinterpret_cast<const float*>(s + row * (W / 4) + row_unit32(row, c >> 2))[c & 3];
+}
+__device__ __forceinline__ f32x4_t mfma32(float a, float b, const f32x4_t& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+template <int DKP, int MODE, int LB>
+__global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || DKP == 128 ? 2 : 4) void linear_chunks_fp32_kernel(
+    LinearArgs a) {
+  constexpr bool LOCAL = MODE == LA_LOCAL;
+  using Lds = ChunkLds32<DKP, LOCAL>;
+  constexpr int WAVES = 4, ALL = LOCAL ? 4 : 8, DVT = 64, NB = DKP / 16;
+  constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;
+  extern __shared__ __attribute__((aligned(256))) f32x4_t s_f32[];
+  f32x4_t* sP = s_f32 + 2 * Lds::kBuffer;  // [tiles (1, 0), (1, 1), (0, 0) of queries and keys][64 lanes]
+  f32x4_t* sO = sP + 3 * 64;               // [column group][query tile][64 lanes]
+  const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool keeps_state = LOCAL || in_all >= WAVES;
+  const int wave = in_all % WAVES;  // of its group: its 16 columns
+  const int dv0 = blockIdx.x * DVT, head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const Span sp = span_of(a, blockIdx.z);
+  const float g = a.log_decay[head], g2 = g * kLog2e;
+  const size_t state0 = ((size_t)(MODE == LA_WHOLE ? sp.seq : sp.item) * a.heads + head) * a.dk * a.dv;
+  const float* state_in = MODE == LA_WHOLE ? a.state_in : LOCAL ? nullptr : a.seg_state;
+  float* state_out = MODE == LA_WHOLE ? a.state_out : LOCAL ? a.seg_state : nullptr;
+
+  auto issue = [&](int pos, int n, f32x4_t* buffer, int ln) {
+    const size_t tok = sp.tok + pos;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (LOADS % ALL != 0 && i * ALL + in_all >= LOADS) continue;
+      const int at = (i * ALL + in_all) * 64 / (16 / LB);  // first unit
+      constexpr int STEP = ALL * 64 / (16 / LB);
+      const bool even = Lds::kQ % STEP == 0 && Lds::kK % STEP == 0;
+      const int by = even ? i * STEP : at;
+      const bool is_q = by < Lds::kQ, is_k = !is_q && by < Lds::kQ + Lds::kK;
+      const int unit = at - (is_q ? 0 : is_k ? Lds::kQ : Lds::kQ + Lds::kK) + ln / (16 / LB);
+      const int units = is_q || is_k ? DKP / 4 : DVT / 4;
+      const int row = unit / units, c = 4 * row_unit32(row, unit % units) + ln % (16 / LB) * (LB / 4);
+      const size_t ld = is_q ? a.ld_q : is_k ? a.ld_k : a.ld_v;
+      const int width = is_q || is_k ? a.dk : a.dv - dv0;
+      const float* base = (is_q   ? static_cast<const float*>(a.q) + (size_t)head * a.dk
+                           : is_k ? static_cast<const float*>(a.k) + (size_t)kv_head * a.dk
+                                  : static_cast<const float*>(a.v) + (size_t)kv_head * a.dv + dv0) +
+                          tok * ld;
+      const void* src = row < n && c < width ? static_cast<const void*>(base + (__umul24(row, (uint32_t)ld) + c)) : g_nothing;
+      auto* dst = (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(buffer) + (i * ALL + in_all) * 64 * LB);
+      if constexpr (LB == 16)
+        __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+      else
+        __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0);
+    }
+  };
+
+  int n = min(LA_C32, sp.len);
+  if (n > 0) issue(0, n, s_f32, lane);
+  // S: rows 16 b + 4 quad + r, column dv0 + 16 wave + col.
+  f32x4_t S[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      S[b][r] = keeps_state && state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
+    }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(S[b]));  // these loads end here, see above
+  // The powers as above, of 32 tokens: 4 for the diagonal tiles and 4 for the
+  // other one, or 2 for the queries and, behind them, 8 for the tokens.
+  float pw[12], fs = 1.0f;
+  int n_left = -1;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int col = lane & 15, quad = lane >> 4;
+    pw[t] = LOCAL ? 0.0f : a.scale * decay_pow(g2, keeps_state ? 16 * (t & 1) + col + 1 : col - 4 * quad - t);
+    pw[4 + t] = LOCAL ? 0.0f : a.scale * decay_pow(g2, 16 + col - 4 * quad - t);
+    pw[8 + t] = 0.0f;
+  }
+  auto put = [&](int pos, int n, int ln) {
+    const int j = dv0 + 16 * wave + 4 * (ln >> 4);
+    float* base = static_cast<float*>(a.out) + (size_t)head * a.dv + (sp.tok + pos) * a.ld_out;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int i = 16 * t + (ln & 15);
+      if (i >= n || j >= a.dv) continue;
+      float* dst = base + (__umul24(i, (uint32_t)a.ld_out) + j);
+      if (j + 4 <= a.dv) {
+        *reinterpret_cast<f32x4_any_t*>(dst) = S[t];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (j + e < a.dv) dst[e] = S[t][e];
+      }
+    }
+  };
+
+  f32x4_t* buffer = s_f32;
+  for (int pos = 0, before = 0; pos < sp.len; pos += n, before = n) {
+    n = min(LA_C32, sp.len - pos);
+    int ln = lane;  // new for the compiler, as above
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int i = 0; i < 12; ++i) asm volatile("" : "+v"(pw[i]));
+    const int col = ln & 15, quad = ln >> 4;
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    __syncthreads();  // the chunk is there, and the one before is read
+    f32x4_t* other = buffer == s_f32 ? s_f32 + Lds::kBuffer : s_f32;
+    if (pos + n < sp.len) issue(pos + n, min(LA_C32, sp.len - pos - n), other, ln);
+    if constexpr (!LOCAL) {
+      if (before && !keeps_state) put(pos - before, before, ln);
+    }
+    const f32x4_t *sQ = buffer, *sK = buffer + Lds::kQ, *sV = sK + Lds::kK;
+    buffer = other;
+
+    if (!LOCAL && !keeps_state) {
+      if (wave < 3) {  // P^T = scale (k q^T) lambda^(i-j), j <= i, one tile each
+        const int qt = wave < 2, kt = wave == 1;
+        f32x4_t p = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const f32x4_t kf = row_frag32<DKP>(sK, 16 * kt + col, 4 * b + quad);
+          const f32x4_t qf = row_frag32<DKP>(sQ, 16 * qt + col, 4 * b + quad);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p = mfma32(kf[r], qf[r], p);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = wave == 0 ? p[r] * pw[4 + r] : col >= 4 * quad + r ? p[r] * pw[r] : 0.0f;
+        sP[wave * 64 + ln] = p;
+      }
+    } else if (!LOCAL) {
+      // (q S)^T, each query's column times scale lambda^(i+1).
+      f32x4_t o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        f32x4_t qf[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) qf[t] = row_frag32<DKP>(sQ, 16 * t + col, 4 * b + quad);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) o[t] = mfma32(S[b][r], qf[t][r], o[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sO[(2 * wave + t) * 64 + ln] = o[t] * pw[t];
+    }
+    if constexpr (!LOCAL) {
+      asm volatile("" ::: "memory");  // as above: no wait for the next chunk's loads
+      __builtin_amdgcn_s_waitcnt(kLdsOnly);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+
+    float v[2][4];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[kt][r] = element32<DVT>(sV, 16 * kt + 4 * quad + r, 16 * wave + col);
+    if (!LOCAL && !keeps_state) {
+      // + (P v)^T; values that are not finite one by one, as above.
+      bool odd = false;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd |= !(fabsf(v[kt][r]) < INFINITY);
+      if (__any(odd)) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(fabsf(v[kt][r]) < INFINITY)) v[kt][r] = 0.0f;
+#pragma unroll 1
+        for (int j = 0; j < LA_C32; ++j) {
+          const f32x4_t v4 = sV[j * (DVT / 4) + row_unit32(j, 4 * wave + quad)];
+#pragma unroll 1
+          for (int t = j >> 4; t < 2; ++t) {
+            const int tile = t == 0 ? 2 : j >> 4;
+            const float p = reinterpret_cast<const float*>(&sP[tile * 64 + 16 * ((j & 15) >> 2) + col])[j & 3];
+            f32x4_t& o = sO[(2 * wave + t) * 64 + ln];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * t + col >= j && !(fabsf(v4[r]) < INFINITY)) o[r] += p * v4[r];
+          }
+        }
+      }
+      f32x4_t o[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) o[t] = sO[(2 * wave + t) * 64 + ln];
+      const f32x4_t p10 = sP[ln], p11 = sP[64 + ln], p00 = sP[128 + ln];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        o[0] = mfma32(v[0][r], p00[r], o[0]);
+        o[1] = mfma32(v[0][r], p10[r], o[1]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[1] = mfma32(v[1][r], p11[r], o[1]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) S[t] = o[t];
+    } else {
+      // S = lambda^n S + k^T (lambda^(n-1-j) v).
+      if (n != n_left) {
+        n_left = n;
+        fs = decay_pow_exact(g, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pw[4 + e] = decay_pow(g2, n - 1 - (16 * (e >> 2) + 4 * quad + (e & 3)));
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) S[b] *= fs;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = v[kt][r] * pw[4 + 4 * kt + r];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            S[b] = mfma32(element32<DKP>(sK, 16 * kt + 4 * quad + r, 16 * b + col), w, S[b]);
+        }
+    }
+  }
+  if constexpr (!LOCAL) {
+    if (sp.len > 0 && !keeps_state) put(sp.len - n, n, lane);
+  }
+  if (!state_out || !keeps_state) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -749,11 +1044,18 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a, size_t s
   const float g = a.log_decay[at / state], full = decay_pow_exact(g, a.seg_len);
   const size_t step = state * a.heads;
   float s = a.state_in ? a.state_in[seq * step + at] : 0.0f;
-  for (int i = item0; i < item1; ++i) {
-    const float own = a.seg_state[i * step + at];
-    a.seg_state[i * step + at] = s;
-    const int n = len - (i - item0) * a.seg_len;
-    s = fmaf(n >= a.seg_len ? full : decay_pow_exact(g, n), s, own);
+  constexpr int AHEAD = 8;  // segments whose loads are in flight together
+  for (int i0 = item0; i0 < item1; i0 += AHEAD) {
+    float own[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) own[j] = a.seg_state[min(i0 + j, item1 - 1) * step + at];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (i0 + j >= item1) continue;
+      a.seg_state[(i0 + j) * step + at] = s;
+      const int n = len - (i0 + j - item0) * a.seg_len;
+      s = fmaf(n >= a.seg_len ? full : decay_pow_exact(g, n), s, own[j]);
+    }
   }
   if (a.state_out) a.state_out[seq * step + at] = s;
 }
@@ -847,24 +1149,31 @@ Status launch_steps(hipStream_t stream, const LinearArgs& a) {
   return Status::Ok();
 }
 
-// The kernel of a call: the bf16 kernel with loads of LB bytes, or (0) the
-// fp32 products, which take any width and alignment.
+// The kernel of a call and the value columns of its workgroups: loads of LB
+// bytes, or (0) the one that takes any width and alignment.
 template <class T, int DKP, int NC, int MODE, int LB>
 struct Chunks {
   static constexpr size_t kLds = (size_t)(2 * LA_C * (DKP + 4) + LA_C * (64 * NC + 4) + LA_C * 68) * 4;
-  static constexpr int kThreads = 256;
-  static constexpr auto kKernel = &linear_chunks_f32_kernel<T, DKP, NC, MODE>;
+  static constexpr int kThreads = 256, kColumns = 64 * NC;
+  static constexpr auto kKernel = &linear_chunks_any_kernel<T, DKP, NC, MODE>;
 };
 template <int DKP, int NC, int MODE, int LB>
 struct ChunksBf16 {
-  static constexpr size_t kLds = ChunkLds<DKP, 4 * NC, MODE == LA_LOCAL>::kBytes;
-  static constexpr int kThreads = 256 * NC;
-  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4 * NC, MODE, LB>;
+  static constexpr int kGroups = MODE == LA_LOCAL ? NC : 1;
+  static constexpr size_t kLds = ChunkLds<DKP, 4 * kGroups, MODE == LA_LOCAL>::kBytes;
+  static constexpr int kThreads = MODE == LA_LOCAL ? 256 * NC : 512, kColumns = 64 * kGroups;
+  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4 * kGroups, MODE, LB>;
 };
 template <int DKP, int NC, int MODE>
 struct Chunks<Bf16, DKP, NC, MODE, 16> : ChunksBf16<DKP, NC, MODE, 16> {};
 template <int DKP, int NC, int MODE>
 struct Chunks<Bf16, DKP, NC, MODE, 4> : ChunksBf16<DKP, NC, MODE, 4> {};
+template <int DKP, int NC, int MODE, int LB>
+struct Chunks<float, DKP, NC, MODE, LB> {
+  static constexpr size_t kLds = ChunkLds32<DKP, MODE == LA_LOCAL>::kBytes;
+  static constexpr int kThreads = MODE == LA_LOCAL ? 256 : 512, kColumns = 64;
+  static constexpr auto kKernel = &linear_chunks_fp32_kernel<DKP, MODE, LB>;
+};
 
 // Calls f with the kernel for a call's type, head widths and loads.
 template <int MODE, class F>
@@ -874,29 +1183,31 @@ Status with_chunks(int dtype, int dk, int dv, int load, F f) {
     constexpr int LB = decltype(lb)::value;
     auto wide = [&](auto dkp) {
       constexpr int D = decltype(dkp)::value;
-      return dv > 64 ? f(Chunks<T, D, 2, MODE, LB>{}, 2) : f(Chunks<T, D, 1, MODE, LB>{}, 1);
+      return dv > 64 ? f(Chunks<T, D, 2, MODE, LB>{}) : f(Chunks<T, D, 1, MODE, LB>{});
     };
     if (dk <= 32) return wide(std::integral_constant<int, 32>{});
     if (dk <= 64) return wide(std::integral_constant<int, 64>{});
     return wide(std::integral_constant<int, 128>{});
   };
-  if (dtype == PSSA_HIP_F32) return typed(0.0f, std::integral_constant<int, 0>{});
-  if (load == 16) return typed(Bf16{}, std::integral_constant<int, 16>{});
-  if (load == 4) return typed(Bf16{}, std::integral_constant<int, 4>{});
+  const std::integral_constant<int, 16> wide_loads;
+  const std::integral_constant<int, 4> short_loads;
+  if (dtype == PSSA_HIP_F32) return load == 16 ? typed(0.0f, wide_loads) : typed(0.0f, short_loads);
+  if (load == 16) return typed(Bf16{}, wide_loads);
+  if (load == 4) return typed(Bf16{}, short_loads);
   return typed(Bf16{}, std::integral_constant<int, 0>{});
 }
 
 // The largest load that every row's and head's start is aligned to.
-int load_bytes(const LinearArgs& a) {
+int load_bytes(int dtype, const LinearArgs& a) {
   const size_t all = (size_t)a.q | (size_t)a.k | (size_t)a.v |
-                     2 * (a.ld_q | a.ld_k | a.ld_v | (size_t)a.dk | (size_t)a.dv);
+                     (dtype == PSSA_HIP_F32 ? 4 : 2) * (a.ld_q | a.ld_k | a.ld_v | (size_t)a.dk | (size_t)a.dv);
   return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 0;
 }
 
 template <int MODE>
 Status launch_chunks(hipStream_t stream, int dtype, const LinearArgs& a) {
-  return with_chunks<MODE>(dtype, a.dk, a.dv, load_bytes(a), [&](auto c, int nc) -> Status {
-    const dim3 grid((a.dv + 64 * nc - 1) / (64 * nc), a.heads, a.items);
+  return with_chunks<MODE>(dtype, a.dk, a.dv, load_bytes(dtype, a), [&](auto c) -> Status {
+    const dim3 grid((a.dv + c.kColumns - 1) / c.kColumns, a.heads, a.items);
     c.kKernel<<<grid, c.kThreads, c.kLds, stream>>>(a);
     PSSA_LAUNCH_CHECK("linear_chunks_kernel");
     return Status::Ok();
@@ -909,7 +1220,7 @@ Status chunks_attributes() {
     for (int dk : {32, 64, 128})
       for (int dv : {64, 128})
         for (int load : {16, 4, 0})
-          PSSA_RETURN_IF(with_chunks<MODE>(dtype, dk, dv, load, [&](auto c, int) -> Status {
+          PSSA_RETURN_IF(with_chunks<MODE>(dtype, dk, dv, load, [&](auto c) -> Status {
             PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(c.kKernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)c.kLds));
             return Status::Ok();
@@ -925,16 +1236,32 @@ Status init_linear_attributes() {
   return chunks_attributes<LA_SEGMENT>();
 }
 
-int linear_segment(size_t n_seqs, size_t longest, size_t tokens, size_t heads, size_t d_val) {
-  if (longest <= (size_t)kLinearSteps) return 0;
-  const size_t tiles = heads * ((d_val + 127) / 128);
-  const size_t blocks = n_seqs * tiles;
-  (void)tokens;
-  if (blocks >= 256 || longest < 512) return 0;
-  // Segments of whole chunks, about one workgroup for each compute unit.
-  const size_t segs = (256 + blocks - 1) / blocks;
-  const size_t len = std::max<size_t>(256, (longest + segs - 1) / segs);
-  return (int)((len + LA_C - 1) / LA_C * LA_C);
+// A walk is the way of a sequence, a head and 64 value columns through the
+// tokens, on a compute unit of its own.  A call is split into the shortest
+// segments that still leave each of them a compute unit.  A split walk's chunk
+// costs twice one of a whole walk, as its state is computed twice, and the
+// passes between take about 12 us, 5 chunks of bf16 heads of 64:
+//                                              whole      split
+//   8192 bf16 tokens, 8 heads of 128            366 us   58 us (segments of 512)
+//   9 fp32 prompts of 5..1000, 12 heads of 64  89.3 us   49 us (of 256)
+//   16 bf16 prompts of 1024, 12 heads of 64      39 us   not split
+// Twice as many segments as compute units took 60 us and 45 us.
+constexpr size_t kComputeUnits = 256;
+int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_val) {
+  const size_t chunks = (longest + LA_C - 1) / LA_C, lanes = heads * ((d_val + 63) / 64);
+  if (n_seqs * lanes > kComputeUnits) return 0;
+  auto fits = [&](size_t c) {
+    size_t items = 0;
+    for (size_t i = 0; i < n_seqs; ++i)
+      items += lens ? std::max<size_t>(1, (lens[i] + c * LA_C - 1) / (c * LA_C)) : (longest + c * LA_C - 1) / (c * LA_C);
+    return items * lanes <= kComputeUnits;
+  };
+  size_t lo = 1, hi = chunks;  // the fewest chunks of a segment that fit; all of them do
+  while (lo < hi) {
+    const size_t mid = (lo + hi) / 2;
+    if (fits(mid)) hi = mid; else lo = mid + 1;
+  }
+  return 2 * lo + 5 <= chunks ? (int)(lo * LA_C) : 0;
 }
 
 Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int longest) {
