@@ -16,6 +16,7 @@
 // as three bf16 parts (8 + 8 + 8 bits, together exact), each a column of its
 // own: the products are exact in fp32 whatever the type.
 #include <algorithm>
+#include <type_traits>
 
 #include "operators.h"
 
@@ -27,6 +28,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef u32x2_t u32x2_any_t __attribute__((aligned(1)));
 
 // The 8 codes of a word as bf16 odd integers: 1, 3 .. 15 by the low three
 // bits, the sign in the fourth; codes 0..3 in the low nibbles, 4..7 above.
@@ -41,23 +44,36 @@ __device__ __forceinline__ bf16x8_t w4_operand(uint32_t w) {
   return __builtin_bit_cast(bf16x8_t, v);
 }
 
-// Codes [n, k], one byte each, into the tiles.
+// Four codes as held: |2 q - 15| / 2 in the low three bits (q ^ 15 below 8,
+// q ^ 8 from there), the sign in the fourth.
+__device__ __forceinline__ uint32_t held4(uint32_t q) {
+  q &= 0x0F0F0F0Fu;
+  return q ^ 0x08080808u ^ (((q >> 3 & 0x01010101u) ^ 0x01010101u) * 7u);
+}
+// Codes [n, k], one byte each, into the tiles: 8 codes to a load.  134 million
+// of them (16384 x 8192) take 36 us, 5.6 TB/s; byte by byte they took 250.
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict__ codes, int n, int k, int kblocks,
                                                       size_t pieces, u32x4_t* __restrict__ out) {
   const size_t piece = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (piece >= pieces) return;
   const int lane = (int)(piece & 63), kb = (int)((piece >> 6) % kblocks);
   const size_t row = (piece >> 6) / kblocks * 16 + (lane & 15);
-  u32x4_t v = {0, 0, 0, 0};
+  u32x4_t v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    const int col = 128 * kb + 32 * j + 8 * (lane >> 4);
+    const uint8_t* src = codes + row * k + col;
+    uint32_t q[2] = {0x08080808u, 0x08080808u};
+    if (row < (size_t)n && col + 8 <= k) {
+      const u32x2_any_t u = *reinterpret_cast<const u32x2_any_t*>(src);
+      q[0] = u[0];
+      q[1] = u[1];
+    } else if (row < (size_t)n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int col = 128 * kb + 32 * j + 8 * (lane >> 4) + i;
-      const uint32_t q = row < (size_t)n && col < k ? codes[row * k + col] & 15u : 8u;
-      const uint32_t held = q >= 8 ? q - 8 : 15 - q;  // magnitude |2q - 15| / 2, and 8 for its sign
-      v[j] |= held << (i < 4 ? 8 * i : 8 * (i - 4) + 4);
+      for (int i = 0; i < 8; ++i)
+        if (col + i < k) q[i >> 2] = (q[i >> 2] & ~(0xFFu << 8 * (i & 3))) | (uint32_t)src[i] << 8 * (i & 3);
     }
+    v[j] = held4(q[0]) | held4(q[1]) << 4;
   }
   out[piece] = v;
 }
@@ -125,6 +141,8 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
     for (int c = 0; c < CT; ++c) total[t][c] = f32x4_t{0, 0, 0, 0};
 
   // What one block of 128 columns needs from memory, fetched one block ahead.
+  // WHOLE: every column is there, and the loads are the same in every block:
+  // behind a load that may not have been made the compiler waits for all.
   struct Block {
     u32x4_t w[NT];
     f32x4_t s[NT][NG];
@@ -132,7 +150,9 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
     u32x4_t xh[F32 ? 1 : 4][F32 ? 1 : CT];
     f32x4_t xf[F32 ? PIECES : 1][2];
   };
-  auto fetch = [&](Block& b, int kb) {
+  const uint8_t* zeros = a.zeros ? a.zeros : reinterpret_cast<const uint8_t*>(a.scales);  // loaded, then not used
+  auto fetch = [&](Block& b, int kb, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const size_t tile = min(tile0 + t, a.tiles - 1);
@@ -141,7 +161,7 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
       for (int g = 0; g < NG; ++g) {
         const size_t at = ((tile * a.kblocks + kb) * NG + g) * 16 + 4 * quad;
         b.s[t][g] = *reinterpret_cast<const f32x4_t*>(a.scales + at);
-        if (a.zeros) b.z[t][g] = *reinterpret_cast<const uint32_t*>(a.zeros + at);
+        b.z[t][g] = *reinterpret_cast<const uint32_t*>(zeros + at);
       }
     }
     if constexpr (F32) {
@@ -149,7 +169,7 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
       for (int q = 0; q < PIECES; ++q) {
         const int piece = min(lane + 64 * q, rows * 16 - 1), r = piece >> 4, c = 128 * kb + 8 * (piece & 15);
         const float* src = static_cast<const float*>(a.x) + (size_t)(row0 + r) * a.ld_x + c;
-        if (c + 8 <= a.k) {
+        if (WHOLE || c + 8 <= a.k) {
           b.xf[q][0] = *reinterpret_cast<const f32x4_any_t*>(src);
           b.xf[q][1] = *reinterpret_cast<const f32x4_any_t*>(src + 4);
         } else {
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
           const int c = 128 * kb + 32 * j + 8 * quad;
           const uint16_t* src =
               static_cast<const uint16_t*>(a.x) + (size_t)(row0 + min(16 * ct + col, rows - 1)) * a.ld_x + c;
-          if (c + 8 <= a.k) {
+          if (WHOLE || c + 8 <= a.k) {
             b.xh[j][ct] = *reinterpret_cast<const u32x4_any_t*>(src);
           } else {
 #pragma unroll
@@ -237,12 +257,18 @@ __global__ __launch_bounds__(512) void matvec_w4_kernel(MatvecArgs a) {
         }
     }
   };
-  Block cur, next;
-  if (kb0 < kb1) fetch(cur, kb0);
-  for (int kb = kb0; kb < kb1; ++kb) {
-    if (kb + 1 < kb1) fetch(next, kb + 1);
+  const int kb_whole = min(kb1, a.k / 128);
+  Block cur;
+  if (kb0 < kb_whole) fetch(cur, kb0, std::true_type{});
+  for (int kb = kb0; kb < kb_whole; ++kb) {
+    Block next;
+    fetch(next, min(kb + 1, kb_whole - 1), std::true_type{});
     compute(cur);
     cur = next;
+  }
+  if (max(kb0, kb_whole) < kb1) {  // the last block, of fewer columns
+    fetch(cur, kb1 - 1, std::false_type{});
+    compute(cur);
   }
 
   // The waves' and the parts' sums, in order.
@@ -282,32 +308,46 @@ Status launch_group(hipStream_t stream, const MatvecArgs& a, int group, int wave
   return launch_one<F32, CT, NT, 128>(stream, a, waves);
 }
 
-template <bool F32>
+template <bool F32, int NT>
 Status launch_columns(hipStream_t stream, const MatvecArgs& a, int group, int waves) {
   const int cols = F32 ? 3 * a.m : a.m;
-  if (cols <= 16) return launch_group<F32, 1, 1>(stream, a, group, waves);
+  if (cols <= 16) return launch_group<F32, 1, NT>(stream, a, group, waves);
   if constexpr (F32)
-    if (cols > 32) return launch_group<F32, 3, 1>(stream, a, group, waves);
-  return launch_group<F32, 2, 1>(stream, a, group, waves);
+    if (cols > 32) return launch_group<F32, 3, NT>(stream, a, group, waves);
+  return launch_group<F32, 2, NT>(stream, a, group, waves);
 }
 
-// Waves that split k: enough for a few thousand in all, a block of 128 for each.
-int split_waves(int tiles, int kblocks) {
+// Waves that split k: enough for some thousands in all, a block of 128 for each.
+int split_waves(int workgroups, int most, int kblocks) {
   int w = 1;
-  while (w < 8 && w * tiles < 4096 && w * 2 <= kblocks) w *= 2;
+  while (w < 8 && w * workgroups < most && w * 2 <= kblocks) w *= 2;
   return w;
 }
 
 }  // namespace
 
-// Fp32 rows of three column tiles stage up to 96 KB.
-Status init_w4_attributes() {
-  const void* k[] = {reinterpret_cast<const void*>(&matvec_w4_kernel<true, 3, 1, 32>),
-                     reinterpret_cast<const void*>(&matvec_w4_kernel<true, 3, 1, 64>),
-                     reinterpret_cast<const void*>(&matvec_w4_kernel<true, 3, 1, 128>)};
-  for (const void* f : k)
-    PSSA_HIP_TRY(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 16 * 48 * 16));
+namespace {
+// Fp32 rows of two or three column tiles stage up to 96 KB.
+template <int CT, int NT, int GROUP>
+Status big_lds() {
+  PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&matvec_w4_kernel<true, CT, NT, GROUP>),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 16 * 48 * 16));
   return Status::Ok();
+}
+template <int NT, int GROUP>
+Status big_lds() {
+  PSSA_RETURN_IF((big_lds<2, NT, GROUP>()));
+  return big_lds<3, NT, GROUP>();
+}
+}  // namespace
+
+Status init_w4_attributes() {
+  PSSA_RETURN_IF((big_lds<1, 32>()));
+  PSSA_RETURN_IF((big_lds<1, 64>()));
+  PSSA_RETURN_IF((big_lds<1, 128>()));
+  PSSA_RETURN_IF((big_lds<2, 32>()));
+  PSSA_RETURN_IF((big_lds<2, 64>()));
+  return big_lds<2, 128>();
 }
 
 size_t w4_packed_bytes(size_t n, size_t k) { return (n + 15) / 16 * ((k + 127) / 128) * 1024; }
@@ -341,9 +381,13 @@ Status launch_matvec_w4(hipStream_t stream, int x_dtype, const void* x, size_t l
   a.k = w.k;
   a.kblocks = (w.k + 127) / 128;
   a.tiles = (w.n + 15) / 16;
-  const int waves = split_waves(a.tiles, a.kblocks);
-  return x_dtype == PSSA_HIP_F32 ? launch_columns<true>(stream, a, w.group, waves)
-                                 : launch_columns<false>(stream, a, w.group, waves);
+  // fp32 rows are split into their parts once for NT tiles: 7 of them with
+  // 16384 x 8192 weights took 35.7, 29.2 and 27.8 us at NT 1, 2 and 4, of
+  // which the last spills with smaller groups.  bf16 rows come as they are:
+  // one of them with 16384 x 768 took 4.8 us at NT 1 and 2.
+  if (x_dtype != PSSA_HIP_F32) return launch_columns<false, 1>(stream, a, w.group, split_waves(a.tiles, 4096, a.kblocks));
+  if (a.tiles < 512) return launch_columns<true, 1>(stream, a, w.group, split_waves(a.tiles, 4096, a.kblocks));
+  return launch_columns<true, 2>(stream, a, w.group, split_waves((a.tiles + 1) / 2, 2048, a.kblocks));
 }
 
 }  // namespace pssa

@@ -468,7 +468,8 @@ def w4_tolerance(x, codes, scales, zp, group):
     (1, 1, 1, 32, False), (1, 16, 128, 32, True), (2, 17, 129, 64, False), (1, 100, 768, 64, False),
     (5, 33, 100, 32, True), (6, 48, 300, 128, True), (10, 64, 257, 64, True), (11, 20, 500, 32, False),
     (16, 31, 640, 128, False), (17, 40, 333, 32, True), (33, 70, 1030, 64, True), (3, 5000, 96, 32, True),
-    (1, 40, 8192, 128, True), (4, 70000, 130, 64, False), (70, 24, 128, 128, True)])
+    (1, 40, 8192, 128, True), (4, 70000, 130, 64, False), (70, 24, 128, 128, True), (9, 8195, 700, 64, True),
+    (11, 8209, 130, 32, False), (6, 8177, 260, 128, True)])
 def test_matvec_w4_matches_64_bits(hip, dtype, m, n, k, group, zeros):
     say(f"w4 {m} x {n} x {k} group {group} {dtype} zeros {zeros}")
     rng = np.random.default_rng(n + k)
