@@ -1,11 +1,11 @@
 // Operators over logit rows: log probabilities of given tokens with entropy
 // and top alternatives, and distillation from a teacher's top logits.
 //
-// Both are one pass of a row through the registers of one workgroup: the
-// loads of a whole row are issued at once, its maximum and its sums are
-// reductions over registers, and what needs the finished sums (the gradient,
-// the alternatives) is computed from the registers again.  Rows past the
-// registers go tile by tile, the statistics merged after each tile.
+// Both pass a row through the registers of one workgroup, tile by tile.  Log
+// probabilities take one pass: a maximum that rises rescales each thread's
+// sums, and tokens that may be among the largest are put aside in LDS.
+// Distillation writes its gradient from the registers that the sums were taken
+// from, or reads a row past them twice.
 #include "operators.h"
 
 namespace pssa {
@@ -19,6 +19,7 @@ typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLowest = -3.0e38f;  // stands for differences that overflow: exp of it is 0, products with 0 stay 0
 constexpr uint32_t kNoToken = PSSA_HIP_NO_TOKEN;
+constexpr size_t kComputeUnits = 256;
 
 struct Bf16 {
   uint16_t bits;
@@ -208,137 +209,195 @@ __device__ __forceinline__ Key wave_merge(Key a, Key b_reversed, int lane) {
 // row's values consist of.
 //
 // Alternatives: the k-th largest of the maxima of some groups of threads (64
-// groups, or every thread for itself where k is large) bounds the row's k-th
-// largest token from below.  The tokens that reach the bound, hardly more
-// than k of them, pass through LDS to one wave that sorts them by value and
-// id.  A row where they are too many (all logits equal, say) takes its
-// tokens one by one, each round the largest behind the one before.
+// groups, or every thread for itself where k is large) bounds the first
+// tile's k-th largest token from below, and with it the row's.  The tokens
+// that pass the bound, hardly more than k of a tile, gather in LDS until one
+// wave sorts them by value and id, at the end or where they are many, which
+// raises the bound.  A tile where they are too many for that (all logits
+// equal, say) gives its k tokens one by one, each round the largest behind
+// the one before.
+//
+// 8192 fp32 rows of 16384: 129 us (4.2 TB/s); 509 bf16 rows of 100003 with 20
+// alternatives: 40 us (2.5 TB/s); one row of 16384: 9 us, mostly latency.
 constexpr int kCandidates = 1024;
+constexpr int kSlots = 8;  // threads of a wave whose vectors are looked through at once
 
-template <class T, int W, int NV>
+// MANY: the row takes several tiles, each loaded while the one before is summed.
+template <class T, int W, int NV, bool MANY>
 __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int N = vec_n<T>(), TILE = 64 * W * NV;
   __shared__ uint32_t s_keys[W * 64];
   __shared__ uint64_t s_round[W];
-  __shared__ float s_sum[2 * W];
-  __shared__ uint32_t s_bound, s_kth;
-  __shared__ int s_count, s_owner;
+  __shared__ float s_max[2][W], s_sum[2 * W];
+  __shared__ int s_owner[2], s_count;
+  __shared__ u32x4_t s_hit[W][kSlots][NV];
+  __shared__ int s_hit_lane[W][kSlots];
+  __shared__ uint32_t s_kth;
   extern __shared__ uint64_t s_cand[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab, top = a.top_k;
   const T* row = static_cast<const T*>(a.logits) + (size_t)blockIdx.x * a.ld;
   const float inv_tau = 1.0f / a.temperature, c2 = kLog2e * inv_tau;
   const uint32_t target = a.targets ? a.targets[blockIdx.x] : kNoToken;
   const float z_target = target < (uint32_t)V ? load1<T>(row + target) : 0.0f;
+  if (tid == 0) {
+    s_count = 0;
+    s_owner[0] = s_owner[1] = 64 * W;
+    s_kth = 0;
+  }
 
-  float m = -INFINITY, S = 0.0f, Tq = 0.0f;
-  uint64_t best = 0;  // wave 0: the largest keys so far, descending
+  float m = -INFINITY, S = 0.0f, Tq = 0.0f;  // the maximum so far; this thread's sums
+  uint64_t best = 0;                         // wave 0: the largest keys so far, descending
   const int vecs = (V + N - 1) / N;
-  for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
-    u32x4_t u[NV];
-    tile_load<T, W, NV>(u, row, V, tile0);
+  // What s_cand has gathered, n of them, into `best`; where the tile that
+  // began behind the first n_before had too many, its tokens from the row.
+  auto settle = [&](int n, int n_before, int tile0) {
+    uint64_t list = 0;
+    if (n > kCandidates) {
+      uint64_t last = ~(uint64_t)0;
+      for (int i = 0; i < top; ++i) {
+        uint64_t mine = 0;
+        for (int e = tile0 * N + tid; e < min(V, (tile0 + TILE) * N); e += 64 * W) {  // from the cache: rare
+          const float v = load1<T>(row + e);
+          const uint64_t key = v > -INFINITY ? token_key(v, e) : 0;
+          if (key < last && key > mine) mine = key;
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) mine = key_step(mine, off, true);
+        if (lane == 0) s_round[wave] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) mine = s_round[w] > mine ? s_round[w] : mine;
+        __syncthreads();
+        last = mine;
+        if (lane == i) list = mine;
+        if (!mine) break;  // uniform
+      }
+      n = n_before;
+    }
+    if (wave == 0) {
+      best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
+#pragma unroll 1
+      for (int c = 0; c < n; c += 64) {
+        const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : (uint64_t)0, lane);
+        best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
+      }
+      if (lane == top - 1) s_kth = (uint32_t)(best >> 32);
+      if (lane == 0) s_count = 0;
+    }
+    __syncthreads();
+  };
+  int gathered = 0;  // before the tile
+  u32x4_t u[NV], ahead[MANY ? NV : 1];
+  tile_load<T, W, NV>(u, row, V, 0);
+  for (int tile0 = 0, p = 0; tile0 < vecs; tile0 += TILE, p ^= 1) {
+    tile_again(u);  // its loads end here
+    if constexpr (MANY) {
+      if (tile0 + TILE < vecs) tile_load<T, W, NV>(ahead, row, V, tile0 + TILE);
+    }
     const float bv = tile_max<T, NV>(u);
     tile_again(u);
-    // The groups' maxima, the tile's, and the bound.
-    float mt;
-    {
-      const bool fine = top > 24;  // every thread a group
-      float gm = bv;
-      if (!fine) {
+    float mt = wave_max(bv);
+    if (lane == 0) s_max[p][wave] = mt;
+    __syncthreads();
 #pragma unroll
-        for (int off = 1; off < W; off <<= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
-      }
-      uint32_t key = value_key(gm);
-      if constexpr (W > 1) {
-        if (fine) {
-          key = wave_sort(key, lane);
-          s_keys[tid] = key;
-        } else if (lane % W == 0) {
-          s_keys[tid / W] = key;
-        }
-      }
-      if (tid == 0) {
-        s_count = 0;
-        s_owner = 64 * W;
-      }
-      __syncthreads();
-      if constexpr (W > 1) {
-        if (fine) {
-#pragma unroll
-          for (int half = W / 2; half >= 1; half >>= 1) {
-            if (wave < half) {
-              key = wave_merge(key, s_keys[(wave + half) * 64 + 63 - lane], lane);
-              s_keys[tid] = key;
-            }
-            __syncthreads();
-          }
-        }
-      }
-      if (wave == 0) {
-        if (W == 1 || !fine) key = wave_sort(W == 1 ? key : s_keys[lane], lane);
-        if (lane == 0) s_bound = key;
-        if (top && lane == top - 1) s_kth = max(key, (uint32_t)(best >> 32));
-      }
-      __syncthreads();
-      mt = key_value((uint64_t)s_bound << 32);
-    }
-    const bool some = mt > -INFINITY;
-    if (bv == mt && some) atomicMin(&s_owner, tid);  // this thread's first maximum is left out of the sums
+    for (int w = 0; w < W; ++w) mt = fmaxf(mt, s_max[p][w]);
+    if (tid == 0) s_owner[p ^ 1] = 64 * W;
+    const bool rises = mt > m;
+    if (rises && bv == mt) atomicMin(&s_owner[p], tid);  // this thread's first maximum is left out of the sums
+    const int n = s_count;
+    uint32_t kth = s_kth;
+    if (top || rises) __syncthreads();  // uniform
     if (top) {
-      const float bound = key_value((uint64_t)s_kth << 32);
-      if (bv >= bound) {
+      if (MANY && n > kCandidates / 2) {
+        settle(n, gathered, tile0 - TILE);
+        kth = s_kth;
+        gathered = 0;
+        __syncthreads();
+      } else {
+        gathered = n;
+      }
+      const bool ties = kth <= value_key(-INFINITY);  // no bound yet; what equals the tile's own may be among the largest
+      if (ties) {
+        const bool fine = top > 24;  // every thread a group
+        float gm = bv;
+        if (!fine) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+          for (int off = 1; off < W; off <<= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
+        }
+        uint32_t key = value_key(gm);
+        if constexpr (W > 1) {
+          if (fine) {
+            key = wave_sort(key, lane);
+            s_keys[tid] = key;
+          } else if (lane % W == 0) {
+            s_keys[tid / W] = key;
+          }
+          __syncthreads();
+          if (fine) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float v = elem<T>(u[k], j);
-            if (v >= bound && v > -INFINITY) {
-              const int at = atomicAdd(&s_count, 1);
-              if (at < kCandidates) s_cand[at] = token_key(v, vec_start<T>(V, tile0 + k * 64 * W + tid) + j);
+            for (int half = W / 2; half >= 1; half >>= 1) {
+              if (wave < half) {
+                key = wave_merge(key, s_keys[(wave + half) * 64 + 63 - lane], lane);
+                s_keys[tid] = key;
+              }
+              __syncthreads();
             }
           }
+        }
+        if (wave == 0) {
+          if (W == 1 || !fine) key = wave_sort(W == 1 ? key : s_keys[lane], lane);
+          if (lane == top - 1) s_kth = key;
+        }
+        __syncthreads();
+        kth = s_kth;
+      }
+      const float bound = key_value((uint64_t)kth << 32);
+      // Threads with such a token hand their vectors over to their wave, a
+      // token for each lane: looked for by the threads themselves, one of 32
+      // here and there would keep the wave as long as the sums do.
+      bool hit = ties ? bv >= bound : bv > bound;
+      for (uint64_t hits = __ballot(hit); hits;) {  // uniform in the wave
+        const int rank = __popcll(hits & (((uint64_t)1 << lane) - 1));
+        const bool now = hit && rank < kSlots;
+        if (now) {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) s_hit[wave][rank][k] = u[k];
+          s_hit_lane[wave][rank] = lane;
+        }
+        wave_sync();
+        const uint64_t done = __ballot(now);
+        const int held = __popcll(done) * NV * N;
+        hits &= ~done;
+        hit = hit && !now;
+        for (int c = 0; c < held; c += 64) {
+          const int at = min(c + lane, held - 1), slot = at / (NV * N), k = at / N % NV, j = at % N;
+          const float v = load1<T>(reinterpret_cast<const T*>(&s_hit[wave][slot][k]) + j);
+          const bool take = c + lane < held && (ties ? v >= bound : v > bound) && v > -INFINITY;
+          const uint64_t taken = __ballot(take);
+          int first = 0;
+          if (lane == 0 && taken) first = atomicAdd(&s_count, __popcll(taken));
+          first = __builtin_amdgcn_readfirstlane(first) + __popcll(taken & (((uint64_t)1 << lane) - 1));
+          if (take && first < kCandidates)
+            s_cand[first] = token_key(v, vec_start<T>(V, tile0 + (k * W + wave) * 64 + s_hit_lane[wave][slot]) + j);
+        }
+        wave_sync();
       }
       tile_again(u);
     }
-    __syncthreads();
-    if (top) {
-      const int n = s_count;
-      if (n <= kCandidates) {
-        if (wave == 0) {
-          for (int c = 0; c < n; c += 64) {
-            const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : (uint64_t)0, lane);
-            best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
-          }
-        }
-      } else {
-        uint64_t last = ~(uint64_t)0, list = 0;
-        for (int i = 0; i < top; ++i) {
-          uint64_t mine = 0;
-          for (int e = tile0 * N + tid; e < min(V, (tile0 + TILE) * N); e += 64 * W) {  // from the cache: rare
-            const float v = load1<T>(row + e);
-            const uint64_t key = v > -INFINITY ? token_key(v, e) : 0;
-            if (key < last && key > mine) mine = key;
-          }
-#pragma unroll
-          for (int off = 32; off >= 1; off >>= 1) mine = key_step(mine, off, true);
-          if (lane == 0) s_round[wave] = mine;
-          __syncthreads();
-#pragma unroll
-          for (int w = 0; w < W; ++w) mine = s_round[w] > mine ? s_round[w] : mine;
-          __syncthreads();
-          last = mine;
-          if (lane == i) list = mine;
-          if (!mine) break;  // uniform
-        }
-        if (wave == 0) best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
-      }
-    }
 
-    // The tile's sums without its first maximum.
-    bool left_out = s_owner != tid;
-    if (!some) mt = 0.0f;
+    // The sums without the first maximum; one that was it becomes a term of the first thread's.
+    if (rises) {
+      const float d = fmaxf(m - mt, kLowest), f = __builtin_amdgcn_exp2f(d * c2);
+      S += tid == 0 && m > -INFINITY ? 1.0f : 0.0f;
+      Tq = fmaf(f, Tq, f * d * S);  // f d first: d alone may be huge where f is 0
+      S *= f;
+      m = mt;
+    }
+    const float at = m > -INFINITY ? m : 0.0f;
+    bool left_out = !rises || s_owner[p] != tid;
     float st = 0.0f, tt = 0.0f;
     auto add = [&](float v) {
-      const float d = v - mt;
+      const float d = v - at;
       const float e = __builtin_amdgcn_exp2f(d * c2);
       st += e;
       tt = fmaf(e, fmaxf(d, kLowest), tt);
@@ -349,7 +408,7 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const float v = elem<T>(u[k], j);
-          const bool now = !left_out && v == mt;
+          const bool now = !left_out && v == m;
           left_out |= now;
           add(now ? -INFINITY : v);
         }
@@ -359,36 +418,32 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int j = 0; j < N; ++j) add(elem<T>(u[k], j));
     }
-    st = wave_sum(st);
-    tt = wave_sum(tt);
-    if constexpr (W > 1) {
-      if (lane == 0) {
-        s_sum[wave] = st;
-        s_sum[W + wave] = tt;
-      }
-      __syncthreads();
-      st = s_sum[0];
-      tt = s_sum[W];
+    S += st;
+    Tq += tt;
+    if constexpr (!MANY) break;
 #pragma unroll
-      for (int w = 1; w < W; ++w) {
-        st += s_sum[w];
-        tt += s_sum[W + w];
-      }
+    for (int k = 0; k < NV; ++k) u[k] = ahead[MANY ? k : 0];
+  }
+  if (top) {
+    __syncthreads();
+    const int n = s_count;
+    __syncthreads();
+    settle(n, gathered, (vecs - 1) / TILE * TILE);
+  }
+  S = wave_sum(S);
+  Tq = wave_sum(Tq);
+  if constexpr (W > 1) {
+    if (lane == 0) {
+      s_sum[wave] = S;
+      s_sum[W + wave] = Tq;
     }
-    __syncthreads();  // the next tile writes LDS again
-    // Joined with the tiles before; the smaller maximum's token becomes a term of the sums.
-    if (!some) {
-      S += st;  // 0, or NaN where the tile holds one
-    } else if (mt > m) {
-      const float d = fmaxf(m - mt, kLowest), f = __builtin_amdgcn_exp2f(d * c2);
-      const float n = m > -INFINITY ? 1.0f : 0.0f;
-      Tq = fmaf(f, Tq, fmaf(f * d, S + n, tt));  // f d first: d alone may be huge where f is 0
-      S = fmaf(f, S + n, st);
-      m = mt;
-    } else {
-      const float d = fmaxf(mt - m, kLowest), f = __builtin_amdgcn_exp2f(d * c2);
-      Tq = fmaf(f, tt, fmaf(f * d, st + 1.0f, Tq));
-      S = fmaf(f, st + 1.0f, S);
+    __syncthreads();
+    S = s_sum[0];
+    Tq = s_sum[W];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      S += s_sum[w];
+      Tq += s_sum[W + w];
     }
   }
 
@@ -581,46 +636,68 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   }
 }
 
-// The smallest workgroup whose registers hold the row.
-template <class T, template <class, int, int> class Launch, class Args>
-Status launch_rows(hipStream_t stream, const Args& a, size_t rows) {
-  const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
-  if (vecs <= 64 * 1 * 4) return Launch<T, 1, 4>::run(stream, a, rows);
-  if (vecs <= 64 * 4 * 4) return Launch<T, 4, 4>::run(stream, a, rows);
-  if (vecs <= 64 * 4 * 8) return Launch<T, 4, 8>::run(stream, a, rows);
-  if (vecs <= 64 * 8 * 8) return Launch<T, 8, 8>::run(stream, a, rows);
-  if (vecs <= 64 * 16 * 8) return Launch<T, 16, 8>::run(stream, a, rows);
-  return Launch<T, 16, 16>::run(stream, a, rows);
+template <class T, int W, int NV, bool MANY>
+Status logprobs(hipStream_t stream, const LogprobArgs& a, size_t rows) {
+  const size_t lds = a.top_k ? kCandidates * 8 : 0;
+  token_logprobs_kernel<T, W, NV, MANY><<<(uint32_t)rows, 64 * W, lds, stream>>>(a);
+  PSSA_LAUNCH_CHECK("token_logprobs_kernel");
+  return Status::Ok();
+}
+template <class T, int W, int NV>
+Status distill(hipStream_t stream, const DistillArgs& a, size_t rows) {
+  distill_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, (size_t)a.teacher_k * 12, stream>>>(a);
+  PSSA_LAUNCH_CHECK("distill_kernel");
+  return Status::Ok();
 }
 
-template <class T, int W, int NV>
-struct LaunchLogprobs {
-  static Status run(hipStream_t stream, const LogprobArgs& a, size_t rows) {
-    const size_t lds = a.top_k ? kCandidates * 8 : 0;
-    token_logprobs_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, lds, stream>>>(a);
-    PSSA_LAUNCH_CHECK("token_logprobs_kernel");
-    return Status::Ok();
-  }
-};
-template <class T, int W, int NV>
-struct LaunchDistill {
-  static Status run(hipStream_t stream, const DistillArgs& a, size_t rows) {
-    distill_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, (size_t)a.teacher_k * 12, stream>>>(a);
-    PSSA_LAUNCH_CHECK("distill_kernel");
-    return Status::Ok();
-  }
-};
+// Waves for a row: so many that the rows fill the chip's compute units, and a
+// tile that holds the row where no more than these are needed for it.
+//   us, with 8 alternatives:      256 rows of          3000 rows of
+//                               65537 100003 bf16    65537 100003 bf16
+//     16 waves                     23     28            261    310
+//     8 waves                      24     31            171    228
+//     4 waves                      35     53            138    195
+template <class T>
+Status launch_logprobs(hipStream_t stream, const LogprobArgs& a, size_t rows) {
+  const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
+  if (vecs <= 64 * 1 * 4) return logprobs<T, 1, 4, false>(stream, a, rows);
+  if (vecs <= 64 * 4 * 4) return logprobs<T, 4, 4, false>(stream, a, rows);
+  if (vecs <= 64 * 4 * 8) return logprobs<T, 4, 8, false>(stream, a, rows);
+  if (rows > 2 * kComputeUnits) return logprobs<T, 4, 4, true>(stream, a, rows);
+  if (vecs <= 64 * 8 * 8) return logprobs<T, 8, 8, false>(stream, a, rows);
+  if (rows > kComputeUnits) return logprobs<T, 8, 4, true>(stream, a, rows);
+  if (vecs <= 64 * 16 * 8) return logprobs<T, 16, 8, false>(stream, a, rows);
+  return logprobs<T, 16, 4, true>(stream, a, rows);
+}
+
+// The smallest workgroup whose registers hold the row, which the gradient is
+// then written from.  A row past them is read again, and so is a bf16 one
+// that would leave no room for a second workgroup, where there are rows for
+// one: a byte of bf16 costs twice the exponentials, which hide behind another
+// workgroup's loads (3000 rows of 65537: 260 us of 8 waves with 4 vectors,
+// 320 of 16 with 16; 256 rows: 33 and 27).
+template <class T>
+Status launch_distillation(hipStream_t stream, const DistillArgs& a, size_t rows) {
+  const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
+  if (vecs <= 64 * 1 * 4) return distill<T, 1, 4>(stream, a, rows);
+  if (vecs <= 64 * 4 * 4) return distill<T, 4, 4>(stream, a, rows);
+  if (vecs <= 64 * 4 * 8) return distill<T, 4, 8>(stream, a, rows);
+  if (vecs <= 64 * 8 * 8) return distill<T, 8, 8>(stream, a, rows);
+  if (vecs > 64 * 16 * 16) return distill<T, 16, 4>(stream, a, rows);
+  if constexpr (sizeof(T) == 2)
+    if (rows > kComputeUnits) return distill<T, 8, 4>(stream, a, rows);
+  if (vecs <= 64 * 16 * 8) return distill<T, 16, 8>(stream, a, rows);
+  return distill<T, 16, 16>(stream, a, rows);
+}
 
 }  // namespace
 
 Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& a, size_t rows) {
-  return dtype == PSSA_HIP_F32 ? launch_rows<float, LaunchLogprobs>(stream, a, rows)
-                               : launch_rows<Bf16, LaunchLogprobs>(stream, a, rows);
+  return dtype == PSSA_HIP_F32 ? launch_logprobs<float>(stream, a, rows) : launch_logprobs<Bf16>(stream, a, rows);
 }
 
 Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& a, size_t rows) {
-  return dtype == PSSA_HIP_F32 ? launch_rows<float, LaunchDistill>(stream, a, rows)
-                               : launch_rows<Bf16, LaunchDistill>(stream, a, rows);
+  return dtype == PSSA_HIP_F32 ? launch_distillation<float>(stream, a, rows) : launch_distillation<Bf16>(stream, a, rows);
 }
 
 }  // namespace pssa

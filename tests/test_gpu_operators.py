@@ -206,6 +206,35 @@ def test_logprobs_masks_ties_and_bad_rows(hip, dtype, vocab, k):
     check_logprobs(hip, z, t, 1.0, k, dtype)
 
 
+@pytest.mark.parametrize("rows,k", [(300, 8), (520, 64), (513, 3), (257, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logprobs_of_many_rows(hip, dtype, rows, k):
+    """Many rows take their tiles one by one: what the alternatives gather in each, with tiles that hold nothing, that
+    hold more and more, and that hold too many."""
+    vocab = 20011
+    say("logprobs of many rows", rows, k, dtype)
+    rng = np.random.default_rng(rows + k)
+    z = logits_like(rng, rows, vocab)
+    z[0] = -np.inf
+    z[1, :18000] = -np.inf
+    z[2] = -np.inf
+    z[2, [5, 9000, 9001, vocab - 1]] = [1.0, 3.0, 3.0, 2.0]
+    z[3] = np.sort(z[3])
+    for i in range(vocab // 1000):
+        z[4, 1000 * i:1000 * i + 150] = 40 + i
+        z[5, 1000 * i:1000 * i + 75] = 40 + i
+    z[6] = 0.25
+    z[7, vocab - 1] = np.nan
+    z[8, 12000] = np.inf
+    z[9] = rng.integers(-2, 3, vocab)
+    z[10, 16000:] = -np.inf
+    z[11] = -40.0
+    z[11, 19000] = 20.0
+    t = some_targets(rng, rows, vocab)
+    t[[0, 7, 8]] = [1, 2, 3]
+    check_logprobs(hip, z, t, 1.0, k, dtype)
+
+
 def test_logprobs_outputs_are_optional_and_the_rest_is_untouched(hip):
     rng = np.random.default_rng(5)
     z = logits_like(rng, 3, 500)
@@ -298,7 +327,7 @@ def teacher(rng, rows, vocab, k, dead=0.1):
 @pytest.mark.parametrize("rows,vocab,k,pad,tau", [
     (1, 1, 1, 0, 1.0), (3, 2, 2, 1, 1.0), (4, 5, 3, 0, 2.0), (2, 9, 9, 0, 1.0), (7, 64, 8, 0, 1.0), (3, 255, 20, 2, 0.7),
     (2, 1025, 64, 0, 1.0), (3, 2048, 100, 0, 4.0), (3, 4099, 8, 1, 1.0), (2, 8193, 20, 0, 1.0), (2, 16384, 64, 0, 2.0),
-    (2, 33001, 1024, 0, 1.0), (1, 65537, 64, 3, 1.5), (2, 140001, 20, 0, 1.0)])
+    (2, 33001, 1024, 0, 1.0), (1, 65537, 64, 3, 1.5), (2, 140001, 20, 0, 1.0), (260, 33001, 20, 1, 1.0)])
 def test_distill_matches_64_bits(hip, dtype, rows, vocab, k, pad, tau):
     say(f"distill {rows} x {vocab} (+{pad}) {dtype} teacher {k} tau {tau}")
     rng = np.random.default_rng(vocab + k)
