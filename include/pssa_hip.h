@@ -589,8 +589,10 @@ int pssa_hip_lanes_stage_times(pssa_hip_lanes* lanes, int enable, const char** n
  * On device-resident arrays (plain device pointers from any allocator),
  * asynchronous on the context stream: work that other streams do on these
  * arrays has to be complete before the call, and pssa_hip_synchronize
- * completes it.  `dtype` is PSSA_HIP_F32 or PSSA_HIP_BF16; sums, statistics and states are
- * fp32.  They have no counterpart in the reference's backend.
+ * completes it.  `dtype` is PSSA_HIP_F32 or PSSA_HIP_BF16; sums, statistics
+ * and states are fp32, their order a matter of the call's sizes alone: the
+ * same call gives the same bits, another number of rows or sequences may give
+ * a row others.  They have no counterpart in the reference's backend.
  */
 
 /* Log probabilities of given tokens under log softmax(logits / temperature),
@@ -689,11 +691,11 @@ int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, f
  * is <= 0 (0: no decay; -inf: only the token itself).  States are fp32
  * [n_seqs, heads, d_key, d_val]: d_state_in NULL starts from zeros,
  * d_state_out (NULL: not kept) receives the states behind the last tokens and
- * may be d_state_in.  out may lie in the buffer of q, k and v in columns of its own (same row stride) and must
- * not overlap them otherwise.  d_key <= 128, d_val <= 4096, n_seqs and heads
- * <= 65535, row strides below 2^24.  bf16 outputs round once; every sum and the states are fp32.  A
- * value that is not finite reaches the outputs from its own token on and no
- * earlier one. */
+ * may be d_state_in.  out may lie in the buffer of q, k and v in columns of
+ * its own (same row stride) and must not overlap them otherwise.  d_key <= 128,
+ * d_val <= 4096, n_seqs and heads <= 65535, row strides below 2^24.  bf16
+ * outputs round once; every sum and the states are fp32.  A value that is not
+ * finite reaches the outputs from its own token on and no earlier one. */
 int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
                                        size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
                                        const float* d_state_in, const uint64_t* lens, size_t n_seqs, size_t seq_len,
