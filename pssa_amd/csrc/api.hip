@@ -2087,8 +2087,8 @@ Status check_batch(const pssa_hip_lanes* L, size_t n_tokens) {
 Status check_w4(size_t n, size_t k, size_t group) {
   PSSA_RETURN_IF(need(n && k, "4-bit weights: dimensions must be positive"));
   PSSA_RETURN_IF(need(group == 32 || group == 64 || group == 128, "4-bit weights: group must be 32, 64 or 128"));
-  // Tiles and columns are counted in 32 bits, the packed bytes in the grid of the layout's kernel.
-  return need(n <= ((size_t)1 << 30) && k <= ((size_t)1 << 24) && n <= ((size_t)1 << 38) / k,
+  // The layout's kernel has a thread for each 16 packed bytes, counted in 32 bits.
+  return need(n <= ((size_t)1 << 30) && k <= ((size_t)1 << 24) && pssa::w4_packed_bytes(n, k) <= (size_t)1 << 35,
               "4-bit weights: too large");
 }
 

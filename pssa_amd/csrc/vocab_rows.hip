@@ -6,6 +6,8 @@
 // sums, and tokens that may be among the largest are put aside in LDS.
 // Distillation writes its gradient from the registers that the sums were taken
 // from, or reads a row past them twice.
+#include <algorithm>
+
 #include "operators.h"
 
 namespace pssa {
@@ -692,12 +694,39 @@ Status launch_distillation(hipStream_t stream, const DistillArgs& a, size_t rows
 
 }  // namespace
 
-Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& a, size_t rows) {
-  return dtype == PSSA_HIP_F32 ? launch_logprobs<float>(stream, a, rows) : launch_logprobs<Bf16>(stream, a, rows);
+// A launch's threads are counted in 32 bits: more rows go in parts.
+constexpr size_t kMostRows = (size_t)1 << 21;
+
+Status launch_token_logprobs(hipStream_t stream, int dtype, const LogprobArgs& args, size_t rows) {
+  LogprobArgs a = args;
+  for (size_t n; rows; rows -= n) {
+    n = std::min(rows, kMostRows);
+    PSSA_RETURN_IF(dtype == PSSA_HIP_F32 ? launch_logprobs<float>(stream, a, n) : launch_logprobs<Bf16>(stream, a, n));
+    a.logits = static_cast<const char*>(a.logits) + n * a.ld * (dtype == PSSA_HIP_F32 ? 4 : 2);
+    if (a.targets) a.targets += n;
+    if (a.logprobs) a.logprobs += n;
+    if (a.entropy) a.entropy += n;
+    if (a.top_ids) a.top_ids += n * a.top_k;
+    if (a.top_logprobs) a.top_logprobs += n * a.top_k;
+  }
+  return Status::Ok();
 }
 
-Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& a, size_t rows) {
-  return dtype == PSSA_HIP_F32 ? launch_distillation<float>(stream, a, rows) : launch_distillation<Bf16>(stream, a, rows);
+Status launch_distill(hipStream_t stream, int dtype, const DistillArgs& args, size_t rows) {
+  DistillArgs a = args;
+  const size_t size = dtype == PSSA_HIP_F32 ? 4 : 2;
+  for (size_t n; rows; rows -= n) {
+    n = std::min(rows, kMostRows);
+    PSSA_RETURN_IF(dtype == PSSA_HIP_F32 ? launch_distillation<float>(stream, a, n)
+                                         : launch_distillation<Bf16>(stream, a, n));
+    a.logits = static_cast<const char*>(a.logits) + n * a.ld * size;
+    a.teacher_ids += n * a.teacher_k;
+    a.teacher_logits += n * a.teacher_k;
+    if (a.row_weights) a.row_weights += n;
+    a.losses += n;
+    if (a.grad) a.grad = static_cast<char*>(a.grad) + n * a.ld_grad * size;
+  }
+  return Status::Ok();
 }
 
 }  // namespace pssa

@@ -762,3 +762,73 @@ def test_a_step_of_a_served_model_runs_through_the_operators(hip):
     assert np.max(np.abs(got[3] - lref[np.arange(streams), targets])) <= U32 * (4 * np.abs(lref).max() + 100)
     np.testing.assert_array_equal(got[4], top64(got[2], K))
     mat.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,h,hk,dk,dv", [([900, 0, 130], 2, 1, 36, 40), ([2000, 5], 1, 1, 64, 64), ([1100, 700], 2, 1, 128, 128)])
+def test_linear_attention_in_segments_with_states_in_place(hip, dtype, lens, h, hk, dk, dv):
+    """Few long walks are split; their states may be written where they were read."""
+    say("linear segments in place", lens, dtype)
+    a = check_linear(hip, lens, h, hk, dk, dv, dtype, True, in_place=True)
+    b = check_linear(hip, lens, h, hk, dk, dv, dtype, True)
+    for x, y in zip(a, b):
+        np.testing.assert_array_equal(x, y)
+    check_linear(hip, lens, h, hk, dk, dv, dtype, True, gap=3, decays=[0.0, -np.inf][:h], in_place=True)
+
+
+def test_linear_attention_of_two_contexts_at_once(hip):
+    """Each context has its stream and its scratch: calls that run beside each other give what each gives alone."""
+    import threading
+
+    from pssa_amd import HipDevice
+
+    rng = np.random.default_rng(3)
+    n, h, d = 1500, 2, 64
+    q, k, v = (rng.normal(0, 1, (n, h, d)) for _ in range(3))
+    g = np.full(h, -0.05, np.float32)
+    alone, last, _ = run_linear(hip, q, k, v, g, [n], 0.3, None, "f32")
+    other = HipDevice(0)
+    got = {}
+
+    def work(dev, name):
+        got[name] = [run_linear(dev, q, k, v, g, [n], 0.3, None, "f32")[:2] for _ in range(8)]
+
+    threads = [threading.Thread(target=work, args=(dev, i)) for i, dev in enumerate((hip, other, hip))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    other.close()
+    assert sorted(got) == [0, 1, 2]
+    for results in got.values():
+        for out, state in results:
+            np.testing.assert_array_equal(out, alone)
+            np.testing.assert_array_equal(state, last)
+
+
+def test_rows_past_one_launch(hip):
+    """More rows than the threads of one launch can be counted for: log p of two tokens is -log(1 + e^(other - own)),
+    whose rounding is the difference's, the exponential's, the logarithm's and the subtraction's."""
+    rows = (1 << 21) + 3
+    say("rows past one launch", rows)
+    rng = np.random.default_rng(8)
+    z = rng.normal(0, 2, (rows, 2)).astype(np.float32)
+    t = rng.integers(0, 2, rows).astype(np.uint32)
+    at = np.arange(rows)
+    d = z[at, 1 - t].astype(np.float64) - z[at, t]
+    ref = -np.logaddexp(0.0, d)
+    p = 1 / (1 + np.exp(d))
+    with Held(hip) as b:
+        x, ids = b.up(z), b.up(t)
+        lp, tid = b.new(rows, np.float32, 7.0), b.new(rows, np.uint32, 7)
+        tlp, tl = b.new(rows, np.float32, 7.0), b.up(np.zeros(rows, np.float32))
+        loss, grad = b.new(rows, np.float32, 7.0), b.new((rows, 2), np.float32, 7.0)
+        hip.token_logprobs_resident(x.ptr, "f32", rows, 2, ids.ptr, lp.ptr, None, 1, tid.ptr, tlp.ptr)
+        hip.distill_resident(x.ptr, "f32", rows, 2, ids.ptr, tl.ptr, 1, loss.ptr, grad.ptr)
+        hip.synchronize()
+        tol = U32 * 32 * (1 + np.abs(d))
+        assert np.all(np.abs(lp.to_host() - ref) <= tol)
+        np.testing.assert_array_equal(tid.to_host(), np.argmax(z, 1))
+        assert np.all(np.abs(loss.to_host() + ref) <= tol)
+        got = grad.to_host()
+        assert np.all(np.abs(got[at, t] - (p - 1)) <= tol) and np.all(np.abs(got[at, 1 - t] - (1 - p)) <= tol)

@@ -102,7 +102,7 @@ W4 = dict(ctx=None, codes=P, scales=P, zeros=None, n=16, k=64, group=32)
 @pytest.mark.parametrize("change,message", [
     ({}, "null context"), ({"codes": None}, "null buffer"), ({"n": 0}, "positive"), ({"k": 0}, "positive"),
     ({"group": 16}, "32, 64 or 128"), ({"group": 0}, "32, 64 or 128"), ({"scales": P + 2}, "misaligned"),
-    ({"n": 1 << 31}, "too large"), ({"k": 1 << 25}, "too large"), ({"n": 1 << 30, "k": 1 << 20}, "too large")])
+    ({"n": 1 << 31}, "too large"), ({"n": 1 << 30, "k": 1}, "too large"), ({"k": 1 << 25}, "too large"), ({"n": 1 << 30, "k": 1 << 20}, "too large")])
 def test_w4_load_refuses(change, message):
     out = C.c_void_p(1)
     refused(_abi.lib().pssa_hip_w4_load_resident, changed(W4, **change) + [C.byref(out)], message)
