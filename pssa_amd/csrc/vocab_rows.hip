@@ -478,7 +478,11 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
 // and its gradient w tau (p - q).  The dense part p is written from the
 // registers that the sums were taken from; the few teacher's tokens are then
 // written again with their q.
-template <class T, int W, int NV>
+// 8192 fp32 rows of 16384: 219 us (4.9 TB/s); 777 bf16 rows of 65537: 63 us
+// (4.6 TB/s with the second read); 37 fp32 rows of 2048: 6 us, latency.
+// MANY: the row takes several tiles, each thread with a maximum and sum of its
+// own until the end, each tile loaded while the one before is summed.
+template <class T, int W, int NV, bool MANY>
 __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   constexpr int N = vec_n<T>(), TILE = 64 * W * NV;
   __shared__ float s_red[2 * W];
@@ -539,19 +543,9 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   }
 
   float m = -INFINITY, S = 0.0f;
-  u32x4_t u[NV];
-  for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
-    tile_load<T, W, NV>(u, row, V, tile0);
-    float mt = tile_max<T, NV>(u);
-    tile_again(u);
-    mt = wave_max(mt);
-    if constexpr (W > 1) {
-      if (lane == 0) s_red[wave] = mt;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < W; ++w) mt = fmaxf(mt, s_red[w]);
-    }
-    const float mn = fmaxf(m, mt), at = mn > -INFINITY ? mn : 0.0f;
+  u32x4_t u[NV], ahead[MANY ? NV : 1];
+  tile_load<T, W, NV>(u, row, V, 0);
+  auto sum = [&](float at) {
     float st = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -560,16 +554,45 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
       for (int j = 0; j < N; ++j) st += __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2);
     }
     tile_again(u);
-    st = wave_sum(st);
-    if constexpr (W > 1) {
-      if (lane == 0) s_red[W + wave] = st;
-      __syncthreads();
-      st = s_red[W];
+    return st;
+  };
+  if constexpr (MANY) {
+    float mine = -INFINITY;
+    for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
+      tile_again(u);  // its loads end here
+      // Behind the last tile comes the first, for the gradient.
+      tile_load<T, W, NV>(ahead, row, V, tile0 + TILE < vecs ? tile0 + TILE : 0);
+      const float mn = fmaxf(mine, tile_max<T, NV>(u)), at = mn > -INFINITY ? mn : 0.0f;
+      tile_again(u);
+      S = (mine > -INFINITY ? S * __builtin_amdgcn_exp2f((mine - at) * c2) : S) + sum(at);
+      mine = mn;
 #pragma unroll
-      for (int w = 1; w < W; ++w) st += s_red[W + w];
+      for (int k = 0; k < NV; ++k) u[k] = ahead[k];
     }
-    S = (m > -INFINITY ? S * __builtin_amdgcn_exp2f((m - at) * c2) : S) + st;
-    m = mn;
+    m = wave_max(mine);
+    if (lane == 0) s_red[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, s_red[w]);
+    if (mine > -INFINITY) S *= __builtin_amdgcn_exp2f((mine - m) * c2);
+  } else {
+    m = wave_max(tile_max<T, NV>(u));
+    tile_again(u);
+    if constexpr (W > 1) {
+      if (lane == 0) s_red[wave] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) m = fmaxf(m, s_red[w]);
+    }
+    S = sum(m > -INFINITY ? m : 0.0f);
+  }
+  S = wave_sum(S);
+  if constexpr (W > 1) {
+    if (lane == 0) s_red[W + wave] = S;
+    __syncthreads();
+    S = s_red[W];
+#pragma unroll
+    for (int w = 1; w < W; ++w) S += s_red[W + w];
   }
   const bool empty = m == -INFINITY;
   const float at = empty ? 0.0f : m;
@@ -609,14 +632,17 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
       }
     }
   };
-  if (vecs <= TILE) {
+  if constexpr (!MANY) {
     write(0);
   } else {
     // In place, a partial vector's load also covers its neighbour's elements,
     // which may be written already: they are masked, as in the sums.
     for (int tile0 = 0; tile0 < vecs; tile0 += TILE) {
-      tile_load<T, W, NV>(u, row, V, tile0);
+      tile_again(u);
+      if (tile0 + TILE < vecs) tile_load<T, W, NV>(ahead, row, V, tile0 + TILE);
       write(tile0);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) u[k] = ahead[k];
     }
   }
   // The dense stores have reached the cache before another thread's store to the same token.
@@ -645,9 +671,9 @@ Status logprobs(hipStream_t stream, const LogprobArgs& a, size_t rows) {
   PSSA_LAUNCH_CHECK("token_logprobs_kernel");
   return Status::Ok();
 }
-template <class T, int W, int NV>
+template <class T, int W, int NV, bool MANY>
 Status distill(hipStream_t stream, const DistillArgs& a, size_t rows) {
-  distill_kernel<T, W, NV><<<(uint32_t)rows, 64 * W, (size_t)a.teacher_k * 12, stream>>>(a);
+  distill_kernel<T, W, NV, MANY><<<(uint32_t)rows, 64 * W, (size_t)a.teacher_k * 12, stream>>>(a);
   PSSA_LAUNCH_CHECK("distill_kernel");
   return Status::Ok();
 }
@@ -673,23 +699,26 @@ Status launch_logprobs(hipStream_t stream, const LogprobArgs& a, size_t rows) {
 }
 
 // The smallest workgroup whose registers hold the row, which the gradient is
-// then written from.  A row past them is read again, and so is a bf16 one
-// that would leave no room for a second workgroup, where there are rows for
-// one: a byte of bf16 costs twice the exponentials, which hide behind another
-// workgroup's loads (3000 rows of 65537: 260 us of 8 waves with 4 vectors,
-// 320 of 16 with 16; 256 rows: 33 and 27).
+// then written from: eight waves with 16 vectors rather than sixteen with 8
+// leave room for a second one (3000 rows of 50257 bf16: 175 and 195 us).  A
+// row past the registers is read again, and so is a bf16 one that would
+// leave no such room, where there are rows for a second workgroup: a byte of
+// bf16 costs twice the exponentials, which hide behind another's loads (us,
+// tiles of 8 waves against 16 waves that hold the row: 3000 rows of 65537 242
+// and 310, of 100003 380 and 395; 256 rows of 100003 33 and 31).  fp32 rows
+// gain from being read once (3000 of 50257: 278 us held, 338 in tiles).
 template <class T>
 Status launch_distillation(hipStream_t stream, const DistillArgs& a, size_t rows) {
   const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
-  if (vecs <= 64 * 1 * 4) return distill<T, 1, 4>(stream, a, rows);
-  if (vecs <= 64 * 4 * 4) return distill<T, 4, 4>(stream, a, rows);
-  if (vecs <= 64 * 4 * 8) return distill<T, 4, 8>(stream, a, rows);
-  if (vecs <= 64 * 8 * 8) return distill<T, 8, 8>(stream, a, rows);
-  if (vecs > 64 * 16 * 16) return distill<T, 16, 4>(stream, a, rows);
+  if (vecs <= 64 * 1 * 4) return distill<T, 1, 4, false>(stream, a, rows);
+  if (vecs <= 64 * 4 * 4) return distill<T, 4, 4, false>(stream, a, rows);
+  if (vecs <= 64 * 4 * 8) return distill<T, 4, 8, false>(stream, a, rows);
+  if (vecs <= 64 * 8 * 8) return distill<T, 8, 8, false>(stream, a, rows);
+  if (vecs <= 64 * 8 * 16) return distill<T, 8, 16, false>(stream, a, rows);
+  if (vecs > 64 * 16 * 16) return distill<T, 16, 4, true>(stream, a, rows);
   if constexpr (sizeof(T) == 2)
-    if (rows > kComputeUnits) return distill<T, 8, 4>(stream, a, rows);
-  if (vecs <= 64 * 16 * 8) return distill<T, 16, 8>(stream, a, rows);
-  return distill<T, 16, 16>(stream, a, rows);
+    if (rows > kComputeUnits) return distill<T, 8, 4, true>(stream, a, rows);
+  return distill<T, 16, 16, false>(stream, a, rows);
 }
 
 }  // namespace
