@@ -416,9 +416,11 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
         }
     } else {
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
+      for (int k = 0; k < NV; ++k) {
+        if (MANY && (tile0 + k * 64 * W) * N >= V) continue;  // uniform: nothing is there
 #pragma unroll
         for (int j = 0; j < N; ++j) add(elem<T>(u[k], j));
+      }
     }
     S += st;
     Tq += tt;
@@ -545,10 +547,11 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
   float m = -INFINITY, S = 0.0f;
   u32x4_t u[NV], ahead[MANY ? NV : 1];
   tile_load<T, W, NV>(u, row, V, 0);
-  auto sum = [&](float at) {
+  auto sum = [&](float at, int tile0) {
     float st = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      if (MANY && (tile0 + k * 64 * W) * N >= V) continue;  // uniform: nothing is there
       if constexpr (NV > 8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < N; ++j) st += __builtin_amdgcn_exp2f((elem<T>(u[k], j) - at) * c2);
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
       tile_load<T, W, NV>(ahead, row, V, tile0 + TILE < vecs ? tile0 + TILE : 0);
       const float mn = fmaxf(mine, tile_max<T, NV>(u)), at = mn > -INFINITY ? mn : 0.0f;
       tile_again(u);
-      S = (mine > -INFINITY ? S * __builtin_amdgcn_exp2f((mine - at) * c2) : S) + sum(at);
+      S = (mine > -INFINITY ? S * __builtin_amdgcn_exp2f((mine - at) * c2) : S) + sum(at, tile0);
       mine = mn;
 #pragma unroll
       for (int k = 0; k < NV; ++k) u[k] = ahead[k];
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(64 * W) void distill_kernel(DistillArgs a) {
 #pragma unroll
       for (int w = 0; w < W; ++w) m = fmaxf(m, s_red[w]);
     }
-    S = sum(m > -INFINITY ? m : 0.0f);
+    S = sum(m > -INFINITY ? m : 0.0f, 0);
   }
   S = wave_sum(S);
   if constexpr (W > 1) {
