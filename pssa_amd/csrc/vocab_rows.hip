@@ -219,8 +219,8 @@ __device__ __forceinline__ Key wave_merge(Key a, Key b_reversed, int lane) {
 // equal, say) gives its k tokens one by one, each round the largest behind
 // the one before.
 //
-// 8192 fp32 rows of 16384: 129 us (4.2 TB/s); 509 bf16 rows of 100003 with 20
-// alternatives: 40 us (2.5 TB/s); one row of 16384: 9 us, mostly latency.
+// 8192 fp32 rows of 16384, 8 alternatives: 129 us (4.2 TB/s); 509 bf16 rows of
+// 100003, 5 of them: 39 us (2.6 TB/s); one row of 16384: 9 us, mostly latency.
 constexpr int kCandidates = 1024;
 constexpr int kSlots = 8;  // threads of a wave whose vectors are looked through at once
 
