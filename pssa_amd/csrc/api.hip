@@ -2133,8 +2133,8 @@ struct LinearPlan {
   std::vector<uint32_t> table;  // first tokens and items, where the arguments do not hold them
   size_t tokens = 0, longest = 0;
 };
-Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_val,
-                      pssa::LinearArgs& a, LinearPlan& p) {
+Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_key,
+                      size_t d_val, pssa::LinearArgs& a, LinearPlan& p) {
   PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "linear attention: sequences must be in 1..=65535"));
   a.n_seqs = (int)n_seqs;
   const size_t most = INT32_MAX;
@@ -2146,7 +2146,7 @@ Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_
     p.longest = std::max(p.longest, len);
     same &= !lens || lens[i] == lens[0];
   }
-  const size_t seg = (size_t)pssa::linear_segment(lens, n_seqs, p.longest, heads, d_val);
+  const size_t seg = (size_t)pssa::linear_segment(lens, n_seqs, p.longest, heads, d_key, d_val);
   a.seg_len = (int)(seg ? seg : std::max<size_t>(p.longest, 1));
   a.uniform_len = same ? (int)p.longest : -1;
   a.uniform_segs = (int)std::max<size_t>(1, (p.longest + a.seg_len - 1) / a.seg_len);
@@ -2477,7 +2477,7 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
                         "linear attention: misaligned buffer"));
     pssa::LinearArgs a;
     LinearPlan plan;
-    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_val, a, plan));
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
     const size_t tokens = plan.tokens;
     size_t n = 0;
     for (size_t ld : {ld_q, ld_k, ld_v, ld_out}) PSSA_RETURN_IF(pssa::checked_count({tokens, ld}, &n, "linear attention"));
@@ -2533,7 +2533,7 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
     PSSA_RETURN_IF(check_heads(heads, d_key, d_val));
     pssa::LinearArgs a;
     LinearPlan plan;
-    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_val, a, plan));
+    PSSA_RETURN_IF(plan_sequences(lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));

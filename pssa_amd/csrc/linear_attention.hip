@@ -441,6 +441,12 @@ constexpr int pair_of(int t, int h) { return t == 3 ? h : t == 2 ? (h ? 5 : 2) :
 // What stands in for rows and columns that are not there.
 __device__ uint32_t g_nothing[4];
 
+// Groups of waves that keep the state, a part of its rows each: two where it
+// is all that a workgroup computes, which otherwise would leave a SIMD one wave
+// (8192 bf16 tokens, 8 heads of 128: 14.7 us against 16.5).
+template <int DKP, bool LOCAL>
+constexpr int kKeepers = LOCAL && DKP >= 64 ? 2 : 1;
+
 // LDS units (16 bytes) of the kernel: two buffers of q | k | v, P, and q S.
 template <int DKP, int WAVES, bool LOCAL>
 struct ChunkLds {
@@ -457,11 +463,12 @@ struct ChunkLds {
 // two workgroups' state passes in between.)
 // LB: bytes of one load, 16 where every row and head is so aligned, else 4.
 template <int DKP, int WAVES, int MODE, int LB>
-__global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA_LOCAL || DKP == 128 ? 2 : 4) void linear_chunks_bf16_kernel(LinearArgs a) {
+__global__ __launch_bounds__((64 * WAVES * (MODE == LA_LOCAL ? kKeepers<DKP, true> : 2)), (MODE == LA_LOCAL || DKP == 128 ? 2 : 4)) void linear_chunks_bf16_kernel(
+    LinearArgs a) {
   constexpr bool LOCAL = MODE == LA_LOCAL;
-  constexpr int ALL = LOCAL ? WAVES : 2 * WAVES;
+  constexpr int KEEPERS = kKeepers<DKP, LOCAL>, ALL = (LOCAL ? 0 : WAVES) + KEEPERS * WAVES;
   using Lds = ChunkLds<DKP, WAVES, LOCAL>;
-  constexpr int DVT = 16 * WAVES, NB = DKP / 16, KP = DKP / 32;
+  constexpr int DVT = 16 * WAVES, NB = DKP / 16 / KEEPERS, KP = DKP / 32;
   constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;  // instructions of a chunk, of a wave
   constexpr int SLOTS = (kPairs + WAVES - 1) / WAVES;
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_bf[];
@@ -469,7 +476,8 @@ __global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA
   f32x4_t* sO = reinterpret_cast<f32x4_t*>(sP + kPairs * 128);  // [column group][query tile][64 lanes]
   const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool keeps_state = LOCAL || in_all >= WAVES;
-  const int wave = LOCAL ? in_all : in_all % WAVES;  // of its group: its 16 columns
+  const int wave = in_all % WAVES;  // of its group: its 16 columns
+  const int b_first = LOCAL ? NB * (in_all / WAVES) : 0;  // of the state's tiles of 16 rows
   const int dv0 = blockIdx.x * DVT, head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
   const Span sp = span_of(a, blockIdx.z);
   const float g = a.log_decay[head], g2 = g * kLog2e;
@@ -538,13 +546,13 @@ __global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA
 
   int n = min(LA_C, sp.len);
   if (n > 0) issue(0, n, s_bf, lane);
-  // S: rows 16 b + 4 quad + r, column dv0 + 16 wave + col.
+  // S: rows 16 (b_first + b) + 4 quad + r, column dv0 + 16 wave + col.
   f32x4_t S[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      const int i = 16 * (b_first + b) + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
       S[b][r] = keeps_state && state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
     }
   // The state's loads end here: waited for in the loop, they would be waited
@@ -738,7 +746,7 @@ __global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA
         }
         constexpr int BG = NB < 4 ? NB : 4;  // tiles whose sums run beside each other
         u32x4_t vf, kf[BG];
-        turned_frags<DVT, DKP, BG>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf, turned_at<DKP>(sK, 32 * h, 0, ln), kf);
+        turned_frags<DVT, DKP, BG>(turned_at<DVT>(sV, 32 * h, 16 * wave, ln), vf, turned_at<DKP>(sK, 32 * h, 16 * b_first, ln), kf);
         u32x4_t w[3];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -751,7 +759,7 @@ __global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA
 #pragma unroll
         for (int b0 = 0; b0 < NB; b0 += BG) {
           if constexpr (NB > 4) {
-            if (b0) turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, ln), kf);
+            if (b0) turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * (b_first + b0), ln), kf);
           }
 #pragma unroll
           for (int b = 0; b < BG; ++b) S[b0 + b] *= fs;
@@ -771,7 +779,7 @@ __global__ __launch_bounds__(64 * WAVES * (MODE == LA_LOCAL ? 1 : 2), MODE == LA
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      const int i = 16 * (b_first + b) + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
       if (i < a.dk && j < a.dv) state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
     }
 }
@@ -808,11 +816,11 @@ __device__ __forceinline__ f32x4_t mfma32(float a, float b, const f32x4_t& c) {
 }
 
 template <int DKP, int MODE, int LB>
-__global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || DKP == 128 ? 2 : 4) void linear_chunks_fp32_kernel(
+__global__ __launch_bounds__((MODE == LA_LOCAL ? 256 * kKeepers<DKP, true> : 512), (MODE == LA_LOCAL || DKP == 128 ? 2 : 4)) void linear_chunks_fp32_kernel(
     LinearArgs a) {
   constexpr bool LOCAL = MODE == LA_LOCAL;
   using Lds = ChunkLds32<DKP, LOCAL>;
-  constexpr int WAVES = 4, ALL = LOCAL ? 4 : 8, DVT = 64, NB = DKP / 16;
+  constexpr int KEEPERS = kKeepers<DKP, LOCAL>, WAVES = 4, ALL = LOCAL ? 4 * KEEPERS : 8, DVT = 64, NB = DKP / 16 / KEEPERS;
   constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;
   extern __shared__ __attribute__((aligned(256))) f32x4_t s_f32[];
   f32x4_t* sP = s_f32 + 2 * Lds::kBuffer;  // [tiles (1, 0), (1, 1), (0, 0) of queries and keys][64 lanes]
@@ -820,6 +828,7 @@ __global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || D
   const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool keeps_state = LOCAL || in_all >= WAVES;
   const int wave = in_all % WAVES;  // of its group: its 16 columns
+  const int b_first = LOCAL ? NB * (in_all / WAVES) : 0;  // of the state's tiles of 16 rows
   const int dv0 = blockIdx.x * DVT, head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
   const Span sp = span_of(a, blockIdx.z);
   const float g = a.log_decay[head], g2 = g * kLog2e;
@@ -857,13 +866,13 @@ __global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || D
 
   int n = min(LA_C32, sp.len);
   if (n > 0) issue(0, n, s_f32, lane);
-  // S: rows 16 b + 4 quad + r, column dv0 + 16 wave + col.
+  // S: rows 16 (b_first + b) + 4 quad + r, column dv0 + 16 wave + col.
   f32x4_t S[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      const int i = 16 * (b_first + b) + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
       S[b][r] = keeps_state && state_in && i < a.dk && j < a.dv ? state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
     }
 #pragma unroll
@@ -1015,7 +1024,7 @@ __global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || D
           const float w = v[kt][r] * pw[4 + 4 * kt + r];
 #pragma unroll
           for (int b = 0; b < NB; ++b)
-            S[b] = mfma32(element32<DKP>(sK, 16 * kt + 4 * quad + r, 16 * b + col), w, S[b]);
+            S[b] = mfma32(element32<DKP>(sK, 16 * kt + 4 * quad + r, 16 * (b_first + b) + col), w, S[b]);
         }
     }
   }
@@ -1027,7 +1036,7 @@ __global__ __launch_bounds__(MODE == LA_LOCAL ? 256 : 512, MODE == LA_LOCAL || D
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
+      const int i = 16 * (b_first + b) + 4 * (lane >> 4) + r, j = dv0 + 16 * wave + (lane & 15);
       if (i < a.dk && j < a.dv) state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
     }
 }
@@ -1159,10 +1168,9 @@ struct Chunks {
 };
 template <int DKP, int NC, int MODE, int LB>
 struct ChunksBf16 {
-  static constexpr int kGroups = MODE == LA_LOCAL ? NC : 1;
-  static constexpr size_t kLds = ChunkLds<DKP, 4 * kGroups, MODE == LA_LOCAL>::kBytes;
-  static constexpr int kThreads = MODE == LA_LOCAL ? 256 * NC : 512, kColumns = 64 * kGroups;
-  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4 * kGroups, MODE, LB>;
+  static constexpr size_t kLds = ChunkLds<DKP, 4, MODE == LA_LOCAL>::kBytes;
+  static constexpr int kThreads = MODE == LA_LOCAL ? 256 * kKeepers<DKP, true> : 512, kColumns = 64;
+  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4, MODE, LB>;
 };
 template <int DKP, int NC, int MODE>
 struct Chunks<Bf16, DKP, NC, MODE, 16> : ChunksBf16<DKP, NC, MODE, 16> {};
@@ -1171,7 +1179,7 @@ struct Chunks<Bf16, DKP, NC, MODE, 4> : ChunksBf16<DKP, NC, MODE, 4> {};
 template <int DKP, int NC, int MODE, int LB>
 struct Chunks<float, DKP, NC, MODE, LB> {
   static constexpr size_t kLds = ChunkLds32<DKP, MODE == LA_LOCAL>::kBytes;
-  static constexpr int kThreads = MODE == LA_LOCAL ? 256 : 512, kColumns = 64;
+  static constexpr int kThreads = MODE == LA_LOCAL ? 256 * kKeepers<DKP, true> : 512, kColumns = 64;
   static constexpr auto kKernel = &linear_chunks_fp32_kernel<DKP, MODE, LB>;
 };
 
@@ -1237,29 +1245,35 @@ Status init_linear_attributes() {
 }
 
 // A walk is the way of a sequence, a head and 64 value columns through the
-// tokens, on a compute unit of its own.  A call is split into the shortest
-// segments that still leave each of them a compute unit.  A split walk's chunk
+// tokens, in a workgroup of its own.  A call is split into the shortest
+// segments that still run all at once: of one chunk if every segment then has
+// a compute unit, else of two or more, two workgroups a compute unit with
+// keys of up to 64 (LDS) and one with wider ones.  A split walk's chunk
 // costs twice one of a whole walk, as its state is computed twice, and the
 // passes between take about 12 us, 5 chunks of bf16 heads of 64:
-//                                              whole      split
-//   8192 bf16 tokens, 8 heads of 128            366 us   58 us (segments of 512)
-//   9 fp32 prompts of 5..1000, 12 heads of 64  89.3 us   49 us (of 256)
-//   16 bf16 prompts of 1024, 12 heads of 64      39 us   not split
-// Twice as many segments as compute units took 60 us and 45 us.
+//                                               whole     split for 256, 512
+//   8192 bf16 tokens, 8 heads of 128             366 us     54   61
+//   9 fp32 prompts of 5..1000, 12 heads of 64     90        49   47
+//   8 fp32 prompts of 1000, 12 heads of 64        92         -   73
+//   16 bf16 prompts of 1500, 8 heads of 32        50         -   40
+// (one chunk or two: a prompt of 700 fp32 tokens, 12 heads of 64 22 us and 27;
+// 4 bf16 prompts of 2000, 4 heads of 64, for which 512 are needed, 27 and 22).
 constexpr size_t kComputeUnits = 256;
-int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_val) {
+int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val) {
   const size_t chunks = (longest + LA_C - 1) / LA_C, lanes = heads * ((d_val + 63) / 64);
-  if (n_seqs * lanes > kComputeUnits) return 0;
-  auto fits = [&](size_t c) {
+  const size_t slots = (d_key <= 64 ? 2 : 1) * kComputeUnits;
+  if (n_seqs * lanes > slots) return 0;
+  auto fits = [&](size_t c, size_t slots) {
     size_t items = 0;
     for (size_t i = 0; i < n_seqs; ++i)
       items += lens ? std::max<size_t>(1, (lens[i] + c * LA_C - 1) / (c * LA_C)) : (longest + c * LA_C - 1) / (c * LA_C);
-    return items * lanes <= kComputeUnits;
+    return items * lanes <= slots;
   };
-  size_t lo = 1, hi = chunks;  // the fewest chunks of a segment that fit; all of them do
+  size_t lo = 2, hi = std::max<size_t>(chunks, 2);  // the fewest chunks of a segment that fit; all of them do
+  if (fits(1, kComputeUnits)) lo = hi = 1;
   while (lo < hi) {
     const size_t mid = (lo + hi) / 2;
-    if (fits(mid)) hi = mid; else lo = mid + 1;
+    if (fits(mid, slots)) hi = mid; else lo = mid + 1;
   }
   return 2 * lo + 5 <= chunks ? (int)(lo * LA_C) : 0;
 }

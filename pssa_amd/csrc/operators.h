@@ -82,7 +82,7 @@ struct LinearArgs {
 };
 Status init_linear_attributes();
 // Tokens of a segment where a call of these sizes is split, else 0.
-int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_val);
+int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val);
 Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int longest);
 
 }  // namespace pssa
