@@ -650,7 +650,8 @@ def check_linear(hip, lens, h, hk, dk, dv, dtype, with_state, gap=0, out_gap=0, 
     ([200], 3, 1, 100, 192, False), ([300, 17], 1, 1, 128, 64, True), ([7] * 300, 1, 1, 16, 16, True),
     (list(range(300)), 1, 1, 16, 24, False), ([1500], 2, 2, 64, 32, True),
     # Split into segments: ragged ends, sequences of one segment and of none, one end on a segment's border.
-    ([900, 0, 3, 513, 256, 512], 2, 1, 24, 72, True), ([1029], 1, 1, 128, 130, True), ([640, 640], 3, 3, 40, 8, False)])
+    ([900, 0, 3, 513, 256, 512], 2, 1, 24, 72, True), ([1029], 1, 1, 128, 130, True), ([640, 640], 3, 3, 40, 8, False),
+    ([1500] + [3] * 299, 1, 1, 16, 16, True)])
 def test_linear_attention_matches_the_recurrence(hip, dtype, lens, h, hk, dk, dv, with_state):
     say(f"linear {len(lens)} sequences, {sum(lens)} tokens, {h}/{hk} heads {dk} x {dv} {dtype}")
     check_linear(hip, lens, h, hk, dk, dv, dtype, with_state)
