@@ -448,7 +448,8 @@ template <int DKP, bool LOCAL>
 constexpr int kKeepers = LOCAL && DKP >= 64 ? 2 : 1;
 
 // LDS units (16 bytes) of the kernel: two buffers of q | k | v, P, and q S.
-template <int DKP, int WAVES, bool LOCAL>
+constexpr int WAVES = 4;  // of a group: 16 value columns each
+template <int DKP, bool LOCAL>
 struct ChunkLds {
   static constexpr int kQ = LOCAL ? 0 : LA_C * DKP / 8, kK = LA_C * DKP / 8, kV = LA_C * 2 * WAVES;
   static constexpr int kBuffer = kQ + kK + kV;
@@ -458,16 +459,15 @@ struct ChunkLds {
 // A tile of 16 WAVES value columns takes two groups of as many waves: one
 // computes P and P v and stores the outputs, the other keeps S, computes q S
 // (handed over through LDS) and the next S.  Both halves of a chunk's work
-// are about as long, and every SIMD has a wave of each.  (One group doing
-// both in turn took 7000 cycles a chunk at heads of 64, two of them with
-// two workgroups' state passes in between.)
+// are about as long, and every SIMD has a wave of each (heads of 64: 5500
+// cycles a chunk, against 7000 of one group that does both in turn).
 // LB: bytes of one load, 16 where every row and head is so aligned, else 4.
-template <int DKP, int WAVES, int MODE, int LB>
+template <int DKP, int MODE, int LB>
 __global__ __launch_bounds__((64 * WAVES * (MODE == LA_LOCAL ? kKeepers<DKP, true> : 2)), (MODE == LA_LOCAL || DKP == 128 ? 2 : 4)) void linear_chunks_bf16_kernel(
     LinearArgs a) {
   constexpr bool LOCAL = MODE == LA_LOCAL;
   constexpr int KEEPERS = kKeepers<DKP, LOCAL>, ALL = (LOCAL ? 0 : WAVES) + KEEPERS * WAVES;
-  using Lds = ChunkLds<DKP, WAVES, LOCAL>;
+  using Lds = ChunkLds<DKP, LOCAL>;
   constexpr int DVT = 16 * WAVES, NB = DKP / 16 / KEEPERS, KP = DKP / 32;
   constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;  // instructions of a chunk, of a wave
   constexpr int SLOTS = (kPairs + WAVES - 1) / WAVES;
@@ -820,7 +820,7 @@ __global__ __launch_bounds__((MODE == LA_LOCAL ? 256 * kKeepers<DKP, true> : 512
     LinearArgs a) {
   constexpr bool LOCAL = MODE == LA_LOCAL;
   using Lds = ChunkLds32<DKP, LOCAL>;
-  constexpr int KEEPERS = kKeepers<DKP, LOCAL>, WAVES = 4, ALL = LOCAL ? 4 * KEEPERS : 8, DVT = 64, NB = DKP / 16 / KEEPERS;
+  constexpr int KEEPERS = kKeepers<DKP, LOCAL>, ALL = LOCAL ? 4 * KEEPERS : 8, DVT = 64, NB = DKP / 16 / KEEPERS;
   constexpr int LOADS = Lds::kBuffer / 64 * (16 / LB), PER = (LOADS + ALL - 1) / ALL;
   extern __shared__ __attribute__((aligned(256))) f32x4_t s_f32[];
   f32x4_t* sP = s_f32 + 2 * Lds::kBuffer;  // [tiles (1, 0), (1, 1), (0, 0) of queries and keys][64 lanes]
@@ -1168,9 +1168,9 @@ struct Chunks {
 };
 template <int DKP, int NC, int MODE, int LB>
 struct ChunksBf16 {
-  static constexpr size_t kLds = ChunkLds<DKP, 4, MODE == LA_LOCAL>::kBytes;
+  static constexpr size_t kLds = ChunkLds<DKP, MODE == LA_LOCAL>::kBytes;
   static constexpr int kThreads = MODE == LA_LOCAL ? 256 * kKeepers<DKP, true> : 512, kColumns = 64;
-  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, 4, MODE, LB>;
+  static constexpr auto kKernel = &linear_chunks_bf16_kernel<DKP, MODE, LB>;
 };
 template <int DKP, int NC, int MODE>
 struct Chunks<Bf16, DKP, NC, MODE, 16> : ChunksBf16<DKP, NC, MODE, 16> {};

@@ -152,14 +152,38 @@ __device__ __forceinline__ float tile_max(const u32x4_t (&u)[NV]) {
   return fmaxf(m0, m1);
 }
 
+// The value of the lane whose number differs in one bit, in registers (`off`
+// constant; every lane active): a step of 8 to 16 cycles, where a shuffle
+// through LDS takes a hundred.
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int off) {
+  switch (off) {
+    case 1: return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);  // quads 1 0 3 2
+    case 2: return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);  // quads 2 3 0 1
+    case 4:  // eights mirrored, then quads
+      return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);
+    case 8: return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);  // sixteens rotated by 8
+    case 16: {
+      const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+      return threadIdx.x & 16 ? r[0] : r[1];
+    }
+    default: {
+      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+      return threadIdx.x & 32 ? r[0] : r[1];
+    }
+  }
+}
+__device__ __forceinline__ float lane_xor(float v, int off) { return __uint_as_float(lane_xor(__float_as_uint(v), off)); }
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v, int off) {
+  return (uint64_t)lane_xor((uint32_t)(v >> 32), off) << 32 | lane_xor((uint32_t)v, off);
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = 32; o >= 1; o >>= 1) v += lane_xor(v, o);
   return v;
 }
 __device__ __forceinline__ float wave_max(float v) {  // NaN never becomes the maximum
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, lane_xor(v, o));
   return v;
 }
 
@@ -177,12 +201,12 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ int key_id(uint64_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ uint64_t key_step(uint64_t a, int off, bool keep_max) {
-  const uint64_t o = __shfl_xor((unsigned long long)a, off, 64);
+  const uint64_t o = lane_xor(a, off);
   return (o > a) == keep_max ? o : a;
 }
 __device__ __forceinline__ uint32_t value_key(float v) { return (uint32_t)(token_key(v, 0) >> 32); }
 __device__ __forceinline__ uint32_t key_step(uint32_t a, int off, bool keep_max) {
-  const uint32_t o = __shfl_xor(a, off, 64);
+  const uint32_t o = lane_xor(a, off);
   return keep_max ? max(o, a) : min(o, a);
 }
 // The wave's 64 keys, largest in lane 0 (bitonic, 21 exchanges).
@@ -254,7 +278,8 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
   // began behind the first n_before had too many, its tokens from the row.
   auto settle = [&](int n, int n_before, int tile0) {
     uint64_t list = 0;
-    if (n > kCandidates) {
+    const bool many = n > kCandidates;
+    if (many) {
       uint64_t last = ~(uint64_t)0;
       for (int i = 0; i < top; ++i) {
         uint64_t mine = 0;
@@ -277,11 +302,14 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
       n = n_before;
     }
     if (wave == 0) {
-      best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
+      if (many) best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
 #pragma unroll 1
       for (int c = 0; c < n; c += 64) {
         const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : (uint64_t)0, lane);
-        best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
+        if (!MANY && c == 0 && !many)
+          best = got;
+        else
+          best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
       }
       if (lane == top - 1) s_kth = (uint32_t)(best >> 32);
       if (lane == 0) s_count = 0;
@@ -324,7 +352,7 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
         float gm = bv;
         if (!fine) {
 #pragma unroll
-          for (int off = 1; off < W; off <<= 1) gm = fmaxf(gm, __shfl_xor(gm, off, 64));
+          for (int off = 1; off < W; off <<= 1) gm = fmaxf(gm, lane_xor(gm, off));
         }
         uint32_t key = value_key(gm);
         if constexpr (W > 1) {
