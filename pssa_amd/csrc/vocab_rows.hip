@@ -176,6 +176,12 @@ __device__ __forceinline__ float lane_xor(float v, int off) { return __uint_as_f
 __device__ __forceinline__ uint64_t lane_xor(uint64_t v, int off) {
   return (uint64_t)lane_xor((uint32_t)(v >> 32), off) << 32 | lane_xor((uint32_t)v, off);
 }
+// The value of lane 63 - lane: sixteens mirrored, then exchanged.
+__device__ __forceinline__ uint64_t lane_reverse(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((uint32_t)v, 0x140, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp((uint32_t)(v >> 32), 0x140, 0xF, 0xF, true);
+  return lane_xor(lane_xor((uint64_t)hi << 32 | lo, 16), 32);
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += lane_xor(v, o);
@@ -243,8 +249,8 @@ __device__ __forceinline__ Key wave_merge(Key a, Key b_reversed, int lane) {
 // equal, say) gives its k tokens one by one, each round the largest behind
 // the one before.
 //
-// 8192 fp32 rows of 16384, 8 alternatives: 129 us (4.2 TB/s); 509 bf16 rows of
-// 100003, 5 of them: 39 us (2.6 TB/s); one row of 16384: 9 us, mostly latency.
+// 8192 fp32 rows of 16384, 8 alternatives: 114 us (4.7 TB/s); 509 bf16 rows of
+// 100003, 5 of them: 36 us (2.8 TB/s); one row of 16384: 7 us, mostly latency.
 constexpr int kCandidates = 1024;
 constexpr int kSlots = 8;  // threads of a wave whose vectors are looked through at once
 
@@ -302,14 +308,14 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
       n = n_before;
     }
     if (wave == 0) {
-      if (many) best = wave_merge(best, (uint64_t)__shfl((unsigned long long)list, 63 - lane, 64), lane);
+      if (many) best = wave_merge(best, lane_reverse(list), lane);
 #pragma unroll 1
       for (int c = 0; c < n; c += 64) {
         const uint64_t got = wave_sort(c + lane < n ? s_cand[c + lane] : (uint64_t)0, lane);
         if (!MANY && c == 0 && !many)
           best = got;
         else
-          best = wave_merge(best, (uint64_t)__shfl((unsigned long long)got, 63 - lane, 64), lane);
+          best = wave_merge(best, lane_reverse(got), lane);
       }
       if (lane == top - 1) s_kth = (uint32_t)(best >> 32);
       if (lane == 0) s_count = 0;
@@ -509,7 +515,7 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
 // registers that the sums were taken from; the few teacher's tokens are then
 // written again with their q.
 // 8192 fp32 rows of 16384: 219 us (4.9 TB/s); 777 bf16 rows of 65537: 63 us
-// (4.6 TB/s with the second read); 37 fp32 rows of 2048: 6 us, latency.
+// (4.6 TB/s with the second read); 37 fp32 rows of 2048: 5 us, latency.
 // MANY: the row takes several tiles, each thread with a maximum and sum of its
 // own until the end, each tile loaded while the one before is summed.
 template <class T, int W, int NV, bool MANY>
@@ -713,9 +719,9 @@ Status distill(hipStream_t stream, const DistillArgs& a, size_t rows) {
 // tile that holds the row where no more than these are needed for it.
 //   us, with 8 alternatives:      256 rows of          3000 rows of
 //                               65537 100003 bf16    65537 100003 bf16
-//     16 waves                     23     28            261    310
-//     8 waves                      24     31            171    228
-//     4 waves                      35     53            138    195
+//     16 waves                     19     24            222    273
+//     8 waves                      21     28            149    204
+//     4 waves                      31     47            122    182
 template <class T>
 Status launch_logprobs(hipStream_t stream, const LogprobArgs& a, size_t rows) {
   const int vecs = (a.vocab + vec_n<T>() - 1) / vec_n<T>();
