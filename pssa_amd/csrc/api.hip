@@ -2027,7 +2027,7 @@ int pssa_hip_dense_scan_reserve(pssa_hip_ctx* ctx, size_t batch, size_t seq_len,
 // 4-bit weights on the device.
 struct pssa_hip_w4 {
   pssa_hip_ctx* ctx = nullptr;
-  DevBuf packed, scales, zeros;
+  DevBuf data;  // codes, scales and zero points, one behind the other
   pssa::W4View view;
 };
 
@@ -2097,15 +2097,16 @@ Status load_w4(pssa_hip_ctx* ctx, const uint8_t* codes, const float* scales, con
                size_t group, std::unique_ptr<pssa_hip_w4>& w) {
   w = std::make_unique<pssa_hip_w4>();
   w->ctx = ctx;
-  const size_t held = pssa::w4_groups_held(n, k, group);
-  PSSA_RETURN_IF(w->packed.alloc(pssa::w4_packed_bytes(n, k)));
-  PSSA_RETURN_IF(w->scales.alloc(held * 4));
-  if (zeros) PSSA_RETURN_IF(w->zeros.alloc(held));
-  PSSA_RETURN_IF(pssa::launch_w4_pack(ctx->stream, codes, scales, zeros, (int)n, (int)k, (int)group, w->packed.p,
-                                      w->scales.as<float>(), w->zeros.as<uint8_t>()));
-  w->view.packed = w->packed.p;
-  w->view.scales = w->scales.as<float>();
-  w->view.zeros = zeros ? w->zeros.as<uint8_t>() : nullptr;
+  const size_t held = pssa::w4_groups_held(n, k, group), packed = pssa::w4_packed_bytes(n, k);
+  PSSA_RETURN_IF(w->data.alloc(packed + held * (zeros ? 5 : 4)));
+  char* base = w->data.as<char>();
+  float* held_scales = reinterpret_cast<float*>(base + packed);
+  uint8_t* held_zeros = zeros ? reinterpret_cast<uint8_t*>(held_scales + held) : nullptr;
+  PSSA_RETURN_IF(
+      pssa::launch_w4_pack(ctx->stream, codes, scales, zeros, (int)n, (int)k, (int)group, base, held_scales, held_zeros));
+  w->view.packed = base;
+  w->view.scales = held_scales;
+  w->view.zeros = held_zeros;
   w->view.n = (int)n;
   w->view.k = (int)k;
   w->view.group = (int)group;
