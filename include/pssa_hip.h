@@ -702,7 +702,11 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
                                        size_t heads, size_t kv_heads, size_t d_key, size_t d_val, float scale,
                                        void* d_out, size_t ld_out, float* d_state_out, char* err, size_t err_len);
 /* Grows the context's scratch (synchronously) to what such a call needs, so
- * that it then allocates nothing and stays asynchronous. */
+ * that it then allocates nothing and stays asynchronous.  More than 256
+ * sequences of unequal lengths take a table of 4 (n_seqs + 1) bytes (twice
+ * that where the call is split) in the scratch; tables of 32 KiB and more go
+ * there through 4 MiB of pinned slots, and a call that finds these full of
+ * tables still on their way waits for the stream. */
 int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
                                       size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len);
 

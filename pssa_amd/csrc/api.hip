@@ -2131,8 +2131,11 @@ bool rows_disjoint(const void* p, size_t ld, size_t w, const void* o, size_t ldo
 
 // The sequences of a linear attention call and their split into work items.
 struct LinearPlan {
-  std::vector<uint32_t> table;  // first tokens and items, where the arguments do not hold them
+  std::vector<uint32_t> table;  // first tokens (and a split call's items), where the arguments do not hold them
   size_t tokens = 0, longest = 0;
+  size_t states = 0;  // bytes of the scratch before the table: a split call's states, one for each item
+
+  size_t scratch_bytes() const { return states + table.size() * 4; }
 };
 Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_key,
                       size_t d_val, pssa::LinearArgs& a, LinearPlan& p) {
@@ -2155,25 +2158,22 @@ Status plan_sequences(const uint64_t* lens, size_t n_seqs, size_t seq_len, size_
     a.items = (int)n_seqs * a.uniform_segs;
   } else {
     const bool inside = n_seqs <= (size_t)pssa::kLinearInline;
-    if (!inside) p.table.resize(2 * (n_seqs + 1));
+    if (!inside) p.table.resize((seg ? 2 : 1) * (n_seqs + 1));
     uint32_t* tok = inside ? a.inline_tokens : p.table.data();
-    uint32_t* item = inside ? a.inline_items : p.table.data() + n_seqs + 1;
+    uint32_t* item = !seg ? nullptr : inside ? a.inline_items : p.table.data() + n_seqs + 1;
     uint32_t t = 0, w = 0;
     for (size_t i = 0; i < n_seqs; ++i) {
       tok[i] = t;
-      item[i] = w;
+      if (item) item[i] = w;
       t += (uint32_t)lens[i];
       w += (uint32_t)std::max<size_t>(1, (lens[i] + a.seg_len - 1) / a.seg_len);
     }
     tok[n_seqs] = t;
-    item[n_seqs] = w;
+    if (item) item[n_seqs] = w;
     a.items = (int)w;
   }
+  if (a.items > a.n_seqs) p.states = ((size_t)a.items * heads * d_key * d_val * 4 + 255) & ~(size_t)255;
   return Status::Ok();
-}
-// Scratch of a split call: a state for each item.
-size_t linear_scratch_bytes(const pssa::LinearArgs& a, size_t heads, size_t d_key, size_t d_val) {
-  return a.items > a.n_seqs ? (size_t)a.items * heads * d_key * d_val * 4 : 0;
 }
 
 Status check_heads(size_t heads, size_t d_key, size_t d_val) {
@@ -2514,14 +2514,12 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
     a.dv = (int)d_val;
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
-    DevBuf dt;
+    PSSA_RETURN_IF(grow_scratch(ctx, plan.scratch_bytes(), false));
+    if (plan.states) a.seg_state = static_cast<float*>(ctx->scratch);
     if (!plan.table.empty()) {
-      PSSA_RETURN_IF(upload(ctx, dt, plan.table.data(), plan.table.size() * 4));
-      a.table = dt.as<uint32_t>();
-    }
-    if (const size_t bytes = linear_scratch_bytes(a, heads, d_key, d_val)) {
-      PSSA_RETURN_IF(grow_scratch(ctx, bytes, false));
-      a.seg_state = static_cast<float*>(ctx->scratch);
+      uint32_t* table = reinterpret_cast<uint32_t*>(static_cast<char*>(ctx->scratch) + plan.states);
+      PSSA_RETURN_IF(ctx->stage.to_device(table, plan.table.data(), plan.table.size() * 4, ctx->stream));
+      a.table = table;
     }
     return pssa::launch_linear_attention(ctx->stream, dtype, a, (int)plan.longest);
   }, err, err_len);
@@ -2538,7 +2536,7 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
-    return grow_scratch(ctx, linear_scratch_bytes(a, heads, d_key, d_val), false);
+    return grow_scratch(ctx, plan.scratch_bytes(), false);
   }, err, err_len);
 }
 

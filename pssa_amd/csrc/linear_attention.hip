@@ -72,7 +72,8 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(Bf16* p, float v) { p->bits = bf16_bits_dev(v); }
 
 // What a workgroup walks: a segment's first token and length, and where its
-// state is (the sequence's, or its own one in the scratch of a split call).
+// state is (the sequence's, or its own one in the scratch of a split call,
+// which seg_state tells from one that is not).
 struct Span {
   int seq, item;
   size_t tok;
@@ -101,13 +102,14 @@ __device__ __forceinline__ Span span_of(const LinearArgs& a, int item) {
     s.tok = (size_t)s.seq * a.uniform_len;
     len = a.uniform_len;
   } else {
-    int lo = 0, hi = a.n_seqs - 1;  // the last sequence that begins at or before the item
+    int lo = item, hi = item;  // not split: the tables have no items
+    if (a.seg_state) lo = 0, hi = a.n_seqs - 1;  // the last sequence that begins at or before the item
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (first_item(a, mid) <= item) lo = mid; else hi = mid - 1;
     }
     s.seq = lo;
-    seg = item - first_item(a, lo);
+    seg = a.seg_state ? item - first_item(a, lo) : 0;
     s.tok = first_token(a, lo);
     len = (int)(first_token(a, lo + 1) - s.tok);
   }

@@ -75,7 +75,7 @@ struct LinearArgs {
   float* seg_state = nullptr;       // [items, heads, dk, dv] of a split call
   int uniform_len = -1;             // every sequence's length, or -1: the tables
   int uniform_segs = 1;             // its segments
-  // [n_seqs + 1] first tokens, then as many first items: on the device, or null and here.
+  // [n_seqs + 1] first tokens and, in a split call, as many first items: on the device, or null and here.
   const uint32_t* table = nullptr;
   uint32_t inline_tokens[kLinearInline + 1] = {};
   uint32_t inline_items[kLinearInline + 1] = {};

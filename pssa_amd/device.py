@@ -352,8 +352,8 @@ class HipDevice:
 
     def linear_attention_reserve(self, dtype: str, heads: int, d_key: int, d_val: int, lens=None, n_seqs: int = 1,
                                  seq_len: int = 1) -> None:
-        """Sizes the context's scratch for linear_attention_resident calls of this shape, so that they allocate
-        nothing."""
+        """Sizes the context's scratch for linear_attention_resident calls of these lengths and widths, so that they
+        allocate nothing."""
         if lens is not None:
             lens, n_seqs = _lens(lens), len(lens)
         _abi.call(self._lib.pssa_hip_linear_attention_reserve, self.handle, _dtype(dtype), lens, n_seqs, seq_len, heads,

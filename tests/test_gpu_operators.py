@@ -833,3 +833,65 @@ def test_rows_past_one_launch(hip):
         assert np.all(np.abs(loss.to_host() + ref) <= tol)
         got = grad.to_host()
         assert np.all(np.abs(got[at, t] - (p - 1)) <= tol) and np.all(np.abs(got[at, 1 - t] - (1 - p)) <= tol)
+
+
+def free_device_bytes():
+    import ctypes as C
+
+    free, total = C.c_size_t(), C.c_size_t()
+    assert C.CDLL("libamdhip64.so").hipMemGetInfo(C.byref(free), C.byref(total)) == 0
+    return free.value
+
+
+@pytest.mark.parametrize("n,most", [(65535, 2), (400, 900)])
+def test_linear_attention_reserved_calls_of_many_ragged_sequences_allocate_nothing(hip, n, most):
+    """After a reservation the tables of many sequences of unequal lengths take no memory either; one or two tokens a
+    sequence against the recurrence, written out."""
+    from pssa_amd import HipDevice
+    from pssa_amd.device import _lens
+
+    say("linear reserved", n, "ragged sequences")
+    rng = np.random.default_rng(n)
+    lens = rng.integers(1, 3, n)
+    lens[n // 2] = most
+    first = np.cumsum(lens) - lens
+    tokens, d, lam = int(lens.sum()), 4, np.float32(-0.5)
+    q, k, v = (rng.normal(0, 1, (tokens, d)).astype(np.float32) for _ in range(3))
+    c_lens = _lens([int(x) for x in lens])
+    others = [HipDevice(0) for _ in range(24)]  # as many tables would be seen in the device's free memory
+    with Held(hip) as b:
+        x, g = [b.up(a) for a in (q, k, v)], b.up(np.full(1, lam))
+        o, s = b.new((tokens, d), np.float32, 7.0), b.new((n, d, d), np.float32, 7.0)
+        hip.synchronize()
+
+        def call(dev):
+            dev.linear_attention_resident(x[0].ptr, x[1].ptr, x[2].ptr, g.ptr, "f32", 1, d, d, o.ptr, c_lens,
+                                          state_out_ptr=s.ptr)
+            dev.synchronize()
+
+        call(hip)  # what the runtime sets up for a first call is there
+        for dev in others:
+            dev.linear_attention_reserve("f32", 1, d, d, c_lens)
+        before = free_device_bytes()
+        for dev in others:
+            call(dev)
+        after = free_device_bytes()
+        out, state = o.to_host(), s.to_host()
+    for dev in others:
+        dev.close()
+    assert after == before
+    f = np.exp(np.float64(lam))
+    outer = k.astype(np.float64)[:, :, None] * v[:, None, :]
+    second = first[lens == 2] + 1
+    sums = outer.copy()
+    sums[second] += f * outer[second - 1]
+    size = np.abs(outer)
+    size[second] += f * size[second - 1]
+    short = lens <= 2
+    at = np.concatenate([first[short], second])
+    ref = np.einsum("td,tdv->tv", q.astype(np.float64), sums)
+    bound = np.einsum("td,tdv->tv", np.abs(q).astype(np.float64), size)
+    # Four products and their sum, one step of the state with the decay's own rounding.
+    assert np.all(np.abs(out[at] - ref[at]) <= U32 * 16 * bound[at])
+    ends = first[short] + lens[short] - 1
+    assert np.all(np.abs(state[short] - sums[ends]) <= U32 * 8 * size[ends])
