@@ -895,3 +895,44 @@ def test_linear_attention_reserved_calls_of_many_ragged_sequences_allocate_nothi
     assert np.all(np.abs(out[at] - ref[at]) <= U32 * 16 * bound[at])
     ends = first[short] + lens[short] - 1
     assert np.all(np.abs(state[short] - sums[ends]) <= U32 * 8 * size[ends])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gap", [2, 3])
+@pytest.mark.parametrize("length,at,dk,dv", [(150, (100,), 32, 40), (70, (69,), 36, 130), (130, (0, 64, 129), 20, 66),
+                                             (700, (300, 301, 640), 32, 40), (700, (63,), 100, 72)])
+def test_linear_attention_of_any_alignment_keeps_what_is_not_finite(hip, dtype, gap, length, at, dk, dv):
+    """As above with loads of 4 bytes and with rows at any element, which take kernels of their own, whole and in
+    segments: values that are not finite in some tokens' v, k or q leave earlier tokens and the other sequence alone."""
+    say("linear not finite, any alignment", gap, length, at, dk, dv, dtype)
+    rng = np.random.default_rng([gap, length, dk])
+    lens, h, hk = [length, 20], 2, 1
+    n = sum(lens)
+    q, k, v = (rng.normal(0, 1, s) for s in ((n, h, dk), (n, hk, dk), (n, hk, dv)))
+    g = np.log(np.array([0.9, 0.99])).astype(np.float32)
+    for which, value in (("v", np.nan), ("v", -np.inf), ("k", np.inf), ("k", np.nan), ("q", np.nan)):
+        x = {"q": q.copy(), "k": k.copy(), "v": v.copy()}
+        for i in at:
+            x[which][i, -1, 3] = value
+        out, last, held = run_linear(hip, x["q"], x["k"], x["v"], g, lens, 1.0, None, dtype, gap, 1)
+        with np.errstate(invalid="ignore"):
+            ref, rlast, (size, ssize) = linear64(*held, g, lens, 1.0, None)
+        fine, sfine = np.isfinite(ref), np.isfinite(rlast)
+        assert fine[:at[0]].all() and fine[length:].all() and not fine.all() and sfine[1].all()
+        assert np.isfinite(out[fine]).all() and not np.isfinite(out[~fine]).any(), which
+        assert np.isfinite(last[sfine]).all() and not np.isfinite(last[~sfine]).any(), which
+        # d_key + 64 terms in a product, one for each of up to 11 chunks' states, powers and products: below 300; two
+        # bf16 parts of the state and of the products of q and k where the inputs are bf16.
+        low = 3 * 2.0 ** -17 if dtype == "bf16" else 0.0
+        tol = (U32 * 300 + low) * size[fine] + (U16 * np.abs(ref[fine]) if dtype == "bf16" else 0)
+        assert np.all(np.abs(out[fine] - ref[fine]) <= tol), which
+        assert np.all(np.abs(last[sfine] - rlast[sfine]) <= U32 * 300 * ssize[sfine]), which
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gap", [0, 3])
+def test_linear_attention_of_a_prompt_beside_single_tokens(hip, dtype, gap):
+    """A prompt and the next token of many streams in one call, more of them than a split call has room for."""
+    say("linear prompt beside single tokens", gap, dtype)
+    check_linear(hip, [1] * 35 + [900] + [1, 0, 2] * 12, 8, 2, 16, 24, dtype, True, gap)
+    check_linear(hip, [1] * 300 + [500] + [1] * 50, 2, 1, 16, 24, dtype, True, gap)
