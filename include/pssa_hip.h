@@ -606,7 +606,8 @@ int pssa_hip_lanes_stage_times(pssa_hip_lanes* lanes, int enable, const char** n
  * A logit of -inf is a token that cannot occur: it has log probability -inf
  * and is never an alternative (places left over hold PSSA_HIP_NO_TOKEN and
  * -inf).  A row of nothing else has entropy 0.  A row with a NaN or +inf has
- * NaN in every value and no alternatives.  temperature in [1e-6, 1e6]. */
+ * NaN in every value and no alternatives.  temperature in [1e-6, 1e6].  The
+ * outputs must not overlap the logits. */
 int pssa_hip_token_logprobs_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t rows, size_t vocab,
                                      size_t ld, const uint32_t* d_targets, float temperature, size_t top_k,
                                      float* d_logprobs, float* d_entropy, uint32_t* d_top_ids,
@@ -622,7 +623,7 @@ int pssa_hip_token_logprobs_resident(pssa_hip_ctx* ctx, const void* d_logits, in
  * has both entries' weight.  d_row_weights [rows] or NULL (1).  d_grad (the
  * logits' type, row r at d_grad + r*ld_grad) or NULL for the loss alone; it
  * may be d_logits itself with ld_grad = ld, and must not overlap it
- * otherwise.  A row of weight 0, or without teacher entries, has loss 0 and
+ * otherwise; neither output may overlap the call's other arrays.  A row of weight 0, or without teacher entries, has loss 0 and
  * gradient 0 whatever it holds.  A teacher's token whose student logit is
  * -inf gives the loss +inf (and a finite gradient); a NaN or +inf among the
  * student's or teacher's logits, or a teacher id >= vocab, makes the row's
@@ -692,7 +693,8 @@ int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, f
  * [n_seqs, heads, d_key, d_val]: d_state_in NULL starts from zeros,
  * d_state_out (NULL: not kept) receives the states behind the last tokens and
  * may be d_state_in.  out may lie in the buffer of q, k and v in columns of
- * its own (same row stride) and must not overlap them otherwise.  d_key <= 128,
+ * its own (same row stride) and must not overlap them, d_log_decay or a state
+ * otherwise.  d_key <= 128,
  * d_val <= 4096, n_seqs and heads <= 65535, row strides below 2^24.  bf16
  * outputs round once; every sum and the states are fp32.  A value that is not
  * finite reaches the outputs from its own token on and no earlier one. */

@@ -2487,7 +2487,14 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
                             rows_disjoint(d_k, ld_k, wk, d_out, ld_out, wo, tokens, size) &&
                             rows_disjoint(d_v, ld_v, wv, d_out, ld_out, wo, tokens, size),
                         "linear attention: the output overlaps its inputs"));
+    if (tokens) {
+      const size_t out_bytes = ((tokens - 1) * ld_out + wo) * size;
+      PSSA_RETURN_IF(need(disjoint(d_log_decay, heads * 4, d_out, out_bytes), "linear attention: the output overlaps its inputs"));
+      PSSA_RETURN_IF(need(!d_state_in || disjoint(d_state_in, n * 4, d_out, out_bytes),
+                          "linear attention: the output overlaps the states"));
+    }
     if (d_state_out) {
+      PSSA_RETURN_IF(need(disjoint(d_log_decay, heads * 4, d_state_out, n * 4), "linear attention: the states overlap"));
       PSSA_RETURN_IF(need(!d_state_in || d_state_in == d_state_out || disjoint(d_state_in, n * 4, d_state_out, n * 4),
                           "linear attention: the states overlap"));
       if (tokens)

@@ -147,3 +147,16 @@ def test_linear_attention_reserve_and_lens_refuse():
     assert list(_lens([3, 0, 5])) == [3, 0, 5]
     with pytest.raises(ValueError, match="negative"):
         _lens([3, -1])
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"state_in": P + 0x30000}, "the output overlaps the states"), ({"state_in": P + 0x30000 + 15 * 384 + 380}, "overlaps the states"),
+    ({"state_in": P + 0x30000 + 15 * 384 + 384}, "null context"), ({"state_in": P + 0x30000 - 12288}, "null context"),
+    ({"state_in": P + 0x30000 - 12284}, "overlaps the states"),
+    ({"decay": P + 0x30000 - 12}, "overlaps its inputs"), ({"decay": P + 0x30000 - 16}, "null context"),
+    ({"decay": P + 0x40000 + 12284}, "states overlap"), ({"decay": P + 0x40000 + 12288}, "null context"),
+    ({"decay": P + 0x30000, "seq_len": 0}, "null context")])
+def test_linear_attention_refuses_outputs_over_what_it_still_reads(change, message):
+    """Heads of a token are written while other workgroups read the entry states and the decays: 16 tokens of 384 bytes
+    out, 2 x 4 states of 16 x 24 values (12288 bytes), 4 decays."""
+    refused(_abi.lib().pssa_hip_linear_attention_resident, changed(LINEAR, **change), message)
