@@ -636,7 +636,9 @@ int pssa_hip_distill_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype
 /* The same on the logits that the last pssa_hip_batch_forward of these lanes
  * left on the device, host arrays in and out, rows in that call's packed
  * token order (n_tokens of them, which must be its token count).
- * targets NULL: the batch's own targets.  Any output may be NULL. */
+ * targets NULL: the batch's own targets.  Any output may be NULL.  In these
+ * host forms a target or teacher id outside the vocabulary that is not
+ * PSSA_HIP_NO_TOKEN is PSSA_HIP_EINVAL. */
 int pssa_hip_batch_token_logprobs(pssa_hip_lanes* lanes, const uint32_t* targets, size_t n_tokens, float temperature,
                                   size_t top_k, float* logprobs, float* entropy, uint32_t* top_ids,
                                   float* top_logprobs, char* err, size_t err_len);

@@ -2084,6 +2084,14 @@ Status check_batch(const pssa_hip_lanes* L, size_t n_tokens) {
   return need(n_tokens == L->tok_row.size(), "token count must be the last batch forward's");
 }
 
+// Token ids of a host array: the model's or none.
+Status check_tokens(const uint32_t* ids, size_t n, size_t V, const char* what) {
+  for (size_t i = 0; i < n; ++i)
+    if (ids[i] >= V && ids[i] != PSSA_HIP_NO_TOKEN)
+      return Status::Invalid(std::string(what) + " token ID " + std::to_string(ids[i]) + " outside model vocabulary");
+  return Status::Ok();
+}
+
 Status check_w4(size_t n, size_t k, size_t group) {
   PSSA_RETURN_IF(need(n && k, "4-bit weights: dimensions must be positive"));
   PSSA_RETURN_IF(need(group == 32 || group == 64 || group == 128, "4-bit weights: group must be 32, 64 or 128"));
@@ -2272,9 +2280,10 @@ int pssa_hip_batch_token_logprobs(pssa_hip_lanes* L, const uint32_t* targets, si
     PSSA_RETURN_IF(need(top_k <= (size_t)pssa::kMaxAlternatives, "token logprobs: top_k must be at most 64"));
     std::lock_guard<std::mutex> g(L->ctx->mu);
     PSSA_RETURN_IF(check_batch(L, n_tokens));
-    PSSA_HIP_TRY(hipSetDevice(L->ctx->device));
     pssa_hip_ctx* ctx = L->ctx;
     const size_t V = L->model->cfg.d_vocab;
+    if (targets) PSSA_RETURN_IF(check_tokens(targets, n_tokens, V, "token logprobs: target"));
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
     std::vector<uint32_t> target_h;
     rows_to_device_order(L->tok_row, targets ? targets : L->tok_target.data(), 1, target_h);
     DevBuf dt, lp, en, id, tl;
@@ -2315,10 +2324,7 @@ int pssa_hip_batch_distill(pssa_hip_lanes* L, const uint32_t* teacher_ids, const
     PSSA_RETURN_IF(check_batch(L, n_tokens));
     pssa_hip_ctx* ctx = L->ctx;
     const size_t V = L->model->cfg.d_vocab;
-    for (size_t i = 0; i < n_tokens * teacher_k; ++i)
-      if (teacher_ids[i] >= V && teacher_ids[i] != PSSA_HIP_NO_TOKEN)
-        return Status::Invalid("distill: teacher token ID " + std::to_string(teacher_ids[i]) +
-                               " outside model vocabulary");
+    PSSA_RETURN_IF(check_tokens(teacher_ids, n_tokens * teacher_k, V, "distill: teacher"));
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     std::vector<uint32_t> ids_h;
     std::vector<float> t_h, w_h;

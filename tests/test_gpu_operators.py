@@ -936,3 +936,23 @@ def test_linear_attention_of_a_prompt_beside_single_tokens(hip, dtype, gap):
     say("linear prompt beside single tokens", gap, dtype)
     check_linear(hip, [1] * 35 + [900] + [1, 0, 2] * 12, 8, 2, 16, 24, dtype, True, gap)
     check_linear(hip, [1] * 300 + [500] + [1] * 50, 2, 1, 16, 24, dtype, True, gap)
+
+
+def test_batch_scores_refuse_targets_outside_the_vocabulary(hip):
+    """Like a teacher's ids; "no token" and the last token are none of these."""
+    from pssa_amd import ModelWeights, PSSAConfig, PSSALayer, Sequence
+
+    say("batch scores refuse targets")
+    cfg = PSSAConfig(depth=1, d_vocab=70, d_latent=16, d_state=8, d_mem_key=8, mem_capacity=10)
+    layer = PSSALayer(hip, ModelWeights.init(cfg, 1, "baseline"), lanes=2, max_tokens=16)
+    ids = np.arange(5, dtype=np.uint32)
+    layer.batch_forward([Sequence(0, ids, ids, True)])
+    own = layer.token_logprobs(top_k=2)
+    for bad in (70, NONE - 1):
+        with pytest.raises(HipError, match="outside model vocabulary"):
+            layer.token_logprobs(targets=np.array([0, 1, bad, 3, 4], np.uint32))
+    got = layer.token_logprobs(targets=np.array([0, 1, 2, 69, NONE], np.uint32), top_k=2)
+    np.testing.assert_array_equal(got["logprobs"][:3], own["logprobs"][:3])
+    np.testing.assert_array_equal(got["top_ids"], own["top_ids"])
+    assert got["logprobs"][4] == 0 and np.isfinite(got["logprobs"]).all()
+    layer.close()
