@@ -956,3 +956,101 @@ def test_batch_scores_refuse_targets_outside_the_vocabulary(hip):
     np.testing.assert_array_equal(got["top_ids"], own["top_ids"])
     assert got["logprobs"][4] == 0 and np.isfinite(got["logprobs"]).all()
     layer.close()
+
+
+# ---------------------------------------------------------------------------
+# Rows far apart: offsets past 32 bits
+
+
+class Rows:
+    """Rows of `width` elements at a stride in one device array that is otherwise not set."""
+
+    def __init__(self, hip, rows, ld, dtype):
+        self.hip, self.ld, self.dtype = hip, ld, np.dtype(dtype)
+        self.buf = hip.empty((rows, ld), dtype)
+
+    def at(self, row, col=0):
+        return self.buf.ptr + (row * self.ld + col) * self.dtype.itemsize
+
+    def put(self, a, col=0):
+        for r, row in enumerate(a):
+            self.buf.write(row, (r * self.ld + col) * self.dtype.itemsize)
+
+    def get(self, rows, width, col=0):
+        import ctypes as C
+
+        out = np.empty((rows, width), self.dtype)
+        for r in range(rows):
+            _abi.call(self.hip._lib.pssa_hip_memcpy, self.hip.handle, out[r].ctypes.data_as(C.c_void_p),
+                      C.c_void_p(self.at(r, col)), width * self.dtype.itemsize, _abi.D2H)
+        return out
+
+
+def test_logit_rows_at_far_offsets(hip):
+    say("logit rows at far offsets")
+    rng = np.random.default_rng(1)
+    rows, vocab, ld, k = 6, 1003, (1 << 30) + 5, 8
+    stored, held = to_bf16(logits_like(rng, rows, vocab))
+    ids, t = teacher(rng, rows, vocab, 12, dead=0.0)
+    targets = rng.integers(0, vocab, rows).astype(np.uint32)
+    far = Rows(hip, rows, ld, np.uint16)
+    with Held(hip) as h:
+        far.put(stored)
+        di, dt, dg = h.up(ids), h.up(t), h.up(targets)
+        lp, loss = h.new(rows, np.float32, 7.0), h.new(rows, np.float32, 7.0)
+        ti, tl = h.new((rows, k), np.uint32, 7), h.new((rows, k), np.float32, 7.0)
+        hip.token_logprobs_resident(far.buf.ptr, "bf16", rows, vocab, dg.ptr, lp.ptr, None, k, ti.ptr, tl.ptr, ld=ld)
+        hip.distill_resident(far.buf.ptr, "bf16", rows, vocab, di.ptr, dt.ptr, 12, loss.ptr, far.buf.ptr, ld=ld)
+        hip.synchronize()
+        got = [a.to_host() for a in (lp, ti, loss)] + [from_bf16(far.get(rows, vocab))]
+    far.buf.close()
+    ref, _, _ = log_softmax64(held, 1.0)
+    assert np.all(np.abs(got[0] - ref[np.arange(rows), targets]) <= U32 * (4 * np.abs(ref).max() + 100))
+    np.testing.assert_array_equal(got[1], top64(held, k))
+    near, grad = run_distill(hip, stored, rows, vocab, vocab, ids, t, 1.0, None, "bf16")
+    np.testing.assert_array_equal(got[2], near)
+    np.testing.assert_array_equal(got[3], from_bf16(grad))
+
+
+@pytest.mark.parametrize("width", [16, 17])
+def test_linear_attention_rows_at_far_offsets(hip, width):
+    """q, k, v and the outputs as columns of rows 2^24 elements apart; heads of 17 take the kernel for any width."""
+    say("linear rows at far offsets", width)
+    rng = np.random.default_rng(width)
+    n, ld = 300, (1 << 24) - 8
+    x = rng.normal(0, 1, (n, 3 * width)).astype(np.float32)
+    stored, held = to_bf16(x)
+    g = np.full(1, -0.05, np.float32)
+    far = Rows(hip, n, ld, np.uint16)
+    with Held(hip) as h:
+        far.put(stored)
+        dg, s = h.up(g), h.new((1, 1, width, width), np.float32, 7.0)
+        hip.linear_attention_resident(far.at(0), far.at(0, width), far.at(0, 2 * width), dg.ptr, "bf16", 1, width, width,
+                                      far.at(0, 3 * width + 1), [n], scale=0.5, state_out_ptr=s.ptr, ld_q=ld, ld_k=ld,
+                                      ld_v=ld, ld_out=ld)
+        hip.synchronize()
+        out, state = from_bf16(far.get(n, width, 3 * width + 1)), s.to_host()
+    far.buf.close()
+    parts = [p.reshape(n, 1, width) for p in np.split(held, 3, 1)]
+    ref, rlast, (so, ss) = linear64(*parts, g, [n], 0.5, None)
+    part = U32 * (width + 64 + 2 * 5 + 12)
+    assert np.all(np.abs(out - ref[:, 0]) <= (part + 3 * 2.0 ** -17) * so[:, 0] + U16 * np.abs(ref[:, 0]) + 1e-30)
+    assert np.all(np.abs(state - rlast) <= part * ss + 1e-30)
+
+
+def test_matvec_w4_rows_at_far_offsets(hip):
+    say("w4 rows at far offsets")
+    rng = np.random.default_rng(2)
+    m, n, k, group, ld = 6, 35, 200, 64, (1 << 30) + 3
+    codes, scales, zp, w = w4_inputs(rng, n, k, group, True)
+    stored, held = to_bf16(rng.normal(0, 1, (m, k)).astype(np.float32))
+    mat = hip.w4_matrix(codes, scales, group, zp)
+    far, y = Rows(hip, m, ld, np.uint16), Rows(hip, m, ld, np.float32)
+    far.put(stored)
+    hip.matvec_w4_resident(far.buf.ptr, "bf16", m, mat, y.buf.ptr, ld_x=ld, ld_y=ld)
+    hip.synchronize()
+    got = y.get(m, n)
+    far.buf.close()
+    y.buf.close()
+    mat.close()
+    assert np.all(np.abs(got - held.astype(np.float64) @ w.T) <= w4_tolerance(held, codes, scales, zp, group))
