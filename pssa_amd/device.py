@@ -51,11 +51,27 @@ class HipDevice:
         self.handle = h
         # Objects holding native state tied to this context; closed first.
         self._children = weakref.WeakSet()
+        # What they hold, as calls that free it: the collector may finalise
+        # this object before them, with the weak references already gone.
+        self._native = {}
+
+    def _own(self, free, *args) -> object:
+        """Registers native state on this context; `_free` of what is returned frees it, once."""
+        key = object()
+        self._native[key] = (free, args)
+        return key
+
+    def _free(self, key) -> None:
+        free, args = self._native.pop(key, (None, ()))
+        if free:
+            free(*args)
 
     def close(self) -> None:
         if self.handle:
             for child in list(self._children):
                 child.close()
+            for key in reversed(list(self._native)):
+                self._free(key)
             self._lib.pssa_hip_destroy(self.handle)
             self.handle = None
 
@@ -417,11 +433,11 @@ class W4Matrix:
 
     def __init__(self, device: HipDevice, handle, n: int, k: int, group: int):
         self.device, self.handle, self.n, self.k, self.group = device, handle, n, k, group
+        self._key = device._own(device._lib.pssa_hip_w4_free, handle)
         device._children.add(self)
 
     def close(self) -> None:
-        if self.handle and self.device.handle:
-            self.device._lib.pssa_hip_w4_free(self.handle)
+        self.device._free(self._key)
         self.handle = None
 
     def __del__(self):  # pragma: no cover
@@ -440,6 +456,7 @@ class DeviceBuffer:
         p = C.c_void_p()
         _abi.call(device._lib.pssa_hip_device_alloc, device.handle, max(nbytes, 1), C.byref(p))
         self.ptr = p.value
+        self._key = device._own(device._lib.pssa_hip_device_free, device.handle, C.c_void_p(self.ptr))
         device._children.add(self)
 
     def to_host(self) -> np.ndarray:
@@ -455,8 +472,7 @@ class DeviceBuffer:
                   a.ctypes.data_as(C.c_void_p), a.nbytes, _abi.H2D)
 
     def close(self) -> None:
-        if self.ptr and self.device.handle:
-            self.device._lib.pssa_hip_device_free(self.device.handle, C.c_void_p(self.ptr))
+        self.device._free(self._key)
         self.ptr = None
 
     def __del__(self):  # pragma: no cover
@@ -499,15 +515,14 @@ class PSSALayer:
             lib.pssa_hip_model_free(m)
             raise
         self.handle = ln
+        # Freed last to first.
+        self._keys = [device._own(lib.pssa_hip_model_free, m), device._own(lib.pssa_hip_lanes_free, ln)]
         device._children.add(self)
 
     def close(self) -> None:
-        if getattr(self, "handle", None):
-            self._lib.pssa_hip_lanes_free(self.handle)
-            self.handle = None
-        if getattr(self, "model", None):
-            self._lib.pssa_hip_model_free(self.model)
-            self.model = None
+        for key in reversed(getattr(self, "_keys", ())):
+            self.device._free(key)
+        self.handle = self.model = None
 
     def __del__(self):  # pragma: no cover
         try:
