@@ -590,8 +590,10 @@ int pssa_hip_lanes_stage_times(pssa_hip_lanes* lanes, int enable, const char** n
  * asynchronous on the context stream: work that other streams do on these
  * arrays has to be complete before the call, and pssa_hip_synchronize
  * completes it.  `dtype` is PSSA_HIP_F32 or PSSA_HIP_BF16; sums, statistics
- * and states are fp32, their order a matter of the call's sizes alone: the
- * same call gives the same bits, another number of rows or sequences may give
+ * and states are fp32.  Their order is a matter of the call's sizes and, for
+ * bf16 linear attention, of whether every row and head starts at a multiple
+ * of 4 bytes, which chooses the kernel: the same call gives the same bits,
+ * another number of rows or sequences, or rows moved by an element, may give
  * a row others.  They have no counterpart in the reference's backend.
  */
 
@@ -697,9 +699,15 @@ int pssa_hip_matvec_w4(pssa_hip_w4* w, const float* x, size_t x_len, size_t m, f
  * may be d_state_in.  out may lie in the buffer of q, k and v in columns of
  * its own (same row stride) and must not overlap them, d_log_decay or a state
  * otherwise.  d_key <= 128,
- * d_val <= 4096, n_seqs and heads <= 65535, row strides below 2^24.  bf16
- * outputs round once; every sum and the states are fp32.  A value that is not
- * finite reaches the outputs from its own token on and no earlier one. */
+ * d_val <= 4096, n_seqs and heads <= 65535, row strides below 2^24.  Every
+ * sum and the states are fp32, and bf16 outputs are these sums rounded once.
+ * Where a sequence of a bf16 call has more than 4 tokens and every row and
+ * head starts at a multiple of 4 bytes, two operands of the products meet q
+ * and v in two bf16 parts, 2^-17 of each value off: the state that a chunk of
+ * 64 tokens is entered with (the state kept and handed on is not rounded) and
+ * the weights exp(log_decay)^(i-j) q_i k_j within the chunk.  Other calls
+ * multiply in fp32.  A value that is not finite reaches the outputs from its
+ * own token on and no earlier one. */
 int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
                                        size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
                                        const float* d_state_in, const uint64_t* lens, size_t n_seqs, size_t seq_len,

@@ -1054,3 +1054,18 @@ def test_matvec_w4_rows_at_far_offsets(hip):
     y.buf.close()
     mat.close()
     assert np.all(np.abs(got - held.astype(np.float64) @ w.T) <= w4_tolerance(held, codes, scales, zp, group))
+
+
+@pytest.mark.parametrize("dtype,gaps", [("f32", (0, 2, 3)), ("bf16", (0, 2))])
+@pytest.mark.parametrize("lens", [[70, 1, 130], [900]])
+def test_linear_attention_loads_do_not_change_the_bits(hip, dtype, gaps, lens):
+    """Loads of 16 and of 4 bytes feed the same sums (only bf16 rows at odd elements take other ones)."""
+    say("linear loads", dtype, lens)
+    rng = np.random.default_rng(sum(lens))
+    n, h, d = sum(lens), 2, 40
+    q, k, v = (rng.normal(0, 1, (n, h, d)) for _ in range(3))
+    g = np.full(h, -0.02, np.float32)
+    got = [run_linear(hip, q, k, v, g, lens, 0.3, None, dtype, gap)[:2] for gap in gaps]
+    for out, state in got[1:]:
+        np.testing.assert_array_equal(out, got[0][0])
+        np.testing.assert_array_equal(state, got[0][1])
