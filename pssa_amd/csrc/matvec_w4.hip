@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t held4(uint32_t q) {
   return q ^ 0x08080808u ^ (((q >> 3 & 0x01010101u) ^ 0x01010101u) * 7u);
 }
 // Codes [n, k], one byte each, into the tiles: 8 codes to a load.  134 million
-// of them (16384 x 8192) take 36 us, 5.6 TB/s; byte by byte they took 250.
+// of them (16384 x 8192) take 38 us, 5.3 TB/s; byte by byte they took 250.
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict__ codes, int n, int k, int kblocks,
                                                       size_t pieces, u32x4_t* __restrict__ out) {
   const size_t piece = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -381,10 +381,11 @@ Status launch_matvec_w4(hipStream_t stream, int x_dtype, const void* x, size_t l
   a.k = w.k;
   a.kblocks = (w.k + 127) / 128;
   a.tiles = (w.n + 15) / 16;
-  // fp32 rows are split into their parts once for NT tiles: 7 of them with
-  // 16384 x 8192 weights took 35.7, 29.2 and 27.8 us at NT 1, 2 and 4, of
-  // which the last spills with smaller groups.  bf16 rows come as they are:
-  // one of them with 16384 x 768 took 4.8 us at NT 1 and 2.
+  // fp32 rows are split into their parts once for NT tiles: with 7 of them and
+  // 16384 x 8192 weights the kernel took 35.7, 29.2 and 27.8 us at NT 1, 2 and
+  // 4 under the profiler, of which the last spills with smaller groups (a call
+  // in a stream takes 26 us).  bf16 rows come as they are: one of them with
+  // 16384 x 768 took 4.8 us at NT 1 and 2.
   if (x_dtype != PSSA_HIP_F32) return launch_columns<false, 1>(stream, a, w.group, split_waves(a.tiles, 4096, a.kblocks));
   if (a.tiles < 512) return launch_columns<true, 1>(stream, a, w.group, split_waves(a.tiles, 4096, a.kblocks));
   return launch_columns<true, 2>(stream, a, w.group, split_waves((a.tiles + 1) / 2, 2048, a.kblocks));

@@ -249,8 +249,11 @@ __device__ __forceinline__ Key wave_merge(Key a, Key b_reversed, int lane) {
 // equal, say) gives its k tokens one by one, each round the largest behind
 // the one before.
 //
-// 8192 fp32 rows of 16384, 8 alternatives: 114 us (4.7 TB/s); 509 bf16 rows of
-// 100003, 5 of them: 36 us (2.8 TB/s); one row of 16384: 7 us, mostly latency.
+// 8192 fp32 rows of 16384, 8 alternatives: 109 us (4.9 TB/s); 509 bf16 rows of
+// 100003, 5 of them: 34 us (3.0 TB/s); one row of 16384: 7.5 us, mostly latency.
+// Tiles that leave fewer tokens than are asked for, with no bound from before,
+// go through LDS whole: 257 and 113 us where the first two keep 4 and 20
+// tokens a row (8 alternatives).
 constexpr int kCandidates = 1024;
 constexpr int kSlots = 8;  // threads of a wave whose vectors are looked through at once
 
@@ -514,8 +517,8 @@ __global__ __launch_bounds__(64 * W) void token_logprobs_kernel(LogprobArgs a) {
 // and its gradient w tau (p - q).  The dense part p is written from the
 // registers that the sums were taken from; the few teacher's tokens are then
 // written again with their q.
-// 8192 fp32 rows of 16384: 219 us (4.9 TB/s); 777 bf16 rows of 65537: 63 us
-// (4.6 TB/s with the second read); 37 fp32 rows of 2048: 5 us, latency.
+// 8192 fp32 rows of 16384: 220 us (4.9 TB/s); 777 bf16 rows of 65537: 69 us
+// (4.4 TB/s with the second read); 37 fp32 rows of 2048: 5.5 us, latency.
 // MANY: the row takes several tiles, each thread with a maximum and sum of its
 // own until the end, each tile loaded while the one before is summed.
 template <class T, int W, int NV, bool MANY>
