@@ -677,7 +677,8 @@ int pssa_hip_w4_quantize(const float* w, size_t w_len, size_t n, size_t k, size_
  * (ld_x >= k), y fp32 with rows d_y + i*ld_y (ld_y >= n), rows at any
  * element; y must not overlap x.  Products and sums are fp32 (x is not
  * rounded); a row's values do not depend on the rows beside it.  An infinity or
- * NaN in a row of x gives values that are not finite in that row. */
+ * NaN in a row of x gives values that are not finite in that row, and so may
+ * values whose sum of 15 |x| over a group passes fp32's range. */
 int pssa_hip_matvec_w4_resident(pssa_hip_w4* w, const void* d_x, int x_dtype, size_t m, size_t ld_x, float* d_y,
                                 size_t ld_y, char* err, size_t err_len);
 /* The same on fp32 host arrays x [m, k], y [m, n]. */
