@@ -723,6 +723,113 @@ int pssa_hip_linear_attention_resident(pssa_hip_ctx* ctx, int dtype, const void*
 int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
                                       size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len);
 
+/* The gated delta rule, the recurrence
+ *   S_t = a_t (1 - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T,   a_t = exp(log_decay_t)
+ *   out_t = scale q_t S_t
+ * over packed sequences (lens, n_seqs, seq_len as above).  q and k [tokens,
+ * key_heads, d_key], v and out [tokens, heads, d_val], all of `dtype`, with
+ * row strides as above; head h reads query and key head h / (heads /
+ * key_heads).  log_decay and beta [tokens, heads] are fp32, token t at t *
+ * ld_gates.  log_decay is <= 0; -inf forgets the state before the token.  Keys
+ * of length one and beta in 0..2 keep the states bounded; other values are
+ * computed as they are.  States are fp32 [n_seqs, heads, d_key, d_val] as
+ * above.  out may lie in the buffer of q, k and v in columns of its own (same
+ * row stride) and must not overlap them, the gates or a state otherwise.
+ * d_key <= 128, d_val <= 4096, n_seqs and heads <= 65535, row strides below
+ * 2^24.  A value that is not finite reaches the outputs from its own token on
+ * and no earlier one. */
+int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
+                                 size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
+                                 const float* d_beta, size_t ld_gates, const float* d_state_in, const uint64_t* lens,
+                                 size_t n_seqs, size_t seq_len, size_t heads, size_t key_heads, size_t d_key,
+                                 size_t d_val, float scale, void* d_out, size_t ld_out, float* d_state_out, char* err,
+                                 size_t err_len);
+/* Grows the context's scratch (synchronously) to what such a call needs, so
+ * that it then allocates nothing and stays asynchronous. */
+int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len);
+
+/* Root-mean-square norm of rows with the residual's addition:
+ *   h = x + residual,   out = gamma h / sqrt(mean(h^2) + eps),
+ * in fp32 from the unrounded h.  Rows of `dtype` at d_x + r*ld_x (likewise the
+ * others), at any element; d_residual NULL: h = x.  Outputs, each of which may
+ * be NULL but not all: d_sum (h, rounded to `dtype`), d_out (`dtype`), and 8-bit codes
+ * with a scale for each row,
+ *   codes = round(t 127 / max|t|), ties to even,   t = gamma h,
+ *   scales = max|t| / 127 / sqrt(mean(h^2) + eps),
+ * d_codes [rows, width] and d_scales [rows] together.  A row of zeros has
+ * codes and scale 0; one whose t is not finite has codes 0 and scale NaN.
+ * gamma is fp32 [width]; 1 <= width <= 65536, eps in [1e-12, 1].  d_sum and d_out may be
+ * d_x or d_residual with their row stride; outputs must not overlap the inputs
+ * or each other otherwise (other columns of the same rows do not). */
+int pssa_hip_rms_norm_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, const void* d_residual,
+                               size_t ld_residual, const float* d_gamma, float eps, size_t rows, size_t width,
+                               void* d_sum, size_t ld_sum, void* d_out, size_t ld_out, int8_t* d_codes,
+                               size_t ld_codes, float* d_scales, char* err, size_t err_len);
+/* 8-bit codes and scales of rows as they are (activations, or a weight's
+ * channels): codes = round(x 127 / max|x|), scales = max|x| / 127. */
+int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, size_t rows, size_t width,
+                                  int8_t* d_codes, size_t ld_codes, float* d_scales, char* err, size_t err_len);
+
+/* y[m, n] = x_scales[i] w_scales[j] sum_l x[i][l] w[j][l] of 8-bit rows x
+ * [m, k] and weights w [n, k] (every code -128..127), with fp32 scales for each
+ * row [m] and channel [n]; rows at any byte, strides ld_x, ld_w >= k.  The sums
+ * are exact (k <= 131071), rounded once to fp32, and y (y_dtype, stride ld_y
+ * >= n) has two more roundings for the scales and one to bf16.  m <= 2^20;
+ * strides below 2^31.  y must not overlap the other arrays. */
+int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scales,
+                                const int8_t* d_w, size_t ld_w, const float* d_w_scales, size_t m, size_t n, size_t k,
+                                void* d_y, int y_dtype, size_t ld_y, char* err, size_t err_len);
+/* Grows the context's scratch (synchronously) to what such a call needs. */
+int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, char* err, size_t err_len);
+
+/* Beam search's selection: of `groups` requests with `beams` rows of logits
+ * each (row g*beams + b at d_logits + row*ld), the `keep` best of
+ *   scores[g][b] + log softmax(logits[row])[v]
+ * over b and v, in descending order, equal ones by beam, then by token:
+ * d_parents (the beam b), d_tokens (v) and d_out_scores [groups, keep].  The
+ * values are computed in 64 bits and rounded once.  d_last [groups, beams] or
+ * NULL: a beam whose last token is `eos` has ended and has one candidate, eos
+ * with its score as it is; its logits are not read.  A beam whose score is not
+ * finite, or whose logits hold a NaN or +inf or nothing but -inf, has none, and
+ * neither has a token with -inf; places left over hold PSSA_HIP_NO_TOKEN twice and
+ * -inf.  beams and keep <= 64.  With keep = beams, d_out_scores may be d_scores
+ * and d_tokens d_last; outputs must not overlap anything otherwise. */
+int pssa_hip_beam_select_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t groups, size_t beams,
+                                  size_t vocab, size_t ld, const float* d_scores, const uint32_t* d_last, uint32_t eos,
+                                  size_t keep, uint32_t* d_parents, uint32_t* d_tokens, float* d_out_scores, char* err,
+                                  size_t err_len);
+/* Grows the context's scratch (synchronously) to what such a call needs. */
+int pssa_hip_beam_select_reserve(pssa_hip_ctx* ctx, size_t groups, size_t beams, size_t vocab, size_t keep, char* err,
+                                 size_t err_len);
+/* States reordered by a selection: row j of group g of the destination becomes
+ * row d_parents[g][j] of the same group of the source (rows of row_bytes; row
+ * i of group g at (g*n_in + i)*ld_src bytes, (g*n_out + j)*ld_dst bytes).  A
+ * row whose parent is not below n_in (PSSA_HIP_NO_TOKEN) stays as it is.  The
+ * rows may be reordered in place (d_dst = d_src, n_out = n_in, equal strides)
+ * and must not overlap otherwise.  n_in, n_out <= 64. */
+int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t ld_src, void* d_dst, size_t ld_dst,
+                                  size_t row_bytes, size_t groups, size_t n_in, const uint32_t* d_parents,
+                                  size_t n_out, char* err, size_t err_len);
+
+/* Beam search on a model's lanes.  Continues the last prefill, of n_groups
+ * lanes (as pssa_hip_decode with first_ids NULL does), each of which becomes
+ * `beams` lanes: lanes g*beams .. of the first n_groups*beams, which must exist.
+ * Every step selects as pssa_hip_beam_select_resident does over ids 1..V-1, as
+ * the greedy choice, and reorders the lanes' carries and penalty windows; the
+ * first one chooses from the prefill's logits, and each later one costs a
+ * forward step of all n_groups*beams lanes.  Beams that chose `eos`
+ * (PSSA_HIP_NO_TOKEN: none does) have ended, keep their score and repeat it.
+ * out_ids [n_groups, beams, steps] are the tokens of the beams that are left,
+ * best first, out_scores [n_groups, beams] their summed log probabilities; a
+ * beam that never had a candidate holds PSSA_HIP_NO_TOKEN and -inf.  The lanes
+ * are left at their last step: the last token of a beam is not yet consumed.
+ * beams <= 64; steps <= 2^20.  Lanes with a repetition penalty or a sampling
+ * temperature are PSSA_HIP_EUNSUPPORTED. */
+int pssa_hip_beam_search(pssa_hip_lanes* lanes, size_t n_groups, size_t beams, size_t steps, uint32_t eos,
+                         uint32_t* out_ids, size_t out_len, float* out_scores, size_t scores_len, char* err,
+                         size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

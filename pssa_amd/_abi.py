@@ -205,6 +205,19 @@ def lib() -> C.CDLL:
         "pssa_hip_linear_attention_resident": ([vp, C.c_int, vp, sz, vp, sz, vp, sz, vp, vp, u64p, sz, sz, sz, sz, sz, sz,
                                                 C.c_float, vp, sz, vp, err_t, sz], C.c_int),
         "pssa_hip_linear_attention_reserve": ([vp, C.c_int, u64p, sz, sz, sz, sz, sz, err_t, sz], C.c_int),
+        "pssa_hip_delta_rule_resident": ([vp, C.c_int, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp, u64p, sz, sz, sz, sz, sz, sz,
+                                          C.c_float, vp, sz, vp, err_t, sz], C.c_int),
+        "pssa_hip_delta_rule_reserve": ([vp, C.c_int, u64p, sz, sz, sz, sz, sz, err_t, sz], C.c_int),
+        "pssa_hip_rms_norm_resident": ([vp, C.c_int, vp, sz, vp, sz, vp, C.c_float, sz, sz, vp, sz, vp, sz, vp, sz, vp,
+                                        err_t, sz], C.c_int),
+        "pssa_hip_quantize_i8_resident": ([vp, C.c_int, vp, sz, sz, sz, vp, sz, vp, err_t, sz], C.c_int),
+        "pssa_hip_matmul_i8_resident": ([vp, vp, sz, vp, vp, sz, vp, sz, sz, sz, vp, C.c_int, sz, err_t, sz], C.c_int),
+        "pssa_hip_matmul_i8_reserve": ([vp, sz, sz, sz, err_t, sz], C.c_int),
+        "pssa_hip_beam_select_resident": ([vp, vp, C.c_int, sz, sz, sz, sz, vp, vp, C.c_uint32, sz, vp, vp, vp, err_t, sz],
+                                          C.c_int),
+        "pssa_hip_beam_select_reserve": ([vp, sz, sz, sz, sz, err_t, sz], C.c_int),
+        "pssa_hip_beam_gather_resident": ([vp, vp, sz, vp, sz, sz, sz, sz, vp, sz, err_t, sz], C.c_int),
+        "pssa_hip_beam_search": ([vp, sz, sz, sz, C.c_uint32, u32p, sz, fp, sz, err_t, sz], C.c_int),
         "pssa_hip_batch_distill": ([vp, u32p, fp, sz, sz, C.c_float, fp, fp, fp, err_t, sz], C.c_int),
     }
     for name, (args, res) in sig.items():

@@ -206,6 +206,7 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_dense_scan_attributes());
     PSSA_RETURN_IF(pssa::init_w4_attributes());
     PSSA_RETURN_IF(pssa::init_linear_attributes());
+    PSSA_RETURN_IF(pssa::init_i8_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));
     *out = ctx.release();
     return Status::Ok();
@@ -2550,6 +2551,489 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     return grow_scratch(ctx, plan.scratch_bytes(), false);
+  }, err, err_len);
+}
+
+}  // extern "C"
+
+namespace {
+
+// The sequences of a delta rule call.
+struct DeltaPlan {
+  std::vector<uint32_t> table;  // first tokens, where the arguments do not hold them
+  size_t tokens = 0, longest = 0;
+
+  size_t scratch_bytes() const { return table.size() * 4; }
+};
+Status plan_delta(const uint64_t* lens, size_t n_seqs, size_t seq_len, pssa::DeltaArgs& a, DeltaPlan& p) {
+  PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "delta rule: sequences must be in 1..=65535"));
+  a.n_seqs = (int)n_seqs;
+  bool same = true;
+  for (size_t i = 0; i < n_seqs; ++i) {
+    const size_t len = lens ? lens[i] : seq_len;
+    PSSA_RETURN_IF(need(len <= INT32_MAX && p.tokens + len <= INT32_MAX, "delta rule: too many tokens"));
+    p.tokens += len;
+    p.longest = std::max(p.longest, len);
+    same &= !lens || lens[i] == lens[0];
+  }
+  a.uniform_len = same ? (int)p.longest : -1;
+  if (same) return Status::Ok();
+  const bool inside = n_seqs <= (size_t)pssa::kDeltaInline;
+  if (!inside) p.table.resize(n_seqs + 1);
+  uint32_t* tok = inside ? a.inline_tokens : p.table.data();
+  uint32_t t = 0;
+  for (size_t i = 0; i < n_seqs; ++i) {
+    tok[i] = t;
+    t += (uint32_t)lens[i];
+  }
+  tok[n_seqs] = t;
+  return Status::Ok();
+}
+Status check_delta_heads(size_t heads, size_t d_key, size_t d_val) {
+  PSSA_RETURN_IF(need(heads && d_key && d_val, "delta rule: dimensions must be positive"));
+  PSSA_RETURN_IF(need(heads <= 65535, "delta rule: at most 65535 heads"));
+  PSSA_RETURN_IF(need(d_key <= (size_t)pssa::kDeltaMaxKey, "delta rule: d_key above 128 is not supported"));
+  return need(d_val <= 4096, "delta rule: d_val above 4096 is not supported");
+}
+
+// Rows `w` bytes wide at stride ld bytes: an array of a call that its outputs must not touch.
+struct Rows {
+  const void* p;
+  size_t rows, ld, w;
+};
+// Apart in memory, or other columns of the same rows.
+bool apart(const Rows& a, const Rows& b) {
+  if (!a.p || !b.p) return true;
+  if (a.rows == b.rows && a.ld && b.ld) return rows_disjoint(a.p, a.ld, a.w, b.p, b.ld, b.w, a.rows, 1);
+  return !a.rows || !b.rows || disjoint(a.p, (a.rows - 1) * a.ld + a.w, b.p, (b.rows - 1) * b.ld + b.w);
+}
+// A matrix of rows: its extent.
+Status check_matrix(size_t rows, size_t width, size_t ld, const char* what) {
+  if (!rows || !width) return Status::Invalid(std::string(what) + ": dimensions must be positive");
+  if (ld < width) return Status::Invalid(std::string(what) + ": row stride below the row");
+  if (rows > INT32_MAX || ld > INT32_MAX) return Status::Invalid(std::string(what) + ": too large");
+  size_t n = 0;
+  return pssa::checked_count({rows, ld}, &n, what);
+}
+Status check_i8(size_t m, size_t n, size_t k) {
+  PSSA_RETURN_IF(need(m && n && k, "8-bit product: dimensions must be positive"));
+  PSSA_RETURN_IF(need(k <= pssa::kI8Depth, "8-bit product: k above 131071 is not supported"));
+  return need(m <= ((size_t)1 << 20) && n <= ((size_t)1 << 24), "8-bit product: too large");
+}
+size_t i8_scratch(size_t m, size_t n, size_t k) {
+  const size_t splits = (size_t)pssa::i8_splits(m, n, k);
+  return splits > 1 ? splits * m * n * 4 : 0;
+}
+Status check_beams(size_t groups, size_t beams, size_t vocab, size_t keep) {
+  PSSA_RETURN_IF(need(groups && vocab, "beam selection: dimensions must be positive"));
+  PSSA_RETURN_IF(need(beams >= 1 && beams <= (size_t)pssa::kMaxBeams && keep >= 1 && keep <= (size_t)pssa::kMaxBeams,
+                      "beam selection: beams and keep must be in 1..=64"));
+  return need(vocab <= ((size_t)1 << 24) && groups <= INT32_MAX / pssa::kMaxBeams, "beam selection: too large");
+}
+
+// The selection of one step on the context's stream, its scratch grown to what it needs.
+Status select_beams(pssa_hip_ctx* ctx, int dtype, pssa::BeamArgs& a, size_t groups) {
+  const pssa::BeamPlan p = pssa::beam_plan(dtype, groups * (size_t)a.beams, (size_t)a.vocab, (size_t)a.keep);
+  PSSA_RETURN_IF(grow_scratch(ctx, p.bytes, false));
+  a.slices = (int)p.slices;
+  a.sums = ctx->scratch;
+  a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(ctx->scratch) + p.sums_bytes);
+  return pssa::launch_beam_select(ctx->stream, dtype, a, groups, p);
+}
+
+Status reorder_rows(pssa_hip_ctx* ctx, const DevBuf& rows, size_t row_bytes, size_t groups, size_t beams,
+                    const uint32_t* parents) {
+  pssa::GatherArgs a;
+  a.src = a.dst = rows.p;
+  a.ld_src = a.ld_dst = a.row_bytes = row_bytes;
+  a.groups = (int)groups;
+  a.n_in = a.n_out = (int)beams;
+  a.parents = parents;
+  return pssa::launch_beam_gather(ctx->stream, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
+                                 size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
+                                 const float* d_beta, size_t ld_gates, const float* d_state_in, const uint64_t* lens,
+                                 size_t n_seqs, size_t seq_len, size_t heads, size_t key_heads, size_t d_key,
+                                 size_t d_val, float scale, void* d_out, size_t ld_out, float* d_state_out, char* err,
+                                 size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_q && d_k && d_v && d_log_decay && d_beta && d_out, "delta rule: null buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(check_delta_heads(heads, d_key, d_val));
+    PSSA_RETURN_IF(need(key_heads && heads % key_heads == 0, "delta rule: key_heads must divide heads"));
+    PSSA_RETURN_IF(need(std::isfinite(scale), "delta rule: scale must be finite"));
+    const size_t size = dtype_size(dtype), wk = key_heads * d_key, wv = heads * d_val;
+    PSSA_RETURN_IF(need(ld_q >= wk && ld_k >= wk && ld_v >= wv && ld_out >= wv && ld_gates >= heads,
+                        "delta rule: row stride below the heads' width"));
+    PSSA_RETURN_IF(need(std::max({ld_q, ld_k, ld_v, ld_out, ld_gates}) < ((size_t)1 << 24),
+                        "delta rule: row strides must be below 2^24"));
+    PSSA_RETURN_IF(need(aligned_to(d_q, size) && aligned_to(d_k, size) && aligned_to(d_v, size) &&
+                            aligned_to(d_out, size) && aligned_to(d_log_decay, 4) && aligned_to(d_beta, 4) &&
+                            aligned_to(d_state_in, 4) && aligned_to(d_state_out, 4),
+                        "delta rule: misaligned buffer"));
+    pssa::DeltaArgs a;
+    DeltaPlan plan;
+    PSSA_RETURN_IF(plan_delta(lens, n_seqs, seq_len, a, plan));
+    const size_t tokens = plan.tokens;
+    size_t n = 0;
+    for (size_t ld : {ld_q, ld_k, ld_v, ld_out, ld_gates})
+      PSSA_RETURN_IF(pssa::checked_count({tokens, ld}, &n, "delta rule"));
+    PSSA_RETURN_IF(pssa::checked_count({n_seqs, heads, d_key, d_val}, &n, "delta rule states"));
+    const Rows out{d_out, tokens, ld_out * size, wv * size}, in{d_state_in, 1, 0, n * 4}, kept{d_state_out, 1, 0, n * 4};
+    for (const Rows& r : {Rows{d_q, tokens, ld_q * size, wk * size}, Rows{d_k, tokens, ld_k * size, wk * size},
+                          Rows{d_v, tokens, ld_v * size, wv * size}, Rows{d_log_decay, tokens, ld_gates * 4, heads * 4},
+                          Rows{d_beta, tokens, ld_gates * 4, heads * 4}}) {
+      PSSA_RETURN_IF(need(apart(r, out), "delta rule: the output overlaps its inputs"));
+      PSSA_RETURN_IF(need(apart(r, kept), "delta rule: the states overlap"));
+    }
+    PSSA_RETURN_IF(need(apart(in, out) && apart(kept, out), "delta rule: the output overlaps the states"));
+    PSSA_RETURN_IF(need(d_state_in == d_state_out || apart(in, kept), "delta rule: the states overlap"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.ld_q = ld_q;
+    a.ld_k = ld_k;
+    a.ld_v = ld_v;
+    a.ld_out = ld_out;
+    a.ld_gates = ld_gates;
+    a.log_decay = d_log_decay;
+    a.beta = d_beta;
+    a.state_in = d_state_in;
+    a.state_out = d_state_out;
+    a.out = d_out;
+    a.scale = scale;
+    a.heads = (int)heads;
+    a.key_heads = (int)key_heads;
+    a.dk = (int)d_key;
+    a.dv = (int)d_val;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    PSSA_RETURN_IF(grow_scratch(ctx, plan.scratch_bytes(), false));
+    if (!plan.table.empty()) {
+      PSSA_RETURN_IF(ctx->stage.to_device(ctx->scratch, plan.table.data(), plan.table.size() * 4, ctx->stream));
+      a.table = static_cast<uint32_t*>(ctx->scratch);
+    }
+    return pssa::launch_delta_rule(ctx->stream, dtype, a, (int)plan.longest);
+  }, err, err_len);
+}
+
+int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
+                                size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(check_delta_heads(heads, d_key, d_val));
+    pssa::DeltaArgs a;
+    DeltaPlan plan;
+    PSSA_RETURN_IF(plan_delta(lens, n_seqs, seq_len, a, plan));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return grow_scratch(ctx, plan.scratch_bytes(), false);
+  }, err, err_len);
+}
+
+int pssa_hip_rms_norm_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, const void* d_residual,
+                               size_t ld_residual, const float* d_gamma, float eps, size_t rows, size_t width,
+                               void* d_sum, size_t ld_sum, void* d_out, size_t ld_out, int8_t* d_codes,
+                               size_t ld_codes, float* d_scales, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_x && d_gamma, "rms norm: null buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(need(eps >= 1e-12f && eps <= 1.0f, "rms norm: eps must be in [1e-12, 1]"));
+    PSSA_RETURN_IF(need(width <= pssa::kRmsWidth, "rms norm: rows above 65536 elements are not supported"));
+    PSSA_RETURN_IF(need(!d_codes == !d_scales, "rms norm: codes and scales belong together"));
+    PSSA_RETURN_IF(need(d_sum || d_out || d_codes, "rms norm: no output asked for"));
+    PSSA_RETURN_IF(check_matrix(rows, width, ld_x, "rms norm"));
+    if (d_residual) PSSA_RETURN_IF(check_matrix(rows, width, ld_residual, "rms norm residual"));
+    if (d_sum) PSSA_RETURN_IF(check_matrix(rows, width, ld_sum, "rms norm sum"));
+    if (d_out) PSSA_RETURN_IF(check_matrix(rows, width, ld_out, "rms norm output"));
+    if (d_codes) PSSA_RETURN_IF(check_matrix(rows, width, ld_codes, "rms norm codes"));
+    const size_t size = dtype_size(dtype);
+    PSSA_RETURN_IF(need(aligned_to(d_x, size) && aligned_to(d_residual, size) && aligned_to(d_sum, size) &&
+                            aligned_to(d_out, size) && aligned_to(d_gamma, 4) && aligned_to(d_scales, 4),
+                        "rms norm: misaligned buffer"));
+    const Rows ins[3] = {{d_x, rows, ld_x * size, width * size}, {d_residual, rows, ld_residual * size, width * size},
+                         {d_gamma, 1, 0, width * 4}};
+    const Rows outs[4] = {{d_sum, rows, ld_sum * size, width * size}, {d_out, rows, ld_out * size, width * size},
+                          {d_codes, rows, ld_codes, width}, {d_scales, 1, 0, rows * 4}};
+    for (int o = 0; o < 4; ++o) {
+      for (int i = 0; i < 3; ++i) {
+        const bool in_place = o < 2 && i < 2 && outs[o].p == ins[i].p && outs[o].ld == ins[i].ld;
+        PSSA_RETURN_IF(need(in_place || apart(outs[o], ins[i]), "rms norm: an output overlaps an input"));
+      }
+      for (int i = 0; i < o; ++i) PSSA_RETURN_IF(need(apart(outs[o], outs[i]), "rms norm: the outputs overlap"));
+    }
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::RmsNormArgs a;
+    a.x = d_x;
+    a.residual = d_residual;
+    a.ld_x = ld_x;
+    a.ld_residual = ld_residual;
+    a.ld_sum = ld_sum;
+    a.ld_out = ld_out;
+    a.ld_codes = ld_codes;
+    a.gamma = d_gamma;
+    a.width = (int)width;
+    a.eps = eps;
+    a.sum = d_sum;
+    a.out = d_out;
+    a.codes = d_codes;
+    a.scales = d_scales;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return pssa::launch_rms_norm(ctx->stream, dtype, a, rows);
+  }, err, err_len);
+}
+
+int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, size_t rows, size_t width,
+                                  int8_t* d_codes, size_t ld_codes, float* d_scales, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_x && d_codes && d_scales, "8-bit rows: null buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
+    PSSA_RETURN_IF(need(width <= pssa::kRmsWidth, "8-bit rows: above 65536 elements are not supported"));
+    PSSA_RETURN_IF(check_matrix(rows, width, ld_x, "8-bit rows"));
+    PSSA_RETURN_IF(check_matrix(rows, width, ld_codes, "8-bit rows' codes"));
+    const size_t size = dtype_size(dtype);
+    PSSA_RETURN_IF(need(aligned_to(d_x, size) && aligned_to(d_scales, 4), "8-bit rows: misaligned buffer"));
+    const Rows x{d_x, rows, ld_x * size, width * size}, codes{d_codes, rows, ld_codes, width}, scales{d_scales, 1, 0, rows * 4};
+    PSSA_RETURN_IF(need(apart(x, codes) && apart(x, scales) && apart(codes, scales), "8-bit rows: the arrays overlap"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::RmsNormArgs a;
+    a.x = d_x;
+    a.ld_x = ld_x;
+    a.ld_codes = ld_codes;
+    a.width = (int)width;
+    a.normed = false;
+    a.codes = d_codes;
+    a.scales = d_scales;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return pssa::launch_rms_norm(ctx->stream, dtype, a, rows);
+  }, err, err_len);
+}
+
+int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scales,
+                                const int8_t* d_w, size_t ld_w, const float* d_w_scales, size_t m, size_t n, size_t k,
+                                void* d_y, int y_dtype, size_t ld_y, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_x && d_x_scales && d_w && d_w_scales && d_y, "8-bit product: null buffer"));
+    PSSA_RETURN_IF(need(dtype_ok(y_dtype), "unknown dtype"));
+    PSSA_RETURN_IF(check_i8(m, n, k));
+    PSSA_RETURN_IF(check_matrix(m, k, ld_x, "8-bit product rows"));
+    PSSA_RETURN_IF(check_matrix(n, k, ld_w, "8-bit product weights"));
+    PSSA_RETURN_IF(check_matrix(m, n, ld_y, "8-bit product output"));
+    const size_t size = dtype_size(y_dtype);
+    PSSA_RETURN_IF(need(aligned_to(d_x_scales, 4) && aligned_to(d_w_scales, 4) && aligned_to(d_y, size),
+                        "8-bit product: misaligned buffer"));
+    const Rows y{d_y, m, ld_y * size, n * size};
+    for (const Rows& r : {Rows{d_x, m, ld_x, k}, Rows{d_w, n, ld_w, k}, Rows{d_x_scales, 1, 0, m * 4},
+                          Rows{d_w_scales, 1, 0, n * 4}})
+      PSSA_RETURN_IF(need(apart(r, y), "8-bit product: the output overlaps its inputs"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::I8Args a;
+    a.x = d_x;
+    a.w = d_w;
+    a.ld_x = ld_x;
+    a.ld_w = ld_w;
+    a.ld_y = ld_y;
+    a.x_scales = d_x_scales;
+    a.w_scales = d_w_scales;
+    a.y = d_y;
+    a.m = (int)m;
+    a.n = (int)n;
+    a.k = (int)k;
+    a.splits = pssa::i8_splits(m, n, k);
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    PSSA_RETURN_IF(grow_scratch(ctx, i8_scratch(m, n, k), false));
+    a.parts = static_cast<int32_t*>(ctx->scratch);
+    return pssa::launch_matmul_i8(ctx->stream, y_dtype, a);
+  }, err, err_len);
+}
+
+int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(check_i8(m, n, k));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return grow_scratch(ctx, i8_scratch(m, n, k), false);
+  }, err, err_len);
+}
+
+int pssa_hip_beam_select_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t groups, size_t beams,
+                                  size_t vocab, size_t ld, const float* d_scores, const uint32_t* d_last, uint32_t eos,
+                                  size_t keep, uint32_t* d_parents, uint32_t* d_tokens, float* d_out_scores, char* err,
+                                  size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_logits && d_scores && d_parents && d_tokens && d_out_scores, "beam selection: null buffer"));
+    PSSA_RETURN_IF(check_beams(groups, beams, vocab, keep));
+    const size_t rows = groups * beams;
+    PSSA_RETURN_IF(check_rows(d_logits, dtype, rows, vocab, ld, "beam selection"));
+    PSSA_RETURN_IF(need(aligned_to(d_scores, 4) && aligned_to(d_last, 4) && aligned_to(d_parents, 4) &&
+                            aligned_to(d_tokens, 4) && aligned_to(d_out_scores, 4),
+                        "beam selection: misaligned buffer"));
+    const size_t size = dtype_size(dtype), kept = groups * keep * 4;
+    const Rows ins[3] = {{d_logits, rows, ld * size, vocab * size}, {d_scores, 1, 0, rows * 4}, {d_last, 1, 0, rows * 4}};
+    const Rows outs[3] = {{d_parents, 1, 0, kept}, {d_out_scores, 1, 0, kept}, {d_tokens, 1, 0, kept}};
+    for (int o = 0; o < 3; ++o) {
+      for (int i = 0; i < 3; ++i) {
+        const bool in_place = o && o == i && keep == beams && outs[o].p == ins[i].p;
+        PSSA_RETURN_IF(need(in_place || apart(outs[o], ins[i]), "beam selection: an output overlaps an input"));
+      }
+      for (int i = 0; i < o; ++i) PSSA_RETURN_IF(need(apart(outs[o], outs[i]), "beam selection: the outputs overlap"));
+    }
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::BeamArgs a;
+    a.logits = d_logits;
+    a.ld = ld;
+    a.vocab = (int)vocab;
+    a.beams = (int)beams;
+    a.keep = (int)keep;
+    a.scores = d_scores;
+    a.last = d_last;
+    a.eos = eos;
+    a.parents = d_parents;
+    a.tokens = d_tokens;
+    a.out_scores = d_out_scores;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return select_beams(ctx, dtype, a, groups);
+  }, err, err_len);
+}
+
+int pssa_hip_beam_select_reserve(pssa_hip_ctx* ctx, size_t groups, size_t beams, size_t vocab, size_t keep, char* err,
+                                 size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(check_beams(groups, beams, vocab, keep));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    const size_t rows = groups * beams;
+    return grow_scratch(ctx, std::max(pssa::beam_plan(PSSA_HIP_F32, rows, vocab, keep).bytes,
+                                      pssa::beam_plan(PSSA_HIP_BF16, rows, vocab, keep).bytes), false);
+  }, err, err_len);
+}
+
+int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t ld_src, void* d_dst, size_t ld_dst,
+                                  size_t row_bytes, size_t groups, size_t n_in, const uint32_t* d_parents,
+                                  size_t n_out, char* err, size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(d_src && d_dst && d_parents, "beam states: null buffer"));
+    PSSA_RETURN_IF(need(row_bytes && groups, "beam states: dimensions must be positive"));
+    PSSA_RETURN_IF(need(n_in >= 1 && n_in <= (size_t)pssa::kMaxBeams && n_out >= 1 && n_out <= (size_t)pssa::kMaxBeams,
+                        "beam states: rows of a group must be in 1..=64"));
+    PSSA_RETURN_IF(need(ld_src >= row_bytes && ld_dst >= row_bytes, "beam states: row stride below the row"));
+    PSSA_RETURN_IF(need(row_bytes <= ((size_t)1 << 38) && groups <= INT32_MAX / pssa::kMaxBeams, "beam states: too large"));
+    size_t n = 0;
+    PSSA_RETURN_IF(pssa::checked_count({groups, n_in, ld_src}, &n, "beam states"));
+    PSSA_RETURN_IF(pssa::checked_count({groups, n_out, ld_dst}, &n, "beam states"));
+    PSSA_RETURN_IF(need(aligned_to(d_parents, 4), "beam states: misaligned buffer"));
+    const Rows src{d_src, groups * n_in, ld_src, row_bytes}, dst{d_dst, groups * n_out, ld_dst, row_bytes};
+    const bool in_place = d_src == d_dst && n_in == n_out && ld_src == ld_dst;
+    PSSA_RETURN_IF(need(in_place || apart(src, dst), "beam states: the rows overlap"));
+    PSSA_RETURN_IF(need(apart(dst, Rows{d_parents, 1, 0, groups * n_out * 4}), "beam states: the rows overlap the parents"));
+    PSSA_RETURN_IF(check_ctx(ctx));
+    pssa::GatherArgs a;
+    a.src = d_src;
+    a.dst = d_dst;
+    a.ld_src = ld_src;
+    a.ld_dst = ld_dst;
+    a.row_bytes = row_bytes;
+    a.groups = (int)groups;
+    a.n_in = (int)n_in;
+    a.n_out = (int)n_out;
+    a.parents = d_parents;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    return pssa::launch_beam_gather(ctx->stream, a);
+  }, err, err_len);
+}
+
+int pssa_hip_beam_search(pssa_hip_lanes* L, size_t n_groups, size_t beams, size_t steps, uint32_t eos,
+                         uint32_t* out_ids, size_t out_len, float* out_scores, size_t scores_len, char* err,
+                         size_t err_len) {
+  return guarded([&]() -> Status {
+    PSSA_RETURN_IF(need(L && out_ids && out_scores, "beam search: null argument"));
+    PSSA_RETURN_IF(need(beams >= 1 && beams <= (size_t)pssa::kMaxBeams, "beam search: beams must be in 1..=64"));
+    PSSA_RETURN_IF(need(steps >= 1 && steps <= (1u << 20), "beam search: steps must be in 1..=2^20"));
+    PSSA_RETURN_IF(need(n_groups >= 1 && n_groups <= L->lanes && n_groups * beams <= L->lanes,
+                        "beam search: n_groups*beams must be in 1..=lanes"));
+    const size_t n = n_groups * beams, V = L->model->cfg.d_vocab;
+    PSSA_RETURN_IF(need(out_len == n * steps && scores_len == n,
+                        "beam search: out_ids must be [n_groups, beams, steps] and out_scores [n_groups, beams]"));
+    PSSA_RETURN_IF(need(V >= 2, "beam search: the vocabulary has no token but 0"));
+    pssa_hip_ctx* ctx = L->ctx;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    PSSA_RETURN_IF(need(L->logit_lanes == n_groups, "beam search continues the last prefill of n_groups lanes"));
+    if (L->rep_penalty != 1.0f || L->temperature > 0.0f)
+      return Status{PSSA_HIP_EUNSUPPORTED, "beam search runs without a repetition penalty or a sampling temperature"};
+    PSSA_RETURN_IF(loops_allow_hybrid(L));
+    PSSA_HIP_TRY(hipSetDevice(ctx->device));
+    const hipStream_t st = ctx->stream;
+    const pssa_hip_config& c = L->model->cfg;
+    const size_t carry = c.depth * L->loops * c.d_latent * c.d_state;
+    DevBuf parents, tokens, scores, start;
+    PSSA_RETURN_IF(parents.alloc(steps * n * 4, &ctx->pool));
+    PSSA_RETURN_IF(tokens.alloc(steps * n * 4, &ctx->pool));
+    PSSA_RETURN_IF(scores.alloc(n * 4, &ctx->pool));
+    PSSA_RETURN_IF(start.alloc(n_groups * 4, &ctx->pool));
+    PSSA_RETURN_IF(pssa::launch_fill_zero(st, start.as<float>(), n_groups));
+    // From here on the lanes are no longer the prefill's.
+    L->staged_lanes = L->staged_len = 0;
+    L->logit_lanes = 0;
+    PSSA_RETURN_IF(pssa::launch_beam_spread(st, L->carry.p, carry, carry, n_groups, beams));
+    PSSA_RETURN_IF(pssa::launch_beam_spread(st, L->hist.p, pssa_hip_lanes::kHist, pssa_hip_lanes::kHist, n_groups, beams));
+    PSSA_RETURN_IF(pssa::launch_beam_spread(st, L->hist_n.p, 1, 1, n_groups, beams));
+    PSSA_RETURN_IF(pssa::launch_beam_spread(st, L->hist_pos.p, 1, 1, n_groups, beams));
+    pssa::BeamArgs a;
+    a.logits = L->logits.as<float>() + 1;
+    a.ld = V;
+    a.vocab = (int)(V - 1);
+    a.first_id = 1;
+    a.eos = eos;
+    a.keep = (int)beams;
+    a.out_scores = scores.as<float>();
+    for (size_t t = 0; t < steps; ++t) {
+      a.parents = parents.as<uint32_t>() + t * n;
+      a.tokens = tokens.as<uint32_t>() + t * n;
+      if (t) {
+        PSSA_RETURN_IF(pssa::launch_beam_feed(st, tokens.as<uint32_t>() + (t - 1) * n, L->ids.as<uint32_t>(), n));
+        PSSA_RETURN_IF(pssa::run_prefill(L, n, 1));
+        a.last = tokens.as<uint32_t>() + (t - 1) * n;
+      }
+      a.beams = (int)(t ? beams : 1);
+      a.scores = t ? scores.as<float>() : start.as<float>();
+      PSSA_RETURN_IF(select_beams(ctx, PSSA_HIP_F32, a, n_groups));
+      if (!t) continue;  // every beam of a group has the same state so far
+      PSSA_RETURN_IF(reorder_rows(ctx, L->carry, carry * 4, n_groups, beams, a.parents));
+      PSSA_RETURN_IF(reorder_rows(ctx, L->hist, pssa_hip_lanes::kHist * 4, n_groups, beams, a.parents));
+      PSSA_RETURN_IF(reorder_rows(ctx, L->hist_n, 4, n_groups, beams, a.parents));
+      PSSA_RETURN_IF(reorder_rows(ctx, L->hist_pos, 4, n_groups, beams, a.parents));
+    }
+    std::vector<uint32_t> from(steps * n), id(steps * n);
+    PSSA_RETURN_IF(download(ctx, from.data(), parents, steps * n * 4));
+    PSSA_RETURN_IF(download(ctx, id.data(), tokens, steps * n * 4));
+    PSSA_RETURN_IF(download(ctx, out_scores, scores, n * 4));
+    PSSA_RETURN_IF(sync(ctx));
+    // Each beam's tokens from its last one back through its parents.
+    for (size_t i = 0; i < n; ++i) {
+      size_t beam = i % beams;
+      const size_t first = i - beam;
+      for (size_t t = steps; t-- > 0;) {
+        out_ids[i * steps + t] = id[t * n + first + beam];
+        const uint32_t p = from[t * n + first + beam];
+        if (t && p < beams) beam = p;
+      }
+    }
+    return Status::Ok();
   }, err, err_len);
 }
 

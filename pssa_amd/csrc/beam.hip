@@ -1,0 +1,390 @@
+// Beam search: the best continuations of a group's beams, and its states
+// reordered by them.
+//
+//   value(b, v) = score[b] + logits[b][v] - log sum_u exp(logits[b][u]),
+//
+// the `keep` largest over a group's beams b and tokens v, equal ones by beam,
+// then by token.  Within a beam the order is the logits' own, so a slice of a
+// row gives its `keep` largest logits and its part of the sum, and a workgroup
+// for each group joins the slices.  Values of different beams lie as near to
+// each other as chance has it: the sums of exponentials, their logarithms and
+// the values are in 64 bits (an fp32 logarithm would pick the wrong one of two
+// candidates in some of 10^4 close calls).
+#include <algorithm>
+
+#include "operators.h"
+
+namespace pssa {
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr uint32_t kNoToken = PSSA_HIP_NO_TOKEN;
+constexpr int kThreads = 256;
+
+struct Bf16 {
+  uint16_t bits;
+};
+template <class T>
+constexpr int vec_n() { return 16 / (int)sizeof(T); }
+
+// Larger for larger values (-0 as 0), and never 0 for one above -inf; 0 stands for none.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t o) {
+  return __uint_as_float(o ^ (~(uint32_t)((int32_t)o >> 31) | 0x80000000u));
+}
+constexpr uint32_t kOrderedLowest = 0x007FFFFFu;  // of -inf
+
+// A logit and its token as one number: by value, then by lower id.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t id) {
+  const uint32_t o = ordered(v);
+  return o > kOrderedLowest ? (uint64_t)o << 32 | (uint32_t)~id : 0;
+}
+
+// What a slice of a row leaves for the join.
+struct SliceSum {
+  double sum;    // of exp(logit - most)
+  float most;
+  uint32_t bad;  // a logit is NaN or +inf
+};
+
+__device__ __forceinline__ bool beam_ended(const BeamArgs& a, int row) {
+  return a.last && a.eos != kNoToken && a.last[row] == a.eos;
+}
+__device__ __forceinline__ bool beam_runs(const BeamArgs& a, int row) {
+  return !beam_ended(a, row) && fabsf(a.scores[row]) < INFINITY;
+}
+
+template <class T>
+__device__ __forceinline__ void load_vec(const T* row, int c, int left, float (&v)[vec_n<T>()]) {
+  constexpr int N = vec_n<T>();
+  if (left >= N) {
+    const u32x4_t u = *reinterpret_cast<const u32x4_any_t*>(row + c);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (sizeof(T) == 4)
+        v[j] = __uint_as_float(u[j]);
+      else
+        v[j] = __uint_as_float(j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[j] = -INFINITY;
+      if (j < left) {
+        if constexpr (sizeof(T) == 4)
+          v[j] = *reinterpret_cast<const float*>(row + c + j);
+        else
+          v[j] = __uint_as_float((uint32_t)row[c + j].bits << 16);
+      }
+    }
+  }
+}
+
+// A slice of a row in the registers of a workgroup, NV pieces of 16 bytes a
+// thread.  The keep-th largest of the threads' own largest keys is a bound:
+// what is below it is none of the keep largest, and only keep threads hold
+// anything that is not.
+template <class T, int NV>
+__global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
+  constexpr int N = vec_n<T>();
+  __shared__ uint64_t s_best[kThreads], s_list[kMaxBeams * NV * N], s_bound;
+  __shared__ double s_sum[4];
+  __shared__ float s_most[4];
+  __shared__ uint32_t s_count;
+  const int row = blockIdx.x, slice = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (!beam_runs(a, row)) return;
+  const T* logits = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
+  const int first = slice * kThreads * NV * N;
+
+  float v[NV][N];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = first + (tid + k * kThreads) * N;
+    load_vec<T>(logits, c, a.vocab - c, v[k]);
+  }
+  float most = -INFINITY;
+  uint64_t best = 0;
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const uint32_t id = first + (tid + k * kThreads) * N;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      bad |= !(v[k][j] < INFINITY);
+      most = fmaxf(most, v[k][j]);
+      const uint64_t key = key_of(v[k][j], id + j);
+      best = key > best ? key : best;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+  if (lane == 0) s_most[wave] = most;
+  s_best[tid] = best;
+  if (tid == 0) s_count = 0, s_bound = 0;
+  const bool any_bad = __syncthreads_or(bad);
+  most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
+
+  double sum = 0.0;
+  if (most > -INFINITY) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float part = 0.0f;  // few terms in fp32, these sums in 64 bits
+#pragma unroll
+      for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((v[k][j] - most) * kLog2e);
+      sum += part;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) s_sum[wave] = sum;
+
+  // The thread's place among the threads' best (equal ones are none, 0).
+  int above = 0;
+  for (int i = 0; i < kThreads; ++i) above += s_best[i] > best;
+  if (above == a.keep - 1 && best) s_bound = best;
+  __syncthreads();
+  const uint64_t bound = s_bound;  // 0 where fewer threads have anything
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const uint32_t id = first + (tid + k * kThreads) * N;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint64_t key = key_of(v[k][j], id + j);
+      if (key && key >= bound) s_list[atomicAdd(&s_count, 1u)] = key;
+    }
+  }
+  __syncthreads();
+  const int count = (int)s_count;
+  const size_t at = (size_t)row * a.slices + slice;
+  uint64_t* out = a.keys + at * a.keep;
+  for (int i = tid; i < count; i += kThreads) {
+    const uint64_t key = s_list[i];
+    int place = 0;
+    for (int j = 0; j < count; ++j) place += s_list[j] > key;
+    if (place < a.keep) out[place] = key;
+  }
+  for (int i = count + tid; i < a.keep; i += kThreads) out[i] = 0;
+  if (tid == 0) {
+    SliceSum s;
+    s.sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    s.most = most;
+    s.bad = any_bad;
+    static_cast<SliceSum*>(a.sums)[at] = s;
+  }
+}
+
+// A candidate: its value, and the beam and token that break ties.
+struct Candidate {
+  double value;
+  uint64_t at;  // beam << 32 | token
+};
+__device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
+  return x.value > y.value || (x.value == y.value && x.at < y.at);
+}
+__device__ __forceinline__ Candidate nothing() { return Candidate{-INFINITY, ~(uint64_t)0}; }
+
+// The join of a group's slices: rounds that each pick the best candidate left,
+// of which only the winner's thread looks for its next one.
+__global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
+  // The scores and which beams have ended, as the outputs may be written over them.
+  __shared__ double s_lse[kMaxBeams], s_score[kMaxBeams];
+  __shared__ bool s_ended[kMaxBeams];
+  __shared__ Candidate s_part[4];
+  const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row0 = group * a.beams;
+  const SliceSum* sums = static_cast<const SliceSum*>(a.sums);
+  // Each running beam's log of the sum; +inf (no candidate) where it has none.
+  for (int b = wave; b < a.beams; b += 4) {
+    double lse = INFINITY;
+    if (beam_runs(a, row0 + b)) {
+      const SliceSum* s = sums + (size_t)(row0 + b) * a.slices;
+      float most = -INFINITY;
+      bool bad = false;
+      for (int i = lane; i < a.slices; i += 64) most = fmaxf(most, s[i].most), bad |= s[i].bad != 0;
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+      double sum = 0.0;
+      for (int i = lane; i < a.slices; i += 64)
+        if (s[i].most > -INFINITY) sum += s[i].sum * exp((double)s[i].most - (double)most);
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      if (!__any(bad) && most > -INFINITY) lse = log(sum) + (double)most;
+    }
+    if (lane == 0) {
+      s_lse[b] = lse;
+      s_score[b] = a.scores[row0 + b];
+      s_ended[b] = beam_ended(a, row0 + b);
+    }
+  }
+  __syncthreads();
+
+  const int per_beam = a.slices * a.keep, all = a.beams * per_beam;
+  auto candidate = [&](int i) -> Candidate {
+    const int b = i / per_beam;
+    const double score = s_score[b];
+    if (s_ended[b])  // it stays as it is
+      return i % per_beam == 0 && fabs(score) < INFINITY ? Candidate{score, (uint64_t)b << 32 | a.eos} : nothing();
+    if (!(s_lse[b] < INFINITY)) return nothing();
+    const uint64_t key = a.keys[(size_t)row0 * per_beam + i];
+    if (!key) return nothing();
+    return Candidate{score + ((double)unordered((uint32_t)(key >> 32)) - s_lse[b]),
+                     (uint64_t)b << 32 | ((uint32_t)~key + a.first_id)};
+  };
+  Candidate mine = nothing();
+  for (int i = tid; i < all; i += kThreads) {
+    const Candidate c = candidate(i);
+    if (better(c, mine)) mine = c;
+  }
+  for (int j = 0; j < a.keep; ++j) {
+    Candidate w = mine;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const Candidate o{__shfl_xor(w.value, off, 64), (uint64_t)__shfl_xor((unsigned long long)w.at, off, 64)};
+      if (better(o, w)) w = o;
+    }
+    if (lane == 0) s_part[wave] = w;
+    __syncthreads();
+    w = s_part[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (better(s_part[i], w)) w = s_part[i];
+    __syncthreads();
+    const bool some = w.value > -INFINITY;
+    if (tid == 0) {
+      const size_t o = (size_t)group * a.keep + j;
+      a.parents[o] = some ? (uint32_t)(w.at >> 32) : kNoToken;
+      a.tokens[o] = some ? (uint32_t)w.at : kNoToken;
+      a.out_scores[o] = some ? (float)w.value : -INFINITY;
+    }
+    if (some && mine.at == w.at) {
+      mine = nothing();
+      for (int i = tid; i < all; i += kThreads) {
+        const Candidate c = candidate(i);
+        if (better(w, c) && better(c, mine)) mine = c;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ states
+// Rows of a group copied from their parents'.  A thread moves one piece of
+// every row, MOST rows at a time.  Where MOST covers a group, all are loaded
+// before the first is stored, and rows may be reordered where they are.
+template <class V, int MOST>
+__global__ __launch_bounds__(kThreads) void beam_gather_kernel(GatherArgs a) {
+  typedef V any_t __attribute__((aligned(1)));
+  const size_t c = ((size_t)blockIdx.x * kThreads + threadIdx.x) * sizeof(V);
+  if (c >= a.row_bytes) return;
+  for (int group = blockIdx.y; group < a.groups; group += gridDim.y) {
+    const uint32_t* parents = a.parents + (size_t)group * a.n_out;
+    const char* src = static_cast<const char*>(a.src) + (size_t)group * a.n_in * a.ld_src + c;
+    char* dst = static_cast<char*>(a.dst) + (size_t)group * a.n_out * a.ld_dst + c;
+    for (int j0 = 0; j0 < a.n_out; j0 += MOST) {
+      V v[MOST];
+#pragma unroll
+      for (int j = 0; j < MOST; ++j)
+        if (j0 + j < a.n_out && parents[j0 + j] < (uint32_t)a.n_in)
+          v[j] = *reinterpret_cast<const any_t*>(src + parents[j0 + j] * a.ld_src);
+#pragma unroll
+      for (int j = 0; j < MOST; ++j)
+        if (j0 + j < a.n_out && parents[j0 + j] < (uint32_t)a.n_in && !(a.src == a.dst && parents[j0 + j] == (uint32_t)(j0 + j)))
+          *reinterpret_cast<any_t*>(dst + (j0 + j) * a.ld_dst) = v[j];
+    }
+  }
+}
+
+// The first row of every group copied to all of the group's, where the first
+// rows are packed at the front: group g's rows begin behind row g, so the last
+// group goes first.
+__global__ __launch_bounds__(kThreads) void beam_spread_kernel(uint32_t* rows, size_t words, size_t ld, int groups, int beams) {
+  const size_t c = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  if (c >= words) return;
+  for (int g = groups - 1; g >= 0; --g) {
+    const uint32_t v = rows[g * ld + c];
+    for (int b = 0; b < beams; ++b) rows[((size_t)g * beams + b) * ld + c] = v;
+  }
+}
+
+// The chosen tokens as the next step's inputs; where there is none, any.
+__global__ __launch_bounds__(kThreads) void beam_feed_kernel(const uint32_t* tokens, uint32_t* ids, size_t n) {
+  const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i < n) ids[i] = tokens[i] == kNoToken ? 0 : tokens[i];
+}
+
+template <class V, int MOST>
+Status launch_pieces(hipStream_t stream, const GatherArgs& a) {
+  const size_t pieces = a.row_bytes / sizeof(V);
+  const dim3 grid((uint32_t)((pieces + kThreads - 1) / kThreads), (uint32_t)std::min(a.groups, 65535));
+  beam_gather_kernel<V, MOST><<<grid, kThreads, 0, stream>>>(a);
+  PSSA_LAUNCH_CHECK("beam_gather_kernel");
+  return Status::Ok();
+}
+
+template <class T>
+Status launch_slices(hipStream_t stream, const BeamArgs& a, size_t rows, int pieces) {
+  const dim3 grid((uint32_t)rows, a.slices);
+  if (pieces == 1)
+    beam_slice_kernel<T, 1><<<grid, kThreads, 0, stream>>>(a);
+  else if (pieces == 2)
+    beam_slice_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a);
+  else if (pieces == 4)
+    beam_slice_kernel<T, 4><<<grid, kThreads, 0, stream>>>(a);
+  else
+    beam_slice_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+  PSSA_LAUNCH_CHECK("beam_slice_kernel");
+  return Status::Ok();
+}
+
+}  // namespace
+
+BeamPlan beam_plan(int dtype, size_t rows, size_t vocab, size_t keep) {
+  BeamPlan p;
+  const size_t per = kThreads * (dtype == PSSA_HIP_F32 ? 4 : 8);
+  for (p.pieces = 1; p.pieces < 8 && rows * ((vocab + per * p.pieces - 1) / (per * p.pieces)) > 2048; p.pieces *= 2) {}
+  p.slices = (vocab + per * p.pieces - 1) / (per * p.pieces);
+  p.sums_bytes = (rows * p.slices * sizeof(SliceSum) + 255) & ~(size_t)255;
+  p.bytes = p.sums_bytes + rows * p.slices * keep * 8;
+  return p;
+}
+
+Status launch_beam_select(hipStream_t stream, int dtype, const BeamArgs& a, size_t groups, const BeamPlan& p) {
+  const size_t rows = groups * (size_t)a.beams;
+  PSSA_RETURN_IF(dtype == PSSA_HIP_F32 ? launch_slices<float>(stream, a, rows, p.pieces)
+                                       : launch_slices<Bf16>(stream, a, rows, p.pieces));
+  beam_join_kernel<<<(uint32_t)groups, kThreads, 0, stream>>>(a);
+  PSSA_LAUNCH_CHECK("beam_join_kernel");
+  return Status::Ok();
+}
+
+// 16 bytes a thread and row up to 16 rows (64 registers), more rows in parts
+// of 16, but for those that are reordered in place: 4 bytes of up to 64 rows.
+Status launch_beam_gather(hipStream_t stream, const GatherArgs& a) {
+  const bool in_place = a.src == a.dst;
+  if (a.row_bytes % 16 == 0 && (a.n_out <= 16 || !in_place)) {
+    if (a.n_out <= 4) return launch_pieces<u32x4_t, 4>(stream, a);
+    if (a.n_out <= 8) return launch_pieces<u32x4_t, 8>(stream, a);
+    return launch_pieces<u32x4_t, 16>(stream, a);
+  }
+  if (a.row_bytes % 4 == 0) return launch_pieces<uint32_t, kMaxBeams>(stream, a);
+  return launch_pieces<uint8_t, kMaxBeams>(stream, a);
+}
+
+Status launch_beam_feed(hipStream_t stream, const uint32_t* tokens, uint32_t* ids, size_t n) {
+  beam_feed_kernel<<<(uint32_t)((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(tokens, ids, n);
+  PSSA_LAUNCH_CHECK("beam_feed_kernel");
+  return Status::Ok();
+}
+
+Status launch_beam_spread(hipStream_t stream, void* rows, size_t words, size_t ld, size_t groups, size_t beams) {
+  beam_spread_kernel<<<(uint32_t)((words + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+      static_cast<uint32_t*>(rows), words, ld, (int)groups, (int)beams);
+  PSSA_LAUNCH_CHECK("beam_spread_kernel");
+  return Status::Ok();
+}
+
+}  // namespace pssa

@@ -1,6 +1,7 @@
 // Language-model operators on device-resident arrays: log probabilities and
 // distillation over logit rows, linear attention with a decay for each head,
-// products with 4-bit weights.
+// the gated delta rule, products with 4-bit weights, norms with 8-bit rows and
+// products of these, beam search.
 #pragma once
 #include "common.h"
 
@@ -84,5 +85,98 @@ Status init_linear_attributes();
 // Tokens of a segment where a call of these sizes is split, else 0.
 int linear_segment(const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val);
 Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& a, int longest);
+
+// ------------------------------------------------------------------- norms
+constexpr size_t kRmsWidth = 65536;  // the widest row: a workgroup's registers
+
+struct RmsNormArgs {
+  const void *x = nullptr, *residual = nullptr;  // row r at r * ld; residual may be null
+  size_t ld_x = 0, ld_residual = 0, ld_sum = 0, ld_out = 0, ld_codes = 0;
+  const float* gamma = nullptr;  // [width], null: ones
+  int width = 0;
+  bool normed = true;  // false: codes of the rows as they are
+  float eps = 0.0f;
+  // Each may be null (codes and scales together); out needs gamma.
+  void *sum = nullptr, *out = nullptr;
+  int8_t* codes = nullptr;
+  float* scales = nullptr;
+};
+Status launch_rms_norm(hipStream_t stream, int dtype, const RmsNormArgs& a, size_t rows);
+
+// ---------------------------------------------------------- 8-bit products
+constexpr size_t kI8Depth = 131071;  // 128 * 128 * k stays below 2^31
+
+struct I8Args {
+  const int8_t *x = nullptr, *w = nullptr;  // rows of k codes
+  size_t ld_x = 0, ld_w = 0, ld_y = 0;
+  const float *x_scales = nullptr, *w_scales = nullptr;  // [m], [n]
+  void* y = nullptr;
+  int m = 0, n = 0, k = 0;
+  int splits = 1;           // parts of k, summed in `parts`
+  int32_t* parts = nullptr; // [splits, m, n]
+};
+// Parts of k of a product of these sizes.
+int i8_splits(size_t m, size_t n, size_t k);
+Status init_i8_attributes();
+Status launch_matmul_i8(hipStream_t stream, int y_dtype, const I8Args& a);
+
+// -------------------------------------------------------- gated delta rule
+constexpr int kDeltaMaxKey = 128;   // d_key held in a workgroup's tiles
+constexpr int kDeltaInline = 256;   // sequences whose offsets travel with the kernel's arguments
+
+struct DeltaArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // token t, head h at t * ld + h * width
+  size_t ld_q = 0, ld_k = 0, ld_v = 0, ld_out = 0, ld_gates = 0;
+  const float *log_decay = nullptr, *beta = nullptr;  // token t, head h at t * ld_gates + h
+  const float* state_in = nullptr;  // [n_seqs, heads, dk, dv] or null (zeros)
+  float* state_out = nullptr;       // likewise, or null
+  void* out = nullptr;
+  float scale = 1.0f;
+  int n_seqs = 0, heads = 0, key_heads = 0, dk = 0, dv = 0;
+  int uniform_len = -1;  // every sequence's length, or -1: the tables
+  // [n_seqs + 1] first tokens: on the device, or null and here.
+  const uint32_t* table = nullptr;
+  uint32_t inline_tokens[kDeltaInline + 1] = {};
+};
+Status launch_delta_rule(hipStream_t stream, int dtype, const DeltaArgs& a, int longest);
+
+// ------------------------------------------------------------- beam search
+constexpr int kMaxBeams = 64;  // of a group, before and after a step
+
+struct BeamArgs {
+  const void* logits = nullptr;  // row g * beams + b at row * ld
+  size_t ld = 0;
+  int vocab = 0, beams = 0, keep = 0;
+  const float* scores = nullptr;   // [groups, beams]
+  const uint32_t* last = nullptr;  // [groups, beams] or null
+  uint32_t eos = PSSA_HIP_NO_TOKEN;
+  uint32_t first_id = 0;  // the token of a row's first logit
+  uint32_t *parents = nullptr, *tokens = nullptr;  // [groups, keep]
+  float* out_scores = nullptr;                     // [groups, keep]
+  int slices = 1;
+  void* sums = nullptr;      // scratch [rows, slices]
+  uint64_t* keys = nullptr;  // scratch [rows, slices, keep]
+};
+// How the rows of a call are cut: pieces of 16 bytes a thread, slices a row,
+// and the scratch (sums, then keys).
+struct BeamPlan {
+  int pieces = 1;
+  size_t slices = 1, sums_bytes = 0, bytes = 0;
+};
+BeamPlan beam_plan(int dtype, size_t rows, size_t vocab, size_t keep);
+Status launch_beam_select(hipStream_t stream, int dtype, const BeamArgs& a, size_t groups, const BeamPlan& p);
+
+struct GatherArgs {
+  const void* src = nullptr;  // row i of group g at (g * n_in + i) * ld_src bytes
+  void* dst = nullptr;        // may be src
+  size_t ld_src = 0, ld_dst = 0, row_bytes = 0;
+  int groups = 0, n_in = 0, n_out = 0;
+  const uint32_t* parents = nullptr;  // [groups, n_out]; a row whose parent is not below n_in stays as it is
+};
+Status launch_beam_gather(hipStream_t stream, const GatherArgs& a);
+// Rows 0 .. groups-1 copied to rows g * beams .. + beams - 1 of the same array.
+Status launch_beam_spread(hipStream_t stream, void* rows, size_t words, size_t ld, size_t groups, size_t beams);
+// The chosen tokens as the next step's inputs (0 where there is none).
+Status launch_beam_feed(hipStream_t stream, const uint32_t* tokens, uint32_t* ids, size_t n);
 
 }  // namespace pssa

@@ -375,6 +375,94 @@ class HipDevice:
         _abi.call(self._lib.pssa_hip_linear_attention_reserve, self.handle, _dtype(dtype), lens, n_seqs, seq_len, heads,
                   d_key, d_val)
 
+    def delta_rule_resident(self, q_ptr: int, k_ptr: int, v_ptr: int, log_decay_ptr: int, beta_ptr: int, dtype: str,
+                            heads: int, d_key: int, d_val: int, out_ptr: int, lens=None, n_seqs: int = 1,
+                            seq_len: int = 1, key_heads: int | None = None, scale: float = 1.0,
+                            state_in_ptr: int | None = None, state_out_ptr: int | None = None, ld_q: int | None = None,
+                            ld_k: int | None = None, ld_v: int | None = None, ld_gates: int | None = None,
+                            ld_out: int | None = None) -> None:
+        """The gated delta rule S_t = a_t (1 - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T with a_t = exp(log_decay_t),
+        out_t = scale q_t S_t, over packed sequences of `lens` tokens (or n_seqs of seq_len), on device arrays: q and k
+        [tokens, key_heads, d_key], v and out [tokens, heads, d_val] with row strides ld_*, f32 gates [tokens, heads]
+        with row stride ld_gates, f32 states [n_seqs, heads, d_key, d_val] (asynchronous on the context stream)."""
+        kh = heads if key_heads is None else key_heads
+        if lens is not None:
+            lens, n_seqs = _lens(lens), len(lens)
+        _abi.call(self._lib.pssa_hip_delta_rule_resident, self.handle, _dtype(dtype), q_ptr,
+                  kh * d_key if ld_q is None else ld_q, k_ptr, kh * d_key if ld_k is None else ld_k, v_ptr,
+                  heads * d_val if ld_v is None else ld_v, log_decay_ptr, beta_ptr, heads if ld_gates is None else ld_gates,
+                  state_in_ptr, lens, n_seqs, seq_len, heads, kh, d_key, d_val, scale, out_ptr,
+                  heads * d_val if ld_out is None else ld_out, state_out_ptr)
+
+    def delta_rule_reserve(self, dtype: str, heads: int, d_key: int, d_val: int, lens=None, n_seqs: int = 1,
+                           seq_len: int = 1) -> None:
+        """Sizes the context's scratch for delta_rule_resident calls of these lengths and widths, so that they allocate
+        nothing."""
+        if lens is not None:
+            lens, n_seqs = _lens(lens), len(lens)
+        _abi.call(self._lib.pssa_hip_delta_rule_reserve, self.handle, _dtype(dtype), lens, n_seqs, seq_len, heads, d_key,
+                  d_val)
+
+    def rms_norm_resident(self, x_ptr: int, dtype: str, rows: int, width: int, gamma_ptr: int,
+                          residual_ptr: int | None = None, sum_ptr: int | None = None, out_ptr: int | None = None,
+                          codes_ptr: int | None = None, scales_ptr: int | None = None, eps: float = 1e-5,
+                          ld_x: int | None = None, ld_residual: int | None = None, ld_sum: int | None = None,
+                          ld_out: int | None = None, ld_codes: int | None = None) -> None:
+        """h = x + residual, out = gamma h / sqrt(mean(h^2) + eps) for rows on the device: h to sum_ptr and the normed
+        rows to out_ptr (both of `dtype`; they may be x_ptr or residual_ptr), and/or in 8 bits to codes_ptr with an f32
+        scale for each row (asynchronous on the context stream)."""
+        ld_x = width if ld_x is None else ld_x
+        ld_residual = width if ld_residual is None else ld_residual
+
+        def of(ptr, ld):  # an output in place has its input's stride
+            if ld is not None or ptr is None:
+                return width if ld is None else ld
+            return ld_x if ptr == x_ptr else ld_residual if ptr == residual_ptr else width
+
+        _abi.call(self._lib.pssa_hip_rms_norm_resident, self.handle, _dtype(dtype), x_ptr, ld_x, residual_ptr, ld_residual,
+                  gamma_ptr, eps, rows, width, sum_ptr, of(sum_ptr, ld_sum), out_ptr, of(out_ptr, ld_out), codes_ptr,
+                  width if ld_codes is None else ld_codes, scales_ptr)
+
+    def quantize_i8_resident(self, x_ptr: int, dtype: str, rows: int, width: int, codes_ptr: int, scales_ptr: int,
+                             ld_x: int | None = None, ld_codes: int | None = None) -> None:
+        """Rows on the device in 8 bits, codes = round(x 127 / max|x|), with an f32 scale max|x| / 127 for each: activations,
+        or a weight's channels (asynchronous on the context stream)."""
+        _abi.call(self._lib.pssa_hip_quantize_i8_resident, self.handle, _dtype(dtype), x_ptr, width if ld_x is None else ld_x,
+                  rows, width, codes_ptr, width if ld_codes is None else ld_codes, scales_ptr)
+
+    def matmul_i8_resident(self, x_ptr: int, x_scales_ptr: int, w_ptr: int, w_scales_ptr: int, m: int, n: int, k: int,
+                           y_ptr: int, y_dtype: str = "f32", ld_x: int | None = None, ld_w: int | None = None,
+                           ld_y: int | None = None) -> None:
+        """y[m, n] = x W^T of 8-bit rows x [m, k] and weights W [n, k] with f32 scales for each row and channel, exact sums
+        (asynchronous on the context stream)."""
+        _abi.call(self._lib.pssa_hip_matmul_i8_resident, self.handle, x_ptr, k if ld_x is None else ld_x, x_scales_ptr,
+                  w_ptr, k if ld_w is None else ld_w, w_scales_ptr, m, n, k, y_ptr, _dtype(y_dtype),
+                  n if ld_y is None else ld_y)
+
+    def matmul_i8_reserve(self, m: int, n: int, k: int) -> None:
+        """Sizes the context's scratch for such a product, so that it allocates nothing."""
+        _abi.call(self._lib.pssa_hip_matmul_i8_reserve, self.handle, m, n, k)
+
+    def beam_select_resident(self, logits_ptr: int, dtype: str, groups: int, beams: int, vocab: int, scores_ptr: int,
+                             keep: int, parents_ptr: int, tokens_ptr: int, out_scores_ptr: int,
+                             last_ptr: int | None = None, eos: int = _abi.NO_TOKEN, ld: int | None = None) -> None:
+        """The `keep` best continuations of each of `groups` requests by scores [groups, beams] + log softmax(logits
+        [groups * beams, vocab]): parents (beams), tokens (both u32) and f32 scores [groups, keep], best first.  A beam
+        whose last token is `eos` stays as it is (asynchronous on the context stream)."""
+        _abi.call(self._lib.pssa_hip_beam_select_resident, self.handle, logits_ptr, _dtype(dtype), groups, beams, vocab,
+                  vocab if ld is None else ld, scores_ptr, last_ptr, eos, keep, parents_ptr, tokens_ptr, out_scores_ptr)
+
+    def beam_select_reserve(self, groups: int, beams: int, vocab: int, keep: int) -> None:
+        """Sizes the context's scratch for such selections, so that they allocate nothing."""
+        _abi.call(self._lib.pssa_hip_beam_select_reserve, self.handle, groups, beams, vocab, keep)
+
+    def beam_gather_resident(self, src_ptr: int, dst_ptr: int, row_bytes: int, groups: int, n_in: int, parents_ptr: int,
+                             n_out: int, ld_src: int | None = None, ld_dst: int | None = None) -> None:
+        """Reorders states: row j of each group of n_out becomes its row parents[group, j] of n_in (rows of row_bytes at
+        strides of ld_* bytes); in place where dst_ptr is src_ptr (asynchronous on the context stream)."""
+        _abi.call(self._lib.pssa_hip_beam_gather_resident, self.handle, src_ptr, row_bytes if ld_src is None else ld_src,
+                  dst_ptr, row_bytes if ld_dst is None else ld_dst, row_bytes, groups, n_in, parents_ptr, n_out)
+
     def w4_matrix_resident(self, codes_ptr: int, scales_ptr: int, n: int, k: int, group: int,
                            zeros_ptr: int | None = None) -> "W4Matrix":
         """4-bit weights from device arrays: u8 codes [n, k], f32 scales [n, ceil(k / group)] and u8 zero points
@@ -703,6 +791,19 @@ class PSSALayer:
                   _abi.ptr(out, C.c_uint32), out.size, _abi.ptr(logits), 0 if logits is None else logits.size)
         self._staged = None
         return (out, logits) if want_logits else out
+
+    def beam_search(self, steps: int, beams: int, eos: int = _abi.NO_TOKEN, n_groups: int | None = None):
+        """Beam search from the last prefill of n_groups lanes (by default as many as it had), each of which becomes
+        `beams` lanes.  Returns ids [n_groups, beams, steps], best first, and their summed log probabilities [n_groups,
+        beams]; a beam that has chosen `eos` ends there and repeats it."""
+        if n_groups is None:
+            n_groups = self._staged[0] if getattr(self, "_staged", None) else 0
+        ids = np.empty((n_groups, beams, steps), np.uint32)
+        scores = np.empty((n_groups, beams), np.float32)
+        _abi.call(self._lib.pssa_hip_beam_search, self.handle, n_groups, beams, steps, eos, _abi.ptr(ids, C.c_uint32),
+                  ids.size, _abi.ptr(scores), scores.size)
+        self._staged = None
+        return ids, scores
 
     def get_taps(self, layer: int, n_lanes: int) -> dict:
         """Block `layer`'s taps of the last plastic decode step over n_lanes lanes:
