@@ -2620,10 +2620,6 @@ Status check_i8(size_t m, size_t n, size_t k) {
   PSSA_RETURN_IF(need(k <= pssa::kI8Depth, "8-bit product: k above 131071 is not supported"));
   return need(m <= ((size_t)1 << 20) && n <= ((size_t)1 << 24), "8-bit product: too large");
 }
-size_t i8_scratch(size_t m, size_t n, size_t k) {
-  const size_t splits = (size_t)pssa::i8_splits(m, n, k);
-  return splits > 1 ? splits * m * n * 4 : 0;
-}
 Status check_beams(size_t groups, size_t beams, size_t vocab, size_t keep) {
   PSSA_RETURN_IF(need(groups && vocab, "beam selection: dimensions must be positive"));
   PSSA_RETURN_IF(need(beams >= 1 && beams <= (size_t)pssa::kMaxBeams && keep >= 1 && keep <= (size_t)pssa::kMaxBeams,
@@ -2849,12 +2845,11 @@ int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_
     a.m = (int)m;
     a.n = (int)n;
     a.k = (int)k;
-    a.splits = pssa::i8_splits(m, n, k);
+    const pssa::I8Plan plan = pssa::i8_plan(m, n, k);
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
-    PSSA_RETURN_IF(grow_scratch(ctx, i8_scratch(m, n, k), false));
-    a.parts = static_cast<int32_t*>(ctx->scratch);
-    return pssa::launch_matmul_i8(ctx->stream, y_dtype, a);
+    PSSA_RETURN_IF(grow_scratch(ctx, plan.bytes(), false));
+    return pssa::launch_matmul_i8(ctx->stream, y_dtype, a, plan, ctx->scratch);
   }, err, err_len);
 }
 
@@ -2864,7 +2859,7 @@ int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, 
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
-    return grow_scratch(ctx, i8_scratch(m, n, k), false);
+    return grow_scratch(ctx, pssa::i8_plan(m, n, k).bytes(), false);
   }, err, err_len);
 }
 

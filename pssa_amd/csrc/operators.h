@@ -112,13 +112,20 @@ struct I8Args {
   const float *x_scales = nullptr, *w_scales = nullptr;  // [m], [n]
   void* y = nullptr;
   int m = 0, n = 0, k = 0;
-  int splits = 1;           // parts of k, summed in `parts`
-  int32_t* parts = nullptr; // [splits, m, n]
+  int splits = 1;            // parts of k
+  int32_t* parts = nullptr;  // [splits, m, n] sums of each, where there are several
 };
-// Parts of k of a product of these sizes.
-int i8_splits(size_t m, size_t n, size_t k);
+constexpr int kI8FewRows = 64;  // up to these the weights go straight to registers
+// Parts of k of a product of these sizes, and its scratch: the parts' sums,
+// and copies of rows and weights that do not lie in units of 16 bytes.
+struct I8Plan {
+  int splits = 1;
+  size_t parts_bytes = 0, pack_bytes = 0;
+  size_t bytes() const { return ((parts_bytes + 255) & ~(size_t)255) + pack_bytes; }
+};
+I8Plan i8_plan(size_t m, size_t n, size_t k);
 Status init_i8_attributes();
-Status launch_matmul_i8(hipStream_t stream, int y_dtype, const I8Args& a);
+Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan& p, void* scratch);
 
 // -------------------------------------------------------- gated delta rule
 constexpr int kDeltaMaxKey = 128;   // d_key held in a workgroup's tiles
