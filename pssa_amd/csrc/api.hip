@@ -207,6 +207,7 @@ int pssa_hip_init(int device, pssa_hip_ctx** out, char* err, size_t err_len) {
     PSSA_RETURN_IF(pssa::init_w4_attributes());
     PSSA_RETURN_IF(pssa::init_linear_attributes());
     PSSA_RETURN_IF(pssa::init_i8_attributes());
+    PSSA_RETURN_IF(pssa::init_delta_attributes());
     PSSA_RETURN_IF(pssa::noalloc_scratch_address(&ctx->noalloc_scratch));
     *out = ctx.release();
     return Status::Ok();
@@ -2558,35 +2559,48 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
 
 namespace {
 
-// The sequences of a delta rule call.
+// The sequences of a delta rule call and the scratch that it takes.
 struct DeltaPlan {
-  std::vector<uint32_t> table;  // first tokens, where the arguments do not hold them
+  std::vector<uint32_t> table;  // first tokens and chunks, where the arguments do not hold them
   size_t tokens = 0, longest = 0;
+  pssa::DeltaScratch scratch;
 
-  size_t scratch_bytes() const { return table.size() * 4; }
+  // What is worked out ahead, row copies, then the table.
+  size_t table_at() const { return scratch.ahead + scratch.rows; }
+  size_t scratch_bytes() const { return table_at() + table.size() * 4; }
 };
-Status plan_delta(const uint64_t* lens, size_t n_seqs, size_t seq_len, pssa::DeltaArgs& a, DeltaPlan& p) {
+Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_key, size_t d_val,
+                  pssa::DeltaArgs& a, DeltaPlan& p) {
   PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "delta rule: sequences must be in 1..=65535"));
   a.n_seqs = (int)n_seqs;
+  const size_t chunk = (size_t)pssa::delta_chunk(dtype);
+  size_t chunks = 0;
   bool same = true;
   for (size_t i = 0; i < n_seqs; ++i) {
     const size_t len = lens ? lens[i] : seq_len;
     PSSA_RETURN_IF(need(len <= INT32_MAX && p.tokens + len <= INT32_MAX, "delta rule: too many tokens"));
     p.tokens += len;
+    chunks += (len + chunk - 1) / chunk;
     p.longest = std::max(p.longest, len);
     same &= !lens || lens[i] == lens[0];
   }
+  a.chunks = (int)chunks;
+  if (p.longest > (size_t)pssa::kDeltaSteps)
+    p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, heads, d_key, d_val);
   a.uniform_len = same ? (int)p.longest : -1;
   if (same) return Status::Ok();
   const bool inside = n_seqs <= (size_t)pssa::kDeltaInline;
-  if (!inside) p.table.resize(n_seqs + 1);
+  if (!inside) p.table.resize(2 * (n_seqs + 1));
   uint32_t* tok = inside ? a.inline_tokens : p.table.data();
-  uint32_t t = 0;
-  for (size_t i = 0; i < n_seqs; ++i) {
+  uint32_t* first = inside ? a.inline_chunks : p.table.data() + n_seqs + 1;
+  uint32_t t = 0, c = 0;
+  for (size_t i = 0; i <= n_seqs; ++i) {
     tok[i] = t;
+    first[i] = c;
+    if (i == n_seqs) break;
     t += (uint32_t)lens[i];
+    c += (uint32_t)((lens[i] + chunk - 1) / chunk);
   }
-  tok[n_seqs] = t;
   return Status::Ok();
 }
 Status check_delta_heads(size_t heads, size_t d_key, size_t d_val) {
@@ -2675,7 +2689,7 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
                         "delta rule: misaligned buffer"));
     pssa::DeltaArgs a;
     DeltaPlan plan;
-    PSSA_RETURN_IF(plan_delta(lens, n_seqs, seq_len, a, plan));
+    PSSA_RETURN_IF(plan_delta(dtype, lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
     const size_t tokens = plan.tokens;
     size_t n = 0;
     for (size_t ld : {ld_q, ld_k, ld_v, ld_out, ld_gates})
@@ -2712,11 +2726,13 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     PSSA_RETURN_IF(grow_scratch(ctx, plan.scratch_bytes(), false));
+    char* scratch = static_cast<char*>(ctx->scratch);
     if (!plan.table.empty()) {
-      PSSA_RETURN_IF(ctx->stage.to_device(ctx->scratch, plan.table.data(), plan.table.size() * 4, ctx->stream));
-      a.table = static_cast<uint32_t*>(ctx->scratch);
+      uint32_t* table = reinterpret_cast<uint32_t*>(scratch + plan.table_at());
+      PSSA_RETURN_IF(ctx->stage.to_device(table, plan.table.data(), plan.table.size() * 4, ctx->stream));
+      a.table = table;
     }
-    return pssa::launch_delta_rule(ctx->stream, dtype, a, (int)plan.longest);
+    return pssa::launch_delta_rule(ctx->stream, dtype, a, tokens, (int)plan.longest, plan.scratch, scratch);
   }, err, err_len);
 }
 
@@ -2727,7 +2743,7 @@ int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* le
     PSSA_RETURN_IF(check_delta_heads(heads, d_key, d_val));
     pssa::DeltaArgs a;
     DeltaPlan plan;
-    PSSA_RETURN_IF(plan_delta(lens, n_seqs, seq_len, a, plan));
+    PSSA_RETURN_IF(plan_delta(dtype, lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));

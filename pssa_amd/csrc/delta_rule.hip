@@ -2,65 +2,47 @@
 //   S_t = a_t (1 - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T,   o_t = scale q_t S_t,
 // a_t = exp(log_decay_t).  With u_t = beta_t (v_t - a_t k_t S_{t-1}) that is
 //   S_t = a_t S_{t-1} + k_t u_t^T,   o_t = scale (a_t q_t S_{t-1} + (q_t k_t) u_t).
+//
+// Prompts run in chunks of 64 tokens (32 in fp32).  With G_i the sum of the
+// chunk's log decays up to token i, and S the state that the chunk is entered
+// with, the tokens' u solve a triangular system:
+//   (1 + A) U = beta (V - e^G K S),   A_ij = beta_i e^(G_i - G_j) k_i k_j for j < i,
+//   O = scale e^G Q S + P U,          P_ij = scale e^(G_i - G_j) q_i k_j for j <= i,
+//   S' = e^(G_n) S + K^T (e^(G_n - G) U).
+// T = (1 + A)^-1 beta and P need no state: a first kernel works them out for
+// all chunks at once (delta_ahead), a second one walks the chunks of a
+// sequence, a head and 64 value columns with S in its registers (delta_walk).
+// There everything follows in registers: the accumulators' layout (lane l
+// holds column l % 16, rows 4 (l / 16) + r) is the next product's operand
+// layout once what meets it is read in the same order.
 #include <algorithm>
 #include <cstddef>
 #include <type_traits>
 
+#include "attention_tiles.h"
 #include "operators.h"
 
 namespace pssa {
 namespace {
 
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-typedef u32x2_t u32x2_any_t __attribute__((aligned(2)));
-
-struct Bf16 {
-  uint16_t bits;
-};
-
-// Four neighbouring elements in fp32, zeros past `left`.
-template <class T>
-__device__ __forceinline__ f32x4_t load4(const T* p, int left);
-template <>
-__device__ __forceinline__ f32x4_t load4<float>(const float* p, int left) {
-  if (left >= 4) return *reinterpret_cast<const f32x4_any_t*>(p);
-  f32x4_t v = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (i < left) v[i] = p[i];
-  return v;
-}
-template <>
-__device__ __forceinline__ f32x4_t load4<Bf16>(const Bf16* p, int left) {
-  f32x4_t v = {0, 0, 0, 0};
-  if (left >= 4) {
-    const u32x2_t u = *reinterpret_cast<const u32x2_any_t*>(p);
-    return f32x4_t{__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xFFFF0000u), __uint_as_float(u[1] << 16),
-                   __uint_as_float(u[1] & 0xFFFF0000u)};
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (i < left) v[i] = __uint_as_float((uint32_t)p[i].bits << 16);
-  return v;
-}
 template <class T>
 __device__ __forceinline__ float load1(const T* p);
 template <>
 __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float load1<Bf16>(const Bf16* p) { return __uint_as_float((uint32_t)p->bits << 16); }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(Bf16* p, float v) { p->bits = bf16_bits_dev(v); }
 
-// The arguments' table is read from the kernel's argument segment, where the
-// arguments lie first: indexing the struct itself would copy it to scratch.
-typedef const __attribute__((address_space(4))) char* kernarg_t;
-__device__ __forceinline__ uint32_t first_token(const DeltaArgs& a, int seq) {
-  if (a.table) return a.table[seq];
+// The arguments lie first in the kernel's argument segment; indexing the
+// struct itself would copy it to scratch.
+__device__ __forceinline__ uint32_t inline_word(size_t offset, int i) {
   return reinterpret_cast<const __attribute__((address_space(4))) uint32_t*>(
-      (kernarg_t)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(DeltaArgs, inline_tokens))[seq];
+      (kernarg_t)__builtin_amdgcn_kernarg_segment_ptr() + offset)[i];
+}
+__device__ __forceinline__ uint32_t first_token(const DeltaArgs& a, int seq) {
+  return a.table ? a.table[seq] : inline_word(offsetof(DeltaArgs, inline_tokens), seq);
+}
+__device__ __forceinline__ int first_chunk(const DeltaArgs& a, int seq) {
+  return (int)(a.table ? a.table[a.n_seqs + 1 + seq] : inline_word(offsetof(DeltaArgs, inline_chunks), seq));
 }
 // A sequence's tokens.
 struct Span {
@@ -118,7 +100,7 @@ __global__ __launch_bounds__(256) void delta_steps_kernel(DeltaArgs a) {
         qk = fmaf(qd, kd, qk);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          S[i][e] *= decay;
+          S[i][e] = decay == 0.0f ? 0.0f : S[i][e] * decay;
           ks[e] = fmaf(kd, S[i][e], ks[e]);
           qs[e] = fmaf(qd, S[i][e], qs[e]);
         }
@@ -183,6 +165,636 @@ __global__ __launch_bounds__(256) void delta_steps_kernel(DeltaArgs a) {
   }
 }
 
+// ------------------------------------------------------------------- chunks
+constexpr double kLog2e = 1.4426950408889634;
+constexpr float kForget = -1e4f;  // a log decay below it forgets all the same, and its sums stay finite
+
+// A chunk's place: its sequence's and its own first token, its tokens.
+struct Place {
+  size_t tok;
+  int n;
+};
+template <int C>
+__device__ __forceinline__ Place place_of(const DeltaArgs& a, int chunk) {
+  if (a.uniform_len >= 0) {
+    const int per = (a.uniform_len + C - 1) / C, seq = chunk / per, pos = (chunk - seq * per) * C;
+    return Place{(size_t)seq * a.uniform_len + pos, min(C, a.uniform_len - pos)};
+  }
+  int lo = 0, hi = a.n_seqs - 1;  // the last sequence whose chunks begin at or before this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_chunk(a, mid) <= chunk) lo = mid; else hi = mid - 1;
+  }
+  const int pos = (chunk - first_chunk(a, lo)) * C;
+  const uint32_t tok = first_token(a, lo);
+  return Place{(size_t)tok + pos, min(C, (int)(first_token(a, lo + 1) - tok) - pos)};
+}
+
+// What is worked out ahead for a chunk and head, in units of 16 bytes: the
+// fragments of T and P where a triangle holds anything, then e^G and
+// e^(G_n - G) of the tokens.  bf16: a fragment is 16 tokens by 32, in two
+// parts; fp32: 16 by 16.
+template <bool B16>
+struct Ahead {
+  static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3;
+  static constexpr int kT = 0, kP = kPairs * (B16 ? 128 : 64), kGamma = 2 * kP, kRest = kGamma + C / 4, kUnits = kGamma + 64;
+};
+// The fragment of token tile t over keys 32 h .. (bf16), 16 h .. (fp32).
+template <bool B16>
+__device__ __forceinline__ constexpr int pair_of(int t, int h) {
+  return B16 ? (t < 2 ? t : 2 * t - 2 + h) : t + h;
+}
+
+// One wave works out a chunk of one head.  A's triangle lies in LDS; its
+// diagonal blocks of 16 x 16 are inverted by forward substitution, a column a
+// lane and the four blocks side by side, the others follow as products:
+//   T_rc = -D_r sum_j A_rj T_jc, c <= j < r.
+template <bool B16, int DKP>
+__global__ __launch_bounds__(64) void delta_ahead_kernel(DeltaArgs a) {
+  using Out = Ahead<B16>;
+  using T = std::conditional_t<B16, Bf16, float>;
+  constexpr int C = Out::C, NT = Out::kTiles, LD = C + 4, KF = B16 ? DKP / 32 : DKP / 16;
+  __shared__ __attribute__((aligned(16))) float s_a[C * LD];
+  __shared__ double s_g[C];
+  __shared__ float s_beta[C];
+  const int lane = threadIdx.x, col = lane & 15, quad = lane >> 4;
+  const int head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads);
+  const Place pl = place_of<C>(a, blockIdx.x);
+  u32x4_t* out = reinterpret_cast<u32x4_t*>(a.ahead) + ((size_t)blockIdx.x * a.heads_here + blockIdx.y) * Out::kUnits;
+
+  // The gates: sums of the log decays in 64 bits, since their differences count.
+  {
+    const bool on = lane < pl.n;
+    float g = on ? a.log_decay[(pl.tok + lane) * a.ld_gates + head] : 0.0f;
+    g = g < kForget ? kForget : g;
+    double sum = g;
+#pragma unroll
+    for (int off = 1; off < C; off <<= 1) {
+      const double o = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += o;
+    }
+    const double all = __shfl(sum, C - 1, 64);
+    if (lane < C) {
+      s_g[lane] = sum;
+      s_beta[lane] = on ? a.beta[(pl.tok + lane) * a.ld_gates + head] : 0.0f;
+      float* f = reinterpret_cast<float*>(out + Out::kGamma);
+      f[lane] = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
+      f[C + lane] = __builtin_amdgcn_exp2f((float)((all - sum) * kLog2e));
+    }
+  }
+  const T* k0 = static_cast<const T*>(a.k) + (size_t)key_head * a.wide_k;
+  const T* q0 = static_cast<const T*>(a.q) + (size_t)key_head * a.wide_q;
+  // Rows in their own order: 16 bytes a lane.
+  auto rows = [&](const T* base, size_t ld, int t, u32x4_t (&f)[KF]) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int i = 16 * t + col;
+#pragma unroll
+    for (int b = 0; b < KF; ++b) {
+      const int c = 4 * N * b + N * quad;
+      f[b] = u32x4_t{0, 0, 0, 0};
+      if (i < pl.n && c < a.dk) f[b] = *reinterpret_cast<const u32x4_t*>(base + (pl.tok + i) * ld + c);
+    }
+  };
+  auto dot = [&](const u32x4_t (&x)[KF], const u32x4_t (&y)[KF]) {
+    f32x4_t s = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < KF; ++b) {
+      if constexpr (B16) {
+        s = mfma(x[b], y[b], s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = mfma32(__uint_as_float(x[b][e]), __uint_as_float(y[b][e]), s);
+      }
+    }
+    return s;
+  };
+  u32x4_t kf[NT][KF];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) rows(k0, a.ld_k, t, kf[t]);
+  wave_sync();
+  double gi[4];
+#pragma unroll
+  for (int r = 0; r < NT; ++r) {
+    // P^T: queries 16 r + col, keys 16 c + 4 quad + e.
+    u32x4_t qf[KF];
+    rows(q0, a.ld_q, r, qf);
+    const double gq = s_g[16 * r + col];
+    f32x4_t p[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) p[c] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c <= r; ++c) {
+      const f32x4_t s = dot(kf[c], qf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = 16 * c + 4 * quad + e;
+        const float w = a.scale * __builtin_amdgcn_exp2f((float)((gq - s_g[key]) * kLog2e));
+        p[c][e] = 16 * r + col >= key ? s[e] * w : 0.0f;
+      }
+    }
+    if constexpr (B16) {
+#pragma unroll
+      for (int h = 0; 2 * h <= r; ++h) {
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t u, l;
+          split2(p[2 * h + (x >> 1)][2 * (x & 1)], p[2 * h + (x >> 1)][2 * (x & 1) + 1], u, l);
+          hi[x] = u;
+          lo[x] = l;
+        }
+        out[Out::kP + 128 * pair_of<B16>(r, h) + lane] = hi;
+        out[Out::kP + 128 * pair_of<B16>(r, h) + 64 + lane] = lo;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c <= r; ++c) out[Out::kP + 64 * pair_of<B16>(r, c) + lane] = __builtin_bit_cast(u32x4_t, p[c]);
+    }
+    // A: rows 16 r + 4 quad + e, columns 16 c + col.
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gi[e] = s_g[16 * r + 4 * quad + e];
+#pragma unroll
+    for (int c = 0; c <= r; ++c) {
+      const f32x4_t s = dot(kf[r], kf[c]);
+      const double gk = s_g[16 * c + col];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * r + 4 * quad + e;
+        const float w = s_beta[i] * __builtin_amdgcn_exp2f((float)((gi[e] - gk) * kLog2e));
+        s_a[i * LD + 16 * c + col] = i > 16 * c + col ? s[e] * w : 0.0f;
+      }
+    }
+  }
+  wave_sync();
+  // The diagonal blocks' inverses, each over its block.
+  {
+    const int r = NT == 4 ? quad : quad & 1;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = i == col ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j4 = 0; j4 < i; j4 += 4) {
+        const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + i) * LD + 16 * r + j4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j4 + e < i) x[i] = fmaf(-w[e], x[j4 + e], x[i]);
+      }
+    }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (quad < NT) s_a[(16 * r + i) * LD + 16 * r + col] = x[i];
+  }
+  wave_sync();
+  f32x4_t t[NT][NT];
+#pragma unroll
+  for (int c = 0; c < NT; ++c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[c][c][e] = s_a[(16 * c + 4 * quad + e) * LD + 16 * c + col];
+#pragma unroll
+    for (int r = c + 1; r < NT; ++r) {
+      f32x4_t z = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = c; j < r; ++j) {
+        const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * j + 4 * quad);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z = mfma32(w[e], t[j][c][e], z);
+      }
+      const f32x4_t d = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * r + 4 * quad);
+      t[r][c] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[r][c] = mfma32(-d[e], z[e], t[r][c]);
+    }
+  }
+  wave_sync();
+#pragma unroll
+  for (int c = 0; c < NT; ++c) {
+    const float beta = s_beta[16 * c + col];
+#pragma unroll
+    for (int r = c; r < NT; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s_a[(16 * r + 4 * quad + e) * LD + 16 * c + col] = t[r][c][e] * beta;
+  }
+  wave_sync();
+#pragma unroll
+  for (int r = 0; r < NT; ++r) {
+    const float* row = s_a + (16 * r + col) * LD + 4 * quad;
+    if constexpr (B16) {
+#pragma unroll
+      for (int h = 0; 2 * h <= r; ++h) {
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          f32x4_t w = {0, 0, 0, 0};
+          if (2 * h + x <= r) w = *reinterpret_cast<const f32x4_t*>(row + 32 * h + 16 * x);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t u, l;
+            split2(w[2 * e], w[2 * e + 1], u, l);
+            hi[2 * x + e] = u;
+            lo[2 * x + e] = l;
+          }
+        }
+        out[Out::kT + 128 * pair_of<B16>(r, h) + lane] = hi;
+        out[Out::kT + 128 * pair_of<B16>(r, h) + 64 + lane] = lo;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c <= r; ++c)
+        out[Out::kT + 64 * pair_of<B16>(r, c) + lane] = *reinterpret_cast<const u32x4_t*>(row + 16 * c);
+    }
+  }
+}
+
+// LDS units of a walk: two buffers of k | q | v | what was worked out ahead.
+template <bool B16, int DKP>
+struct WalkLds {
+  static constexpr int C = Ahead<B16>::C, N = B16 ? 8 : 4;  // elements of a unit
+  static constexpr int kK = C * DKP / N, kQ = kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
+  static constexpr size_t kBytes = 2 * 16 * (size_t)kBuffer;
+};
+
+// The walk of a sequence, a head and 64 value columns through its chunks, 16
+// columns a wave.
+template <bool B16, int DKP>
+__global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
+  using In = Ahead<B16>;
+  using Lds = WalkLds<B16, DKP>;
+  using T = std::conditional_t<B16, Bf16, float>;
+  constexpr int C = In::C, NT = In::kTiles, NB = DKP / 16, N = Lds::N;
+  constexpr int LOADS = Lds::kBuffer / 64, PER = (LOADS + 3) / 4;
+  extern __shared__ __attribute__((aligned(256))) u32x4_t s_walk[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int dv0 = blockIdx.x * 64, head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads), seq = blockIdx.z;
+  const Span sp = span_of(a, seq);
+  const int chunk0 = a.uniform_len >= 0 ? seq * ((a.uniform_len + C - 1) / C) : first_chunk(a, seq);
+  const size_t state0 = ((size_t)seq * a.heads + head) * a.dk * a.dv;
+  const int j = dv0 + 16 * wave + col;  // the lane's column
+
+  auto issue = [&](int pos, int n, u32x4_t* buffer) {
+    const size_t tok = sp.tok + pos;
+    const u32x4_t* ahead = reinterpret_cast<const u32x4_t*>(a.ahead) +
+                           ((size_t)(chunk0 + pos / C) * a.heads_here + blockIdx.y) * In::kUnits;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (LOADS % 4 != 0 && i * 4 + wave >= LOADS) continue;
+      const int at = (i * 4 + wave) * 64;  // first unit
+      const bool is_k = at < Lds::kK, is_q = !is_k && at < Lds::kK + Lds::kQ, is_v = !is_k && !is_q && at < Lds::kK + Lds::kQ + Lds::kV;
+      const void* src;
+      if (is_k || is_q || is_v) {
+        const int unit = at - (is_k ? 0 : is_q ? Lds::kK : Lds::kK + Lds::kQ) + lane;
+        const int units = is_v ? 64 / N : DKP / N, row = unit / units, u = unit % units;
+        int c;
+        if constexpr (B16)
+          c = N * (is_v ? row_unit<64>(row, u) : row_unit<DKP>(row, u));
+        else
+          c = N * row_unit32(row, u);
+        const size_t ld = is_k ? a.ld_k : is_q ? a.ld_q : a.ld_v;
+        const T* base = is_k   ? static_cast<const T*>(a.k) + (size_t)key_head * a.wide_k
+                        : is_q ? static_cast<const T*>(a.q) + (size_t)key_head * a.wide_q
+                               : static_cast<const T*>(a.v) + (size_t)head * a.wide_v + dv0;
+        const int width = is_v ? a.dv - dv0 : a.dk;
+        src = row < n && c < width ? static_cast<const void*>(base + (tok + row) * ld + c) : g_nothing;
+      } else {
+        src = ahead + (at - Lds::kK - Lds::kQ - Lds::kV) + lane;
+      }
+      auto* dst = (__attribute__((address_space(3))) void*)(buffer + at);
+      __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+    }
+  };
+  if (sp.len > 0) issue(0, min(C, sp.len), s_walk);
+  // S: rows 16 b + 4 quad + r of the lane's column.
+  f32x4_t S[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * quad + r;
+      S[b][r] = a.state_in && i < a.dk && j < a.dv ? a.state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
+    }
+  // These loads end here: in the loop they would be waited for with every next chunk's.
+#pragma unroll
+  for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(S[b]));
+
+  // A chunk's outputs, tokens 16 t + col by columns 16 wave + 4 quad .., are
+  // stored in the next one's course: every memory operation of a chunk has to
+  // end before the next begins.
+  u32x4_t held[NT];
+  int hold_n = 0;
+  auto put = [&](int pos) {
+    const int c = dv0 + 16 * wave + 4 * quad;
+    T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv + c;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int i = 16 * t + col;
+      if (i >= hold_n || c >= a.dv) continue;
+      T* dst = out + (size_t)i * a.ld_out;
+      if (c + 4 <= a.dv) {
+        if constexpr (B16)
+          *reinterpret_cast<u32x2_any_t*>(dst) = u32x2_t{held[t][0], held[t][1]};
+        else
+          *reinterpret_cast<f32x4_any_t*>(dst) = __builtin_bit_cast(f32x4_t, held[t]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+          if (c + e >= a.dv) continue;
+          if constexpr (B16)
+            dst[e].bits = (uint16_t)(held[t][e >> 1] >> (16 * (e & 1)));
+          else
+            dst[e] = __uint_as_float(held[t][e]);
+        }
+      }
+    }
+  };
+
+  u32x4_t* buffer = s_walk;
+  for (int pos = 0; pos < sp.len; pos += C) {
+    const int n = min(C, sp.len - pos);
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    __syncthreads();  // the chunk is there, and the one before is read
+    u32x4_t* other = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
+    if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), other);
+    if (hold_n) put(pos - hold_n);
+    hold_n = 0;
+    const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV, *sP = sT + In::kP;
+    const float *gamma = reinterpret_cast<const float*>(sT + In::kGamma), *rest = gamma + C;
+    const f32x4_t *K32 = reinterpret_cast<const f32x4_t*>(sK), *Q32 = reinterpret_cast<const f32x4_t*>(sQ),
+                  *V32 = reinterpret_cast<const f32x4_t*>(sV);
+    buffer = other;
+
+    // K S (rows: tokens) and (Q S)^T (columns: tokens).
+    f32x4_t x[NT], o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = o[t] = f32x4_t{0, 0, 0, 0};
+    if constexpr (B16) {
+#pragma unroll
+      for (int kp = 0; kp < DKP / 32; ++kp) {
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t u, l;
+          split2(S[2 * kp + (e >> 1)][2 * (e & 1)], S[2 * kp + (e >> 1)][2 * (e & 1) + 1], u, l);
+          hi[e] = u;
+          lo[e] = l;
+        }
+        u32x4_t kf[NT], qf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) kf[t] = order_frag<DKP>(sK, 16 * t + col, kp, quad);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) qf[t] = order_frag<DKP>(sQ, 16 * t + col, kp, quad);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], lo, x[t]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] = mfma(lo, qf[t], o[t]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], hi, x[t]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] = mfma(hi, qf[t], o[t]);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        f32x4_t kf[NT], qf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) kf[t] = row_frag32<DKP>(K32, 16 * t + col, 4 * b + quad);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) qf[t] = row_frag32<DKP>(Q32, 16 * t + col, 4 * b + quad);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[t] = mfma32(kf[t][r], S[b][r], x[t]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[t] = mfma32(S[b][r], qf[t][r], o[t]);
+        }
+      }
+    }
+    // X = V - e^G K S, U = T X.
+    f32x4_t u[NT];
+    if constexpr (B16) {
+      u32x4_t vf[2], hi[2], lo[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) turned_frag<64>(turned_at<64>(sV, 32 * h, 16 * wave, lane), vf[h]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4_t g = *reinterpret_cast<const f32x4_t*>(gamma + 16 * t + 4 * quad);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w = vf[t >> 1][2 * (t & 1) + e];
+          const float x0 = fmaf(-g[2 * e], x[t][2 * e], __uint_as_float(w << 16));
+          const float x1 = fmaf(-g[2 * e + 1], x[t][2 * e + 1], __uint_as_float(w & 0xFFFF0000u));
+          uint32_t p, l;
+          split2(x0, x1, p, l);
+          hi[t >> 1][2 * (t & 1) + e] = p;
+          lo[t >> 1][2 * (t & 1) + e] = l;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        u[t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; 2 * h <= t; ++h) {
+          const u32x4_t th = sT[128 * pair_of<B16>(t, h) + lane], tl = sT[128 * pair_of<B16>(t, h) + 64 + lane];
+          u[t] = mfma(tl, hi[h], u[t]);
+          u[t] = mfma(th, lo[h], u[t]);
+          u[t] = mfma(th, hi[h], u[t]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4_t g = *reinterpret_cast<const f32x4_t*>(gamma + 16 * t + 4 * quad);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t][r] = fmaf(-g[r], x[t][r], element32<64>(V32, 16 * t + 4 * quad + r, 16 * wave + col));
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        u[t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h <= t; ++h) {
+          const f32x4_t tf = __builtin_bit_cast(f32x4_t, sT[64 * pair_of<B16>(t, h) + lane]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) u[t] = mfma32(tf[r], x[h][r], u[t]);
+        }
+      }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[t][r]) < INFINITY);
+    T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv;
+    if (__any(odd)) {
+      // Something is not finite; in the products 0 times it would reach
+      // tokens before it.  The chunk's tokens run one by one.
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const size_t at = (sp.tok + pos + i) * a.ld_gates + head;
+        const float decay = expf(a.log_decay[at]), beta = a.beta[at];
+        f32x4_t kv[NB], qv[NB];
+        float v;
+        if constexpr (B16) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const u32x2_t w = four_of<DKP>(sK, i, 16 * b + 4 * quad), y = four_of<DKP>(sQ, i, 16 * b + 4 * quad);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              kv[b][r] = __uint_as_float(r & 1 ? w[r >> 1] & 0xFFFF0000u : w[r >> 1] << 16);
+              qv[b][r] = __uint_as_float(r & 1 ? y[r >> 1] & 0xFFFF0000u : y[r >> 1] << 16);
+            }
+          }
+          const u32x2_t w = four_of<64>(sV, i, 16 * wave + (col & ~3));
+          const uint32_t y = col & 2 ? w[1] : w[0];
+          v = __uint_as_float(col & 1 ? y & 0xFFFF0000u : y << 16);
+        } else {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            kv[b] = row_frag32<DKP>(K32, i, 4 * b + quad);
+            qv[b] = row_frag32<DKP>(Q32, i, 4 * b + quad);
+          }
+          v = element32<64>(V32, i, 16 * wave + col);
+        }
+        float ks = 0.0f, qs = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            S[b][r] = decay == 0.0f ? 0.0f : S[b][r] * decay;
+            ks = fmaf(kv[b][r], S[b][r], ks);
+          }
+        ks += __shfl_xor(ks, 16, 64);
+        ks += __shfl_xor(ks, 32, 64);
+        const float w = beta * (v - ks);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // Rows past d_key stay empty, whatever w is.
+            S[b][r] = 16 * b + 4 * quad + r < a.dk ? fmaf(kv[b][r], w, S[b][r]) : 0.0f;
+            qs = fmaf(qv[b][r], S[b][r], qs);
+          }
+        qs += __shfl_xor(qs, 16, 64);
+        qs += __shfl_xor(qs, 32, 64);
+        if (quad == 0 && j < a.dv) store1(out + (size_t)i * a.ld_out + j, qs * a.scale);
+      }
+      continue;
+    }
+    // O^T = scale e^G (Q S)^T + (P U)^T.
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
+    if constexpr (B16) {
+      u32x4_t hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t p, l;
+        split2(u[e >> 1][2 * (e & 1)], u[e >> 1][2 * (e & 1) + 1], p, l);
+        hi[e >> 2][e & 3] = p;
+        lo[e >> 2][e & 3] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; 2 * h <= t; ++h) {
+          const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
+          o[t] = mfma(lo[h], ph, o[t]);
+          o[t] = mfma(hi[h], pl, o[t]);
+          o[t] = mfma(hi[h], ph, o[t]);
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h <= t; ++h) {
+          const f32x4_t pf = __builtin_bit_cast(f32x4_t, sP[64 * pair_of<B16>(t, h) + lane]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t] = mfma32(u[h][r], pf[r], o[t]);
+        }
+    }
+    // S = e^(G_n) S + K^T (e^(G_n - G) U).
+    const float last = gamma[C - 1];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) S[b] *= last;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) u[t] *= *reinterpret_cast<const f32x4_t*>(rest + 16 * t + 4 * quad);
+    if constexpr (B16) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4_t w[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t p0, p1, p2;
+          split3(u[2 * h + (e >> 1)][2 * (e & 1)], u[2 * h + (e >> 1)][2 * (e & 1) + 1], p0, p1, p2);
+          w[0][e] = p0;
+          w[1][e] = p1;
+          w[2][e] = p2;
+        }
+        constexpr int BG = NB < 4 ? NB : 4;
+#pragma unroll
+        for (int b0 = 0; b0 < NB; b0 += BG) {
+          u32x4_t kf[BG];
+          if constexpr (BG == 4) {
+            turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, lane), kf);
+          } else {
+#pragma unroll
+            for (int b = 0; b < BG; ++b) turned_frag<DKP>(turned_at<DKP>(sK, 32 * h, 16 * (b0 + b), lane), kf[b]);
+          }
+#pragma unroll
+          for (int p = 2; p >= 0; --p)
+#pragma unroll
+            for (int b = 0; b < BG; ++b) S[b0 + b] = mfma(kf[b], w[p], S[b0 + b]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
+    }
+    if constexpr (B16) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        held[t][0] = bf16x2_bits(o[t][0], o[t][1]);
+        held[t][1] = bf16x2_bits(o[t][2], o[t][3]);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) held[t] = __builtin_bit_cast(u32x4_t, o[t]);
+    }
+    hold_n = n;
+  }
+  put(sp.len - hold_n);
+  if (!a.state_out) return;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * quad + r;
+      if (i < a.dk && j < a.dv) a.state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
+    }
+}
+
+// Rows at any element copied to rows of whole 16-byte units: heads of `width`
+// columns to heads of `to`, zeros behind.
+template <class T>
+__global__ __launch_bounds__(256) void delta_rows_kernel(const T* src, size_t ld, int heads, int width, T* dst, int to, size_t tokens) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int units = to / N;
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, row = (size_t)heads * units;
+  if (at >= tokens * row) return;
+  const size_t tok = at / row;
+  const int in = (int)(at - tok * row), head = in / units, c = in % units * N;
+  T v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = c + e < width ? src[tok * ld + (size_t)head * width + c + e] : T{};
+  u32x4_t w;
+  __builtin_memcpy(&w, v, 16);
+  *reinterpret_cast<u32x4_t*>(dst + at * N) = w;
+}
+
 template <class T>
 Status launch_steps(hipStream_t stream, const DeltaArgs& a) {
   const dim3 grid((a.dv + 63) / 64, a.heads, a.n_seqs);
@@ -196,10 +808,100 @@ Status launch_steps(hipStream_t stream, const DeltaArgs& a) {
   return Status::Ok();
 }
 
+// Calls f with the kernels for a call's type and key width.
+template <bool B16, int DKP>
+struct Chunked {
+  static constexpr bool kBf16 = B16;
+  static constexpr size_t kLds = WalkLds<B16, DKP>::kBytes;
+  static constexpr auto kAhead = &delta_ahead_kernel<B16, DKP>;
+  static constexpr auto kWalk = &delta_walk_kernel<B16, DKP>;
+};
+template <class F>
+Status with_chunks(int dtype, int dk, F f) {
+  auto wide = [&](auto b16) {
+    constexpr bool B = decltype(b16)::value;
+    if (dk <= 32) return f(Chunked<B, 32>{});
+    if (dk <= 64) return f(Chunked<B, 64>{});
+    return f(Chunked<B, 128>{});
+  };
+  return dtype == PSSA_HIP_BF16 ? wide(std::true_type{}) : wide(std::false_type{});
+}
+
+size_t unit_of(int dtype) { return dtype == PSSA_HIP_BF16 ? 8 : 4; }  // elements of 16 bytes
+size_t whole(size_t width, size_t unit) { return (width + unit - 1) / unit * unit; }
+// Rows and heads in whole 16-byte units.
+bool in_units(const void* p, size_t ld, size_t width, size_t unit) {
+  return (uintptr_t)p % 16 == 0 && ld % unit == 0 && width % unit == 0;
+}
+
+template <class T>
+Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, int width, int& to, size_t tokens, char*& scratch) {
+  to = (int)whole(width, 16 / sizeof(T));
+  const size_t units = tokens * heads * (to * sizeof(T) / 16);
+  delta_rows_kernel<T><<<(uint32_t)((units + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(p), ld, heads, width,
+                                                                          reinterpret_cast<T*>(scratch), to, tokens);
+  PSSA_LAUNCH_CHECK("delta_rows_kernel");
+  p = scratch;
+  ld = (size_t)heads * to;
+  scratch += (units * 16 + 255) & ~(size_t)255;
+  return Status::Ok();
+}
+
 }  // namespace
 
-Status launch_delta_rule(hipStream_t stream, int dtype, const DeltaArgs& a, int longest) {
-  return dtype == PSSA_HIP_F32 ? launch_steps<float>(stream, a) : launch_steps<Bf16>(stream, a);
+int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ahead<false>::C; }
+
+// What is worked out ahead takes 25 KiB a chunk and head (bf16; 7 KiB fp32):
+// past 1 GiB of it the heads run in several launches.
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t heads, size_t d_key, size_t d_val) {
+  DeltaScratch s;
+  const size_t size = dtype == PSSA_HIP_BF16 ? 2 : 4, unit = unit_of(dtype);
+  const size_t one = chunks * 16 * (dtype == PSSA_HIP_BF16 ? Ahead<true>::kUnits : Ahead<false>::kUnits);
+  s.heads_here = (int)std::max<size_t>(1, std::min(heads, ((size_t)1 << 30) / std::max<size_t>(one, 1)));
+  s.ahead = (one * s.heads_here + 255) & ~(size_t)255;
+  s.rows = 2 * ((tokens * heads * whole(d_key, unit) * size + 255) & ~(size_t)255) +
+           ((tokens * heads * whole(d_val, unit) * size + 255) & ~(size_t)255);
+  return s;
+}
+
+Status init_delta_attributes() {
+  for (int dtype : {PSSA_HIP_F32, PSSA_HIP_BF16})
+    for (int dk : {32, 64, 128})
+      PSSA_RETURN_IF(with_chunks(dtype, dk, [&](auto c) -> Status {
+        PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(c.kWalk), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)c.kLds));
+        return Status::Ok();
+      }));
+  return Status::Ok();
+}
+
+Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t tokens, int longest, const DeltaScratch& s,
+                         char* scratch) {
+  if (longest <= kDeltaSteps)
+    return dtype == PSSA_HIP_F32 ? launch_steps<float>(stream, a) : launch_steps<Bf16>(stream, a);
+  a.ahead = scratch;
+  char* rows = scratch + s.ahead;
+  const size_t unit = unit_of(dtype);
+  const bool b16 = dtype == PSSA_HIP_BF16;
+  auto in_place = [&](const void*& p, size_t& ld, int heads, int width, int& to) -> Status {
+    to = width;
+    if (in_units(p, ld, width, unit)) return Status::Ok();
+    return b16 ? launch_rows<Bf16>(stream, p, ld, heads, width, to, tokens, rows)
+               : launch_rows<float>(stream, p, ld, heads, width, to, tokens, rows);
+  };
+  PSSA_RETURN_IF(in_place(a.q, a.ld_q, a.key_heads, a.dk, a.wide_q));
+  PSSA_RETURN_IF(in_place(a.k, a.ld_k, a.key_heads, a.dk, a.wide_k));
+  PSSA_RETURN_IF(in_place(a.v, a.ld_v, a.heads, a.dv, a.wide_v));
+  return with_chunks(dtype, a.dk, [&](auto c) -> Status {
+    for (a.head0 = 0; a.head0 < a.heads; a.head0 += s.heads_here) {
+      a.heads_here = std::min(s.heads_here, a.heads - a.head0);
+      c.kAhead<<<dim3(a.chunks, a.heads_here), 64, 0, stream>>>(a);
+      PSSA_LAUNCH_CHECK("delta_ahead_kernel");
+      c.kWalk<<<dim3((a.dv + 63) / 64, a.heads_here, a.n_seqs), 256, c.kLds, stream>>>(a);
+      PSSA_LAUNCH_CHECK("delta_walk_kernel");
+    }
+    return Status::Ok();
+  });
 }
 
 }  // namespace pssa

@@ -129,6 +129,7 @@ Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan&
 
 // -------------------------------------------------------- gated delta rule
 constexpr int kDeltaMaxKey = 128;   // d_key held in a workgroup's tiles
+constexpr int kDeltaSteps = 4;      // up to this length a sequence runs token by token
 constexpr int kDeltaInline = 256;   // sequences whose offsets travel with the kernel's arguments
 
 struct DeltaArgs {
@@ -141,11 +142,28 @@ struct DeltaArgs {
   float scale = 1.0f;
   int n_seqs = 0, heads = 0, key_heads = 0, dk = 0, dv = 0;
   int uniform_len = -1;  // every sequence's length, or -1: the tables
-  // [n_seqs + 1] first tokens: on the device, or null and here.
+  // Where the call runs in chunks: what is worked out for each of them ahead,
+  // [chunks, heads of one launch], and the launch's first head.
+  char* ahead = nullptr;
+  int head0 = 0, heads_here = 0, chunks = 0;
+  int wide_q = 0, wide_k = 0, wide_v = 0;  // elements from a head to the next in rows that may be copies
+  // [n_seqs + 1] first tokens and, behind them, first chunks: on the device, or null and here.
   const uint32_t* table = nullptr;
   uint32_t inline_tokens[kDeltaInline + 1] = {};
+  uint32_t inline_chunks[kDeltaInline + 1] = {};
 };
-Status launch_delta_rule(hipStream_t stream, int dtype, const DeltaArgs& a, int longest);
+// Tokens of a chunk of a type, and the scratch of a call: what is worked out
+// ahead for the heads of one launch, and copies of rows that do not lie in
+// units of 16 bytes.
+int delta_chunk(int dtype);
+struct DeltaScratch {
+  size_t ahead = 0, rows = 0;  // bytes
+  int heads_here = 0;          // heads of a launch
+};
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t heads, size_t d_key, size_t d_val);
+Status init_delta_attributes();
+Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t tokens, int longest, const DeltaScratch& s,
+                         char* scratch);
 
 // ------------------------------------------------------------- beam search
 constexpr int kMaxBeams = 64;  // of a group, before and after a step
