@@ -162,6 +162,8 @@ __device__ __forceinline__ void turned_frags(uint32_t ak, u32x4_t (&k)[4]) {
   for (int i = 0; i < 4; ++i) k[i] = u32x4_t{k0[i][0], k0[i][1], k1[i][0], k1[i][1]};
 }
 
+constexpr int kLdsOnly = 0xF | (0x3 << 14) | (0x7 << 4);  // s_waitcnt lgkmcnt(0)
+
 // Element i of bf16 values in a register or LDS.
 template <class V>
 __device__ __forceinline__ float bf16_at(const V* p, int i) {

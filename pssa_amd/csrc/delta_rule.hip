@@ -415,17 +415,56 @@ struct WalkLds {
   static constexpr size_t kBytes = 2 * 16 * (size_t)kBuffer;
 };
 
-// The walk of a sequence, a head and 64 value columns through its chunks, 16
-// columns a wave.
+// The state's row of register r of tile b: as rows of k are read, 16 bytes a
+// lane, so that the state's tiles are operands without a move.
+template <bool B16>
+__device__ __forceinline__ int state_row(int b, int quad, int r) {
+  return B16 ? 32 * (b >> 1) + 8 * quad + 4 * (b & 1) + r : 16 * b + 4 * quad + r;
+}
+// Tokens row0 + 4 quad .. + 3 and 16 more of the state's rows of N tiles (4 or
+// 2): transposed LDS reads, with their wait (the builtin would wait for the
+// loads into the other buffer).
+template <int W>
+__device__ __forceinline__ uint32_t state_turned_at(const u32x4_t* s, int row0, int lane) {
+  const int row = row0 + 4 * (lane >> 4) + ((lane >> 2) & 3);
+  const u32x4_t* unit = s + row * (W / 8) + row_unit<W>(row, lane & 3);
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)unit;
+}
+template <int W>
+__device__ __forceinline__ void state_turned(uint32_t at, u32x4_t (&k)[4]) {
+  u32x2_t k0[4], k1[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%c12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%c12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(k0[0]), "=&v"(k1[0]), "=&v"(k0[1]), "=&v"(k1[1]), "=&v"(k0[2]), "=&v"(k1[2]), "=&v"(k0[3]), "=&v"(k1[3])
+      : "v"(at), "v"(at ^ 8), "v"(at ^ 64), "v"(at ^ 72), "i"(32 * W)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = u32x4_t{k0[i][0], k0[i][1], k1[i][0], k1[i][1]};
+}
+template <int W>
+__device__ __forceinline__ void state_turned(uint32_t at, u32x4_t (&k)[2]) {
+  turned_frag<W>(at, k[0]);
+  turned_frag<W>(at ^ 8, k[1]);
+}
+
+// The walk of a sequence, a head and 64 value columns through its chunks: four
+// waves compute, 16 columns each, and four bring the next chunk (where the
+// same waves did both, issuing the loads took 2.3 of a chunk's 5.7 us, heads
+// of 128).
+constexpr int kWalkers = 4;
 template <bool B16, int DKP>
-__global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a) {
   using In = Ahead<B16>;
   using Lds = WalkLds<B16, DKP>;
   using T = std::conditional_t<B16, Bf16, float>;
   constexpr int C = In::C, NT = In::kTiles, NB = DKP / 16, N = Lds::N;
   constexpr int LOADS = Lds::kBuffer / 64, PER = (LOADS + 3) / 4;
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_walk[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = in_all % kWalkers;
   const int col = lane & 15, quad = lane >> 4;
   const int dv0 = blockIdx.x * 64, head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads), seq = blockIdx.z;
   const Span sp = span_of(a, seq);
@@ -464,65 +503,41 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
       __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
     }
   };
-  if (sp.len > 0) issue(0, min(C, sp.len), s_walk);
-  // S: rows 16 b + 4 quad + r of the lane's column.
+  auto meet = [&]() {  // without __syncthreads' wait for outputs on their way
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kLdsOnly);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (in_all >= kWalkers) {
+    u32x4_t* to = s_walk;
+    if (sp.len > 0) issue(0, min(C, sp.len), to);
+    for (int pos = 0; pos < sp.len; pos += C) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      meet();  // the chunk is there, and the one before is read
+      to = to == s_walk ? s_walk + Lds::kBuffer : s_walk;
+      if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), to);
+    }
+    return;
+  }
+  // S: the rows of the lane's column.
   f32x4_t S[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * quad + r;
+      const int i = state_row<B16>(b, quad, r);
       S[b][r] = a.state_in && i < a.dk && j < a.dv ? a.state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
     }
-  // These loads end here: in the loop they would be waited for with every next chunk's.
-#pragma unroll
-  for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(S[b]));
-
-  // A chunk's outputs, tokens 16 t + col by columns 16 wave + 4 quad .., are
-  // stored in the next one's course: every memory operation of a chunk has to
-  // end before the next begins.
-  u32x4_t held[NT];
-  int hold_n = 0;
-  auto put = [&](int pos) {
-    const int c = dv0 + 16 * wave + 4 * quad;
-    T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv + c;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int i = 16 * t + col;
-      if (i >= hold_n || c >= a.dv) continue;
-      T* dst = out + (size_t)i * a.ld_out;
-      if (c + 4 <= a.dv) {
-        if constexpr (B16)
-          *reinterpret_cast<u32x2_any_t*>(dst) = u32x2_t{held[t][0], held[t][1]};
-        else
-          *reinterpret_cast<f32x4_any_t*>(dst) = __builtin_bit_cast(f32x4_t, held[t]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e) {
-          if (c + e >= a.dv) continue;
-          if constexpr (B16)
-            dst[e].bits = (uint16_t)(held[t][e >> 1] >> (16 * (e & 1)));
-          else
-            dst[e] = __uint_as_float(held[t][e]);
-        }
-      }
-    }
-  };
-
-  u32x4_t* buffer = s_walk;
+  const u32x4_t* buffer = s_walk;
   for (int pos = 0; pos < sp.len; pos += C) {
     const int n = min(C, sp.len - pos);
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-    __syncthreads();  // the chunk is there, and the one before is read
-    u32x4_t* other = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
-    if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), other);
-    if (hold_n) put(pos - hold_n);
-    hold_n = 0;
+    meet();
     const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV, *sP = sT + In::kP;
     const float *gamma = reinterpret_cast<const float*>(sT + In::kGamma), *rest = gamma + C;
     const f32x4_t *K32 = reinterpret_cast<const f32x4_t*>(sK), *Q32 = reinterpret_cast<const f32x4_t*>(sQ),
                   *V32 = reinterpret_cast<const f32x4_t*>(sV);
-    buffer = other;
+    buffer = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
 
     // K S (rows: tokens) and (Q S)^T (columns: tokens).
     f32x4_t x[NT], o[NT];
@@ -541,9 +556,9 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
         }
         u32x4_t kf[NT], qf[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) kf[t] = order_frag<DKP>(sK, 16 * t + col, kp, quad);
+        for (int t = 0; t < NT; ++t) kf[t] = row_frag<DKP>(sK, 16 * t + col, 4 * kp + quad);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) qf[t] = order_frag<DKP>(sQ, 16 * t + col, kp, quad);
+        for (int t = 0; t < NT; ++t) qf[t] = row_frag<DKP>(sQ, 16 * t + col, 4 * kp + quad);
 #pragma unroll
         for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], lo, x[t]);
 #pragma unroll
@@ -637,7 +652,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
         if constexpr (B16) {
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            const u32x2_t w = four_of<DKP>(sK, i, 16 * b + 4 * quad), y = four_of<DKP>(sQ, i, 16 * b + 4 * quad);
+            const u32x2_t w = four_of<DKP>(sK, i, state_row<B16>(b, quad, 0)), y = four_of<DKP>(sQ, i, state_row<B16>(b, quad, 0));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               kv[b][r] = __uint_as_float(r & 1 ? w[r >> 1] & 0xFFFF0000u : w[r >> 1] << 16);
@@ -671,7 +686,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             // Rows past d_key stay empty, whatever w is.
-            S[b][r] = 16 * b + 4 * quad + r < a.dk ? fmaf(kv[b][r], w, S[b][r]) : 0.0f;
+            S[b][r] = state_row<B16>(b, quad, r) < a.dk ? fmaf(kv[b][r], w, S[b][r]) : 0.0f;
             qs = fmaf(qv[b][r], S[b][r], qs);
           }
         qs += __shfl_xor(qs, 16, 64);
@@ -733,12 +748,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
 #pragma unroll
         for (int b0 = 0; b0 < NB; b0 += BG) {
           u32x4_t kf[BG];
-          if constexpr (BG == 4) {
-            turned_frags<DKP>(turned_at<DKP>(sK, 32 * h, 16 * b0, lane), kf);
-          } else {
-#pragma unroll
-            for (int b = 0; b < BG; ++b) turned_frag<DKP>(turned_at<DKP>(sK, 32 * h, 16 * (b0 + b), lane), kf[b]);
-          }
+          state_turned<DKP>(state_turned_at<DKP>(sK, 32 * h, lane) ^ (32 * b0), kf);
 #pragma unroll
           for (int p = 2; p >= 0; --p)
 #pragma unroll
@@ -754,25 +764,31 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs a) {
           for (int b = 0; b < NB; ++b)
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
     }
-    if constexpr (B16) {
+    // Tokens 16 t + col, columns 16 wave + 4 quad ..
+    const int c = dv0 + 16 * wave + 4 * quad;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        held[t][0] = bf16x2_bits(o[t][0], o[t][1]);
-        held[t][1] = bf16x2_bits(o[t][2], o[t][3]);
+    for (int t = 0; t < NT; ++t) {
+      const int i = 16 * t + col;
+      if (i >= n || c >= a.dv) continue;
+      T* dst = out + (size_t)i * a.ld_out + c;
+      if (c + 4 <= a.dv) {
+        if constexpr (B16)
+          *reinterpret_cast<u32x2_any_t*>(dst) = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
+        else
+          *reinterpret_cast<f32x4_any_t*>(dst) = o[t];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (c + e < a.dv) store1(dst + e, o[t][e]);
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) held[t] = __builtin_bit_cast(u32x4_t, o[t]);
     }
-    hold_n = n;
   }
-  put(sp.len - hold_n);
   if (!a.state_out) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * b + 4 * quad + r;
+      const int i = state_row<B16>(b, quad, r);
       if (i < a.dk && j < a.dv) a.state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
     }
 }
@@ -897,7 +913,7 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
       a.heads_here = std::min(s.heads_here, a.heads - a.head0);
       c.kAhead<<<dim3(a.chunks, a.heads_here), 64, 0, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_ahead_kernel");
-      c.kWalk<<<dim3((a.dv + 63) / 64, a.heads_here, a.n_seqs), 256, c.kLds, stream>>>(a);
+      c.kWalk<<<dim3((a.dv + 63) / 64, a.heads_here, a.n_seqs), 128 * kWalkers, c.kLds, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_walk_kernel");
     }
     return Status::Ok();

@@ -277,7 +277,6 @@ __global__ __launch_bounds__(256) void linear_chunks_any_kernel(LinearArgs a) {
 // two LDS buffers while the other one's chunk is worked on.
 // Of a chunk's P the pairs of a query tile and a key half that hold anything,
 // the largest first: a wave computes one or two.
-constexpr int kLdsOnly = 0xF | (0x3 << 14) | (0x7 << 4);  // s_waitcnt lgkmcnt(0)
 constexpr int kPairs = 6;
 __device__ __forceinline__ int pair_query(int p) { return (0x201233 >> (4 * p)) & 3; }
 __device__ __forceinline__ int pair_half(int p) { return (0x100010 >> (4 * p)) & 1; }
