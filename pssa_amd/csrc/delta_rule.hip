@@ -9,9 +9,9 @@
 //   (1 + A) U = beta (V - e^G K S),   A_ij = beta_i e^(G_i - G_j) k_i k_j for j < i,
 //   O = scale e^G Q S + P U,          P_ij = scale e^(G_i - G_j) q_i k_j for j <= i,
 //   S' = e^(G_n) S + K^T (e^(G_n - G) U).
-// T = (1 + A)^-1 beta and P need no state: a first kernel works them out for
-// all chunks at once (delta_ahead), a second one walks the chunks of a
-// sequence, a head and 64 value columns with S in its registers (delta_walk).
+// T = (1 + A)^-1 beta needs no state: a first kernel works it out for all
+// chunks at once (delta_ahead), a second one walks the chunks of a sequence, a
+// head and 64 value columns with S in its registers (delta_walk).
 // There everything follows in registers: the accumulators' layout (lane l
 // holds column l % 16, rows 4 (l / 16) + r) is the next product's operand
 // layout once what meets it is read in the same order.
@@ -191,39 +191,76 @@ __device__ __forceinline__ Place place_of(const DeltaArgs& a, int chunk) {
 }
 
 // What is worked out ahead for a chunk and head, in units of 16 bytes: the
-// fragments of T and P where a triangle holds anything, then e^G and
-// e^(G_n - G) of the tokens.  bf16: a fragment is 16 tokens by 32, in two
-// parts; fp32: 16 by 16.
+// fragments of T where its triangle holds anything, then of the tokens e^G,
+// e^(G_n - G) and G itself, in 64 bits since differences of it count.  bf16:
+// a fragment is 16 tokens by 32, in two parts; fp32: 16 by 16.
 template <bool B16>
 struct Ahead {
-  static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3;
-  static constexpr int kT = 0, kP = kPairs * (B16 ? 128 : 64), kGamma = 2 * kP, kRest = kGamma + C / 4, kUnits = kGamma + 64;
+  static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3, kFrag = B16 ? 128 : 64;
+  static constexpr int kGamma = kPairs * kFrag, kRest = kGamma + C / 4, kSum = kRest + C / 4, kUnits = kGamma + 64;
 };
 // The fragment of token tile t over keys 32 h .. (bf16), 16 h .. (fp32).
 template <bool B16>
 __device__ __forceinline__ constexpr int pair_of(int t, int h) {
   return B16 ? (t < 2 ? t : 2 * t - 2 + h) : t + h;
 }
+// The tiles of a lower triangle in a row: the row of the i-th, and its column.
+__device__ __forceinline__ int triangle_row(int i) { return i >= 6 ? 3 : i >= 3 ? 2 : i >= 1 ? 1 : 0; }
+__device__ __forceinline__ int triangle_col(int i) { return i - triangle_row(i) * (triangle_row(i) + 1) / 2; }
 
-// One wave works out a chunk of one head.  A's triangle lies in LDS; its
-// diagonal blocks of 16 x 16 are inverted by forward substitution, a column a
-// lane and the four blocks side by side, the others follow as products:
+// Units of a row of W elements of a type lie exchanged in LDS, so that rows
+// read at one unit hit different banks.
+template <bool B16, int W>
+__device__ __forceinline__ int unit_in_row(int row, int u) {
+  if constexpr (B16) return row_unit<W>(row, u);
+  return row_unit32(row, u);
+}
+// Rows x .. + 15 times rows y .. + 15 of two tiles in LDS: lane l holds row
+// y + l % 16 and rows x + 4 (l / 16) + e.
+template <bool B16, int DKP>
+__device__ __forceinline__ f32x4_t tile_product(const u32x4_t* sx, int x, const u32x4_t* sy, int y, int lane) {
+  const int col = lane & 15, quad = lane >> 4;
+  f32x4_t s = {0, 0, 0, 0};
+#pragma unroll
+  for (int b = 0; b < DKP / (B16 ? 32 : 16); ++b) {
+    constexpr int ROW = DKP / (B16 ? 8 : 4);
+    const u32x4_t xf = sx[(x + col) * ROW + unit_in_row<B16, DKP>(x + col, 4 * b + quad)];
+    const u32x4_t yf = sy[(y + col) * ROW + unit_in_row<B16, DKP>(y + col, 4 * b + quad)];
+    if constexpr (B16) {
+      s = mfma(xf, yf, s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = mfma32(__uint_as_float(xf[e]), __uint_as_float(yf[e]), s);
+    }
+  }
+  return s;
+}
+
+// A chunk of one head, a wave for each 16 tokens.  A's triangle lies in LDS;
+// each wave inverts one of its diagonal blocks by substitution, a column a
+// lane, and follows one column of blocks down:
 //   T_rc = -D_r sum_j A_rj T_jc, c <= j < r.
 template <bool B16, int DKP>
-__global__ __launch_bounds__(64) void delta_ahead_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs a) {
   using Out = Ahead<B16>;
   using T = std::conditional_t<B16, Bf16, float>;
-  constexpr int C = Out::C, NT = Out::kTiles, LD = C + 4, KF = B16 ? DKP / 32 : DKP / 16;
+  constexpr int C = Out::C, NT = Out::kTiles, LD = C + 4, N = 16 / (int)sizeof(T), ROW = DKP / N;
+  __shared__ __attribute__((aligned(256))) u32x4_t s_k[C * ROW];
   __shared__ __attribute__((aligned(16))) float s_a[C * LD];
   __shared__ double s_g[C];
   __shared__ float s_beta[C];
-  const int lane = threadIdx.x, col = lane & 15, quad = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   const int head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads);
   const Place pl = place_of<C>(a, blockIdx.x);
   u32x4_t* out = reinterpret_cast<u32x4_t*>(a.ahead) + ((size_t)blockIdx.x * a.heads_here + blockIdx.y) * Out::kUnits;
-
-  // The gates: sums of the log decays in 64 bits, since their differences count.
-  {
+  const T* k0 = static_cast<const T*>(a.k) + pl.tok * a.ld_k + (size_t)key_head * a.wide_k;
+#pragma unroll
+  for (int i = 0; i < C * ROW / (64 * NT); ++i) {
+    const int at = (i * NT + wave) * 64, unit = at + lane, row = unit / ROW, c = N * unit_in_row<B16, DKP>(row, unit % ROW);
+    const void* src = row < pl.n && c < a.dk ? static_cast<const void*>(k0 + row * a.ld_k + c) : g_nothing;
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)(s_k + at), 16, 0, 0);
+  }
+  if (wave == 0) {
     const bool on = lane < pl.n;
     float g = on ? a.log_decay[(pl.tok + lane) * a.ld_gates + head] : 0.0f;
     g = g < kForget ? kForget : g;
@@ -240,179 +277,118 @@ __global__ __launch_bounds__(64) void delta_ahead_kernel(DeltaArgs a) {
       float* f = reinterpret_cast<float*>(out + Out::kGamma);
       f[lane] = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
       f[C + lane] = __builtin_amdgcn_exp2f((float)((all - sum) * kLog2e));
+      reinterpret_cast<double*>(out + Out::kSum)[lane] = sum;
     }
   }
-  const T* k0 = static_cast<const T*>(a.k) + (size_t)key_head * a.wide_k;
-  const T* q0 = static_cast<const T*>(a.q) + (size_t)key_head * a.wide_q;
-  // Rows in their own order: 16 bytes a lane.
-  auto rows = [&](const T* base, size_t ld, int t, u32x4_t (&f)[KF]) {
-    constexpr int N = 16 / (int)sizeof(T);
-    const int i = 16 * t + col;
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  __syncthreads();
+  // A: rows 16 r + 4 quad + e, columns 16 c + col.
 #pragma unroll
-    for (int b = 0; b < KF; ++b) {
-      const int c = 4 * N * b + N * quad;
-      f[b] = u32x4_t{0, 0, 0, 0};
-      if (i < pl.n && c < a.dk) f[b] = *reinterpret_cast<const u32x4_t*>(base + (pl.tok + i) * ld + c);
-    }
-  };
-  auto dot = [&](const u32x4_t (&x)[KF], const u32x4_t (&y)[KF]) {
-    f32x4_t s = {0, 0, 0, 0};
+  for (int i = 0; i < (NT * (NT + 1) / 2 + NT - 1) / NT; ++i) {
+    const int at = min(i * NT + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
+    const f32x4_t s = tile_product<B16, DKP>(s_k, 16 * r, s_k, 16 * c, lane);
+    const double gk = s_g[16 * c + col];
 #pragma unroll
-    for (int b = 0; b < KF; ++b) {
-      if constexpr (B16) {
-        s = mfma(x[b], y[b], s);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s = mfma32(__uint_as_float(x[b][e]), __uint_as_float(y[b][e]), s);
-      }
-    }
-    return s;
-  };
-  u32x4_t kf[NT][KF];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) rows(k0, a.ld_k, t, kf[t]);
-  wave_sync();
-  double gi[4];
-#pragma unroll
-  for (int r = 0; r < NT; ++r) {
-    // P^T: queries 16 r + col, keys 16 c + 4 quad + e.
-    u32x4_t qf[KF];
-    rows(q0, a.ld_q, r, qf);
-    const double gq = s_g[16 * r + col];
-    f32x4_t p[NT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) p[c] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c <= r; ++c) {
-      const f32x4_t s = dot(kf[c], qf);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = 16 * c + 4 * quad + e;
-        const float w = a.scale * __builtin_amdgcn_exp2f((float)((gq - s_g[key]) * kLog2e));
-        p[c][e] = 16 * r + col >= key ? s[e] * w : 0.0f;
-      }
-    }
-    if constexpr (B16) {
-#pragma unroll
-      for (int h = 0; 2 * h <= r; ++h) {
-        u32x4_t hi, lo;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t u, l;
-          split2(p[2 * h + (x >> 1)][2 * (x & 1)], p[2 * h + (x >> 1)][2 * (x & 1) + 1], u, l);
-          hi[x] = u;
-          lo[x] = l;
-        }
-        out[Out::kP + 128 * pair_of<B16>(r, h) + lane] = hi;
-        out[Out::kP + 128 * pair_of<B16>(r, h) + 64 + lane] = lo;
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c <= r; ++c) out[Out::kP + 64 * pair_of<B16>(r, c) + lane] = __builtin_bit_cast(u32x4_t, p[c]);
-    }
-    // A: rows 16 r + 4 quad + e, columns 16 c + col.
-#pragma unroll
-    for (int e = 0; e < 4; ++e) gi[e] = s_g[16 * r + 4 * quad + e];
-#pragma unroll
-    for (int c = 0; c <= r; ++c) {
-      const f32x4_t s = dot(kf[r], kf[c]);
-      const double gk = s_g[16 * c + col];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 16 * r + 4 * quad + e;
-        const float w = s_beta[i] * __builtin_amdgcn_exp2f((float)((gi[e] - gk) * kLog2e));
-        s_a[i * LD + 16 * c + col] = i > 16 * c + col ? s[e] * w : 0.0f;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * r + 4 * quad + e;
+      const float w = s_beta[row] * __builtin_amdgcn_exp2f((float)((s_g[row] - gk) * kLog2e));
+      s_a[row * LD + 16 * c + col] = row > 16 * c + col ? s[e] * w : 0.0f;
     }
   }
-  wave_sync();
-  // The diagonal blocks' inverses, each over its block.
+  __syncthreads();
+  // The inverse of the wave's diagonal block, over its block: each row as soon
+  // as it is known leaves the rows below.
   {
-    const int r = NT == 4 ? quad : quad & 1;
+    float* block = s_a + 16 * wave * LD + 16 * wave;
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] = i == col ? 1.0f : 0.0f;
+    for (int i = 0; i < 16; ++i) x[i] = i == col ? 1.0f : 0.0f;
+    auto leave = [&](auto first) {
+      constexpr int J = decltype(first)::value;
+      f32x4_t w[16 - J];
 #pragma unroll
-      for (int j4 = 0; j4 < i; j4 += 4) {
-        const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + i) * LD + 16 * r + j4);
+      for (int i = 1; i < 16 - J; ++i) w[i] = *reinterpret_cast<const f32x4_t*>(block + (J + i) * LD + J);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j4 + e < i) x[i] = fmaf(-w[e], x[j4 + e], x[i]);
-      }
-    }
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 1; i < 16 - J; ++i)
+          if (i > e) x[J + i] = fmaf(-w[i][e], x[J + e], x[J + i]);
+    };
+    leave(std::integral_constant<int, 0>{});
+    leave(std::integral_constant<int, 4>{});
+    leave(std::integral_constant<int, 8>{});
+    leave(std::integral_constant<int, 12>{});
     wave_sync();
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (quad < NT) s_a[(16 * r + i) * LD + 16 * r + col] = x[i];
+      if (quad == (i & 3)) block[i * LD + col] = x[i];
   }
-  wave_sync();
-  f32x4_t t[NT][NT];
+  __syncthreads();
+  // The wave's column of blocks.
+  f32x4_t t[NT];
 #pragma unroll
-  for (int c = 0; c < NT; ++c) {
+  for (int e = 0; e < 4; ++e) t[0][e] = s_a[(16 * wave + 4 * quad + e) * LD + 16 * wave + col];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[c][c][e] = s_a[(16 * c + 4 * quad + e) * LD + 16 * c + col];
+  for (int d = 1; d < NT; ++d) {  // the block d rows below the diagonal
+    const int r = wave + d;
+    t[d] = f32x4_t{0, 0, 0, 0};
+    if (r >= NT) continue;  // uniform
+    f32x4_t z = {0, 0, 0, 0};
 #pragma unroll
-    for (int r = c + 1; r < NT; ++r) {
-      f32x4_t z = {0, 0, 0, 0};
+    for (int j = 0; j < d; ++j) {
+      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * (wave + j) + 4 * quad);
 #pragma unroll
-      for (int j = c; j < r; ++j) {
-        const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * j + 4 * quad);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z = mfma32(w[e], t[j][c][e], z);
-      }
-      const f32x4_t d = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * r + 4 * quad);
-      t[r][c] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[r][c] = mfma32(-d[e], z[e], t[r][c]);
+      for (int e = 0; e < 4; ++e) z = mfma32(w[e], t[j][e], z);
     }
+    const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 16 * r + 4 * quad);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[d] = mfma32(-inv[e], z[e], t[d]);
   }
-  wave_sync();
+  __syncthreads();
+  const float beta = s_beta[16 * wave + col];
 #pragma unroll
-  for (int c = 0; c < NT; ++c) {
-    const float beta = s_beta[16 * c + col];
+  for (int d = 0; d < NT; ++d) {
+    if (wave + d >= NT) continue;
 #pragma unroll
-    for (int r = c; r < NT; ++r)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s_a[(16 * r + 4 * quad + e) * LD + 16 * c + col] = t[r][c][e] * beta;
+    for (int e = 0; e < 4; ++e) s_a[(16 * (wave + d) + 4 * quad + e) * LD + 16 * wave + col] = t[d][e] * beta;
   }
-  wave_sync();
+  __syncthreads();
+  // T's rows as fragments.
 #pragma unroll
-  for (int r = 0; r < NT; ++r) {
-    const float* row = s_a + (16 * r + col) * LD + 4 * quad;
+  for (int i = 0; i < (Out::kPairs + NT - 1) / NT; ++i) {
+    const int at = i * NT + wave;
+    if (at >= Out::kPairs) continue;
     if constexpr (B16) {
+      const int r = at < 2 ? at : 2 + (at - 2) / 2, h = at < 2 ? 0 : at & 1;
+      u32x4_t hi, lo;
 #pragma unroll
-      for (int h = 0; 2 * h <= r; ++h) {
-        u32x4_t hi, lo;
+      for (int x = 0; x < 2; ++x) {
+        f32x4_t w = {0, 0, 0, 0};
+        if (2 * h + x <= r) w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 32 * h + 16 * x + 4 * quad);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          f32x4_t w = {0, 0, 0, 0};
-          if (2 * h + x <= r) w = *reinterpret_cast<const f32x4_t*>(row + 32 * h + 16 * x);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t u, l;
-            split2(w[2 * e], w[2 * e + 1], u, l);
-            hi[2 * x + e] = u;
-            lo[2 * x + e] = l;
-          }
+        for (int e = 0; e < 2; ++e) {
+          uint32_t u, l;
+          split2(w[2 * e], w[2 * e + 1], u, l);
+          hi[2 * x + e] = u;
+          lo[2 * x + e] = l;
         }
-        out[Out::kT + 128 * pair_of<B16>(r, h) + lane] = hi;
-        out[Out::kT + 128 * pair_of<B16>(r, h) + 64 + lane] = lo;
       }
+      out[128 * at + lane] = hi;
+      out[128 * at + 64 + lane] = lo;
     } else {
-#pragma unroll
-      for (int c = 0; c <= r; ++c)
-        out[Out::kT + 64 * pair_of<B16>(r, c) + lane] = *reinterpret_cast<const u32x4_t*>(row + 16 * c);
+      const int r = triangle_row(at), c = triangle_col(at);
+      out[64 * at + lane] = *reinterpret_cast<const u32x4_t*>(s_a + (16 * r + col) * LD + 16 * c + 4 * quad);
     }
   }
 }
 
-// LDS units of a walk: two buffers of k | q | v | what was worked out ahead.
+// LDS units of a walk: two buffers of k | q | v | what was worked out ahead, and P.
 template <bool B16, int DKP>
 struct WalkLds {
   static constexpr int C = Ahead<B16>::C, N = B16 ? 8 : 4;  // elements of a unit
   static constexpr int kK = C * DKP / N, kQ = kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
-  static constexpr size_t kBytes = 2 * 16 * (size_t)kBuffer;
+  static constexpr int kP = Ahead<B16>::kPairs * Ahead<B16>::kFrag;
+  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + kP);
 };
 
 // The state's row of register r of tile b: as rows of k are read, 16 bytes a
@@ -452,9 +428,9 @@ __device__ __forceinline__ void state_turned(uint32_t at, u32x4_t (&k)[2]) {
 }
 
 // The walk of a sequence, a head and 64 value columns through its chunks: four
-// waves compute, 16 columns each, and four bring the next chunk (where the
-// same waves did both, issuing the loads took 2.3 of a chunk's 5.7 us, heads
-// of 128).
+// waves compute, 16 columns each, and four bring the next chunk and work out
+// P (where the same waves did all, issuing the loads took 2.3 of a chunk's
+// 5.7 us, heads of 128).
 constexpr int kWalkers = 4;
 template <bool B16, int DKP>
 __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a) {
@@ -509,14 +485,53 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  u32x4_t* sP = s_walk + 2 * Lds::kBuffer;
   if (in_all >= kWalkers) {
+    if constexpr (B16) {  // the halves of fragments that P does not reach
+      if (wave < 2) {
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          reinterpret_cast<u32x2_t*>(sP + In::kFrag * pair_of<B16>(2 * wave, wave) + 64 * part + lane)[1] = u32x2_t{0, 0};
+      }
+    }
     u32x4_t* to = s_walk;
     if (sp.len > 0) issue(0, min(C, sp.len), to);
     for (int pos = 0; pos < sp.len; pos += C) {
       __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
       meet();  // the chunk is there, and the one before is read
+      const u32x4_t *sK = to, *sQ = sK + Lds::kK;
+      const double* sum = reinterpret_cast<const double*>(sQ + Lds::kQ + Lds::kV + In::kSum);
       to = to == s_walk ? s_walk + Lds::kBuffer : s_walk;
       if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), to);
+      // P^T: queries 16 r + col, keys 16 c + 4 quad + e.
+#pragma unroll
+      for (int i = 0; i < (NT * (NT + 1) / 2 + 3) / 4; ++i) {
+        const int at = min(4 * i + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
+        f32x4_t p = tile_product<B16, DKP>(sK, 16 * c, sQ, 16 * r, lane);
+        const double gq = sum[16 * r + col];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = 16 * c + 4 * quad + e;
+          const float w = a.scale * __builtin_amdgcn_exp2f((float)((gq - sum[key]) * kLog2e));
+          p[e] = 16 * r + col >= key ? p[e] * w : 0.0f;
+        }
+        if constexpr (B16) {
+          u32x2_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t u, l;
+            split2(p[2 * e], p[2 * e + 1], u, l);
+            hi[e] = u;
+            lo[e] = l;
+          }
+          u32x4_t* to_p = sP + In::kFrag * pair_of<B16>(r, c >> 1) + lane;
+          reinterpret_cast<u32x2_t*>(to_p)[c & 1] = hi;
+          reinterpret_cast<u32x2_t*>(to_p + 64)[c & 1] = lo;
+        } else {
+          sP[In::kFrag * pair_of<B16>(r, c) + lane] = __builtin_bit_cast(u32x4_t, p);
+        }
+      }
+      meet();  // P is there
     }
     return;
   }
@@ -533,7 +548,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
   for (int pos = 0; pos < sp.len; pos += C) {
     const int n = min(C, sp.len - pos);
     meet();
-    const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV, *sP = sT + In::kP;
+    const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV;
     const float *gamma = reinterpret_cast<const float*>(sT + In::kGamma), *rest = gamma + C;
     const f32x4_t *K32 = reinterpret_cast<const f32x4_t*>(sK), *Q32 = reinterpret_cast<const f32x4_t*>(sQ),
                   *V32 = reinterpret_cast<const f32x4_t*>(sV);
@@ -693,38 +708,21 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
         qs += __shfl_xor(qs, 32, 64);
         if (quad == 0 && j < a.dv) store1(out + (size_t)i * a.ld_out + j, qs * a.scale);
       }
+      meet();
       continue;
     }
-    // O^T = scale e^G (Q S)^T + (P U)^T.
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
+    u32x4_t u_hi[2], u_lo[2];
     if constexpr (B16) {
-      u32x4_t hi[2], lo[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         uint32_t p, l;
         split2(u[e >> 1][2 * (e & 1)], u[e >> 1][2 * (e & 1) + 1], p, l);
-        hi[e >> 2][e & 3] = p;
-        lo[e >> 2][e & 3] = l;
+        u_hi[e >> 2][e & 3] = p;
+        u_lo[e >> 2][e & 3] = l;
       }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int h = 0; 2 * h <= t; ++h) {
-          const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
-          o[t] = mfma(lo[h], ph, o[t]);
-          o[t] = mfma(hi[h], pl, o[t]);
-          o[t] = mfma(hi[h], ph, o[t]);
-        }
     } else {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int h = 0; h <= t; ++h) {
-          const f32x4_t pf = __builtin_bit_cast(f32x4_t, sP[64 * pair_of<B16>(t, h) + lane]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[t] = mfma32(u[h][r], pf[r], o[t]);
-        }
+      for (int t = 0; t < NT; ++t) u_hi[t] = __builtin_bit_cast(u32x4_t, u[t]);
     }
     // S = e^(G_n) S + K^T (e^(G_n - G) U).
     const float last = gamma[C - 1];
@@ -763,6 +761,30 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
 #pragma unroll
           for (int b = 0; b < NB; ++b)
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
+    }
+    meet();  // P is there
+    // O^T = scale e^G (Q S)^T + (P U)^T.
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
+    if constexpr (B16) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; 2 * h <= t; ++h) {
+          const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
+          o[t] = mfma(u_lo[h], ph, o[t]);
+          o[t] = mfma(u_hi[h], pl, o[t]);
+          o[t] = mfma(u_hi[h], ph, o[t]);
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h <= t; ++h) {
+          const f32x4_t pf = __builtin_bit_cast(f32x4_t, sP[64 * pair_of<B16>(t, h) + lane]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t] = mfma32(__uint_as_float(u_hi[h][r]), pf[r], o[t]);
+        }
     }
     // Tokens 16 t + col, columns 16 wave + 4 quad ..
     const int c = dv0 + 16 * wave + 4 * quad;
@@ -867,7 +889,7 @@ Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, in
 
 int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ahead<false>::C; }
 
-// What is worked out ahead takes 25 KiB a chunk and head (bf16; 7 KiB fp32):
+// What is worked out ahead takes 13 KiB a chunk and head (bf16; 4 KiB fp32):
 // past 1 GiB of it the heads run in several launches.
 DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t heads, size_t d_key, size_t d_val) {
   DeltaScratch s;
@@ -911,7 +933,7 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
   return with_chunks(dtype, a.dk, [&](auto c) -> Status {
     for (a.head0 = 0; a.head0 < a.heads; a.head0 += s.heads_here) {
       a.heads_here = std::min(s.heads_here, a.heads - a.head0);
-      c.kAhead<<<dim3(a.chunks, a.heads_here), 64, 0, stream>>>(a);
+      c.kAhead<<<dim3(a.chunks, a.heads_here), c.kBf16 ? 256 : 128, 0, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_ahead_kernel");
       c.kWalk<<<dim3((a.dv + 63) / 64, a.heads_here, a.n_seqs), 128 * kWalkers, c.kLds, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_walk_kernel");
