@@ -236,6 +236,12 @@ __device__ __forceinline__ f32x4_t tile_product(const u32x4_t* sx, int x, const 
   return s;
 }
 
+// e^(gi - gj) where `on`, else 0: no branch, as the loads of either would wait in it.
+__device__ __forceinline__ float decay_between(double gi, double gj, bool on) {
+  const float d = (float)((gi - gj) * kLog2e);
+  return __builtin_amdgcn_exp2f(on ? d : -INFINITY);
+}
+
 // A chunk of one head, a wave for each 16 tokens.  A's triangle lies in LDS;
 // each wave inverts one of its diagonal blocks by substitution, a column a
 // lane, and follows one column of blocks down:
@@ -288,11 +294,16 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
     const int at = min(i * NT + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
     const f32x4_t s = tile_product<B16, DKP>(s_k, 16 * r, s_k, 16 * c, lane);
     const double gk = s_g[16 * c + col];
+    float w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = 16 * r + 4 * quad + e;
-      const float w = s_beta[row] * __builtin_amdgcn_exp2f((float)((s_g[row] - gk) * kLog2e));
-      s_a[row * LD + 16 * c + col] = row > 16 * c + col ? s[e] * w : 0.0f;
+      w[e] = s_beta[row] * decay_between(s_g[row], gk, row > 16 * c + col);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * r + 4 * quad + e;
+      s_a[row * LD + 16 * c + col] = row > 16 * c + col ? s[e] * w[e] : 0.0f;
     }
   }
   __syncthreads();
@@ -382,13 +393,18 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
   }
 }
 
-// LDS units of a walk: two buffers of k | q | v | what was worked out ahead, and P.
+// LDS units of a walk: two buffers of k | q | v | what was worked out ahead,
+// P, and what the computing waves hand over: S as operands, U (its first part
+// in v's place where it is bf16), and which waves ran token by token.
 template <bool B16, int DKP>
 struct WalkLds {
   static constexpr int C = Ahead<B16>::C, N = B16 ? 8 : 4;  // elements of a unit
   static constexpr int kK = C * DKP / N, kQ = kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
-  static constexpr int kP = Ahead<B16>::kPairs * Ahead<B16>::kFrag;
-  static constexpr size_t kBytes = 16 * (size_t)(2 * kBuffer + kP);
+  static constexpr int kP = 2 * kBuffer, kS = kP + Ahead<B16>::kPairs * Ahead<B16>::kFrag;
+  static constexpr int kState = B16 ? DKP / 32 * 2 * 64 : DKP / 16 * 64;  // of a wave
+  static constexpr int kU = kS + 4 * kState, kOdd = kU + 4 * 128, kUnits = kOdd + 1;
+  static constexpr size_t kBytes = 16 * (size_t)kUnits;
+  static_assert(kBytes <= 160 * 1024, "a compute unit's LDS");
 };
 
 // The state's row of register r of tile b: as rows of k are read, 16 bytes a
@@ -397,40 +413,29 @@ template <bool B16>
 __device__ __forceinline__ int state_row(int b, int quad, int r) {
   return B16 ? 32 * (b >> 1) + 8 * quad + 4 * (b & 1) + r : 16 * b + 4 * quad + r;
 }
-// Tokens row0 + 4 quad .. + 3 and 16 more of the state's rows of N tiles (4 or
-// 2): transposed LDS reads, with their wait (the builtin would wait for the
-// loads into the other buffer).
-template <int W>
-__device__ __forceinline__ uint32_t state_turned_at(const u32x4_t* s, int row0, int lane) {
-  const int row = row0 + 4 * (lane >> 4) + ((lane >> 2) & 3);
-  const u32x4_t* unit = s + row * (W / 8) + row_unit<W>(row, lane & 3);
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)unit;
-}
-template <int W>
-__device__ __forceinline__ void state_turned(uint32_t at, u32x4_t (&k)[4]) {
-  u32x2_t k0[4], k1[4];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%c12\n\t"
-      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%c12\n\t"
-      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%c12\n\t"
-      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%c12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(k0[0]), "=&v"(k1[0]), "=&v"(k0[1]), "=&v"(k1[1]), "=&v"(k0[2]), "=&v"(k1[2]), "=&v"(k0[3]), "=&v"(k1[3])
-      : "v"(at), "v"(at ^ 8), "v"(at ^ 64), "v"(at ^ 72), "i"(32 * W)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k[i] = u32x4_t{k0[i][0], k0[i][1], k1[i][0], k1[i][1]};
-}
-template <int W>
-__device__ __forceinline__ void state_turned(uint32_t at, u32x4_t (&k)[2]) {
-  turned_frag<W>(at, k[0]);
-  turned_frag<W>(at ^ 8, k[1]);
+// Rows row0 + 4 quad .. + 3 and 16 more at a lane's column: 16 lanes read a 4 x
+// 16 block, 4 columns each, and are handed its columns.  The lanes' columns are
+// c0 + STEP (lane % 4) .. + 3.  The waves that compute bring nothing into LDS,
+// so these loads wait for none.
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+template <int W, int STEP>
+__device__ __forceinline__ u32x4_t turned(const u32x4_t* s, int row0, int c0, int lane) {
+  const int row = row0 + 4 * (lane >> 4) + ((lane >> 2) & 3), c = c0 + STEP * (lane & 3);
+  const u32x2_t* at = reinterpret_cast<const u32x2_t*>(s + row * (W / 8) + row_unit<W>(row, c >> 3)) + ((c >> 2) & 1);
+  auto read = [](const u32x2_t* p) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) i16x4_t*)(const_cast<u32x2_t*>(p))));
+  };
+  const u32x2_t x = read(at), y = read(at + 16 * (W / 4));
+  return u32x4_t{x[0], x[1], y[0], y[1]};
 }
 
-// The walk of a sequence, a head and 64 value columns through its chunks: four
-// waves compute, 16 columns each, and four bring the next chunk and work out
-// P (where the same waves did all, issuing the loads took 2.3 of a chunk's
-// 5.7 us, heads of 128).
+// The walk of a sequence, a head and 64 value columns through its chunks. Four
+// waves, 16 columns each, go from S to the next S; four others bring the next
+// chunk, work out P and turn the S and U that they are handed into outputs, so
+// that nothing but the states' own chain runs from chunk to chunk (where the
+// same waves did all, issuing the loads alone took 2.3 of a chunk's 5.7 us,
+// heads of 128).
 constexpr int kWalkers = 4;
 template <bool B16, int DKP>
 __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a) {
@@ -485,7 +490,13 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  u32x4_t* sP = s_walk + 2 * Lds::kBuffer;
+  u32x4_t *sP = s_walk + Lds::kP, *sS = s_walk + Lds::kS + wave * Lds::kState, *sU = s_walk + Lds::kU + wave * 128;
+  uint32_t* s_odd = reinterpret_cast<uint32_t*>(s_walk + Lds::kOdd);
+  // U's first parts in v's place: the wave's own columns, 2 units of each row.
+  auto u_place = [&](const u32x4_t* v, int h) {
+    const int i = 64 * h + lane, row = i >> 1;
+    return const_cast<u32x4_t*>(v) + row * 8 + row_unit<64>(row, 2 * wave + (i & 1));
+  };
   if (in_all >= kWalkers) {
     if constexpr (B16) {  // the halves of fragments that P does not reach
       if (wave < 2) {
@@ -494,27 +505,66 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           reinterpret_cast<u32x2_t*>(sP + In::kFrag * pair_of<B16>(2 * wave, wave) + 64 * part + lane)[1] = u32x2_t{0, 0};
       }
     }
-    u32x4_t* to = s_walk;
-    if (sp.len > 0) issue(0, min(C, sp.len), to);
+    // A chunk's outputs, tokens 16 t + col by columns 16 wave + 4 quad .., leave
+    // in the next one's course: every memory operation of a chunk has to end
+    // before the next begins.
+    std::conditional_t<B16, u32x2_t, f32x4_t> held[NT];
+    int held_n = 0;
+    const int c_out = dv0 + 16 * wave + 4 * quad;
+    auto put = [&](int pos) {
+      typedef std::conditional_t<B16, u32x2_any_t, f32x4_any_t> any_t;
+      T* dst = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv + (__umul24(col, (uint32_t)a.ld_out) + c_out);
+      if (held_n == C && dv0 + 64 <= a.dv) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<any_t*>(dst + (size_t)(16 * t) * a.ld_out) = held[t];
+        return;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (16 * t + col >= held_n || c_out >= a.dv) continue;
+        T* to = dst + (size_t)(16 * t) * a.ld_out;
+        if (c_out + 4 <= a.dv) {
+          *reinterpret_cast<any_t*>(to) = held[t];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 3; ++e) {
+            if (c_out + e >= a.dv) continue;
+            if constexpr (B16)
+              to[e].bits = (uint16_t)(held[t][e >> 1] >> (16 * (e & 1)));
+            else
+              to[e] = held[t][e];
+          }
+        }
+      }
+    };
+    const u32x4_t* buffer = s_walk;
+    if (sp.len > 0) issue(0, min(C, sp.len), s_walk);
     for (int pos = 0; pos < sp.len; pos += C) {
+      const int n = min(C, sp.len - pos);
       __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
       meet();  // the chunk is there, and the one before is read
-      const u32x4_t *sK = to, *sQ = sK + Lds::kK;
-      const double* sum = reinterpret_cast<const double*>(sQ + Lds::kQ + Lds::kV + In::kSum);
-      to = to == s_walk ? s_walk + Lds::kBuffer : s_walk;
-      if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), to);
+      const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV;
+      const float* gamma = reinterpret_cast<const float*>(sT + In::kGamma);
+      const double* sum = reinterpret_cast<const double*>(sT + In::kSum);
+      u32x4_t* other = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
+      buffer = other;
+      if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), other);
+      put(pos - held_n);
+      held_n = 0;
       // P^T: queries 16 r + col, keys 16 c + 4 quad + e.
 #pragma unroll
       for (int i = 0; i < (NT * (NT + 1) / 2 + 3) / 4; ++i) {
         const int at = min(4 * i + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
         f32x4_t p = tile_product<B16, DKP>(sK, 16 * c, sQ, 16 * r, lane);
         const double gq = sum[16 * r + col];
+        float d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = 16 * c + 4 * quad + e;
-          const float w = a.scale * __builtin_amdgcn_exp2f((float)((gq - sum[key]) * kLog2e));
-          p[e] = 16 * r + col >= key ? p[e] * w : 0.0f;
+          d[e] = a.scale * decay_between(gq, sum[key], 16 * r + col >= key);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = 16 * r + col >= 16 * c + 4 * quad + e ? p[e] * d[e] : 0.0f;
         if constexpr (B16) {
           u32x2_t hi, lo;
 #pragma unroll
@@ -531,8 +581,79 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           sP[In::kFrag * pair_of<B16>(r, c) + lane] = __builtin_bit_cast(u32x4_t, p);
         }
       }
-      meet();  // P is there
+      meet();  // P, S and U are there
+      if (s_odd[wave]) continue;  // uniform: the other wave stores these
+      // O^T = scale e^G (Q S)^T + (P U)^T.
+      f32x4_t o[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0, 0, 0, 0};
+      if constexpr (B16) {
+#pragma unroll
+        for (int kp = 0; kp < DKP / 32; ++kp) {
+          const u32x4_t hi = sS[128 * kp + lane], lo = sS[128 * kp + 64 + lane];
+          u32x4_t qf[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) qf[t] = row_frag<DKP>(sQ, 16 * t + col, 4 * kp + quad);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[t] = mfma(lo, qf[t], o[t]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[t] = mfma(hi, qf[t], o[t]);
+        }
+      } else {
+        const f32x4_t* Q32 = reinterpret_cast<const f32x4_t*>(sQ);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const f32x4_t sf = __builtin_bit_cast(f32x4_t, sS[64 * b + lane]);
+          f32x4_t qf[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) qf[t] = row_frag32<DKP>(Q32, 16 * t + col, 4 * b + quad);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] = mfma32(sf[r], qf[t][r], o[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
+      if constexpr (B16) {
+        u32x4_t hi[2], lo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          hi[h] = *u_place(sV, h);
+          lo[h] = sU[64 * h + lane];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int h = 0; 2 * h <= t; ++h) {
+            const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
+            o[t] = mfma(lo[h], ph, o[t]);
+            o[t] = mfma(hi[h], pl, o[t]);
+            o[t] = mfma(hi[h], ph, o[t]);
+          }
+      } else {
+        f32x4_t u[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) u[t] = __builtin_bit_cast(f32x4_t, sU[64 * t + lane]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int h = 0; h <= t; ++h) {
+            const f32x4_t pf = __builtin_bit_cast(f32x4_t, sP[64 * pair_of<B16>(t, h) + lane]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t] = mfma32(u[h][r], pf[r], o[t]);
+          }
+      }
+      held_n = n;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (B16)
+          held[t] = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
+        else
+          held[t] = o[t];
+      }
     }
+    put(sp.len - held_n);
     return;
   }
   // S: the rows of the lane's column.
@@ -554,10 +675,10 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
                   *V32 = reinterpret_cast<const f32x4_t*>(sV);
     buffer = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
 
-    // K S (rows: tokens) and (Q S)^T (columns: tokens).
-    f32x4_t x[NT], o[NT];
+    // K S (rows: tokens).
+    f32x4_t x[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) x[t] = o[t] = f32x4_t{0, 0, 0, 0};
+    for (int t = 0; t < NT; ++t) x[t] = f32x4_t{0, 0, 0, 0};
     if constexpr (B16) {
 #pragma unroll
       for (int kp = 0; kp < DKP / 32; ++kp) {
@@ -569,35 +690,27 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           hi[e] = u;
           lo[e] = l;
         }
-        u32x4_t kf[NT], qf[NT];
+        sS[128 * kp + lane] = hi;
+        sS[128 * kp + 64 + lane] = lo;
+        u32x4_t kf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) kf[t] = row_frag<DKP>(sK, 16 * t + col, 4 * kp + quad);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) qf[t] = row_frag<DKP>(sQ, 16 * t + col, 4 * kp + quad);
-#pragma unroll
         for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], lo, x[t]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o[t] = mfma(lo, qf[t], o[t]);
-#pragma unroll
         for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], hi, x[t]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t] = mfma(hi, qf[t], o[t]);
       }
     } else {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        f32x4_t kf[NT], qf[NT];
+        sS[64 * b + lane] = __builtin_bit_cast(u32x4_t, S[b]);
+        f32x4_t kf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) kf[t] = row_frag32<DKP>(K32, 16 * t + col, 4 * b + quad);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) qf[t] = row_frag32<DKP>(Q32, 16 * t + col, 4 * b + quad);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int t = 0; t < NT; ++t) x[t] = mfma32(kf[t][r], S[b][r], x[t]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t] = mfma32(S[b][r], qf[t][r], o[t]);
-        }
       }
     }
     // X = V - e^G K S, U = T X.
@@ -605,7 +718,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     if constexpr (B16) {
       u32x4_t vf[2], hi[2], lo[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) turned_frag<64>(turned_at<64>(sV, 32 * h, 16 * wave, lane), vf[h]);
+      for (int h = 0; h < 2; ++h) vf[h] = turned<64, 4>(sV, 32 * h, 16 * wave, lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const f32x4_t g = *reinterpret_cast<const f32x4_t*>(gamma + 16 * t + 4 * quad);
@@ -649,13 +762,36 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
         }
       }
     }
-    bool odd = false;
+    float odd = 0.0f;  // NaN once a value is not finite
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[t][r]) < INFINITY);
-    T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv;
-    if (__any(odd)) {
+      for (int r = 0; r < 4; ++r) odd = fmaf(u[t][r], 0.0f, odd);
+    const bool one_by_one = __any(odd != odd);
+    if (lane == 0) s_odd[wave] = one_by_one;
+    if (!one_by_one) {
+      if constexpr (B16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4_t p, l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t hi, lo;
+            split2(u[2 * h + (e >> 1)][2 * (e & 1)], u[2 * h + (e >> 1)][2 * (e & 1) + 1], hi, lo);
+            p[e] = hi;
+            l[e] = lo;
+          }
+          *u_place(sV, h) = p;
+          sU[64 * h + lane] = l;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sU[64 * t + lane] = __builtin_bit_cast(u32x4_t, u[t]);
+      }
+    }
+    meet();  // S and U are there
+    if (one_by_one) {
+      T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv;
       // Something is not finite; in the products 0 times it would reach
       // tokens before it.  The chunk's tokens run one by one.
 #pragma unroll 1
@@ -708,21 +844,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
         qs += __shfl_xor(qs, 32, 64);
         if (quad == 0 && j < a.dv) store1(out + (size_t)i * a.ld_out + j, qs * a.scale);
       }
-      meet();
       continue;
-    }
-    u32x4_t u_hi[2], u_lo[2];
-    if constexpr (B16) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint32_t p, l;
-        split2(u[e >> 1][2 * (e & 1)], u[e >> 1][2 * (e & 1) + 1], p, l);
-        u_hi[e >> 2][e & 3] = p;
-        u_lo[e >> 2][e & 3] = l;
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) u_hi[t] = __builtin_bit_cast(u32x4_t, u[t]);
     }
     // S = e^(G_n) S + K^T (e^(G_n - G) U).
     const float last = gamma[C - 1];
@@ -746,7 +868,8 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
 #pragma unroll
         for (int b0 = 0; b0 < NB; b0 += BG) {
           u32x4_t kf[BG];
-          state_turned<DKP>(state_turned_at<DKP>(sK, 32 * h, lane) ^ (32 * b0), kf);
+#pragma unroll
+          for (int b = 0; b < BG; ++b) kf[b] = turned<DKP, 8>(sK, 32 * h, state_row<B16>(b0 + b, 0, 0), lane);
 #pragma unroll
           for (int p = 2; p >= 0; --p)
 #pragma unroll
@@ -761,48 +884,6 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
 #pragma unroll
           for (int b = 0; b < NB; ++b)
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
-    }
-    meet();  // P is there
-    // O^T = scale e^G (Q S)^T + (P U)^T.
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
-    if constexpr (B16) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int h = 0; 2 * h <= t; ++h) {
-          const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
-          o[t] = mfma(u_lo[h], ph, o[t]);
-          o[t] = mfma(u_hi[h], pl, o[t]);
-          o[t] = mfma(u_hi[h], ph, o[t]);
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int h = 0; h <= t; ++h) {
-          const f32x4_t pf = __builtin_bit_cast(f32x4_t, sP[64 * pair_of<B16>(t, h) + lane]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[t] = mfma32(__uint_as_float(u_hi[h][r]), pf[r], o[t]);
-        }
-    }
-    // Tokens 16 t + col, columns 16 wave + 4 quad ..
-    const int c = dv0 + 16 * wave + 4 * quad;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int i = 16 * t + col;
-      if (i >= n || c >= a.dv) continue;
-      T* dst = out + (size_t)i * a.ld_out + c;
-      if (c + 4 <= a.dv) {
-        if constexpr (B16)
-          *reinterpret_cast<u32x2_any_t*>(dst) = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
-        else
-          *reinterpret_cast<f32x4_any_t*>(dst) = o[t];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (c + e < a.dv) store1(dst + e, o[t][e]);
-      }
     }
   }
   if (!a.state_out) return;
