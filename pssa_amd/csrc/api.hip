@@ -2565,8 +2565,8 @@ struct DeltaPlan {
   size_t tokens = 0, longest = 0;
   pssa::DeltaScratch scratch;
 
-  // What is worked out ahead, row copies, then the table.
-  size_t table_at() const { return scratch.ahead + scratch.rows; }
+  // What is worked out ahead, row copies, the segments' states and transitions, then the table.
+  size_t table_at() const { return scratch.ahead + scratch.rows + scratch.state + scratch.move; }
   size_t scratch_bytes() const { return table_at() + table.size() * 4; }
 };
 Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len, size_t heads, size_t d_key, size_t d_val,
@@ -2574,33 +2574,42 @@ Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len
   PSSA_RETURN_IF(need(n_seqs >= 1 && n_seqs <= 65535, "delta rule: sequences must be in 1..=65535"));
   a.n_seqs = (int)n_seqs;
   const size_t chunk = (size_t)pssa::delta_chunk(dtype);
-  size_t chunks = 0;
   bool same = true;
   for (size_t i = 0; i < n_seqs; ++i) {
     const size_t len = lens ? lens[i] : seq_len;
     PSSA_RETURN_IF(need(len <= INT32_MAX && p.tokens + len <= INT32_MAX, "delta rule: too many tokens"));
     p.tokens += len;
-    chunks += (len + chunk - 1) / chunk;
     p.longest = std::max(p.longest, len);
     same &= !lens || lens[i] == lens[0];
   }
-  a.chunks = (int)chunks;
-  if (p.longest > (size_t)pssa::kDeltaSteps)
-    p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, heads, d_key, d_val);
   a.uniform_len = same ? (int)p.longest : -1;
-  if (same) return Status::Ok();
+  const bool chunked = p.longest > (size_t)pssa::kDeltaSteps;
+  a.seg_chunks = chunked ? pssa::delta_segment(dtype, lens, n_seqs, p.longest, heads, d_key, d_val) : 0;
+  const size_t seg = (size_t)a.seg_chunks * chunk;
+  auto segments = [&](size_t len) { return seg ? std::max<size_t>(1, (len + seg - 1) / seg) : 1; };
+  size_t chunks = 0, items = 0;
   const bool inside = n_seqs <= (size_t)pssa::kDeltaInline;
-  if (!inside) p.table.resize(2 * (n_seqs + 1));
+  if (!same && !inside) p.table.resize((seg ? 3 : 2) * (n_seqs + 1));
   uint32_t* tok = inside ? a.inline_tokens : p.table.data();
   uint32_t* first = inside ? a.inline_chunks : p.table.data() + n_seqs + 1;
-  uint32_t t = 0, c = 0;
+  uint32_t* item = inside ? a.inline_items : p.table.data() + 2 * (n_seqs + 1);
+  uint32_t t = 0;
   for (size_t i = 0; i <= n_seqs; ++i) {
-    tok[i] = t;
-    first[i] = c;
+    if (!same) {
+      tok[i] = t;
+      first[i] = (uint32_t)chunks;
+      if (seg) item[i] = (uint32_t)items;
+    }
     if (i == n_seqs) break;
-    t += (uint32_t)lens[i];
-    c += (uint32_t)((lens[i] + chunk - 1) / chunk);
+    const size_t len = lens ? lens[i] : seq_len;
+    t += (uint32_t)len;
+    chunks += (len + chunk - 1) / chunk;
+    items += segments(len);
   }
+  a.chunks = (int)chunks;
+  a.items = (int)items;
+  a.uniform_segs = (int)segments(p.longest);
+  if (chunked) p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, seg ? items : 0, heads, d_key, d_val);
   return Status::Ok();
 }
 Status check_delta_heads(size_t heads, size_t d_key, size_t d_val) {

@@ -44,6 +44,9 @@ __device__ __forceinline__ uint32_t first_token(const DeltaArgs& a, int seq) {
 __device__ __forceinline__ int first_chunk(const DeltaArgs& a, int seq) {
   return (int)(a.table ? a.table[a.n_seqs + 1 + seq] : inline_word(offsetof(DeltaArgs, inline_chunks), seq));
 }
+__device__ __forceinline__ int first_item(const DeltaArgs& a, int seq) {
+  return (int)(a.table ? a.table[2 * (a.n_seqs + 1) + seq] : inline_word(offsetof(DeltaArgs, inline_items), seq));
+}
 // A sequence's tokens.
 struct Span {
   size_t tok;
@@ -393,16 +396,20 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
   }
 }
 
+// How a walk runs: the whole of an unsplit call, a segment's own state and
+// transition, or a segment's outputs from its entry state.
+enum { DR_WHOLE, DR_LOCAL, DR_SEGMENT };
+
 // LDS units of a walk: two buffers of k | q | v | what was worked out ahead,
 // P, and what the computing waves hand over: S as operands, U (its first part
 // in v's place where it is bf16), and which waves ran token by token.
-template <bool B16, int DKP>
+template <bool B16, int DKP, bool LOCAL>
 struct WalkLds {
   static constexpr int C = Ahead<B16>::C, N = B16 ? 8 : 4;  // elements of a unit
-  static constexpr int kK = C * DKP / N, kQ = kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
-  static constexpr int kP = 2 * kBuffer, kS = kP + Ahead<B16>::kPairs * Ahead<B16>::kFrag;
-  static constexpr int kState = B16 ? DKP / 32 * 2 * 64 : DKP / 16 * 64;  // of a wave
-  static constexpr int kU = kS + 4 * kState, kOdd = kU + 4 * 128, kUnits = kOdd + 1;
+  static constexpr int kK = C * DKP / N, kQ = LOCAL ? 0 : kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
+  static constexpr int kP = 2 * kBuffer, kS = kP + (LOCAL ? 0 : Ahead<B16>::kPairs * Ahead<B16>::kFrag);
+  static constexpr int kState = LOCAL ? 0 : B16 ? DKP / 32 * 2 * 64 : DKP / 16 * 64;  // of a wave
+  static constexpr int kU = kS + 4 * kState, kOdd = kU + (LOCAL ? 0 : 4 * 128), kUnits = kOdd + (LOCAL ? 0 : 1);
   static constexpr size_t kBytes = 16 * (size_t)kUnits;
   static_assert(kBytes <= 160 * 1024, "a compute unit's LDS");
 };
@@ -430,37 +437,90 @@ __device__ __forceinline__ u32x4_t turned(const u32x4_t* s, int row0, int c0, in
   return u32x4_t{x[0], x[1], y[0], y[1]};
 }
 
+// What a workgroup walks: a sequence's or segment's first chunk, its first
+// token and its tokens.
+template <int C>
+struct Walk {
+  int seq, chunk0;
+  Span span;
+};
+template <int C, int MODE>
+__device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
+  Walk<C> w;
+  int seg = 0;
+  if (MODE == DR_WHOLE) {
+    w.seq = item;
+  } else if (a.uniform_len >= 0) {
+    w.seq = item / a.uniform_segs;
+    seg = item - w.seq * a.uniform_segs;
+  } else {
+    int lo = 0, hi = a.n_seqs - 1;  // the last sequence that begins at or before the item
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_item(a, mid) <= item) lo = mid; else hi = mid - 1;
+    }
+    w.seq = lo;
+    seg = item - first_item(a, lo);
+  }
+  w.span = span_of(a, w.seq);
+  w.chunk0 = a.uniform_len >= 0 ? w.seq * ((a.uniform_len + C - 1) / C) : first_chunk(a, w.seq);
+  if (MODE != DR_WHOLE) {
+    w.chunk0 += seg * a.seg_chunks;
+    w.span.tok += (size_t)seg * a.seg_chunks * C;
+    w.span.len = min(w.span.len - seg * a.seg_chunks * C, a.seg_chunks * C);
+  }
+  return w;
+}
+
 // The walk of a sequence, a head and 64 value columns through its chunks. Four
 // waves, 16 columns each, go from S to the next S; four others bring the next
 // chunk, work out P and turn the S and U that they are handed into outputs, so
 // that nothing but the states' own chain runs from chunk to chunk (where the
 // same waves did all, issuing the loads alone took 2.3 of a chunk's 5.7 us,
 // heads of 128).
+// A segment's own state and its transition need no outputs, and two waves bring
+// their chunks, so that two workgroups fit a compute unit.  The transition is
+// the state that the unit matrix becomes without values: more columns.
 constexpr int kWalkers = 4;
-template <bool B16, int DKP>
-__global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a) {
+template <int MODE>
+constexpr int kHelpers = MODE == DR_LOCAL ? 2 : 4;
+template <bool B16, int DKP, int MODE>
+__global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_kernel(DeltaArgs a) {
+  constexpr bool LOCAL = MODE == DR_LOCAL;
+  constexpr int HELPERS = kHelpers<MODE>;
   using In = Ahead<B16>;
-  using Lds = WalkLds<B16, DKP>;
+  using Lds = WalkLds<B16, DKP, LOCAL>;
   using T = std::conditional_t<B16, Bf16, float>;
   constexpr int C = In::C, NT = In::kTiles, NB = DKP / 16, N = Lds::N;
-  constexpr int LOADS = Lds::kBuffer / 64, PER = (LOADS + 3) / 4;
+  constexpr int LOADS = Lds::kBuffer / 64, PER = (LOADS + HELPERS - 1) / HELPERS;
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_walk[];
   const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = in_all % kWalkers;
   const int col = lane & 15, quad = lane >> 4;
-  const int dv0 = blockIdx.x * 64, head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads), seq = blockIdx.z;
-  const Span sp = span_of(a, seq);
-  const int chunk0 = a.uniform_len >= 0 ? seq * ((a.uniform_len + C - 1) / C) : first_chunk(a, seq);
-  const size_t state0 = ((size_t)seq * a.heads + head) * a.dk * a.dv;
+  const int head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads);
+  const Walk<C> wk = walk_of<C, MODE>(a, blockIdx.z);
+  const Span sp = wk.span;
+  // The columns: of the values, or (behind them) of the transition.
+  const int tiles_v = (a.dv + 63) / 64;
+  const bool moves = LOCAL && (int)blockIdx.x >= tiles_v;
+  const int dv0 = 64 * ((int)blockIdx.x - (moves ? tiles_v : 0)), width = moves ? a.dk : a.dv;
+  const size_t item_head = (size_t)blockIdx.z * a.heads_here + blockIdx.y;
+  const float* state_in = MODE == DR_WHOLE     ? a.state_in ? a.state_in + ((size_t)wk.seq * a.heads + head) * a.dk * a.dv : nullptr
+                          : MODE == DR_SEGMENT ? a.seg_state + item_head * a.dk * a.dv
+                                               : nullptr;
+  float* state_out = MODE == DR_WHOLE   ? a.state_out ? a.state_out + ((size_t)wk.seq * a.heads + head) * a.dk * a.dv : nullptr
+                     : MODE == DR_LOCAL ? (moves ? a.seg_move + item_head * a.dk * a.dk : a.seg_state + item_head * a.dk * a.dv)
+                                        : nullptr;
   const int j = dv0 + 16 * wave + col;  // the lane's column
 
   auto issue = [&](int pos, int n, u32x4_t* buffer) {
     const size_t tok = sp.tok + pos;
     const u32x4_t* ahead = reinterpret_cast<const u32x4_t*>(a.ahead) +
-                           ((size_t)(chunk0 + pos / C) * a.heads_here + blockIdx.y) * In::kUnits;
+                           ((size_t)(wk.chunk0 + pos / C) * a.heads_here + blockIdx.y) * In::kUnits;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (LOADS % 4 != 0 && i * 4 + wave >= LOADS) continue;
-      const int at = (i * 4 + wave) * 64;  // first unit
+      const int load = i * HELPERS + in_all - kWalkers;
+      if (LOADS % HELPERS != 0 && load >= LOADS) continue;
+      const int at = load * 64;  // first unit
       const bool is_k = at < Lds::kK, is_q = !is_k && at < Lds::kK + Lds::kQ, is_v = !is_k && !is_q && at < Lds::kK + Lds::kQ + Lds::kV;
       const void* src;
       if (is_k || is_q || is_v) {
@@ -475,8 +535,8 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
         const T* base = is_k   ? static_cast<const T*>(a.k) + (size_t)key_head * a.wide_k
                         : is_q ? static_cast<const T*>(a.q) + (size_t)key_head * a.wide_q
                                : static_cast<const T*>(a.v) + (size_t)head * a.wide_v + dv0;
-        const int width = is_v ? a.dv - dv0 : a.dk;
-        src = row < n && c < width ? static_cast<const void*>(base + (tok + row) * ld + c) : g_nothing;
+        const int there = is_v ? (moves ? 0 : a.dv - dv0) : a.dk;
+        src = row < n && c < there ? static_cast<const void*>(base + (tok + row) * ld + c) : g_nothing;
       } else {
         src = ahead + (at - Lds::kK - Lds::kQ - Lds::kV) + lane;
       }
@@ -490,6 +550,19 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  if constexpr (LOCAL) {
+    if (in_all >= kWalkers) {
+      u32x4_t* to = s_walk;
+      if (sp.len > 0) issue(0, min(C, sp.len), to);
+      for (int pos = 0; pos < sp.len; pos += C) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+        meet();  // the chunk is there, and the one before is read
+        to = to == s_walk ? s_walk + Lds::kBuffer : s_walk;
+        if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), to);
+      }
+      return;
+    }
+  }
   u32x4_t *sP = s_walk + Lds::kP, *sS = s_walk + Lds::kS + wave * Lds::kState, *sU = s_walk + Lds::kU + wave * 128;
   uint32_t* s_odd = reinterpret_cast<uint32_t*>(s_walk + Lds::kOdd);
   // U's first parts in v's place: the wave's own columns, 2 units of each row.
@@ -497,7 +570,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     const int i = 64 * h + lane, row = i >> 1;
     return const_cast<u32x4_t*>(v) + row * 8 + row_unit<64>(row, 2 * wave + (i & 1));
   };
-  if (in_all >= kWalkers) {
+  if (!LOCAL && in_all >= kWalkers) {
     if constexpr (B16) {  // the halves of fragments that P does not reach
       if (wave < 2) {
 #pragma unroll
@@ -663,7 +736,9 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = state_row<B16>(b, quad, r);
-      S[b][r] = a.state_in && i < a.dk && j < a.dv ? a.state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
+      S[b][r] = moves                                    ? (i == j && i < a.dk ? 1.0f : 0.0f)
+                : state_in && i < a.dk && j < a.dv ? state_in[(size_t)i * a.dv + j]
+                                                   : 0.0f;
     }
   const u32x4_t* buffer = s_walk;
   for (int pos = 0; pos < sp.len; pos += C) {
@@ -690,8 +765,10 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           hi[e] = u;
           lo[e] = l;
         }
-        sS[128 * kp + lane] = hi;
-        sS[128 * kp + 64 + lane] = lo;
+        if constexpr (!LOCAL) {
+          sS[128 * kp + lane] = hi;
+          sS[128 * kp + 64 + lane] = lo;
+        }
         u32x4_t kf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) kf[t] = row_frag<DKP>(sK, 16 * t + col, 4 * kp + quad);
@@ -703,7 +780,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
     } else {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        sS[64 * b + lane] = __builtin_bit_cast(u32x4_t, S[b]);
+        if constexpr (!LOCAL) sS[64 * b + lane] = __builtin_bit_cast(u32x4_t, S[b]);
         f32x4_t kf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) kf[t] = row_frag32<DKP>(K32, 16 * t + col, 4 * b + quad);
@@ -768,8 +845,8 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
 #pragma unroll
       for (int r = 0; r < 4; ++r) odd = fmaf(u[t][r], 0.0f, odd);
     const bool one_by_one = __any(odd != odd);
-    if (lane == 0) s_odd[wave] = one_by_one;
-    if (!one_by_one) {
+    if (!LOCAL && lane == 0) s_odd[wave] = one_by_one;
+    if (!LOCAL && !one_by_one) {
       if constexpr (B16) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -789,7 +866,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
         for (int t = 0; t < NT; ++t) sU[64 * t + lane] = __builtin_bit_cast(u32x4_t, u[t]);
       }
     }
-    meet();  // S and U are there
+    if constexpr (!LOCAL) meet();  // S and U are there
     if (one_by_one) {
       T* out = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv;
       // Something is not finite; in the products 0 times it would reach
@@ -831,7 +908,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           }
         ks += __shfl_xor(ks, 16, 64);
         ks += __shfl_xor(ks, 32, 64);
-        const float w = beta * (v - ks);
+        const float w = beta * ((moves ? 0.0f : v) - ks);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -842,7 +919,7 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
           }
         qs += __shfl_xor(qs, 16, 64);
         qs += __shfl_xor(qs, 32, 64);
-        if (quad == 0 && j < a.dv) store1(out + (size_t)i * a.ld_out + j, qs * a.scale);
+        if (!LOCAL && quad == 0 && j < a.dv) store1(out + (size_t)i * a.ld_out + j, qs * a.scale);
       }
       continue;
     }
@@ -886,14 +963,95 @@ __global__ __launch_bounds__(128 * kWalkers) void delta_walk_kernel(DeltaArgs a)
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
     }
   }
-  if (!a.state_out) return;
+  if (!state_out) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = state_row<B16>(b, quad, r);
-      if (i < a.dk && j < a.dv) a.state_out[state0 + (size_t)i * a.dv + j] = S[b][r];
+      if (i < a.dk && j < width) state_out[(size_t)i * width + j] = S[b][r];
     }
+}
+
+// The scan over a sequence's segments: S goes to its transition times S plus
+// its own state; every segment's own state becomes its entry state, and the
+// last one's exit is the sequence's.  A workgroup takes 16 columns, a wave
+// every fourth 16 of the rows; products in fp32.  The next segment's matrices
+// are on their way meanwhile.
+template <int DKP>
+__global__ __launch_bounds__(256) void delta_scan_kernel(DeltaArgs a) {
+  constexpr int NB = DKP / 16, MINE = (NB + 3) / 4;
+  __shared__ f32x4_t s_state[2][NB * 64];  // as operands: lane l holds rows 16 b + 4 (l / 16) + r
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
+  const int j = blockIdx.x * 16 + col, head = a.head0 + blockIdx.y, seq = blockIdx.z;
+  const int item0 = a.uniform_len >= 0 ? seq * a.uniform_segs : first_item(a, seq);
+  const int item1 = a.uniform_len >= 0 ? item0 + a.uniform_segs : first_item(a, seq + 1);
+  const size_t state0 = ((size_t)seq * a.heads + head) * a.dk * a.dv;
+  auto own = [&](int item) { return a.seg_state + ((size_t)item * a.heads_here + blockIdx.y) * a.dk * a.dv; };
+  auto row_of = [&](int m, int r) { return 16 * (wave + 4 * m) + 4 * quad + r; };
+  f32x4_t S[MINE], B[MINE], M[MINE][NB];
+#pragma unroll
+  for (int m = 0; m < MINE; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      S[m][r] = a.state_in && row_of(m, r) < a.dk && j < a.dv ? a.state_in[state0 + (size_t)row_of(m, r) * a.dv + j] : 0.0f;
+  auto load = [&](int item) {
+    const float* move = a.seg_move + ((size_t)item * a.heads_here + blockIdx.y) * a.dk * a.dk;
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      const int row = 16 * (wave + 4 * m) + col;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int c = 16 * b + 4 * quad;
+        M[m][b] = row < a.dk && c < a.dk ? load4<float>(move + (size_t)row * a.dk + c, a.dk - c) : f32x4_t{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) B[m][r] = row_of(m, r) < a.dk && j < a.dv ? own(item)[(size_t)row_of(m, r) * a.dv + j] : 0.0f;
+    }
+  };
+  load(item0);
+  for (int item = item0; item < item1; ++item) {
+    f32x4_t* s = s_state[(item - item0) & 1];
+#pragma unroll
+    for (int m = 0; m < MINE; ++m)
+      if (wave + 4 * m < NB) s[64 * (wave + 4 * m) + lane] = S[m];
+    __syncthreads();
+    f32x4_t next[MINE];
+    bool keeps = false;  // a transition of zeros forgets whatever the state is
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      next[m] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) keeps |= M[m][b][r] != 0.0f;
+    }
+    if (__any(keeps)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const f32x4_t w = s[64 * b + lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int m = 0; m < MINE; ++m) next[m] = mfma32(M[m][b][r], w[r], next[m]);
+      }
+    }
+    float* entry = own(item);
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (row_of(m, r) < a.dk && j < a.dv) entry[(size_t)row_of(m, r) * a.dv + j] = S[m][r];
+      S[m] = next[m] + B[m];
+    }
+    if (item + 1 < item1) load(item + 1);
+  }
+  if (!a.state_out) return;
+#pragma unroll
+  for (int m = 0; m < MINE; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (row_of(m, r) < a.dk && j < a.dv) a.state_out[state0 + (size_t)row_of(m, r) * a.dv + j] = S[m][r];
 }
 
 // Rows at any element copied to rows of whole 16-byte units: heads of `width`
@@ -931,9 +1089,22 @@ Status launch_steps(hipStream_t stream, const DeltaArgs& a) {
 template <bool B16, int DKP>
 struct Chunked {
   static constexpr bool kBf16 = B16;
-  static constexpr size_t kLds = WalkLds<B16, DKP>::kBytes;
   static constexpr auto kAhead = &delta_ahead_kernel<B16, DKP>;
-  static constexpr auto kWalk = &delta_walk_kernel<B16, DKP>;
+  static constexpr auto kScan = &delta_scan_kernel<DKP>;
+  template <int MODE>
+  static Status walk(hipStream_t stream, const DeltaArgs& a) {
+    const dim3 grid((a.dv + 63) / 64 + (MODE == DR_LOCAL ? (a.dk + 63) / 64 : 0), a.heads_here, MODE == DR_WHOLE ? a.n_seqs : a.items);
+    delta_walk_kernel<B16, DKP, MODE>
+        <<<grid, 64 * (kWalkers + kHelpers<MODE>), WalkLds<B16, DKP, MODE == DR_LOCAL>::kBytes, stream>>>(a);
+    PSSA_LAUNCH_CHECK("delta_walk_kernel");
+    return Status::Ok();
+  }
+  template <int MODE>
+  static Status attributes() {
+    PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&delta_walk_kernel<B16, DKP, MODE>),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)WalkLds<B16, DKP, MODE == DR_LOCAL>::kBytes));
+    return Status::Ok();
+  }
 };
 template <class F>
 Status with_chunks(int dtype, int dk, F f) {
@@ -972,12 +1143,14 @@ int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ah
 
 // What is worked out ahead takes 13 KiB a chunk and head (bf16; 4 KiB fp32):
 // past 1 GiB of it the heads run in several launches.
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t heads, size_t d_key, size_t d_val) {
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items, size_t heads, size_t d_key, size_t d_val) {
   DeltaScratch s;
   const size_t size = dtype == PSSA_HIP_BF16 ? 2 : 4, unit = unit_of(dtype);
   const size_t one = chunks * 16 * (dtype == PSSA_HIP_BF16 ? Ahead<true>::kUnits : Ahead<false>::kUnits);
   s.heads_here = (int)std::max<size_t>(1, std::min(heads, ((size_t)1 << 30) / std::max<size_t>(one, 1)));
   s.ahead = (one * s.heads_here + 255) & ~(size_t)255;
+  s.state = (items * s.heads_here * d_key * d_val * 4 + 255) & ~(size_t)255;
+  s.move = (items * s.heads_here * d_key * d_key * 4 + 255) & ~(size_t)255;
   s.rows = 2 * ((tokens * heads * whole(d_key, unit) * size + 255) & ~(size_t)255) +
            ((tokens * heads * whole(d_val, unit) * size + 255) & ~(size_t)255);
   return s;
@@ -987,11 +1160,40 @@ Status init_delta_attributes() {
   for (int dtype : {PSSA_HIP_F32, PSSA_HIP_BF16})
     for (int dk : {32, 64, 128})
       PSSA_RETURN_IF(with_chunks(dtype, dk, [&](auto c) -> Status {
-        PSSA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(c.kWalk), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)c.kLds));
-        return Status::Ok();
+        PSSA_RETURN_IF(c.template attributes<DR_WHOLE>());
+        PSSA_RETURN_IF(c.template attributes<DR_LOCAL>());
+        return c.template attributes<DR_SEGMENT>();
       }));
   return Status::Ok();
+}
+
+// A walk's chunk takes about 3.1 us, one of a segment's own state 2.3 us, a
+// step of the scan over the segments 1.5 us, and the passes between some 12 us
+// (figures at the machine's 256 compute units, a workgroup each).  A call is
+// split where that makes it the faster, into segments of whichever length
+// costs least.
+constexpr size_t kComputeUnits = 256;
+int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val) {
+  const size_t chunk = (size_t)delta_chunk(dtype), most = (longest + chunk - 1) / chunk;
+  const size_t tiles = (d_val + 63) / 64, moves = (d_key + 63) / 64;
+  auto rounds = [](size_t n) { return (double)((n + kComputeUnits - 1) / kComputeUnits); };
+  auto items_of = [&](size_t seg) {
+    size_t items = 0;
+    for (size_t i = 0; i < (lens ? n_seqs : 1); ++i) items += std::max<size_t>(1, ((lens ? lens[i] : longest) + seg * chunk - 1) / (seg * chunk));
+    return lens ? items : items * n_seqs;
+  };
+  double best = rounds(n_seqs * heads * tiles) * most * 3.1;
+  int at = 0;
+  for (size_t seg = 2; 2 * seg <= most; seg += std::max<size_t>(1, seg / 4)) {
+    const size_t items = items_of(seg), steps = (most + seg - 1) / seg;
+    if (items > 65535) continue;
+    const double cost = rounds(items * heads * (tiles + moves)) * seg * 2.3 + steps * 1.5 + rounds(items * heads * tiles) * seg * 3.1 + 12;
+    if (cost < best) {
+      best = cost;
+      at = (int)seg;
+    }
+  }
+  return at;
 }
 
 Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t tokens, int longest, const DeltaScratch& s,
@@ -999,6 +1201,8 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
   if (longest <= kDeltaSteps)
     return dtype == PSSA_HIP_F32 ? launch_steps<float>(stream, a) : launch_steps<Bf16>(stream, a);
   a.ahead = scratch;
+  a.seg_state = reinterpret_cast<float*>(scratch + s.ahead + s.rows);
+  a.seg_move = reinterpret_cast<float*>(scratch + s.ahead + s.rows + s.state);
   char* rows = scratch + s.ahead;
   const size_t unit = unit_of(dtype);
   const bool b16 = dtype == PSSA_HIP_BF16;
@@ -1016,8 +1220,14 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
       a.heads_here = std::min(s.heads_here, a.heads - a.head0);
       c.kAhead<<<dim3(a.chunks, a.heads_here), c.kBf16 ? 256 : 128, 0, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_ahead_kernel");
-      c.kWalk<<<dim3((a.dv + 63) / 64, a.heads_here, a.n_seqs), 128 * kWalkers, c.kLds, stream>>>(a);
-      PSSA_LAUNCH_CHECK("delta_walk_kernel");
+      if (!a.seg_chunks) {
+        PSSA_RETURN_IF(c.template walk<DR_WHOLE>(stream, a));
+        continue;
+      }
+      PSSA_RETURN_IF(c.template walk<DR_LOCAL>(stream, a));
+      c.kScan<<<dim3((a.dv + 15) / 16, a.heads_here, a.n_seqs), 256, 0, stream>>>(a);
+      PSSA_LAUNCH_CHECK("delta_scan_kernel");
+      PSSA_RETURN_IF(c.template walk<DR_SEGMENT>(stream, a));
     }
     return Status::Ok();
   });

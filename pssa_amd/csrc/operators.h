@@ -147,20 +147,28 @@ struct DeltaArgs {
   char* ahead = nullptr;
   int head0 = 0, heads_here = 0, chunks = 0;
   int wide_q = 0, wide_k = 0, wide_v = 0;  // elements from a head to the next in rows that may be copies
-  // [n_seqs + 1] first tokens and, behind them, first chunks: on the device, or null and here.
+  // The work items: whole sequences, or (split) their segments of seg_chunks
+  // chunks, whose own states and transitions are [items, heads of one launch].
+  int items = 0, seg_chunks = 0, uniform_segs = 1;
+  float *seg_state = nullptr, *seg_move = nullptr;
+  // [n_seqs + 1] first tokens, behind them first chunks and, in a split call,
+  // first items: on the device, or null and here.
   const uint32_t* table = nullptr;
   uint32_t inline_tokens[kDeltaInline + 1] = {};
   uint32_t inline_chunks[kDeltaInline + 1] = {};
+  uint32_t inline_items[kDeltaInline + 1] = {};
 };
 // Tokens of a chunk of a type, and the scratch of a call: what is worked out
 // ahead for the heads of one launch, and copies of rows that do not lie in
 // units of 16 bytes.
 int delta_chunk(int dtype);
 struct DeltaScratch {
-  size_t ahead = 0, rows = 0;  // bytes
-  int heads_here = 0;          // heads of a launch
+  size_t ahead = 0, rows = 0, state = 0, move = 0;  // bytes
+  int heads_here = 0;                               // heads of a launch
 };
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t heads, size_t d_key, size_t d_val);
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items, size_t heads, size_t d_key, size_t d_val);
+// Chunks of a segment where a call of these sizes is split, else 0.
+int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val);
 Status init_delta_attributes();
 Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t tokens, int longest, const DeltaScratch& s,
                          char* scratch);

@@ -430,6 +430,31 @@ def test_delta_rule_values_that_are_not_finite(hip, dtype, what, n, at):
         assert np.isfinite(S[1]).all() and np.isfinite(np.delete(S[0, 1], col, 1)).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,heads,key_heads,dk,dv", [([3000], 1, 1, 64, 64), ([2177], 2, 1, 128, 72), ([1300, 1300], 1, 1, 32, 40),
+                                                        ([1700, 3, 0, 900, 64], 2, 2, 64, 64), ([1601], 1, 1, 100, 130)])
+def test_delta_rule_in_segments(hip, dtype, lens, heads, key_heads, dk, dv):
+    """Few long walks are split; a forgotten state is forgotten across segments, and a NaN stays behind its token."""
+    say("segments", dtype, lens, heads, dk, dv)
+    rng = np.random.default_rng(sum(lens))
+    c = delta_case(rng, lens, heads, key_heads, dk, dv, True, pace=0.01)
+    c["g"][lens[0] // 2] = -np.inf
+    check_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, reserve=True)
+    check_delta(hip, delta_case(rng, lens, heads, key_heads, dk, dv, False, pace=0.1), lens, heads, key_heads, dk, dv, dtype,
+                layout="row")
+    clean = run_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, 1.0)
+    at, again = lens[0] // 3, lens[0] // 2
+    c["v"][at, 0, 1] = np.nan
+    c["state"][0, 0, 0, 0] = np.nan
+    out = run_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, 1.0)
+    bad = np.zeros(clean[3].shape, bool)
+    bad[at:again, 0, 1] = bad[:again, 0, 0] = True  # what is forgotten is no more
+    np.testing.assert_array_equal(np.isnan(out[3]), bad)
+    assert np.isfinite(out[4]).all()
+    scale = np.abs(clean[3]).max()
+    assert np.abs(out[3] - clean[3])[~bad].max() <= scale * ((U16 * 2 if dtype == "bf16" else 0) + delta_steps(dk, dtype) * 64 * U32)
+
+
 def test_delta_rule_single_tokens_continue_a_prompt(hip):
     """A prompt, then single tokens from its state, equal the whole sequence."""
     rng = np.random.default_rng(13)
