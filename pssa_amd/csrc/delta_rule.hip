@@ -496,26 +496,30 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_walk[];
   const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = in_all % kWalkers;
   const int col = lane & 15, quad = lane >> 4;
-  const int head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads);
-  const Walk<C> wk = walk_of<C, MODE>(a, blockIdx.z);
-  const Span sp = wk.span;
   // The columns: of the values, or (behind them) of the transition.
-  const int tiles_v = (a.dv + 63) / 64;
-  const bool moves = LOCAL && (int)blockIdx.x >= tiles_v;
-  const int dv0 = 64 * ((int)blockIdx.x - (moves ? tiles_v : 0)), width = moves ? a.dk : a.dv;
-  const size_t item_head = (size_t)blockIdx.z * a.heads_here + blockIdx.y;
-  const float* state_in = MODE == DR_WHOLE     ? a.state_in ? a.state_in + ((size_t)wk.seq * a.heads + head) * a.dk * a.dv : nullptr
-                          : MODE == DR_SEGMENT ? a.seg_state + item_head * a.dk * a.dv
-                                               : nullptr;
-  float* state_out = MODE == DR_WHOLE   ? a.state_out ? a.state_out + ((size_t)wk.seq * a.heads + head) * a.dk * a.dv : nullptr
-                     : MODE == DR_LOCAL ? (moves ? a.seg_move + item_head * a.dk * a.dk : a.seg_state + item_head * a.dk * a.dv)
-                                        : nullptr;
+  const int tiles_v = (a.dv + 63) / 64, tiles = tiles_v + (LOCAL ? (a.dk + 63) / 64 : 0);
+  // Workgroups of one item that read the same keys follow one another on one
+  // of the eight XCDs, so that its L2 has them once.
+  const int shared = a.share * tiles, slot = blockIdx.x / 8, group = slot / shared * 8 + blockIdx.x % 8;
+  const int key_groups = a.heads_here / a.share, item = group / key_groups;
+  if (item >= (MODE == DR_WHOLE ? a.n_seqs : a.items)) return;
+  const int tile = slot % shared % tiles, head_here = group % key_groups * a.share + slot % shared / tiles;
+  const int head = a.head0 + head_here, key_head = head / (a.heads / a.key_heads);
+  const Walk<C> wk = walk_of<C, MODE>(a, item);
+  const Span sp = wk.span;
+  const bool moves = LOCAL && tile >= tiles_v;
+  const int dv0 = 64 * (tile - (moves ? tiles_v : 0));
+  const size_t item_head = (size_t)item * a.heads_here + head_here;
+  // The state's element at the lane's first row and its column; the others are whole rows further.
+  const size_t state0 = (((size_t)wk.seq * a.heads + head) * a.dk + state_row<B16>(0, quad, 0)) * a.dv + dv0 + 16 * wave + col;
+  // A segment's state lies as the waves hold it: [16 columns][tile][lane].
+  f32x4_t* seg_state = reinterpret_cast<f32x4_t*>(a.seg_state) + (item_head * ((a.dv + 15) / 16) + dv0 / 16 + wave) * NB * 64 + lane;
   const int j = dv0 + 16 * wave + col;  // the lane's column
 
   auto issue = [&](int pos, int n, u32x4_t* buffer) {
     const size_t tok = sp.tok + pos;
     const u32x4_t* ahead = reinterpret_cast<const u32x4_t*>(a.ahead) +
-                           ((size_t)(wk.chunk0 + pos / C) * a.heads_here + blockIdx.y) * In::kUnits;
+                           ((size_t)(wk.chunk0 + pos / C) * a.heads_here + head_here) * In::kUnits;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int load = i * HELPERS + in_all - kWalkers;
@@ -732,14 +736,20 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
   // S: the rows of the lane's column.
   f32x4_t S[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
+    if constexpr (MODE == DR_SEGMENT) {
+      S[b] = dv0 + 16 * wave < a.dv ? seg_state[64 * b] : f32x4_t{0, 0, 0, 0};
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = state_row<B16>(b, quad, r);
-      S[b][r] = moves                                    ? (i == j && i < a.dk ? 1.0f : 0.0f)
-                : state_in && i < a.dk && j < a.dv ? state_in[(size_t)i * a.dv + j]
-                                                   : 0.0f;
+      for (int r = 0; r < 4; ++r) {
+        const int i = state_row<B16>(b, quad, r);
+        if constexpr (LOCAL)
+          S[b][r] = moves && i == j && i < a.dk ? 1.0f : 0.0f;
+        else
+          S[b][r] = a.state_in && i < a.dk && j < a.dv ? (a.state_in + state0)[(size_t)state_row<B16>(b, 0, r) * a.dv] : 0.0f;
+      }
     }
+  }
   const u32x4_t* buffer = s_walk;
   for (int pos = 0; pos < sp.len; pos += C) {
     const int n = min(C, sp.len - pos);
@@ -963,95 +973,127 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
     }
   }
-  if (!state_out) return;
+  if (LOCAL && moves) {  // whole rows and columns, zeros past d_key
+    float* move = a.seg_move + item_head * DKP * DKP + j;
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = state_row<B16>(b, quad, r);
-      if (i < a.dk && j < width) state_out[(size_t)i * width + j] = S[b][r];
-    }
+      for (int r = 0; r < 4; ++r)
+        if (j < DKP) move[state_row<B16>(b, quad, r) * DKP] = S[b][r];
+  } else if (LOCAL) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (dv0 + 16 * wave < a.dv) seg_state[64 * b] = S[b];
+  } else if (MODE == DR_WHOLE && a.state_out) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = state_row<B16>(b, quad, r);
+        if (i < a.dk && j < a.dv) (a.state_out + state0)[(size_t)state_row<B16>(b, 0, r) * a.dv] = S[b][r];
+      }
+  }
 }
 
 // The scan over a sequence's segments: S goes to its transition times S plus
 // its own state; every segment's own state becomes its entry state, and the
-// last one's exit is the sequence's.  A workgroup takes 16 columns, a wave
-// every fourth 16 of the rows; products in fp32.  The next segment's matrices
-// are on their way meanwhile.
+// last one's exit is the sequence's.  A workgroup takes 16 columns, a wave one
+// of the state's tiles; products in fp32.  The matrices of the next segments
+// are on their way meanwhile; a step of 128 x 128 still takes 2.7 us, in which
+// a compute unit reads its 64 KiB (25 bytes a ns).
 template <int DKP>
-__global__ __launch_bounds__(256) void delta_scan_kernel(DeltaArgs a) {
-  constexpr int NB = DKP / 16, MINE = (NB + 3) / 4;
-  __shared__ f32x4_t s_state[2][NB * 64];  // as operands: lane l holds rows 16 b + 4 (l / 16) + r
+constexpr int kScanWaves = DKP / 16;
+template <bool B16, int DKP>
+__global__ __launch_bounds__(64 * kScanWaves<DKP>) void delta_scan_kernel(DeltaArgs a) {
+  constexpr int NB = DKP / 16, WAVES = kScanWaves<DKP>, MINE = NB / WAVES;
+  __shared__ f32x4_t s_state[2][NB * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   const int j = blockIdx.x * 16 + col, head = a.head0 + blockIdx.y, seq = blockIdx.z;
   const int item0 = a.uniform_len >= 0 ? seq * a.uniform_segs : first_item(a, seq);
   const int item1 = a.uniform_len >= 0 ? item0 + a.uniform_segs : first_item(a, seq + 1);
   const size_t state0 = ((size_t)seq * a.heads + head) * a.dk * a.dv;
-  auto own = [&](int item) { return a.seg_state + ((size_t)item * a.heads_here + blockIdx.y) * a.dk * a.dv; };
-  auto row_of = [&](int m, int r) { return 16 * (wave + 4 * m) + 4 * quad + r; };
-  f32x4_t S[MINE], B[MINE], M[MINE][NB];
+  const size_t own_step = (size_t)a.heads_here * gridDim.x * NB * 64, move_step = (size_t)a.heads_here * DKP * DKP;
+  f32x4_t* own = reinterpret_cast<f32x4_t*>(a.seg_state) + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * NB * 64 + lane;
+  const float* move = a.seg_move + (size_t)blockIdx.y * DKP * DKP;
+  struct Part {
+    f32x4_t own[MINE], move[MINE][NB];
+  };
+  f32x4_t S[MINE];
 #pragma unroll
   for (int m = 0; m < MINE; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      S[m][r] = a.state_in && row_of(m, r) < a.dk && j < a.dv ? a.state_in[state0 + (size_t)row_of(m, r) * a.dv + j] : 0.0f;
-  auto load = [&](int item) {
-    const float* move = a.seg_move + ((size_t)item * a.heads_here + blockIdx.y) * a.dk * a.dk;
+    for (int r = 0; r < 4; ++r) {
+      const int i = state_row<B16>(wave + WAVES * m, quad, r);
+      S[m][r] = a.state_in && i < a.dk && j < a.dv ? a.state_in[state0 + (size_t)i * a.dv + j] : 0.0f;
+    }
+  auto load = [&](int item, Part& p) {
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
-      const int row = 16 * (wave + 4 * m) + col;
+      const int b = wave + WAVES * m;
+      p.own[m] = own[item * own_step + 64 * b];
+      // Operands: the lane's row of tile b, columns as a tile's rows lie.
+      const float* row = move + item * move_step + state_row<B16>(b, col >> 2, col & 3) * DKP;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int c = 16 * b + 4 * quad;
-        M[m][b] = row < a.dk && c < a.dk ? load4<float>(move + (size_t)row * a.dk + c, a.dk - c) : f32x4_t{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) B[m][r] = row_of(m, r) < a.dk && j < a.dv ? own(item)[(size_t)row_of(m, r) * a.dv + j] : 0.0f;
+      for (int k = 0; k < NB; ++k) p.move[m][k] = *reinterpret_cast<const f32x4_t*>(row + state_row<B16>(k, quad, 0));
     }
   };
-  load(item0);
-  for (int item = item0; item < item1; ++item) {
+  auto step = [&](int item, const Part& p) {
     f32x4_t* s = s_state[(item - item0) & 1];
 #pragma unroll
-    for (int m = 0; m < MINE; ++m)
-      if (wave + 4 * m < NB) s[64 * (wave + 4 * m) + lane] = S[m];
-    __syncthreads();
+    for (int m = 0; m < MINE; ++m) s[64 * (wave + WAVES * m) + lane] = S[m];
+    asm volatile("" ::: "memory");  // the next segment's loads stay in flight
+    __builtin_amdgcn_s_waitcnt(kLdsOnly);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     f32x4_t next[MINE];
-    bool keeps = false;  // a transition of zeros forgets whatever the state is
+    uint32_t keeps = 0;  // a transition of zeros forgets whatever the state is
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
       next[m] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int k = 0; k < NB; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) keeps |= M[m][b][r] != 0.0f;
+        for (int r = 0; r < 4; ++r) keeps |= __float_as_uint(p.move[m][k][r]) << 1;
     }
-    if (__any(keeps)) {
+    if (__any(keeps != 0)) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const f32x4_t w = s[64 * b + lane];
+      for (int k = 0; k < NB; ++k) {
+        const f32x4_t w = s[64 * k + lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int m = 0; m < MINE; ++m) next[m] = mfma32(M[m][b][r], w[r], next[m]);
+          for (int m = 0; m < MINE; ++m) next[m] = mfma32(p.move[m][k][r], w[r], next[m]);
       }
     }
-    float* entry = own(item);
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (row_of(m, r) < a.dk && j < a.dv) entry[(size_t)row_of(m, r) * a.dv + j] = S[m][r];
-      S[m] = next[m] + B[m];
+      own[item * own_step + 64 * (wave + WAVES * m)] = S[m];
+      S[m] = next[m] + p.own[m];
     }
-    if (item + 1 < item1) load(item + 1);
+  };
+  constexpr int DEEP = DKP == 128 ? 3 : 4;
+  Part p[DEEP];
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d) load(min(item0 + d, item1 - 1), p[d]);
+  int item = item0;
+  for (; item + DEEP <= item1; item += DEEP) {
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      step(item + d, p[d]);
+      load(min(item + d + DEEP, item1 - 1), p[d]);
+    }
   }
+#pragma unroll
+  for (int d = 0; d < DEEP - 1; ++d)
+    if (item + d < item1) step(item + d, p[d]);
   if (!a.state_out) return;
 #pragma unroll
   for (int m = 0; m < MINE; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (row_of(m, r) < a.dk && j < a.dv) a.state_out[state0 + (size_t)row_of(m, r) * a.dv + j] = S[m][r];
+    for (int r = 0; r < 4; ++r) {
+      const int i = state_row<B16>(wave + WAVES * m, quad, r);
+      if (i < a.dk && j < a.dv) a.state_out[state0 + (size_t)i * a.dv + j] = S[m][r];
+    }
 }
 
 // Rows at any element copied to rows of whole 16-byte units: heads of `width`
@@ -1090,10 +1132,13 @@ template <bool B16, int DKP>
 struct Chunked {
   static constexpr bool kBf16 = B16;
   static constexpr auto kAhead = &delta_ahead_kernel<B16, DKP>;
-  static constexpr auto kScan = &delta_scan_kernel<DKP>;
+  static constexpr auto kScan = &delta_scan_kernel<B16, DKP>;
+  static constexpr int kScanThreads = 64 * kScanWaves<DKP>;
   template <int MODE>
   static Status walk(hipStream_t stream, const DeltaArgs& a) {
-    const dim3 grid((a.dv + 63) / 64 + (MODE == DR_LOCAL ? (a.dk + 63) / 64 : 0), a.heads_here, MODE == DR_WHOLE ? a.n_seqs : a.items);
+    const size_t shared = (size_t)a.share * ((a.dv + 63) / 64 + (MODE == DR_LOCAL ? (a.dk + 63) / 64 : 0));
+    const size_t groups = (size_t)(MODE == DR_WHOLE ? a.n_seqs : a.items) * (a.heads_here / a.share);
+    const uint32_t grid = (uint32_t)((groups + 7) / 8 * 8 * shared);
     delta_walk_kernel<B16, DKP, MODE>
         <<<grid, 64 * (kWalkers + kHelpers<MODE>), WalkLds<B16, DKP, MODE == DR_LOCAL>::kBytes, stream>>>(a);
     PSSA_LAUNCH_CHECK("delta_walk_kernel");
@@ -1149,8 +1194,9 @@ DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items
   const size_t one = chunks * 16 * (dtype == PSSA_HIP_BF16 ? Ahead<true>::kUnits : Ahead<false>::kUnits);
   s.heads_here = (int)std::max<size_t>(1, std::min(heads, ((size_t)1 << 30) / std::max<size_t>(one, 1)));
   s.ahead = (one * s.heads_here + 255) & ~(size_t)255;
-  s.state = (items * s.heads_here * d_key * d_val * 4 + 255) & ~(size_t)255;
-  s.move = (items * s.heads_here * d_key * d_key * 4 + 255) & ~(size_t)255;
+  const size_t keys = d_key <= 32 ? 32 : d_key <= 64 ? 64 : 128;  // as the kernels hold them
+  s.state = items * s.heads_here * keys * whole(d_val, 16) * 4;
+  s.move = items * s.heads_here * keys * keys * 4;
   s.rows = 2 * ((tokens * heads * whole(d_key, unit) * size + 255) & ~(size_t)255) +
            ((tokens * heads * whole(d_val, unit) * size + 255) & ~(size_t)255);
   return s;
@@ -1218,6 +1264,8 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
   return with_chunks(dtype, a.dk, [&](auto c) -> Status {
     for (a.head0 = 0; a.head0 < a.heads; a.head0 += s.heads_here) {
       a.heads_here = std::min(s.heads_here, a.heads - a.head0);
+      const int rep = a.heads / a.key_heads;  // heads of the same keys
+      a.share = a.head0 % rep == 0 && a.heads_here % rep == 0 ? rep : 1;
       c.kAhead<<<dim3(a.chunks, a.heads_here), c.kBf16 ? 256 : 128, 0, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_ahead_kernel");
       if (!a.seg_chunks) {
@@ -1225,7 +1273,7 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
         continue;
       }
       PSSA_RETURN_IF(c.template walk<DR_LOCAL>(stream, a));
-      c.kScan<<<dim3((a.dv + 15) / 16, a.heads_here, a.n_seqs), 256, 0, stream>>>(a);
+      c.kScan<<<dim3((a.dv + 15) / 16, a.heads_here, a.n_seqs), c.kScanThreads, 0, stream>>>(a);
       PSSA_LAUNCH_CHECK("delta_scan_kernel");
       PSSA_RETURN_IF(c.template walk<DR_SEGMENT>(stream, a));
     }

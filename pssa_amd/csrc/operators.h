@@ -146,6 +146,7 @@ struct DeltaArgs {
   // [chunks, heads of one launch], and the launch's first head.
   char* ahead = nullptr;
   int head0 = 0, heads_here = 0, chunks = 0;
+  int share = 1;  // neighbouring heads of the launch that read the same keys
   int wide_q = 0, wide_k = 0, wide_v = 0;  // elements from a head to the next in rows that may be copies
   // The work items: whole sequences, or (split) their segments of seg_chunks
   // chunks, whose own states and transitions are [items, heads of one launch].
