@@ -473,26 +473,25 @@ __device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
 }
 
 // The walk of a sequence, a head and 64 value columns through its chunks. Four
-// waves, 16 columns each, go from S to the next S; four others bring the next
-// chunk, work out P and turn the S and U that they are handed into outputs, so
-// that nothing but the states' own chain runs from chunk to chunk (where the
-// same waves did all, issuing the loads alone took 2.3 of a chunk's 5.7 us,
-// heads of 128).
+// waves, 16 columns each, go from S to the next S; four bring the next chunk,
+// four turn the S and U that they are handed into outputs, and these eight
+// work out P, so that nothing but the states' own chain runs from chunk to
+// chunk (where the same waves did all, issuing the loads alone took 2.3 of a
+// chunk's 5.7 us, heads of 128).
 // A segment's own state and its transition need no outputs, and two waves bring
 // their chunks, so that two workgroups fit a compute unit.  The transition is
 // the state that the unit matrix becomes without values: more columns.
 constexpr int kWalkers = 4;
 template <int MODE>
-constexpr int kHelpers = MODE == DR_LOCAL ? 2 : 4;
+constexpr int kHelpers = MODE == DR_LOCAL ? 2 : 8;
 template <bool B16, int DKP, int MODE>
 __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_kernel(DeltaArgs a) {
   constexpr bool LOCAL = MODE == DR_LOCAL;
-  constexpr int HELPERS = kHelpers<MODE>;
   using In = Ahead<B16>;
   using Lds = WalkLds<B16, DKP, LOCAL>;
   using T = std::conditional_t<B16, Bf16, float>;
   constexpr int C = In::C, NT = In::kTiles, NB = DKP / 16, N = Lds::N;
-  constexpr int LOADS = Lds::kBuffer / 64, PER = (LOADS + HELPERS - 1) / HELPERS;
+  constexpr int BRING = LOCAL ? 2 : 4, LOADS = Lds::kBuffer / 64, PER = (LOADS + BRING - 1) / BRING;
   extern __shared__ __attribute__((aligned(256))) u32x4_t s_walk[];
   const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = in_all % kWalkers;
   const int col = lane & 15, quad = lane >> 4;
@@ -522,8 +521,8 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
                            ((size_t)(wk.chunk0 + pos / C) * a.heads_here + head_here) * In::kUnits;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int load = i * HELPERS + in_all - kWalkers;
-      if (LOADS % HELPERS != 0 && load >= LOADS) continue;
+      const int load = i * BRING + in_all - kWalkers;
+      if (LOADS % BRING != 0 && load >= LOADS) continue;
       const int at = load * 64;  // first unit
       const bool is_k = at < Lds::kK, is_q = !is_k && at < Lds::kK + Lds::kQ, is_v = !is_k && !is_q && at < Lds::kK + Lds::kQ + Lds::kV;
       const void* src;
@@ -582,56 +581,26 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
           reinterpret_cast<u32x2_t*>(sP + In::kFrag * pair_of<B16>(2 * wave, wave) + 64 * part + lane)[1] = u32x2_t{0, 0};
       }
     }
-    // A chunk's outputs, tokens 16 t + col by columns 16 wave + 4 quad .., leave
-    // in the next one's course: every memory operation of a chunk has to end
-    // before the next begins.
-    std::conditional_t<B16, u32x2_t, f32x4_t> held[NT];
-    int held_n = 0;
-    const int c_out = dv0 + 16 * wave + 4 * quad;
-    auto put = [&](int pos) {
-      typedef std::conditional_t<B16, u32x2_any_t, f32x4_any_t> any_t;
-      T* dst = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv + (__umul24(col, (uint32_t)a.ld_out) + c_out);
-      if (held_n == C && dv0 + 64 <= a.dv) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) *reinterpret_cast<any_t*>(dst + (size_t)(16 * t) * a.ld_out) = held[t];
-        return;
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (16 * t + col >= held_n || c_out >= a.dv) continue;
-        T* to = dst + (size_t)(16 * t) * a.ld_out;
-        if (c_out + 4 <= a.dv) {
-          *reinterpret_cast<any_t*>(to) = held[t];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 3; ++e) {
-            if (c_out + e >= a.dv) continue;
-            if constexpr (B16)
-              to[e].bits = (uint16_t)(held[t][e >> 1] >> (16 * (e & 1)));
-            else
-              to[e] = held[t][e];
-          }
-        }
-      }
-    };
+    const int helper = in_all - kWalkers;
+    const bool brings = helper < 4;
     const u32x4_t* buffer = s_walk;
-    if (sp.len > 0) issue(0, min(C, sp.len), s_walk);
+    if (brings && sp.len > 0) issue(0, min(C, sp.len), s_walk);
     for (int pos = 0; pos < sp.len; pos += C) {
       const int n = min(C, sp.len - pos);
-      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      if (brings) __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
       meet();  // the chunk is there, and the one before is read
       const u32x4_t *sK = buffer, *sQ = sK + Lds::kK, *sV = sQ + Lds::kQ, *sT = sV + Lds::kV;
       const float* gamma = reinterpret_cast<const float*>(sT + In::kGamma);
       const double* sum = reinterpret_cast<const double*>(sT + In::kSum);
       u32x4_t* other = buffer == s_walk ? s_walk + Lds::kBuffer : s_walk;
       buffer = other;
-      if (pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), other);
-      put(pos - held_n);
-      held_n = 0;
+      if (brings && pos + C < sp.len) issue(pos + C, min(C, sp.len - pos - C), other);
       // P^T: queries 16 r + col, keys 16 c + 4 quad + e.
 #pragma unroll
-      for (int i = 0; i < (NT * (NT + 1) / 2 + 3) / 4; ++i) {
-        const int at = min(4 * i + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
+      for (int i = 0; i < (NT * (NT + 1) / 2 + 7) / 8; ++i) {
+        // The waves that bring nothing take the second round.
+        const int at = i ? 8 + helper - 4 : helper, r = triangle_row(at), c = triangle_col(at);
+        if (at < 8 * i || at >= NT * (NT + 1) / 2) continue;  // uniform
         f32x4_t p = tile_product<B16, DKP>(sK, 16 * c, sQ, 16 * r, lane);
         const double gq = sum[16 * r + col];
         float d[4];
@@ -659,7 +628,7 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
         }
       }
       meet();  // P, S and U are there
-      if (s_odd[wave]) continue;  // uniform: the other wave stores these
+      if (brings || s_odd[wave]) continue;  // uniform; odd: the walking wave stores these
       // O^T = scale e^G (Q S)^T + (P U)^T.
       f32x4_t o[NT];
 #pragma unroll
@@ -721,16 +690,33 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
             for (int r = 0; r < 4; ++r) o[t] = mfma32(u[h][r], pf[r], o[t]);
           }
       }
-      held_n = n;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      // Tokens 16 t + col, columns 16 wave + 4 quad ..
+      const int c = dv0 + 16 * wave + 4 * quad;
+      T* dst = static_cast<T*>(a.out) + (sp.tok + pos) * a.ld_out + (size_t)head * a.dv + (__umul24(col, (uint32_t)a.ld_out) + c);
+      auto store = [&](T* to, const f32x4_t& v) {
         if constexpr (B16)
-          held[t] = u32x2_t{bf16x2_bits(o[t][0], o[t][1]), bf16x2_bits(o[t][2], o[t][3])};
+          *reinterpret_cast<u32x2_any_t*>(to) = u32x2_t{bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3])};
         else
-          held[t] = o[t];
+          *reinterpret_cast<f32x4_any_t*>(to) = v;
+      };
+      if (n == C && dv0 + 64 <= a.dv) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) store(dst + (size_t)(16 * t) * a.ld_out, o[t]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (16 * t + col >= n || c >= a.dv) continue;
+          T* to = dst + (size_t)(16 * t) * a.ld_out;
+          if (c + 4 <= a.dv) {
+            store(to, o[t]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (c + e < a.dv) store1(to + e, o[t][e]);
+          }
+        }
       }
     }
-    put(sp.len - held_n);
     return;
   }
   // S: the rows of the lane's column.
