@@ -16,6 +16,8 @@ namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
 // Rows start at any element.
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 typedef u32x2_t u32x2_any_t __attribute__((aligned(1)));
@@ -27,12 +29,6 @@ struct Bf16 {
 template <class T>
 constexpr int vec_n() { return 16 / (int)sizeof(T); }
 
-template <class T>
-__device__ __forceinline__ float load1(const T* p);
-template <>
-__device__ __forceinline__ float load1<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float load1<Bf16>(const Bf16* p) { return __uint_as_float((uint32_t)p->bits << 16); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(Bf16* p, float v) { p->bits = bf16_bits_dev(v); }
 
@@ -46,16 +42,21 @@ __device__ __forceinline__ void widen(u32x4_t u, float (&v)[vec_n<T>()]) {
       v[j] = __uint_as_float(j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
   }
 }
-// Elements c .. of a row: N of them, or the `left` that there are, then zeros.
+// Elements c .. of a row: a piece of them, or the `left` that there are, then zeros.
 template <class T>
-__device__ __forceinline__ void load_vec(const T* row, int c, int left, float (&v)[vec_n<T>()]) {
+__device__ __forceinline__ u32x4_t load_piece(const T* row, int c, int left) {
   constexpr int N = vec_n<T>();
-  if (left >= N) {
-    widen<T>(*reinterpret_cast<const u32x4_any_t*>(row + c), v);
-  } else {
+  if (left >= N) return *reinterpret_cast<const u32x4_any_t*>(row + c);
+  u32x4_t u = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = j < left ? load1<T>(row + c + j) : 0.0f;
+  for (int j = 0; j < N; ++j) {
+    if (j >= left) continue;
+    if constexpr (sizeof(T) == 4)
+      u[j] = __float_as_uint(row[c + j]);
+    else
+      u[j >> 1] |= (uint32_t)row[c + j].bits << (16 * (j & 1));
   }
+  return u;
 }
 template <class T>
 __device__ __forceinline__ void store_vec(T* row, int c, int left, const float (&v)[vec_n<T>()]) {
@@ -121,117 +122,163 @@ __device__ __forceinline__ void row_reduce(float& sum, float& most, float (*s_pa
 }
 
 // W waves hold a row, NV pieces a thread; where a row takes one wave, four of
-// them share a workgroup.
+// them share a workgroup.  A workgroup goes through several rows: gamma stays
+// in its registers, and the next row is on its way while one is summed.
 template <class T, int W, int NV>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNormArgs a, int rows) {
-  constexpr int N = vec_n<T>();
+  constexpr int N = vec_n<T>(), PER = W == 1 ? 4 : 1;  // rows of a workgroup at a time
+  constexpr bool kAhead = NV * N <= 32 && W < 16;      // registers for gamma and a second row
   __shared__ float s_part[W][2];
-  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (W == 1 && r >= rows) return;  // a wave of its own: no barrier follows
-  const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const T* x = static_cast<const T*>(a.x) + (size_t)r * a.ld_x;
-  const T* res = static_cast<const T*>(a.residual) + (a.residual ? (size_t)r * a.ld_residual : 0);
-
-  float h[NV][N];
+  int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+  int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  float gamma[kAhead ? NV : 1][N];
+  auto gamma_of = [&](int k, float (&g)[N]) {
+    const int c = (tid + k * 64 * W) * N;
+    if (a.gamma && c + N <= a.width) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (tid + k * 64 * W) * N, left = a.width - c;
-    load_vec<T>(x, c, left, h[k]);
-  }
-  if (a.residual) {
+      for (int j4 = 0; j4 < N; j4 += 4) {
+        const f32x4_t v = *reinterpret_cast<const f32x4_any_t*>(a.gamma + c + j4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[j4 + e] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) g[j] = c + j >= a.width ? 0.0f : a.gamma ? a.gamma[c + j] : 1.0f;
+    }
+  };
+  u32x4_t next[kAhead ? NV : 1], next_res[kAhead ? NV : 1];
+  auto fetch = [&](int row) {
+    const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ld_x;
+    const T* res = static_cast<const T*>(a.residual) + (size_t)row * a.ld_residual;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * 64 * W) * N, left = a.width - c;
-      float v[N];
-      load_vec<T>(res, c, left, v);
-#pragma unroll
-      for (int j = 0; j < N; ++j) h[k][j] += v[j];
+      const int c = (tid + k * 64 * W) * N;
+      next[kAhead ? k : 0] = load_piece<T>(x, c, a.width - c);
     }
+    if (a.residual) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * 64 * W) * N;
+        next_res[kAhead ? k : 0] = load_piece<T>(res, c, a.width - c);
+      }
+    }
+  };
+  if constexpr (kAhead) {
+    if (r < rows) fetch(r);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) gamma_of(k, gamma[k]);
   }
-  // The sum of squares; the largest |gamma h|, infinite where one is not a
-  // number (a maximum passes over it).
-  float ss = 0.0f, most = 0.0f;
+  for (; r < rows; r += PER * gridDim.x) {
+    // New for the compiler with each row: addresses kept for all pieces would take more registers than the row.
+    if constexpr (!kAhead) asm volatile("" : "+v"(tid));
+    float h[NV][N];
+    const T* x = static_cast<const T*>(a.x) + (size_t)r * a.ld_x;
+    const T* res = static_cast<const T*>(a.residual) + (size_t)r * a.ld_residual;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (tid + k * 64 * W) * N, left = a.width - c;
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * 64 * W) * N;
+      widen<T>(kAhead ? next[kAhead ? k : 0] : load_piece<T>(x, c, a.width - c), h[k]);
+    }
+    if (a.residual) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) ss = fmaf(h[k][j], h[k][j], ss);
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * 64 * W) * N;
+        float v[N];
+        widen<T>(kAhead ? next_res[kAhead ? k : 0] : load_piece<T>(res, c, a.width - c), v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[k][j] += v[j];
+      }
+    }
+    if constexpr (kAhead) {
+      const int r_next = r + PER * (int)gridDim.x;
+      if (r_next < rows) fetch(r_next);
+    }
+    // The sum of squares; the largest |gamma h|, infinite where one is not a
+    // number (a maximum passes over it).
+    float ss = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) ss = fmaf(h[k][j], h[k][j], ss);
+      if (a.codes) {
+        float g[N];
+        if constexpr (!kAhead) gamma_of(k, g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float t = fabsf(h[k][j] * (kAhead ? gamma[kAhead ? k : 0][j] : g[j]));
+          most = fmaxf(most, t < INFINITY ? t : INFINITY);
+        }
+      }
+    }
+    row_reduce<W>(ss, most, s_part);
+    float inv = 1.0f / sqrtf(ss / (float)a.width + a.eps);
+    if (ss == INFINITY) {
+      // Squares past fp32's range: again with the row scaled down (an infinity
+      // in the row comes out the same).
+      constexpr float kDown = 5.42101086242752217e-20f;  // 2^-64
+      float low = 0.0f, none = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) low = fmaf(h[k][j] * kDown, h[k][j] * kDown, low);
+      row_reduce<W>(low, none, s_part);
+      inv = kDown / sqrtf(low / (float)a.width);
+    }
+    if (!a.normed) inv = 1.0f;
+
+    if (a.sum) {
+      T* sum = static_cast<T*>(a.sum) + (size_t)r * a.ld_sum;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * 64 * W) * N, left = a.width - c;
+        if (left > 0) store_vec<T>(sum, c, left, h[k]);
+      }
+    }
+    if (a.out) {
+      T* out = static_cast<T*>(a.out) + (size_t)r * a.ld_out;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * 64 * W) * N, left = a.width - c;
+        if (left <= 0) continue;
+        float v[N], g[N];
+        if constexpr (!kAhead) gamma_of(k, g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = h[k][j] * inv * (kAhead ? gamma[kAhead ? k : 0][j] : g[j]);
+        store_vec<T>(out, c, left, v);
+      }
+    }
     if (a.codes) {
-      float g[N];
-      if (a.gamma) {
+      // A row that is not finite has the scale NaN, which its products take on.
+      const bool fine = most < INFINITY;
+      // Maxima so small that 127 / max would overflow are scaled up, exactly.
+      const float up = most < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 2^64
+      const float by = 127.0f / (most * up);
+      int8_t* codes = a.codes + (size_t)r * a.ld_codes;
 #pragma unroll
-        for (int j = 0; j < N; ++j) g[j] = j < left ? a.gamma[c + j] : 0.0f;
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * 64 * W) * N, left = a.width - c;
+        if (left <= 0) continue;
+        int q[N];
+        float g[N];
+        if constexpr (!kAhead) gamma_of(k, g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float t = h[k][j] * (kAhead ? gamma[kAhead ? k : 0][j] : g[j]);
+          q[j] = fine && most > 0.0f ? (int)fminf(fmaxf(rintf(t * up * by), -127.0f), 127.0f) : 0;
+        }
+        store_codes<N>(codes, c, left, q);
       }
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float t = fabsf(a.gamma ? h[k][j] * g[j] : h[k][j]);
-        most = fmaxf(most, t < INFINITY ? t : INFINITY);
-      }
+      if (tid == 0) a.scales[r] = fine ? most / 127.0f * inv : NAN;
     }
-  }
-  row_reduce<W>(ss, most, s_part);
-  float inv = 1.0f / sqrtf(ss / (float)a.width + a.eps);
-  if (ss == INFINITY) {
-    // Squares past fp32's range: again with the row scaled down (an infinity
-    // in the row comes out the same).
-    constexpr float kDown = 5.42101086242752217e-20f;  // 2^-64
-    float low = 0.0f, none = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < N; ++j) low = fmaf(h[k][j] * kDown, h[k][j] * kDown, low);
-    row_reduce<W>(low, none, s_part);
-    inv = kDown / sqrtf(low / (float)a.width);
-  }
-  if (!a.normed) inv = 1.0f;
-
-  if (a.sum) {
-    T* sum = static_cast<T*>(a.sum) + (size_t)r * a.ld_sum;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * 64 * W) * N, left = a.width - c;
-      if (left > 0) store_vec<T>(sum, c, left, h[k]);
-    }
-  }
-  if (a.out) {
-    T* out = static_cast<T*>(a.out) + (size_t)r * a.ld_out;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * 64 * W) * N, left = a.width - c;
-      if (left <= 0) continue;
-      float v[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = h[k][j] * inv * (j < left ? a.gamma[c + j] : 0.0f);
-      store_vec<T>(out, c, left, v);
-    }
-  }
-  if (a.codes) {
-    // A row that is not finite has the scale NaN, which its products take on.
-    const bool fine = most < INFINITY;
-    // Maxima so small that 127 / max would overflow are scaled up, exactly.
-    const float up = most < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 2^64
-    const float by = 127.0f / (most * up);
-    int8_t* codes = a.codes + (size_t)r * a.ld_codes;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * 64 * W) * N, left = a.width - c;
-      if (left <= 0) continue;
-      int q[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float t = a.gamma ? h[k][j] * (j < left ? a.gamma[c + j] : 0.0f) : h[k][j];
-        q[j] = fine && most > 0.0f ? (int)fminf(fmaxf(rintf(t * up * by), -127.0f), 127.0f) : 0;
-      }
-      store_codes<N>(codes, c, left, q);
-    }
-    if (tid == 0) a.scales[r] = fine ? most / 127.0f * inv : NAN;
   }
 }
 
 template <class T, int W, int NV>
 Status launch_rows(hipStream_t stream, const RmsNormArgs& a, size_t rows) {
-  const uint32_t grid = (uint32_t)(W == 1 ? (rows + 3) / 4 : rows);
-  rms_norm_kernel<T, W, NV><<<grid, W == 1 ? 256 : 64 * W, 0, stream>>>(a, (int)rows);
+  constexpr int WAVES = W == 1 ? 4 : W;
+  // As many workgroups as the machine holds at once, 16 waves a compute unit.
+  const size_t all = W == 1 ? (rows + 3) / 4 : rows, most = 256 * std::max(1, 16 / WAVES);
+  rms_norm_kernel<T, W, NV><<<(uint32_t)std::min(all, most), 64 * WAVES, 0, stream>>>(a, (int)rows);
   PSSA_LAUNCH_CHECK("rms_norm_kernel");
   return Status::Ok();
 }
