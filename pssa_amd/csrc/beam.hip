@@ -60,121 +60,165 @@ __device__ __forceinline__ bool beam_runs(const BeamArgs& a, int row) {
   return !beam_ended(a, row) && fabsf(a.scores[row]) < INFINITY;
 }
 
+// A piece of a row: 16 bytes, or the `left` elements that there are, then -inf.
 template <class T>
-__device__ __forceinline__ void load_vec(const T* row, int c, int left, float (&v)[vec_n<T>()]) {
+__device__ __forceinline__ u32x4_t load_piece(const T* row, int c, int left) {
   constexpr int N = vec_n<T>();
-  if (left >= N) {
-    const u32x4_t u = *reinterpret_cast<const u32x4_any_t*>(row + c);
+  if (left >= N) return *reinterpret_cast<const u32x4_any_t*>(row + c);
+  u32x4_t u;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if constexpr (sizeof(T) == 4)
-        v[j] = __uint_as_float(u[j]);
-      else
-        v[j] = __uint_as_float(j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
-    }
-  } else {
+  for (int e = 0; e < 4; ++e) u[e] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      v[j] = -INFINITY;
-      if (j < left) {
-        if constexpr (sizeof(T) == 4)
-          v[j] = *reinterpret_cast<const float*>(row + c + j);
-        else
-          v[j] = __uint_as_float((uint32_t)row[c + j].bits << 16);
-      }
-    }
+  for (int j = 0; j < N; ++j) {
+    if (j >= left) continue;
+    if constexpr (sizeof(T) == 4)
+      u[j] = __float_as_uint(row[c + j]);
+    else
+      u[j >> 1] = j & 1 ? (u[j >> 1] & 0xFFFFu) | (uint32_t)row[c + j].bits << 16 : (u[j >> 1] & 0xFFFF0000u) | row[c + j].bits;
   }
+  return u;
+}
+template <class T>
+__device__ __forceinline__ float elem(const u32x4_t& u, int j) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(u[j]);
+  return __uint_as_float(j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
 }
 
+// Of the 64 values of a wave's lanes the keep-th largest, in every lane.
+__device__ __forceinline__ float keepth_largest(float v, int keep) {
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)) > v;
+  // The least of those that fewer than keep lie above.
+  float least = above < keep ? v : INFINITY;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) least = fminf(least, __shfl_xor(least, off, 64));
+  return least;
+}
+
+// Places of the candidates that a workgroup puts aside; past them (rows of
+// equal logits) it goes through its candidates in rounds.
+constexpr int kAside = 1024;
+
 // A slice of a row in the registers of a workgroup, NV pieces of 16 bytes a
-// thread.  The keep-th largest of the threads' own largest keys is a bound:
-// what is below it is none of the keep largest, and only keep threads hold
-// anything that is not.
+// thread.  The largest logits of 64 groups of threads: the keep-th of these is
+// a bound that keep logits reach, and few others do.  What reaches it is put
+// aside and ordered.
 template <class T, int NV>
 __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
   constexpr int N = vec_n<T>();
-  __shared__ uint64_t s_best[kThreads], s_list[kMaxBeams * NV * N], s_bound;
+  __shared__ uint64_t s_list[kAside], s_best[4];
+  __shared__ float s_group[4][64], s_bound;
   __shared__ double s_sum[4];
-  __shared__ float s_most[4];
   __shared__ uint32_t s_count;
   const int row = blockIdx.x, slice = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (!beam_runs(a, row)) return;
   const T* logits = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
   const int first = slice * kThreads * NV * N;
 
-  float v[NV][N];
+  u32x4_t raw[NV];
+  float piece[NV], mine = -INFINITY;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = first + (tid + k * kThreads) * N;
-    load_vec<T>(logits, c, a.vocab - c, v[k]);
+    raw[k] = load_piece<T>(logits, c, a.vocab - c);
   }
-  float most = -INFINITY;
-  uint64_t best = 0;
-  bool bad = false;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const uint32_t id = first + (tid + k * kThreads) * N;
+    piece[k] = elem<T>(raw[k], 0);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      bad |= !(v[k][j] < INFINITY);
-      most = fmaxf(most, v[k][j]);
-      const uint64_t key = key_of(v[k][j], id + j);
-      best = key > best ? key : best;
-    }
+    for (int j = 1; j < N; ++j) piece[k] = fmaxf(piece[k], elem<T>(raw[k], j));
+    mine = fmaxf(mine, piece[k]);  // passes over a NaN
   }
+  s_group[wave][lane] = mine;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  const float group = fmaxf(fmaxf(s_group[0][lane], s_group[1][lane]), fmaxf(s_group[2][lane], s_group[3][lane]));
+  float most = group;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-  if (lane == 0) s_most[wave] = most;
-  s_best[tid] = best;
-  if (tid == 0) s_count = 0, s_bound = 0;
-  const bool any_bad = __syncthreads_or(bad);
-  most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
-
+  if (wave == ((row + slice) & 3)) {  // one wave, another SIMD's in neighbouring workgroups
+    const float b = keepth_largest(group, a.keep);
+    if (lane == 0) s_bound = b;
+  }
+  // A NaN makes the sum NaN; a slice of nothing else and -inf has no sum.
   double sum = 0.0;
-  if (most > -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float part = 0.0f;  // few terms in fp32, these sums in 64 bits
+  for (int k = 0; k < NV; ++k) {
+    asm volatile("" : "+v"(raw[k]));  // widened again: kept, the elements would take twice the registers
+    float part = 0.0f;                // few terms in fp32, these sums in 64 bits
 #pragma unroll
-      for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((v[k][j] - most) * kLog2e);
-      sum += part;
+    for (int j = 0; j < N; ++j) {
+      const float v = elem<T>(raw[k], j);
+      part += most > -INFINITY ? __builtin_amdgcn_exp2f((v - most) * kLog2e) : v != v ? v : 0.0f;
     }
+    sum += part;
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
 
-  // The thread's place among the threads' best (equal ones are none, 0).
-  int above = 0;
-  for (int i = 0; i < kThreads; ++i) above += s_best[i] > best;
-  if (above == a.keep - 1 && best) s_bound = best;
-  __syncthreads();
-  const uint64_t bound = s_bound;  // 0 where fewer threads have anything
+  // The few pieces that reach the bound are read again, so that the others
+  // need no registers.
+  const float bound = s_bound;
+  uint32_t reach = 0;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const uint32_t id = first + (tid + k * kThreads) * N;
+  for (int k = 0; k < NV; ++k) reach |= (piece[k] >= bound ? 1u : 0u) << k;
+  auto keys = [&](auto use) {
+    for (uint32_t left = reach; left; left &= left - 1) {
+      const int c = first + (tid + __builtin_ctz(left) * kThreads) * N;
+      const u32x4_t u = load_piece<T>(logits, c, a.vocab - c);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const uint64_t key = key_of(v[k][j], id + j);
-      if (key && key >= bound) s_list[atomicAdd(&s_count, 1u)] = key;
+      for (int j = 0; j < N; ++j) {
+        const float v = elem<T>(u, j);
+        const uint64_t key = key_of(v, c + j);
+        if (key && v >= bound) use(key);
+      }
     }
-  }
+  };
+  keys([&](uint64_t key) {
+    const uint32_t at = atomicAdd(&s_count, 1u);
+    if (at < kAside) s_list[at] = key;
+  });
   __syncthreads();
+
   const int count = (int)s_count;
   const size_t at = (size_t)row * a.slices + slice;
   uint64_t* out = a.keys + at * a.keep;
-  for (int i = tid; i < count; i += kThreads) {
-    const uint64_t key = s_list[i];
-    int place = 0;
-    for (int j = 0; j < count; ++j) place += s_list[j] > key;
-    if (place < a.keep) out[place] = key;
+  if (count <= kAside) {
+    for (int i = tid; i < count; i += kThreads) {
+      const uint64_t key = s_list[i];
+      int place = 0;
+      for (int j = 0; j < count; ++j) place += s_list[j] > key;
+      if (place < a.keep) out[place] = key;
+    }
+    for (int i = count + tid; i < a.keep; i += kThreads) out[i] = 0;
+  } else {
+    uint64_t last = ~(uint64_t)0;
+    for (int i = 0; i < a.keep; ++i) {
+      uint64_t best = 0;
+      keys([&](uint64_t key) { best = key < last && key > best ? key : best; });
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) {
+        const uint64_t o = __shfl_xor((unsigned long long)best, off, 64);
+        best = o > best ? o : best;
+      }
+      if (lane == 0) s_best[wave] = best;
+      __syncthreads();
+      best = s_best[0];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) best = s_best[w] > best ? s_best[w] : best;
+      __syncthreads();
+      if (tid == 0) out[i] = best;
+      last = best;
+    }
   }
-  for (int i = count + tid; i < a.keep; i += kThreads) out[i] = 0;
   if (tid == 0) {
     SliceSum s;
     s.sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
     s.most = most;
-    s.bad = any_bad;
+    s.bad = !(most < INFINITY) || s.sum != s.sum;
     static_cast<SliceSum*>(a.sums)[at] = s;
   }
 }
@@ -189,34 +233,36 @@ __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
 }
 __device__ __forceinline__ Candidate nothing() { return Candidate{-INFINITY, ~(uint64_t)0}; }
 
-// The join of a group's slices: rounds that each pick the best candidate left,
-// of which only the winner's thread looks for its next one.
+// The join of a group's slices, with the same bound over its candidates.
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   // The scores and which beams have ended, as the outputs may be written over them.
   __shared__ double s_lse[kMaxBeams], s_score[kMaxBeams];
+  __shared__ float s_group[4][64];
   __shared__ bool s_ended[kMaxBeams];
-  __shared__ Candidate s_part[4];
+  __shared__ Candidate s_list[kAside], s_part[4];
+  __shared__ uint32_t s_count;
   const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row0 = group * a.beams;
   const SliceSum* sums = static_cast<const SliceSum*>(a.sums);
+  if (tid == 0) s_count = 0;
   // Each running beam's log of the sum; +inf (no candidate) where it has none.
-  for (int b = wave; b < a.beams; b += 4) {
-    double lse = INFINITY;
-    if (beam_runs(a, row0 + b)) {
-      const SliceSum* s = sums + (size_t)(row0 + b) * a.slices;
-      float most = -INFINITY;
-      bool bad = false;
-      for (int i = lane; i < a.slices; i += 64) most = fmaxf(most, s[i].most), bad |= s[i].bad != 0;
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-      double sum = 0.0;
-      for (int i = lane; i < a.slices; i += 64)
-        if (s[i].most > -INFINITY) sum += s[i].sum * exp((double)s[i].most - (double)most);
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-      if (!__any(bad) && most > -INFINITY) lse = log(sum) + (double)most;
+  // A beam's slices take as many lanes as let all beams be joined at once.
+  const int lanes = a.beams <= 4 ? 64 : a.beams <= 16 ? 16 : 4, b = tid / lanes;
+  if (b < a.beams) {
+    const SliceSum* s = sums + (size_t)(row0 + b) * a.slices;
+    const int in = tid & (lanes - 1), slices = beam_runs(a, row0 + b) ? a.slices : 0;
+    float most = -INFINITY;
+    bool bad = false;
+    for (int i = in; i < slices; i += lanes) most = fmaxf(most, s[i].most), bad |= s[i].bad != 0;
+    for (int off = lanes >> 1; off >= 1; off >>= 1) {
+      most = fmaxf(most, __shfl_xor(most, off, 64));
+      bad |= (bool)__shfl_xor((int)bad, off, 64);
     }
-    if (lane == 0) {
-      s_lse[b] = lse;
+    double sum = 0.0;
+    for (int i = in; i < slices; i += lanes)
+      if (s[i].most > -INFINITY) sum += s[i].sum * exp((double)s[i].most - (double)most);
+    for (int off = lanes >> 1; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (in == 0) {
+      s_lse[b] = !bad && most > -INFINITY ? log(sum) + (double)most : INFINITY;
       s_score[b] = a.scores[row0 + b];
       s_ended[b] = beam_ended(a, row0 + b);
     }
@@ -228,7 +274,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     const int b = i / per_beam;
     const double score = s_score[b];
     if (s_ended[b])  // it stays as it is
-      return i % per_beam == 0 && fabs(score) < INFINITY ? Candidate{score, (uint64_t)b << 32 | a.eos} : nothing();
+      return i == b * per_beam && fabs(score) < INFINITY ? Candidate{score, (uint64_t)b << 32 | a.eos} : nothing();
     if (!(s_lse[b] < INFINITY)) return nothing();
     const uint64_t key = a.keys[(size_t)row0 * per_beam + i];
     if (!key) return nothing();
@@ -240,6 +286,37 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     const Candidate c = candidate(i);
     if (better(c, mine)) mine = c;
   }
+  s_group[wave][lane] = (float)mine.value;  // rounding keeps the order
+  __syncthreads();
+  const float bound = keepth_largest(fmaxf(fmaxf(s_group[0][lane], s_group[1][lane]), fmaxf(s_group[2][lane], s_group[3][lane])), a.keep);
+  for (int i = tid; i < all; i += kThreads) {
+    const Candidate c = candidate(i);
+    if (c.value > -INFINITY && (float)c.value >= bound) {
+      const uint32_t at = atomicAdd(&s_count, 1u);
+      if (at < kAside) s_list[at] = c;
+    }
+  }
+  __syncthreads();
+  const int count = (int)s_count;
+  auto put = [&](int place, const Candidate& c) {
+    const size_t o = (size_t)group * a.keep + place;
+    const bool some = c.value > -INFINITY;
+    a.parents[o] = some ? (uint32_t)(c.at >> 32) : kNoToken;
+    a.tokens[o] = some ? (uint32_t)c.at : kNoToken;
+    a.out_scores[o] = some ? (float)c.value : -INFINITY;
+  };
+  if (count <= kAside) {
+    for (int i = tid; i < count; i += kThreads) {
+      const Candidate c = s_list[i];
+      int place = 0;
+      for (int j = 0; j < count; ++j) place += better(s_list[j], c);
+      if (place < a.keep) put(place, c);
+    }
+    for (int i = count + tid; i < a.keep; i += kThreads) put(i, nothing());
+    return;
+  }
+  // Rounds that each pick the best candidate left, of which only the winner's
+  // thread looks for its next one.
   for (int j = 0; j < a.keep; ++j) {
     Candidate w = mine;
 #pragma unroll
@@ -254,14 +331,8 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     for (int i = 1; i < 4; ++i)
       if (better(s_part[i], w)) w = s_part[i];
     __syncthreads();
-    const bool some = w.value > -INFINITY;
-    if (tid == 0) {
-      const size_t o = (size_t)group * a.keep + j;
-      a.parents[o] = some ? (uint32_t)(w.at >> 32) : kNoToken;
-      a.tokens[o] = some ? (uint32_t)w.at : kNoToken;
-      a.out_scores[o] = some ? (float)w.value : -INFINITY;
-    }
-    if (some && mine.at == w.at) {
+    if (tid == 0) put(j, w);
+    if (w.value > -INFINITY && mine.at == w.at) {
       mine = nothing();
       for (int i = tid; i < all; i += kThreads) {
         const Candidate c = candidate(i);
