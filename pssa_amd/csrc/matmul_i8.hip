@@ -140,7 +140,10 @@ __global__ __launch_bounds__(256) void matmul_i8_rows_kernel(I8Args a) {
 }
 
 // ----------------------------------------------------------------- many rows
-__device__ uint32_t g_zeros[4];  // codes behind a row's end
+constexpr int kLdsDone = ~(0xF << 8);  // of an s_waitcnt: lgkmcnt(0)
+
+// Channels of a row of parts: whole units of 16 bytes.
+__host__ __device__ __forceinline__ size_t parts_ld(size_t n) { return (n + 3) / 4 * 4; }
 
 // Consecutive workgroups lie on different XCDs: each of the eight gets
 // neighbouring tiles, walked in bands of 8 rows of tiles, so that what runs at
@@ -156,8 +159,16 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int& 
 }
 
 // BM rows by BN channels, WM x WN waves; rows and weights at multiples of 16
-// bytes, k a multiple of 16.
-template <class T, int BM, int BN, int WM, int WN>
+// bytes, k a multiple of 16.  Slabs of 128 codes, whole cache lines, pass
+// through R LDS buffers, 2 or 4.  A step of 32 codes' fragments are read while
+// the step before is multiplied, across the slabs' border too, and the loads of
+// the slab R - 1 ahead go out over R steps between the products: the L1 takes
+// 16 cycles for each, all at once they held the products up.  At the end a
+// wave's 32 rows at a time turn in LDS, so that what it stores is whole lines.
+// 8192 x 8192 x 8192: 475 to 550 us, by the card's clock, which falls to 1.7
+// GHz under this load (2.0 to 2.3 POP/s; stores of 8 bytes a row took 70 us
+// more, rows whose units lay two to a bank 20).
+template <class T, int BM, int BN, int WM, int WN, int R>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a, int tiles_m, int tiles_n) {
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int UNITS = (BM + BN) * 8, PER = UNITS / THREADS;  // of 16 bytes; of a thread
@@ -170,24 +181,29 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a,
   const int slabs = (a.k + 127) / 128, first = (int)((int64_t)blockIdx.y * slabs / a.splits),
             last = (int)((int64_t)(blockIdx.y + 1) * slabs / a.splits);
 
-  // A slab row is 8 units of 16 codes; unit u of row r lies at u ^ (r & 7), so
-  // that rows read at one unit hit different banks.
-  const int8_t* src[PER];
-  int unit_k;
+  // A slab row is 4 units of 16 codes; unit u of row r lies at u ^ (r / 2 & 3),
+  // so that rows read at one unit hit different banks.  What a slab has behind
+  // k, and slabs behind the last, are other codes of the row.
+  uint32_t from[PER];  // the row, of the tile's first
+  const int unit_k = 16 * ((threadIdx.x & 7) ^ (threadIdx.x >> 4 & 7));  // THREADS / 8 rows further it is the same
+  constexpr int OF_X = BM * 8 / THREADS;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int row = (i * THREADS + (int)threadIdx.x) / 8, u = (threadIdx.x & 7) ^ (row & 7);
-    unit_k = 16 * u;  // THREADS / 8 is a multiple of 8: the same for all of a thread's rows
-    src[i] = row < BM ? a.x + (size_t)min(m0 + row, a.m - 1) * a.ld_x + 16 * u
-                      : a.w + (size_t)min(n0 + row - BM, a.n - 1) * a.ld_w + 16 * u;
+    const int row = (i * THREADS + (int)threadIdx.x) / 8;
+    from[i] = i < OF_X ? (uint32_t)min(row, a.m - 1 - m0) * (uint32_t)a.ld_x : (uint32_t)min(row - BM, a.n - 1 - n0) * (uint32_t)a.ld_w;
   }
-  auto issue = [&](int slab, i32x4_t* buffer) {
-    const bool there = 128 * slab + unit_k < a.k;
+  const int8_t *x = a.x + (size_t)m0 * a.ld_x, *w = a.w + (size_t)n0 * a.ld_w;
+  // Loads begin .. end - 1 of a slab.
+  auto issue = [&](int slab, int begin, int end) {
+    const int k0 = 128 * min(slab, last - 1);
+    const uint32_t at = k0 + unit_k < a.k ? k0 + unit_k : k0;
+    i32x4_t* buffer = s_tile + (slab - first) % R * UNITS;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const void* from = there ? static_cast<const void*>(src[i] + (size_t)slab * 128) : g_zeros;
+      if (i < begin || i >= end) continue;
       auto* to = (__attribute__((address_space(3))) void*)(buffer + i * THREADS + wave * 64);
-      __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+      const void* codes = (i < OF_X ? x : w) + (from[i] + at);
+      __builtin_amdgcn_global_load_lds(codes, to, 16, 0, 0);
     }
   };
   i32x16_t acc[TN][TM];
@@ -197,76 +213,165 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a,
     for (int t = 0; t < TM; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[b][t][e] = 0;
-
-  i32x4_t* buffer = s_tile;
-  if (first < last) issue(first, buffer);
-  for (int slab = first; slab < last; ++slab) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-    __syncthreads();  // the slab is there, and the one before is read
-    i32x4_t* other = buffer == s_tile ? s_tile + UNITS : s_tile;
-    if (slab + 1 < last) issue(slab + 1, other);
+  // Slab s is there for all waves, and s - 1 read by them.  Slabs behind the last are of zeros.
+  auto meet = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(vmcnt_only((R - 2) * PER) & kLdsDone);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  i32x4_t xf[2][TM], wf[2][TN];
+  auto read = [&](int slab, auto step) {
+    constexpr int S = decltype(step)::value;
+    const i32x4_t* buffer = s_tile + (slab - first) % R * UNITS;
     const i32x4_t *sx = buffer + (wm * TM * 32 + l32) * 8, *sw = buffer + (BM + wn * TN * 32 + l32) * 8;
+    const int u = (2 * S + half) ^ (l32 >> 1 & 7);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int u = (2 * ks + half) ^ (l32 & 7);
-      i32x4_t xf[TM], wf[TN];
+    for (int b = 0; b < TN; ++b) wf[S & 1][b] = sw[b * 256 + u];
 #pragma unroll
-      for (int b = 0; b < TN; ++b) wf[b] = sw[b * 256 + u];
+    for (int t = 0; t < TM; ++t) xf[S & 1][t] = sx[t * 256 + u];
+  };
+  auto multiply = [&](int slab, auto step, bool end) {
+    constexpr int S = decltype(step)::value;
+    if (end)  // the sums may end inside the slab
 #pragma unroll
-      for (int t = 0; t < TM; ++t) xf[t] = sx[t * 256 + u];
-#pragma unroll
-      for (int b = 0; b < TN; ++b)
-#pragma unroll
-        for (int t = 0; t < TM; ++t) acc[b][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[b], xf[t], acc[b][t], 0, 0, 0);
-    }
-    buffer = other;
-  }
-  // A lane holds a row's channels 8 g + 4 half .. + 3 of each 32.
-#pragma unroll
-  for (int t = 0; t < TM; ++t) {
-    const int i = m0 + (wm * TM + t) * 32 + l32;
-    if (i >= a.m) continue;
-    const float scale = a.x_scales[i];
+      for (int t = 0; t < TM; ++t)
+        if (128 * slab + 32 * S + 16 * half >= a.k) xf[S & 1][t] = i32x4_t{0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < TN; ++b)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int j = n0 + (wn * TN + b) * 32 + 8 * g + 4 * half, left = a.n - j;
-        if (left <= 0) continue;
-        if (a.splits > 1) {
-          int32_t* part = a.parts + ((size_t)blockIdx.y * a.m + i) * a.n + j;
+      for (int t = 0; t < TM; ++t) acc[b][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[S & 1][b], xf[S & 1][t], acc[b][t], 0, 0, 0);
+    // Reads and loads between the products.
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < left) part[r] = acc[b][t][4 * g + r];
-          continue;
-        }
-        f32x4_t y;
+    for (int i = 0; i < TM * TN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, TM + TN, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::integral_constant<int, 0> zero;
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 3> three;
+  constexpr int P = PER / R;  // loads of a step
+  for (int r = 0; r < R - 1; ++r) issue(first + r, 0, PER);
+  issue(first + R - 1, 0, P);
+  meet();
+  read(first, zero);
+  auto pass = [&](int slab, bool end) {
+    read(slab, one);
+    issue(slab + R - 1, P, 2 * P);
+    multiply(slab, zero, end);
+    read(slab, two);
+    if constexpr (R > 2) issue(slab + R - 1, 2 * P, 3 * P);
+    multiply(slab, one, end);
+    read(slab, three);
+    if constexpr (R > 2) issue(slab + R - 1, 3 * P, 4 * P);
+    multiply(slab, two, end);
+    meet();
+    issue(slab + R, 0, P);
+    read(slab + 1, zero);
+    multiply(slab, three, end);
+  };
+  for (int slab = first; slab < last - 1; ++slab) pass(slab, false);
+  pass(last - 1, true);
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  meet();  // all have read the slabs, and none is on its way
+  // A lane holds channels 8 g + 4 half .. + 3 of each 32 of a row; a unit is 4
+  // channels, unit u of row r lies at u ^ (r & 15).
+  constexpr int ROW = TN * 8;
+  static_assert(ROW == 16);
+  i32x4_t* s_out = s_tile + wave * 32 * ROW;
+  const int row0 = m0 + wm * TM * 32, ch0 = n0 + wn * TN * 32;
+  auto each = [&](auto units, auto out) {
+    constexpr int U = decltype(units)::value, AT_ONCE = 64 / (ROW / U);  // a lane's units, an instruction's rows
+    const int u = lane % (ROW / U) * U, j = ch0 + 4 * u;
+    float scales[4 * U];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = (float)acc[b][t][4 * g + r] * scale * a.w_scales[min(j + r, a.n - 1)];
-        store4(static_cast<T*>(a.y) + (size_t)i * a.ld_y + j, y, left);
+    for (int c = 0; c < 4 * U; ++c) scales[c] = a.w_scales[min(j + c, a.n - 1)];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          s_out[l32 * ROW + ((8 * b + 2 * g + half) ^ (l32 & 15))] = i32x4_t{acc[b][t][4 * g], acc[b][t][4 * g + 1], acc[b][t][4 * g + 2], acc[b][t][4 * g + 3]};
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+        const int r = r0 + lane / (ROW / U), i = row0 + 32 * t + r;
+        i32x4_t v[U];
+#pragma unroll
+        for (int e = 0; e < U; ++e) v[e] = s_out[r * ROW + ((u + e) ^ (r & 15))];
+        if (i < a.m && j < a.n) out(i, j, v, scales);
       }
-  }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  if (a.splits > 1)
+    each(one, [&](int i, int j, const i32x4_t* v, const float*) {
+      *reinterpret_cast<i32x4_t*>(a.parts + ((size_t)blockIdx.y * a.m + i) * parts_ld(a.n) + j) = v[0];
+    });
+  else if constexpr (sizeof(T) == 2)
+    each(two, [&](int i, int j, const i32x4_t* v, const float* scales) {
+      const float scale = a.x_scales[i];
+      T* y = static_cast<T*>(a.y) + (size_t)i * a.ld_y + j;
+      f32x4_t f[2];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) f[c / 4][c % 4] = (float)v[c / 4][c % 4] * scale * scales[c];
+      if (a.n - j >= 8)
+        *reinterpret_cast<i32x4_any_t*>(y) = i32x4_t{(int)bf16x2_bits(f[0][0], f[0][1]), (int)bf16x2_bits(f[0][2], f[0][3]),
+                                                     (int)bf16x2_bits(f[1][0], f[1][1]), (int)bf16x2_bits(f[1][2], f[1][3])};
+      else {
+        store4(y, f[0], a.n - j);
+        store4(y + 4, f[1], a.n - j - 4);
+      }
+    });
+  else
+    each(one, [&](int i, int j, const i32x4_t* v, const float* scales) {
+      const float scale = a.x_scales[i];
+      f32x4_t f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) f[c] = (float)v[0][c] * scale * scales[c];
+      store4(static_cast<T*>(a.y) + (size_t)i * a.ld_y + j, f, a.n - j);
+    });
 }
 
-// The parts of k summed, and scaled.
+// The parts of k summed, and scaled: four channels a thread, rows along y.
 template <class T>
 __global__ __launch_bounds__(256) void matmul_i8_join_kernel(I8Args a) {
-  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, all = (size_t)a.m * a.n;
+  const size_t ld = parts_ld(a.n), all = a.m * ld, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= all) return;
-  int sum = 0;
-  for (int s = 0; s < a.splits; ++s) sum += a.parts[s * all + at];
-  const size_t i = at / a.n, j = at - i * a.n;
-  store1(static_cast<T*>(a.y) + i * a.ld_y + j, (float)sum * a.x_scales[i] * a.w_scales[j]);
+  i32x4_t sum = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) sum += *reinterpret_cast<const i32x4_t*>(a.parts + s * all + at);
+  const size_t i = at / ld;
+  const int j = (int)(at - i * ld);
+  const float scale = a.x_scales[i];
+  f32x4_t y;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) y[c] = (float)sum[c] * scale * a.w_scales[min(j + c, a.n - 1)];
+  store4(static_cast<T*>(a.y) + i * a.ld_y + j, y, a.n - j);
 }
 
-// Rows of k codes at any byte, copied to rows of whole units with zeros behind.
-__global__ __launch_bounds__(256) void i8_pack_kernel(const int8_t* src, size_t ld, int k, int8_t* dst, size_t ld_dst, int rows) {
-  const int units = (int)(ld_dst / 16);
-  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (size_t)rows * units) return;
+// Rows of k codes at any byte, copied to rows of whole units with zeros behind:
+// x's and the weights' in one launch.
+struct Packed {
+  const int8_t* src;
+  size_t ld;
+  int8_t* dst;
+  int rows;  // 0 where the rows are used as they are
+};
+__global__ __launch_bounds__(256) void i8_pack_kernel(Packed x, Packed w, int k, int units) {
+  size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t of_x = (size_t)x.rows * units;
+  const Packed p = at < of_x ? x : w;
+  if (at >= of_x) at -= of_x;
+  if (at >= (size_t)p.rows * units) return;
   const size_t row = at / units;
   const int u = (int)(at - row * units);
-  *reinterpret_cast<i32x4_t*>(dst + row * ld_dst + 16 * u) = load16(src + row * ld + 16 * u, k - 16 * u);
+  *reinterpret_cast<i32x4_t*>(p.dst + (row * units + u) * 16) = load16(p.src + row * p.ld + 16 * u, k - 16 * u);
 }
 
 template <class T, int MT, int NC>
@@ -287,16 +392,18 @@ Status launch_few(hipStream_t stream, const I8Args& a) {
   return launch_rows_of<T, 4, 2>(stream, a);
 }
 
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, int R>
 struct Tiles {
-  static constexpr size_t kLds = 2 * (size_t)(BM + BN) * 128;
+  static constexpr size_t kLds = R * (size_t)(BM + BN) * 128;
   static constexpr int kRows = BM, kChannels = BN, kThreads = 64 * WM * WN;
-  static constexpr auto kKernel = &matmul_i8_tiles_kernel<T, BM, BN, WM, WN>;
+  static constexpr auto kKernel = &matmul_i8_tiles_kernel<T, BM, BN, WM, WN, R>;
 };
 template <class T>
-using Large = Tiles<T, 256, 256, 2, 4>;
+using Large = Tiles<T, 256, 256, 2, 4, 2>;
 template <class T>
-using Small = Tiles<T, 128, 128, 2, 2>;
+using Small = Tiles<T, 128, 128, 2, 2, 2>;
+template <class T>
+using Deep = Tiles<T, 128, 128, 2, 2, 4>;
 
 template <class C, class T>
 Status launch_tiles(hipStream_t stream, const I8Args& a) {
@@ -304,7 +411,7 @@ Status launch_tiles(hipStream_t stream, const I8Args& a) {
   C::kKernel<<<dim3((uint32_t)tiles_m * tiles_n, a.splits), C::kThreads, C::kLds, stream>>>(a, tiles_m, tiles_n);
   PSSA_LAUNCH_CHECK("matmul_i8_tiles_kernel");
   if (a.splits > 1) {
-    matmul_i8_join_kernel<T><<<(uint32_t)(((size_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(a);
+    matmul_i8_join_kernel<T><<<(uint32_t)((a.m * parts_ld(a.n) / 4 + 255) / 256), 256, 0, stream>>>(a);
     PSSA_LAUNCH_CHECK("matmul_i8_join_kernel");
   }
   return Status::Ok();
@@ -316,19 +423,15 @@ bool large_tiles(size_t m, size_t n) { return tiles_of(m, n, 256) >= 3 * kComput
 template <class T>
 Status launch_typed(hipStream_t stream, const I8Args& a) {
   if (a.m <= kI8FewRows) return launch_few<T>(stream, a);
-  return large_tiles(a.m, a.n) ? launch_tiles<Large<T>, T>(stream, a) : launch_tiles<Small<T>, T>(stream, a);
+  if (large_tiles(a.m, a.n)) return launch_tiles<Large<T>, T>(stream, a);
+  // A workgroup a compute unit has room for four buffers (1024 x 4096 x 4096:
+  // 25 us, with two 28), more than that share it with two each (1024 x 5120 x
+  // 4096: 34 us, one after the other 40).
+  return tiles_of(a.m, a.n, 128) * a.splits <= kComputeUnits ? launch_tiles<Deep<T>, T>(stream, a) : launch_tiles<Small<T>, T>(stream, a);
 }
 
-Status launch_pack(hipStream_t stream, const int8_t*& p, size_t& ld, int k, int rows, char*& scratch) {
-  const size_t to = ((size_t)k + 15) / 16 * 16;
-  i8_pack_kernel<<<(uint32_t)((rows * (to / 16) + 255) / 256), 256, 0, stream>>>(p, ld, k, reinterpret_cast<int8_t*>(scratch), to, rows);
-  PSSA_LAUNCH_CHECK("i8_pack_kernel");
-  p = reinterpret_cast<int8_t*>(scratch);
-  ld = to;
-  scratch += (rows * to + 255) & ~(size_t)255;
-  return Status::Ok();
-}
-bool in_units(const void* p, size_t ld, size_t k) { return ((uintptr_t)p | ld | k) % 16 == 0; }
+// Whole units, and offsets inside a tile's rows of 32 bits.
+bool in_units(const void* p, size_t ld, size_t k) { return ((uintptr_t)p | ld | k) % 16 == 0 && ld <= (size_t)1 << 24; }
 
 }  // namespace
 
@@ -338,11 +441,12 @@ I8Plan i8_plan(size_t m, size_t n, size_t k) {
   const size_t rows = (k + 15) / 16 * 16;
   p.pack_bytes = ((m * rows + 255) & ~(size_t)255) + ((n * rows + 255) & ~(size_t)255);
   if (!large_tiles(m, n)) {
-    // Two workgroups a compute unit, parts of four slabs or more.
+    // Parts of four slabs or more, for a workgroup a compute unit: two, of half
+    // the slabs each, have twice the sums to join (1024 x 4096 x 4096 37 us, so 28).
     const size_t tiles = tiles_of(m, n, 128), slabs = (k + 127) / 128;
-    p.splits = (int)std::max<size_t>(1, std::min(kComputeUnits * 2 / tiles, slabs / 4));
+    p.splits = (int)std::max<size_t>(1, std::min(kComputeUnits / tiles, slabs / 4));
   }
-  p.parts_bytes = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
+  p.parts_bytes = p.splits > 1 ? p.splits * m * parts_ld(n) * 4 : 0;
   return p;
 }
 
@@ -353,6 +457,8 @@ Status init_i8_attributes() {
   };
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Large<float>::kKernel), Large<float>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Large<Bf16>::kKernel), Large<Bf16>::kLds));
+  PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Deep<float>::kKernel), Deep<float>::kLds));
+  PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Deep<Bf16>::kKernel), Deep<Bf16>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Small<float>::kKernel), Small<float>::kLds));
   return set(reinterpret_cast<const void*>(Small<Bf16>::kKernel), Small<Bf16>::kLds);
 }
@@ -362,8 +468,15 @@ Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan&
     a.splits = p.splits;
     a.parts = static_cast<int32_t*>(scratch);
     char* at = static_cast<char*>(scratch) + ((p.parts_bytes + 255) & ~(size_t)255);
-    if (!in_units(a.x, a.ld_x, (size_t)a.k)) PSSA_RETURN_IF(launch_pack(stream, a.x, a.ld_x, a.k, a.m, at));
-    if (!in_units(a.w, a.ld_w, (size_t)a.k)) PSSA_RETURN_IF(launch_pack(stream, a.w, a.ld_w, a.k, a.n, at));
+    const size_t units = ((size_t)a.k + 15) / 16;
+    Packed x{a.x, a.ld_x, reinterpret_cast<int8_t*>(at), in_units(a.x, a.ld_x, (size_t)a.k) ? 0 : a.m};
+    Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * units * 16 + 255) & ~(size_t)255)), in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
+    if (x.rows || w.rows) {
+      i8_pack_kernel<<<(uint32_t)((((size_t)x.rows + w.rows) * units + 255) / 256), 256, 0, stream>>>(x, w, a.k, (int)units);
+      PSSA_LAUNCH_CHECK("i8_pack_kernel");
+    }
+    if (x.rows) a.x = x.dst, a.ld_x = units * 16;
+    if (w.rows) a.w = w.dst, a.ld_w = units * 16;
     a.k = (a.k + 15) / 16 * 16;
   }
   return y_dtype == PSSA_HIP_F32 ? launch_typed<float>(stream, a) : launch_typed<Bf16>(stream, a);
