@@ -193,14 +193,18 @@ __device__ __forceinline__ Place place_of(const DeltaArgs& a, int chunk) {
   return Place{(size_t)tok + pos, min(C, (int)(first_token(a, lo + 1) - tok) - pos)};
 }
 
-// What is worked out ahead for a chunk and head, in units of 16 bytes: the
-// fragments of T where its triangle holds anything, then of the tokens e^G,
-// e^(G_n - G) and G itself, in 64 bits since differences of it count.  bf16:
-// a fragment is 16 tokens by 32, in two parts; fp32: 16 by 16.
+// What is worked out ahead for a chunk and head, in units of 16 bytes: T's
+// tiles of 16 x 16 where its triangle holds anything, in fp32 for both types,
+// then of the tokens e^G, e^(G_n - G) and G itself, in 64 bits since differences
+// of it count.  T as two bf16 parts had the products for U at half the time (a
+// chunk 0.4 us of 2.6), but what they drop comes back in every chunk's state,
+// and grows where keys are alike: states were off by 5e-6 of their size, and
+// are by 2e-7 so.  P's fragments are 16 tokens by 32 in two parts (bf16), 16 by
+// 16 (fp32): it only reaches the outputs.
 template <bool B16>
 struct Ahead {
   static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3, kFrag = B16 ? 128 : 64;
-  static constexpr int kGamma = kPairs * kFrag, kRest = kGamma + C / 4, kSum = kRest + C / 4, kUnits = kGamma + 64;
+  static constexpr int kTriangle = kTiles * (kTiles + 1) / 2, kGamma = kTriangle * 64, kRest = kGamma + C / 4, kSum = kRest + C / 4, kUnits = kGamma + 64;
 };
 // The fragment of token tile t over keys 32 h .. (bf16), 16 h .. (fp32).
 template <bool B16>
@@ -369,30 +373,10 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
   __syncthreads();
   // T's rows as fragments.
 #pragma unroll
-  for (int i = 0; i < (Out::kPairs + NT - 1) / NT; ++i) {
-    const int at = i * NT + wave;
-    if (at >= Out::kPairs) continue;
-    if constexpr (B16) {
-      const int r = at < 2 ? at : 2 + (at - 2) / 2, h = at < 2 ? 0 : at & 1;
-      u32x4_t hi, lo;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        f32x4_t w = {0, 0, 0, 0};
-        if (2 * h + x <= r) w = *reinterpret_cast<const f32x4_t*>(s_a + (16 * r + col) * LD + 32 * h + 16 * x + 4 * quad);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t u, l;
-          split2(w[2 * e], w[2 * e + 1], u, l);
-          hi[2 * x + e] = u;
-          lo[2 * x + e] = l;
-        }
-      }
-      out[128 * at + lane] = hi;
-      out[128 * at + 64 + lane] = lo;
-    } else {
-      const int r = triangle_row(at), c = triangle_col(at);
+  for (int i = 0; i < (Out::kTriangle + NT - 1) / NT; ++i) {
+    const int at = i * NT + wave, r = triangle_row(at), c = triangle_col(at);
+    if (at < Out::kTriangle)
       out[64 * at + lane] = *reinterpret_cast<const u32x4_t*>(s_a + (16 * r + col) * LD + 16 * c + 4 * quad);
-    }
   }
 }
 
@@ -753,25 +737,26 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
     if constexpr (B16) {
 #pragma unroll
       for (int kp = 0; kp < DKP / 32; ++kp) {
-        u32x4_t hi, lo;
+        u32x4_t w[3];  // the outputs, in bf16, do with two
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          uint32_t u, l;
-          split2(S[2 * kp + (e >> 1)][2 * (e & 1)], S[2 * kp + (e >> 1)][2 * (e & 1) + 1], u, l);
-          hi[e] = u;
-          lo[e] = l;
+          uint32_t p0, p1, p2;
+          split3(S[2 * kp + (e >> 1)][2 * (e & 1)], S[2 * kp + (e >> 1)][2 * (e & 1) + 1], p0, p1, p2);
+          w[0][e] = p0;
+          w[1][e] = p1;
+          w[2][e] = p2;
         }
         if constexpr (!LOCAL) {
-          sS[128 * kp + lane] = hi;
-          sS[128 * kp + 64 + lane] = lo;
+          sS[128 * kp + lane] = w[0];
+          sS[128 * kp + 64 + lane] = w[1];
         }
         u32x4_t kf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) kf[t] = row_frag<DKP>(sK, 16 * t + col, 4 * kp + quad);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], lo, x[t]);
+        for (int p = 2; p >= 0; --p)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], hi, x[t]);
+          for (int t = 0; t < NT; ++t) x[t] = mfma(kf[t], w[p], x[t]);
       }
     } else {
 #pragma unroll
@@ -787,34 +772,17 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
       }
     }
     // X = V - e^G K S, U = T X.
-    f32x4_t u[NT];
     if constexpr (B16) {
-      u32x4_t vf[2], hi[2], lo[2];
+      u32x4_t vf[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) vf[h] = turned<64, 4>(sV, 32 * h, 16 * wave, lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const f32x4_t g = *reinterpret_cast<const f32x4_t*>(gamma + 16 * t + 4 * quad);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t w = vf[t >> 1][2 * (t & 1) + e];
-          const float x0 = fmaf(-g[2 * e], x[t][2 * e], __uint_as_float(w << 16));
-          const float x1 = fmaf(-g[2 * e + 1], x[t][2 * e + 1], __uint_as_float(w & 0xFFFF0000u));
-          uint32_t p, l;
-          split2(x0, x1, p, l);
-          hi[t >> 1][2 * (t & 1) + e] = p;
-          lo[t >> 1][2 * (t & 1) + e] = l;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        u[t] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; 2 * h <= t; ++h) {
-          const u32x4_t th = sT[128 * pair_of<B16>(t, h) + lane], tl = sT[128 * pair_of<B16>(t, h) + 64 + lane];
-          u[t] = mfma(tl, hi[h], u[t]);
-          u[t] = mfma(th, lo[h], u[t]);
-          u[t] = mfma(th, hi[h], u[t]);
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t w = vf[t >> 1][2 * (t & 1) + (r >> 1)];
+          x[t][r] = fmaf(-g[r], x[t][r], __uint_as_float(r & 1 ? w & 0xFFFF0000u : w << 16));
         }
       }
     } else {
@@ -824,16 +792,19 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_k
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[t][r] = fmaf(-g[r], x[t][r], element32<64>(V32, 16 * t + 4 * quad + r, 16 * wave + col));
       }
+    }
+    f32x4_t u[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        u[t] = f32x4_t{0, 0, 0, 0};
+    for (int t = 0; t < NT; ++t) u[t] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h <= t; ++h) {
-          const f32x4_t tf = __builtin_bit_cast(f32x4_t, sT[64 * pair_of<B16>(t, h) + lane]);
+    for (int h = 0; h < NT; ++h) {
+      f32x4_t tf[NT];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) u[t] = mfma32(tf[r], x[h][r], u[t]);
-        }
-      }
+      for (int t = h; t < NT; ++t) tf[t] = __builtin_bit_cast(f32x4_t, sT[64 * (t * (t + 1) / 2 + h) + lane]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = h; t < NT; ++t) u[t] = mfma32(tf[t][r], x[h][r], u[t]);
     }
     float odd = 0.0f;  // NaN once a value is not finite
 #pragma unroll
@@ -1172,7 +1143,7 @@ Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, in
 
 int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ahead<false>::C; }
 
-// What is worked out ahead takes 13 KiB a chunk and head (bf16; 4 KiB fp32):
+// What is worked out ahead takes 11 KiB a chunk and head (bf16; 4 KiB fp32):
 // past 1 GiB of it the heads run in several launches.
 DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items, size_t heads, size_t d_key, size_t d_val) {
   DeltaScratch s;
