@@ -142,16 +142,14 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
     if (lane == 0) s_bound = b;
   }
   // A NaN makes the sum NaN; a slice of nothing else and -inf has no sum.
+  const float base = most > -INFINITY ? most : 0.0f;
   double sum = 0.0;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     asm volatile("" : "+v"(raw[k]));  // widened again: kept, the elements would take twice the registers
     float part = 0.0f;                // few terms in fp32, these sums in 64 bits
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float v = elem<T>(raw[k], j);
-      part += most > -INFINITY ? __builtin_amdgcn_exp2f((v - most) * kLog2e) : v != v ? v : 0.0f;
-    }
+    for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((elem<T>(raw[k], j) - base) * kLog2e);
     sum += part;
   }
 #pragma unroll
