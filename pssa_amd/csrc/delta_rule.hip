@@ -314,32 +314,54 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
     }
   }
   __syncthreads();
-  // The inverse of the wave's diagonal block, over its block: each row as soon
-  // as it is known leaves the rows below.
+  // The inverse of the wave's diagonal block, over its block.  First of its two
+  // halves of 8 x 8, a column a lane: each row as soon as it is known leaves the
+  // rows below (16 x 16 at once takes three times the products, and registers
+  // that let three waves share a SIMD).
   {
     float* block = s_a + 16 * wave * LD + 16 * wave;
-    float x[16];
+    const float* half = block + (col >> 3) * 8 * (LD + 1);
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = i == col ? 1.0f : 0.0f;
+    for (int i = 0; i < 8; ++i) x[i] = i == (col & 7) ? 1.0f : 0.0f;
     auto leave = [&](auto first) {
       constexpr int J = decltype(first)::value;
-      f32x4_t w[16 - J];
+      f32x4_t w[8 - J];
 #pragma unroll
-      for (int i = 1; i < 16 - J; ++i) w[i] = *reinterpret_cast<const f32x4_t*>(block + (J + i) * LD + J);
+      for (int i = 1; i < 8 - J; ++i) w[i] = *reinterpret_cast<const f32x4_t*>(half + (J + i) * LD + J);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 1; i < 16 - J; ++i)
+        for (int i = 1; i < 8 - J; ++i)
           if (i > e) x[J + i] = fmaf(-w[i][e], x[J + e], x[J + i]);
     };
     leave(std::integral_constant<int, 0>{});
     leave(std::integral_constant<int, 4>{});
-    leave(std::integral_constant<int, 8>{});
-    leave(std::integral_constant<int, 12>{});
     wave_sync();
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (quad == (i & 3)) block[i * LD + col] = x[i];
+    for (int i = 0; i < 8; ++i)
+      if (quad == (i & 3)) block[((col & 8) + i) * LD + col] = x[i];
+    wave_sync();
+    // The block between them: -X2 (A21 X1), an element a lane; the block above
+    // holds A21 X1 meanwhile.
+    const int r = lane >> 3, c = lane & 7;
+    auto times = [&](const float* left, const float* right) {
+      const f32x4_t l0 = *reinterpret_cast<const f32x4_t*>(left + r * LD), l1 = *reinterpret_cast<const f32x4_t*>(left + r * LD + 4);
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(l0[e], right[e * LD + c], sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fmaf(l1[e], right[(4 + e) * LD + c], sum);
+      return sum;
+    };
+    const float y = times(block + 8 * LD, block);
+    wave_sync();
+    block[r * LD + 8 + c] = y;
+    wave_sync();
+    const float z = times(block + 8 * LD + 8, block + 8);
+    wave_sync();
+    block[(8 + r) * LD + c] = -z;
+    block[r * LD + 8 + c] = 0.0f;
   }
   __syncthreads();
   // The wave's column of blocks.
