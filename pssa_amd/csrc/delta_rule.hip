@@ -487,11 +487,12 @@ __device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
 // A segment's own state and its transition need no outputs, and two waves bring
 // their chunks, so that two workgroups fit a compute unit.  The transition is
 // the state that the unit matrix becomes without values: more columns.
+// (Where a segment's own bf16 walk takes over 168 registers, only one of the two fits.)
 constexpr int kWalkers = 4;
 template <int MODE>
 constexpr int kHelpers = MODE == DR_LOCAL ? 2 : 8;
 template <bool B16, int DKP, int MODE>
-__global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>)) void delta_walk_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL ? 1 : B16 || DKP < 128 ? 3 : 2) void delta_walk_kernel(DeltaArgs a) {
   constexpr bool LOCAL = MODE == DR_LOCAL;
   using In = Ahead<B16>;
   using Lds = WalkLds<B16, DKP, LOCAL>;
