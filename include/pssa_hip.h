@@ -736,8 +736,11 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
  * above.  out may lie in the buffer of q, k and v in columns of its own (same
  * row stride) and must not overlap them, the gates or a state otherwise.
  * d_key <= 128, d_val <= 4096, n_seqs and heads <= 65535, row strides below
- * 2^24.  A value that is not finite reaches the outputs from its own token on
- * and no earlier one. */
+ * 2^24.  The states are those of fp32 products and sums for both types; a bf16
+ * call of more than 4 tokens takes the state that a chunk of 64 is entered with,
+ * the corrections of its tokens and their weights in two bf16 parts for the
+ * outputs, up to 2^-16 of each value off.  A value that is not finite reaches
+ * the outputs from its own token on and no earlier one. */
 int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
                                  size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,
                                  const float* d_beta, size_t ld_gates, const float* d_state_in, const uint64_t* lens,
@@ -745,7 +748,9 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
                                  size_t d_val, float scale, void* d_out, size_t ld_out, float* d_state_out, char* err,
                                  size_t err_len);
 /* Grows the context's scratch (synchronously) to what such a call needs, so
- * that it then allocates nothing and stays asynchronous. */
+ * that it then allocates nothing and stays asynchronous.  More than 256
+ * sequences of unequal lengths take a table of 8 (n_seqs + 1) bytes (12 where
+ * the call is split), which goes there as linear attention's does. */
 int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,
                                 size_t heads, size_t d_key, size_t d_val, char* err, size_t err_len);
 
@@ -787,13 +792,13 @@ int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, 
  * each (row g*beams + b at d_logits + row*ld), the `keep` best of
  *   scores[g][b] + log softmax(logits[row])[v]
  * over b and v, in descending order, equal ones by beam, then by token:
- * d_parents (the beam b), d_tokens (v) and d_out_scores [groups, keep].  The
- * values are computed in 64 bits and rounded once.  d_last [groups, beams] or
+ * d_parents (the beam b), d_tokens (v) and d_out_scores [groups, keep].  Sums
+ * and values are computed in 64 bits, of exponentials in fp32, and rounded once.  d_last [groups, beams] or
  * NULL: a beam whose last token is `eos` has ended and has one candidate, eos
  * with its score as it is; its logits are not read.  A beam whose score is not
  * finite, or whose logits hold a NaN or +inf or nothing but -inf, has none, and
  * neither has a token with -inf; places left over hold PSSA_HIP_NO_TOKEN twice and
- * -inf.  beams and keep <= 64.  With keep = beams, d_out_scores may be d_scores
+ * -inf.  beams and keep <= 64, groups * beams < 2^24.  With keep = beams, d_out_scores may be d_scores
  * and d_tokens d_last; outputs must not overlap anything otherwise. */
 int pssa_hip_beam_select_resident(pssa_hip_ctx* ctx, const void* d_logits, int dtype, size_t groups, size_t beams,
                                   size_t vocab, size_t ld, const float* d_scores, const uint32_t* d_last, uint32_t eos,

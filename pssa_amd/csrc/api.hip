@@ -2606,10 +2606,11 @@ Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len
     chunks += (len + chunk - 1) / chunk;
     items += segments(len);
   }
+  PSSA_RETURN_IF(need(chunks < ((size_t)1 << 24), "delta rule: too many tokens"));
   a.chunks = (int)chunks;
   a.items = (int)items;
   a.uniform_segs = (int)segments(p.longest);
-  if (chunked) p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, seg ? items : 0, heads, d_key, d_val);
+  if (chunked) p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, n_seqs, seg ? items : 0, heads, d_key, d_val);
   return Status::Ok();
 }
 Status check_delta_heads(size_t heads, size_t d_key, size_t d_val) {
@@ -2647,7 +2648,7 @@ Status check_beams(size_t groups, size_t beams, size_t vocab, size_t keep) {
   PSSA_RETURN_IF(need(groups && vocab, "beam selection: dimensions must be positive"));
   PSSA_RETURN_IF(need(beams >= 1 && beams <= (size_t)pssa::kMaxBeams && keep >= 1 && keep <= (size_t)pssa::kMaxBeams,
                       "beam selection: beams and keep must be in 1..=64"));
-  return need(vocab <= ((size_t)1 << 24) && groups <= INT32_MAX / pssa::kMaxBeams, "beam selection: too large");
+  return need(vocab <= ((size_t)1 << 24) && groups <= (((size_t)1 << 24) - 1) / beams, "beam selection: too large");
 }
 
 // The selection of one step on the context's stream, its scratch grown to what it needs.

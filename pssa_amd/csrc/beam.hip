@@ -388,6 +388,7 @@ __global__ __launch_bounds__(kThreads) void beam_feed_kernel(const uint32_t* tok
 template <class V, int MOST>
 Status launch_pieces(hipStream_t stream, const GatherArgs& a) {
   const size_t pieces = a.row_bytes / sizeof(V);
+  if (pieces >> 32) return Status::Invalid("beam states: too large");
   const dim3 grid((uint32_t)((pieces + kThreads - 1) / kThreads), (uint32_t)std::min(a.groups, 65535));
   beam_gather_kernel<V, MOST><<<grid, kThreads, 0, stream>>>(a);
   PSSA_LAUNCH_CHECK("beam_gather_kernel");

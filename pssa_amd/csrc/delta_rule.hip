@@ -1167,12 +1167,15 @@ Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, in
 int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ahead<false>::C; }
 
 // What is worked out ahead takes 11 KiB a chunk and head (bf16; 4 KiB fp32):
-// past 1 GiB of it the heads run in several launches.
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items, size_t heads, size_t d_key, size_t d_val) {
+// past 1 GiB of it the heads run in several launches, and where a launch would
+// have 2^32 threads.
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key,
+                           size_t d_val) {
   DeltaScratch s;
   const size_t size = dtype == PSSA_HIP_BF16 ? 2 : 4, unit = unit_of(dtype);
   const size_t one = chunks * 16 * (dtype == PSSA_HIP_BF16 ? Ahead<true>::kUnits : Ahead<false>::kUnits);
-  s.heads_here = (int)std::max<size_t>(1, std::min(heads, ((size_t)1 << 30) / std::max<size_t>(one, 1)));
+  const size_t walks = std::max(n_seqs, items) * ((d_val + 63) / 64 + (items ? (d_key + 63) / 64 : 0));
+  s.heads_here = (int)std::max<size_t>(1, std::min({heads, ((size_t)1 << 30) / std::max<size_t>(one, 1), 5000000 / walks}));
   s.ahead = (one * s.heads_here + 255) & ~(size_t)255;
   const size_t keys = d_key <= 32 ? 32 : d_key <= 64 ? 64 : 128;  // as the kernels hold them
   s.state = items * s.heads_here * keys * whole(d_val, 16) * 4;

@@ -167,7 +167,9 @@ struct DeltaScratch {
   size_t ahead = 0, rows = 0, state = 0, move = 0;  // bytes
   int heads_here = 0;                               // heads of a launch
 };
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t items, size_t heads, size_t d_key, size_t d_val);
+// `items` segments, 0 where the call is not split.
+DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key,
+                           size_t d_val);
 // Chunks of a segment where a call of these sizes is split, else 0.
 int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val);
 Status init_delta_attributes();

@@ -217,6 +217,15 @@ def test_matmul_i8(hip, m, n, k):
     check_i8(hip, m, n, k, "bf16", pads=(-k % 4, -k % 4, 1), offset=4)
 
 
+@pytest.mark.parametrize("m,n,k", [(3300, 4200, 272), (2000, 2500, 528), (1025, 2100, 1000), (70, 16400, 16)])
+def test_matmul_i8_of_many_tiles(hip, m, n, k):
+    """Each size of tiles, and k that ends in a slab's first and later units."""
+    say("i8 tiles", m, n, k)
+    check_i8(hip, m, n, k)
+    check_i8(hip, m, n, k, "bf16", pads=(16, 0, 3))
+    check_i8(hip, m, n, k, "bf16", pads=(3, 1, 5), offset=1)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 64, 131071), (2, 2, 131071), (130, 130, 2048)])
 def test_matmul_i8_of_the_largest_codes(hip, m, n, k):
     """Sums of -128 squared: the largest that 32 bits hold."""
@@ -333,7 +342,8 @@ def run_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, scale, layout="pack
 
 def delta_steps(dk, dtype):
     """Roundings of a step, in u: sums over d_key and a chunk's 64 tokens with some across lanes, the exponentials, the
-    factors; in bf16 three products in a row of operands held in two bf16 parts, 2^-17 of each."""
+    factors; in bf16 three products in a row of operands held in two bf16 parts, 2^-17 of each (outputs; states have
+    none)."""
     return 2 * (dk + 64) + 32 + (3 * 2 * 2.0 ** -17 / U32 if dtype == "bf16" else 0)
 
 
@@ -344,7 +354,7 @@ def check_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, scale=0.5, **kw):
                                       c["state"], heads, key_heads)
     steps = delta_steps(dk, dtype) * U32
     within(out, want, steps * oerr + (U16 if dtype == "bf16" else U32) * np.abs(want), "outputs")
-    within(S, state, steps * serr[:, :, None, :] + U32 * np.abs(state), "states")
+    within(S, state, delta_steps(dk, "f32") * U32 * serr[:, :, None, :] + U32 * np.abs(state), "states")
 
 
 DELTA_SHAPES = [  # lens, heads, key heads, d_key, d_val
@@ -787,3 +797,124 @@ def test_two_contexts_at_once(hip):
             check_i8(hip, 40, 40, 20000)
     finally:
         other.close()
+
+
+# ---------------------------------------------------------------------------
+# Offsets past 31 and 32 bits
+
+
+class Far(Held):
+    """Arrays of rows far apart, of which only the rows are written and read."""
+
+    def rows(self, values, ld):
+        b = self.dev.empty(((len(values) - 1) * ld + values.shape[1],), values.dtype)
+        self.bufs.append(b)
+        for i, row in enumerate(values):
+            b.write(row, i * ld * values.itemsize)
+        return b
+
+    def back(self, buf, n, width, ld):
+        out = np.empty((n, width), buf.dtype)
+        for i in range(n):
+            _abi.call(self.dev._lib.pssa_hip_memcpy, self.dev.handle, out[i].ctypes.data, buf.ptr + i * ld * out.itemsize,
+                      out[i].nbytes, _abi.D2H)
+        return out
+
+
+def test_norm_rows_far_apart(hip):
+    rng = np.random.default_rng(61)
+    rows, width, ld = 3, 100, 2 ** 31 - 1
+    stored, held = to_bf16(stream(rng, rows, width))
+    g = rng.normal(1, 0.2, width).astype(np.float32)
+    with Far(hip) as h:
+        x, codes = h.rows(stored, ld), h.rows(np.zeros((rows, width), np.int8), ld)
+        dg, sc, out = h.up(g), h.new(rows, np.float32, 0), h.new((rows, width), np.uint16, 0)
+        hip.rms_norm_resident(x.ptr, "bf16", rows, width, dg.ptr, sum_ptr=x.ptr, out_ptr=out.ptr, codes_ptr=codes.ptr,
+                              scales_ptr=sc.ptr, ld_x=ld, ld_sum=ld, ld_codes=ld)
+        hip.synchronize()
+        np.testing.assert_array_equal(h.back(x, rows, width, ld), stored)  # no residual: the sum is x
+        np.testing.assert_array_equal(h.back(codes, rows, width, ld), codes32((held * g).astype(np.float32))[0])
+        h64 = held.astype(np.float64)
+        want = h64 / np.sqrt((h64 ** 2).mean(1, keepdims=True) + 1e-5) * g
+        within(from_bf16(out.to_host()), want, np.abs(want) * (45 * U32 + U16), "out")
+
+
+@pytest.mark.parametrize("m,ld", [(3, 2 ** 24), (70, 2 ** 24), (70, 2 ** 24 + 16)])
+def test_matmul_i8_rows_far_apart(hip, m, ld):
+    rng = np.random.default_rng(62)
+    n, k = 300, 80
+    x, w = rng.integers(-128, 128, (m, k)).astype(np.int8), rng.integers(-128, 128, (n, k)).astype(np.int8)
+    with Far(hip) as h:
+        dx, dw, ones, y = h.rows(x, ld), h.rows(w, ld), h.up(np.ones(max(m, n), np.float32)), h.new((m, n), np.float32, 0)
+        hip.matmul_i8_resident(dx.ptr, ones.ptr, dw.ptr, ones.ptr, m, n, k, y.ptr, ld_x=ld, ld_w=ld)
+        hip.synchronize()
+        np.testing.assert_array_equal(y.to_host(), x.astype(np.float64) @ w.astype(np.float64).T)  # below 2^24: exact
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_delta_rule_rows_far_apart(hip, dtype):
+    rng = np.random.default_rng(63)
+    n, ld = 150, 2 ** 24 - 8
+    c = delta_case(rng, [n], 1, 1, 64, 64, False)
+    (sq, hq), (sk, hk), (sv, hv) = (typed(c[x].reshape(n, 64), dtype) for x in "qkv")
+    gates = np.concatenate([c["g"], c["beta"]], 1).astype(np.float32)
+    with Far(hip) as h:
+        q, k, v, out = h.up(sq), h.rows(sk, ld), h.rows(sv, ld), h.rows(np.zeros((n, 64), sv.dtype), ld)
+        dg = h.up(gates)
+        hip.delta_rule_resident(q.ptr, k.ptr, v.ptr, dg.ptr, dg.ptr + 4, dtype, 1, 64, 64, out.ptr, n_seqs=1, seq_len=n,
+                                scale=0.5, ld_k=ld, ld_v=ld, ld_gates=2, ld_out=ld)
+        hip.synchronize()
+        got = h.back(out, n, 64, ld)
+    got = from_bf16(got) if dtype == "bf16" else got
+    q, k, v = (a.astype(np.float64).reshape(n, 1, 64) for a in (hq, hk, hv))
+    want, _, oerr, _ = delta64(q, k, v, gates[:, :1].astype(np.float64), gates[:, 1:].astype(np.float64), 0.5, [n], None, 1, 1)
+    within(got.reshape(want.shape), want, delta_steps(64, dtype) * U32 * oerr + (U16 if dtype == "bf16" else U32) * np.abs(want), "outputs")
+
+
+def test_beams_far_apart(hip):
+    rng = np.random.default_rng(64)
+    beams, vocab, ld = 9, 1000, 2 ** 28 + 1
+    stored, held = to_bf16(rng.normal(0, 2.5, (beams, vocab)))
+    scores = rng.normal(-20, 1, beams).astype(np.float32)
+    with Far(hip) as h:
+        z, sc = h.rows(stored, ld), h.up(scores)
+        par, tok, out = h.new(beams, np.uint32, 7), h.new(beams, np.uint32, 7), h.new(beams, np.float32, 7)
+        hip.beam_select_resident(z.ptr, "bf16", 1, beams, vocab, sc.ptr, beams, par.ptr, tok.ptr, out.ptr, ld=ld)
+        hip.synchronize()
+        val = candidates64(held, scores, None, NONE).ravel()
+        order = np.argsort(-val, kind="stable")[:beams]
+        np.testing.assert_array_equal(par.to_host().astype(np.int64) * vocab + tok.to_host(), order)
+        within(out.to_host(), val[order], U32 * np.abs(val[order]) + 4 * U32, "scores")
+        src, parents = rng.integers(0, 256, (3, 48)).astype(np.uint8), np.array([2, 2, 0], np.uint32)
+        far = 2 ** 31 + 16
+        a, dp, b = h.rows(src, far), h.up(parents), h.new((3, 48), np.uint8, 0)
+        hip.beam_gather_resident(a.ptr, b.ptr, 48, 1, 3, dp.ptr, 3, ld_src=far, ld_dst=48)
+        hip.beam_gather_resident(a.ptr, a.ptr, 48, 1, 3, dp.ptr, 3, ld_src=far, ld_dst=far)
+        hip.synchronize()
+        np.testing.assert_array_equal(b.to_host(), src[parents])
+        np.testing.assert_array_equal(h.back(a, 3, 48, far), src[parents])
+
+
+def test_calls_one_behind_another(hip):
+    """Calls that share the scratch, in a row without a wait, two rounds of them: the second equals the first."""
+    rng = np.random.default_rng(65)
+    m, n, k, t, heads, vocab = 100, 500, 5000, 300, 2, 4000
+    with Held(hip) as h:
+        x, w, s = h.up(rng.integers(-128, 128, (m, k)).astype(np.int8)), h.up(rng.integers(-128, 128, (n, k)).astype(np.int8)), h.up(rng.uniform(0.1, 1, n).astype(np.float32))
+        q, kk, v = (h.up(typed(rng.normal(0, 0.1, (t, heads * 64)), "bf16")[0]) for _ in range(3))
+        g = h.up(np.concatenate([-rng.exponential(0.1, (t, heads)), rng.uniform(0, 1, (t, heads))], 1).astype(np.float32))
+        z, sc = h.up(rng.normal(0, 2, (4, vocab)).astype(np.float32)), h.up(np.zeros(4, np.float32))
+        outs = []
+        for _ in range(2):
+            y, o, S = h.new((m, n), np.float32, 0), h.new((t, heads * 64), np.uint16, 0), h.new((1, heads, 64, 64), np.float32, 0)
+            par, tok, best = h.new(4, np.uint32, 0), h.new(4, np.uint32, 0), h.new(4, np.float32, 0)
+            hip.matmul_i8_resident(x.ptr, s.ptr, w.ptr, s.ptr, m, n, k, y.ptr)
+            hip.delta_rule_resident(q.ptr, kk.ptr, v.ptr, g.ptr, g.ptr + 4 * heads, "bf16", heads, 64, 64, o.ptr, n_seqs=1,
+                                    seq_len=t, ld_gates=2 * heads, state_out_ptr=S.ptr)
+            hip.beam_select_resident(z.ptr, "f32", 1, 4, vocab, sc.ptr, 4, par.ptr, tok.ptr, best.ptr)
+            outs.append([y, o, S, par, tok, best])
+        hip.synchronize()
+        for a, b in zip(*outs):
+            np.testing.assert_array_equal(a.to_host(), b.to_host())
+        want = (x.to_host().astype(np.float64) @ w.to_host().astype(np.float64).T) * s.to_host()[:m, None].astype(np.float64) * s.to_host().astype(np.float64)
+        within(outs[0][0].to_host(), want, np.abs(want) * 3.01 * U32, "product")

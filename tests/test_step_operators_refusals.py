@@ -90,7 +90,7 @@ DELTA = dict(ctx=None, dtype=_abi.F32, q=P, ld_q=32, k=P + 0x10000, ld_k=32, v=P
     ({"dtype": 3}, "unknown dtype"), ({"heads": 0}, "positive"), ({"d_val": 0}, "positive"), ({"key_heads": 0}, "divide"),
     ({"key_heads": 3}, "divide"), ({"d_key": 129}, "128"), ({"d_val": 4097}, "4096"), ({"heads": 65536, "key_heads": 1}, "65535"),
     ({"n_seqs": 0}, "sequences"), ({"n_seqs": 65536}, "sequences"), ({"seq_len": 1 << 31}, "too many tokens"),
-    ({"n_seqs": 60000, "seq_len": 1 << 20}, "too many tokens"), ({"ld_q": 31}, "row stride"), ({"ld_k": 31}, "row stride"),
+    ({"n_seqs": 60000, "seq_len": 1 << 20}, "too many tokens"), ({"n_seqs": 1, "seq_len": 1 << 30}, "too many tokens"), ({"ld_q": 31}, "row stride"), ({"ld_k": 31}, "row stride"),
     ({"ld_v": 95}, "row stride"), ({"ld_out": 95}, "row stride"), ({"ld_gates": 3}, "row stride"), ({"ld_k": 1 << 24}, "2^24"),
     ({"scale": float("nan")}, "scale"), ({"q": P + 2}, "misaligned"), ({"beta": P + 0x38002}, "misaligned"),
     ({"state_out": P + 0x50002}, "misaligned"), ({"out": P}, "overlaps its inputs"), ({"out": P + 0x30000}, "overlaps its inputs"),
@@ -123,7 +123,7 @@ BEAM = dict(ctx=None, logits=P, dtype=_abi.F32, groups=2, beams=4, vocab=100, ld
     ({"last": None}, "null context"), ({"dtype": 4}, "unknown dtype"), ({"groups": 0}, "positive"), ({"vocab": 0}, "positive"),
     ({"beams": 0}, "1..=64"), ({"beams": 65}, "1..=64"), ({"keep": 0}, "1..=64"), ({"keep": 65}, "1..=64"),
     ({"ld": 99}, "row stride"), ({"vocab": (1 << 24) + 1, "ld": 1 << 25}, "too large"), ({"groups": 1 << 40}, "too large"),
-    ({"logits": P + 2}, "misaligned"), ({"parents": P + 0x10202}, "misaligned"),
+    ({"groups": 1 << 22}, "too large"), ({"logits": P + 2}, "misaligned"), ({"parents": P + 0x10202}, "misaligned"),
     ({"out_scores": P + 0x10000, "tokens": P + 0x10100}, "null context"), ({"out_scores": P + 0x10000, "keep": 3}, "overlaps an input"),
     ({"out_scores": P + 0x10004}, "overlaps an input"), ({"tokens": P + 0x10000}, "overlaps an input"),
     ({"parents": P + 0x10100}, "overlaps an input"), ({"parents": P}, "overlaps an input"), ({"tokens": P + 0x10200}, "outputs overlap")])
