@@ -953,13 +953,14 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
             S[b] = mfma32(element32<DKP>(K32, 16 * t + 4 * quad + r, 16 * b + col), u[t][r], S[b]);
     }
   }
-  if (LOCAL && moves) {  // whole rows and columns, zeros past d_key
-    float* move = a.seg_move + item_head * DKP * DKP + j;
+  if (LOCAL && moves) {  // whole rows and columns, zeros past d_key, as the scan's lanes read them: 16 bytes each
+    const int k = B16 ? j / 32 * 2 + (j >> 2 & 1) : j / 16, at = B16 ? j >> 3 & 3 : j >> 2 & 3;  // j = state_row(k, at, j % 4)
+    float* move = a.seg_move + item_head * DKP * DKP + (k * 64 + at * 16 + 4 * quad) * 4 + j % 4;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (j < DKP) move[state_row<B16>(b, quad, r) * DKP] = S[b][r];
+        if (j < DKP) move[(b * NB * 64 + r) * 4] = S[b][r];
   } else if (LOCAL) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -1012,9 +1013,9 @@ __global__ __launch_bounds__(64 * kScanWaves<DKP>) void delta_scan_kernel(DeltaA
       const int b = wave + WAVES * m;
       p.own[m] = own[item * own_step + 64 * b];
       // Operands: the lane's row of tile b, columns as a tile's rows lie.
-      const float* row = move + item * move_step + state_row<B16>(b, col >> 2, col & 3) * DKP;
+      const f32x4_t* at = reinterpret_cast<const f32x4_t*>(move + item * move_step) + b * NB * 64 + lane;
 #pragma unroll
-      for (int k = 0; k < NB; ++k) p.move[m][k] = *reinterpret_cast<const f32x4_t*>(row + state_row<B16>(k, quad, 0));
+      for (int k = 0; k < NB; ++k) p.move[m][k] = at[64 * k];
     }
   };
   auto step = [&](int item, const Part& p) {
