@@ -45,21 +45,39 @@ __device__ __forceinline__ void store4(T* p, const f32x4_t& v, int left) {
   }
 }
 
-// 16 codes, zeros past `left`.
-__device__ __forceinline__ i32x4_t load16(const int8_t* p, int left) {
-  if (left >= 16) return *reinterpret_cast<const i32x4_any_t*>(p);
-  i32x4_t v = {0, 0, 0, 0};
+// 16 codes at any byte: the dwords that hold them, moved into place.  A load of
+// 16 bytes that does not begin at a dword takes the L1 several times as long
+// (28 x 183 x 5817: 34 us, so 18).
+__device__ __forceinline__ i32x4_t load_odd(const int8_t* p) {
+  const uintptr_t at = (uintptr_t)p;
+  const i32x4_t v = *reinterpret_cast<const i32x4_any_t*>(at & ~(uintptr_t)3);
+  const int e = *reinterpret_cast<const int*>((at + 15) & ~(uintptr_t)3);
+  const uint32_t by = (uint32_t)at & 3;
+  return i32x4_t{(int)__builtin_amdgcn_alignbyte(v[1], v[0], by), (int)__builtin_amdgcn_alignbyte(v[2], v[1], by),
+                 (int)__builtin_amdgcn_alignbyte(v[3], v[2], by), (int)__builtin_amdgcn_alignbyte(e, v[3], by)};
+}
+// 16 codes of a row of k, zeros past the `left` that the row still has: its last
+// 16 moved down, in one load (byte by byte a row's end took 7 us).
+__device__ __forceinline__ i32x4_t load16(const int8_t* p, int left, int k) {
+  if (k < 16) {  // uniform
+    i32x4_t v = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 15; ++i)
-    if (i < left) v[i >> 2] |= (int)(uint8_t)p[i] << (8 * (i & 3));
-  return v;
+    for (int i = 0; i < 15; ++i)
+      if (i < left) v[i >> 2] |= (int)(uint8_t)p[i] << (8 * (i & 3));
+    return v;
+  }
+  const i32x4_t v = load_odd(p + min(left - 16, 0));
+  const int off = 8 * max(16 - left, 0);  // bits
+  const uint64_t lo = (uint32_t)v[0] | (uint64_t)(uint32_t)v[1] << 32, hi = (uint32_t)v[2] | (uint64_t)(uint32_t)v[3] << 32;
+  const uint64_t l = off >= 128 ? 0 : off >= 64 ? hi >> (off & 63) : off ? lo >> off | hi << (64 - off) : lo, h = off >= 64 ? 0 : hi >> off;
+  return i32x4_t{(int)l, (int)(l >> 32), (int)h, (int)(h >> 32)};
 }
 
 // ---------------------------------------------------------------- few rows
 // A wave multiplies 16 MT rows by 16 NC channels over its part of k: WK waves
 // of a workgroup share the channels, 4 / WK... of them lie side by side, and
-// the parts meet in LDS.  Rows at any byte.
-template <class T, int MT, int NC, int WK>
+// the parts meet in LDS.  Rows at any dword, or (ODD) at any byte.
+template <class T, int MT, int NC, int WK, bool ODD>
 __global__ __launch_bounds__(256) void matmul_i8_rows_kernel(I8Args a) {
   constexpr int WN = 4 / WK, DEEP = MT * NC >= 4 ? 2 : 4;  // steps of 64 codes whose loads are in flight together
   __shared__ i32x4_t s_acc[WK > 1 ? (WK - 1) * MT * NC * 64 : 1];
@@ -77,15 +95,16 @@ __global__ __launch_bounds__(256) void matmul_i8_rows_kernel(I8Args a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[c][t] = i32x4_t{0, 0, 0, 0};
   const int steps = a.k / 64, first = wk * steps / WK, last = (wk + 1) * steps / WK;
+  auto load = [&](const int8_t* p) { return ODD ? load_odd(p) : *reinterpret_cast<const i32x4_any_t*>(p); };
   auto some = [&](int s, auto n) {
     constexpr int N = decltype(n)::value;
     i32x4_t xf[N][MT], wf[N][NC];
 #pragma unroll
     for (int d = 0; d < N; ++d) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) wf[d][c] = *reinterpret_cast<const i32x4_any_t*>(w[c] + 64 * (s + d));
+      for (int c = 0; c < NC; ++c) wf[d][c] = load(w[c] + 64 * (s + d));
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xf[d][t] = *reinterpret_cast<const i32x4_any_t*>(x[t] + 64 * (s + d));
+      for (int t = 0; t < MT; ++t) xf[d][t] = load(x[t] + 64 * (s + d));
     }
 #pragma unroll
     for (int d = 0; d < N; ++d)
@@ -101,9 +120,9 @@ __global__ __launch_bounds__(256) void matmul_i8_rows_kernel(I8Args a) {
     const int left = a.k - 64 * steps - 16 * quad;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const i32x4_t wf = load16(w[c] + 64 * steps, left);
+      const i32x4_t wf = load16(w[c] + 64 * steps, left, a.k);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, load16(x[t] + 64 * steps, left), acc[c][t], 0, 0, 0);
+      for (int t = 0; t < MT; ++t) acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, load16(x[t] + 64 * steps, left, a.k), acc[c][t], 0, 0, 0);
     }
   }
   if constexpr (WK > 1) {
@@ -371,25 +390,34 @@ __global__ __launch_bounds__(256) void i8_pack_kernel(Packed x, Packed w, int k,
   if (at >= (size_t)p.rows * units) return;
   const size_t row = at / units;
   const int u = (int)(at - row * units);
-  *reinterpret_cast<i32x4_t*>(p.dst + (row * units + u) * 16) = load16(p.src + row * p.ld + 16 * u, k - 16 * u);
+  *reinterpret_cast<i32x4_t*>(p.dst + (row * units + u) * 16) = load16(p.src + row * p.ld + 16 * u, k - 16 * u, k);
 }
 
-template <class T, int MT, int NC>
+template <class T, int MT, int NC, bool ODD>
 Status launch_rows_of(hipStream_t stream, const I8Args& a) {
   const int tiles = (a.n + 16 * NC - 1) / (16 * NC), rows = (a.m + 16 * MT - 1) / (16 * MT);
   // A workgroup's four waves share the channels of one tile where the tiles alone would not fill the machine.
   if (tiles * rows >= 2048)
-    matmul_i8_rows_kernel<T, MT, NC, 1><<<dim3((tiles + 3) / 4, rows), 256, 0, stream>>>(a);
+    matmul_i8_rows_kernel<T, MT, NC, 1, ODD><<<dim3((tiles + 3) / 4, rows), 256, 0, stream>>>(a);
   else
-    matmul_i8_rows_kernel<T, MT, NC, 4><<<dim3(tiles, rows), 256, 0, stream>>>(a);
+    matmul_i8_rows_kernel<T, MT, NC, 4, ODD><<<dim3(tiles, rows), 256, 0, stream>>>(a);
   PSSA_LAUNCH_CHECK("matmul_i8_rows_kernel");
   return Status::Ok();
 }
+template <class T, bool ODD>
+Status launch_few_at(hipStream_t stream, const I8Args& a) {
+  // 32 channels a workgroup leave most of the machine idle below some 2000 of
+  // them: 16 by 16 rows read the codes more often, in more places at once (64 x
+  // 2048 x 4096: 14.7 -> 9.1 us, 28 x 183 x 5817: 18 -> 9.5; 64 x 4096 x 4096 would
+  // lose a tenth).
+  if (a.m <= 16 || a.n <= 2048) return launch_rows_of<T, 1, 1, ODD>(stream, a);
+  if (a.m <= 32) return launch_rows_of<T, 2, 2, ODD>(stream, a);
+  return launch_rows_of<T, 4, 2, ODD>(stream, a);
+}
 template <class T>
 Status launch_few(hipStream_t stream, const I8Args& a) {
-  if (a.m <= 16) return launch_rows_of<T, 1, 1>(stream, a);
-  if (a.m <= 32) return launch_rows_of<T, 2, 2>(stream, a);
-  return launch_rows_of<T, 4, 2>(stream, a);
+  const bool odd = ((uintptr_t)a.x | a.ld_x | (uintptr_t)a.w | a.ld_w) % 4 != 0;
+  return odd ? launch_few_at<T, true>(stream, a) : launch_few_at<T, false>(stream, a);
 }
 
 template <class T, int BM, int BN, int WM, int WN, int R>
