@@ -60,7 +60,9 @@ __device__ __forceinline__ Span span_of(const DeltaArgs& a, int seq) {
 
 // The recurrence itself, the state read and written once.  A workgroup's
 // threads lie over 64 of the state's columns, four each, and its rows, 16
-// apart: 16 x 16.  k S and q S of a token meet in LDS together.
+// apart: 16 x 16.  k S and q S of a token meet in LDS together.  Bound by the
+// states' way through memory: 256 streams of one token, 12 heads of 64 x 64, 22.5
+// us, 4.5 TB/s.
 template <class T, int ROWS>
 __global__ __launch_bounds__(256) void delta_steps_kernel(DeltaArgs a) {
   __shared__ float s_kq[2][2][kDeltaMaxKey];
@@ -253,6 +255,8 @@ __device__ __forceinline__ float decay_between(double gi, double gj, bool on) {
 // each wave inverts one of its diagonal blocks by substitution, a column a
 // lane, and follows one column of blocks down:
 //   T_rc = -D_r sum_j A_rj T_jc, c <= j < r.
+// Some 7 us a workgroup's way, six of them to a compute unit: 3072 chunks and heads
+// of 64 in 23 us, waits between its steps, no unit over a third busy.
 template <bool B16, int DKP>
 __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs a) {
   using Out = Ahead<B16>;
@@ -483,7 +487,9 @@ __device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
 // four turn the S and U that they are handed into outputs, and these eight
 // work out P, so that nothing but the states' own chain runs from chunk to
 // chunk (where the same waves did all, issuing the loads alone took 2.3 of a
-// chunk's 5.7 us, heads of 128).
+// chunk's 5.7 us, heads of 128).  A chunk takes 3 us at heads of 64, 4.5 at 128:
+// the chain's matrix products 0.9 and 1.2 us, the rest its LDS reads, splits and
+// two meetings; matrix cores and VALU are 0.3 busy each.
 // A segment's own state and its transition need no outputs, and two waves bring
 // their chunks, so that two workgroups fit a compute unit.  The transition is
 // the state that the unit matrix becomes without values: more columns.
@@ -980,8 +986,8 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
 // its own state; every segment's own state becomes its entry state, and the
 // last one's exit is the sequence's.  A workgroup takes 16 columns, a wave one
 // of the state's tiles; products in fp32.  The matrices of the next segments
-// are on their way meanwhile; a step of 128 x 128 still takes 2.7 us, in which
-// a compute unit reads its 64 KiB (25 bytes a ns).
+// are on their way meanwhile; a step of 128 x 128 still takes 1.7 us, in which
+// a compute unit reads its 64 KiB (2.3 us while a load's lanes lay in 64 places).
 template <int DKP>
 constexpr int kScanWaves = DKP / 16;
 template <bool B16, int DKP>
@@ -1199,9 +1205,12 @@ Status init_delta_attributes() {
 
 // A walk's chunk takes about 3.1 us, one of a segment's own state 2.3 us, a
 // step of the scan over the segments 1.5 us, and the passes between some 12 us
-// (figures at the machine's 256 compute units, a workgroup each).  A call is
+// (at heads of 64 and the machine's 256 compute units, a workgroup each; wider
+// heads take half as much again of all, which leaves the choice).  A call is
 // split where that makes it the faster, into segments of whichever length
-// costs least.
+// costs least: ten calls of 600 to 16 x 1000 tokens ran within 5% of the best of
+// segments of 4, 8, 12, 16 and 32 chunks and of none (8192 tokens, 8 heads of 128:
+// 132 us, unsplit 480; 600 tokens, 2 heads of 64: 29 us, unsplit 34).
 constexpr size_t kComputeUnits = 256;
 int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val) {
   const size_t chunk = (size_t)delta_chunk(dtype), most = (longest + chunk - 1) / chunk;
