@@ -255,8 +255,8 @@ __device__ __forceinline__ float decay_between(double gi, double gj, bool on) {
 // each wave inverts one of its diagonal blocks by substitution, a column a
 // lane, and follows one column of blocks down:
 //   T_rc = -D_r sum_j A_rj T_jc, c <= j < r.
-// Some 7 us a workgroup's way, six of them to a compute unit: 3072 chunks and heads
-// of 64 in 23 us, waits between its steps, no unit over a third busy.
+// Some 7 us a workgroup's way, six of them to a compute unit: 16 x 1024 tokens, 12
+// heads of 64 in 23 us, waits between its steps, no unit over a third busy.
 template <bool B16, int DKP>
 __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs a) {
   using Out = Ahead<B16>;
