@@ -326,7 +326,18 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     return;
   }
   // Rounds that each pick the best candidate left, of which only the winner's
-  // thread looks for its next one.
+  // thread looks for its next one: over all of its own, as values that a large
+  // score has rounded to one lie in the logits' order.
+  auto next = [&](auto left) {
+    Candidate best = nothing();
+    for (int list = list0; list < lists; list += step)
+      for (int r = sub; r < a.keep; r += each) {
+        const Candidate c = candidate(list, r);
+        if (left(c) && better(c, best)) best = c;
+      }
+    return best;
+  };
+  mine = next([](const Candidate&) { return true; });
   for (int j = 0; j < a.keep; ++j) {
     Candidate w = mine;
 #pragma unroll
@@ -342,14 +353,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
       if (better(s_part[i], w)) w = s_part[i];
     __syncthreads();
     if (tid == 0) put(j, w);
-    if (w.value > -INFINITY && mine.at == w.at) {
-      mine = nothing();
-      for (int list = list0; list < lists; list += step)
-        for (int r = sub; r < a.keep; r += each) {
-          const Candidate c = candidate(list, r);
-          if (better(w, c) && better(c, mine)) mine = c;
-        }
-    }
+    if (w.value > -INFINITY && mine.at == w.at) mine = next([&](const Candidate& c) { return better(w, c); });
   }
 }
 

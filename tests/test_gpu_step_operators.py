@@ -918,3 +918,18 @@ def test_calls_one_behind_another(hip):
             np.testing.assert_array_equal(a.to_host(), b.to_host())
         want = (x.to_host().astype(np.float64) @ w.to_host().astype(np.float64).T) * s.to_host()[:m, None].astype(np.float64) * s.to_host().astype(np.float64)
         within(outs[0][0].to_host(), want, np.abs(want) * 3.01 * U32, "product")
+
+
+def test_beam_select_of_scores_that_round_the_logits_away(hip):
+    """Values of a beam that are one in 64 bits: as many as there are, each once, in the places' order."""
+    rng = np.random.default_rng(71)
+    for vocab, beams, keep in [(40, 4, 16), (60, 64, 64)]:
+        z = rng.normal(0, 1e-6, (2, beams, vocab)).astype(np.float32)
+        with Held(hip) as h:
+            dz, ds = h.up(z), h.up(np.full((2, beams), -1e14, np.float32))
+            par, tok, out = h.new((2, keep), np.uint32, 7), h.new((2, keep), np.uint32, 7), h.new((2, keep), np.float32, 7.0)
+            hip.beam_select_resident(dz.ptr, "f32", 2, beams, vocab, ds.ptr, keep, par.ptr, tok.ptr, out.ptr)
+            hip.synchronize()
+            got = par.to_host().astype(np.int64) * vocab + tok.to_host()
+            assert (got < beams * vocab).all() and (out.to_host() == np.float32(-1e14)).all()
+            assert (np.diff(got, axis=1) > 0).all()
