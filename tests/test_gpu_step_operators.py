@@ -933,3 +933,55 @@ def test_beam_select_of_scores_that_round_the_logits_away(hip):
             got = par.to_host().astype(np.int64) * vocab + tok.to_host()
             assert (got < beams * vocab).all() and (out.to_host() == np.float32(-1e14)).all()
             assert (np.diff(got, axis=1) > 0).all()
+
+
+def test_beam_search_of_more_beams_than_tokens(hip):
+    """The first steps leave beams without a candidate, whose lanes run idle until there are enough."""
+    cfg = PSSAConfig(depth=2, d_vocab=4, d_latent=64, d_state=16, d_mem_key=16, mem_capacity=32)
+    w = ModelWeights.init(cfg, 5, "baseline")
+    w.unembed *= 40.0
+    layer = PSSALayer(hip, w, lanes=12, max_tokens=12 * 16)
+    prompts = np.random.default_rng(72).integers(1, 4, (2, 5))
+    for steps in (1, 2, 4):
+        layer.reset_recurrent_state()
+        layer.prefill_inference(prompts)
+        ids, scores = layer.beam_search(steps, 6)
+        want, ws = search64(layer, prompts, 6, steps, NONE)
+        there = np.isfinite(ws)
+        np.testing.assert_array_equal(np.isfinite(scores), there)
+        np.testing.assert_array_equal(ids[there], want[there])
+        assert (ids[~there] == NONE).all()
+        np.testing.assert_allclose(scores[there], ws[there], rtol=0, atol=1e-4 * steps * np.abs(ws[there]).max())
+    layer.close()
+
+
+def test_beam_search_with_bf16_weights(hip):
+    """The beams are different, best first, and have their tokens' summed log probabilities."""
+    layer, steps, beams = small_layer(hip, 8, dtype="bf16"), 5, 4
+    prompts = np.random.default_rng(73).integers(1, 97, (2, 7))
+    layer.prefill_inference(prompts)
+    ids, scores = layer.beam_search(steps, beams)
+    assert (np.diff(scores, axis=1) <= 0).all()
+    for g in range(2):
+        assert len({tuple(t) for t in ids[g].tolist()}) == beams
+        for b in range(beams):
+            total, gate = 0.0, 0.0
+            for t in range(steps):
+                layer.reset_recurrent_state()
+                z = layer.prefill_inference(np.array([list(prompts[g]) + ids[g, b, :t].tolist()]))[0].astype(np.float64)[1:]
+                total += z[ids[g, b, t] - 1] - (np.log(np.exp(z - z.max()).sum()) + z.max())
+                gate += 2 * 2e-2 * np.abs(z).max()  # the bf16 forward's gate, of the logit and of the sum's
+            assert abs(scores[g, b] - total) <= gate
+    layer.close()
+
+
+def test_beam_search_behind_prompts_of_different_lengths(hip):
+    rng = np.random.default_rng(74)
+    prompts = [rng.integers(1, 97, n) for n in (9, 2, 5)]
+    layer = small_layer(hip, 9)
+    layer.prefill_ragged(prompts)
+    ids, scores = layer.beam_search(4, 3)
+    want, ws = search64(layer, prompts, 3, 4, NONE)
+    np.testing.assert_array_equal(ids, want)
+    np.testing.assert_allclose(scores, ws, rtol=0, atol=1e-4 * 4 * np.abs(ws).max())
+    layer.close()
