@@ -163,6 +163,8 @@ __global__ __launch_bounds__(256) void matmul_i8_rows_kernel(I8Args a) {
 // ----------------------------------------------------------------- many rows
 constexpr int kLdsDone = ~(0xF << 8);  // of an s_waitcnt: lgkmcnt(0)
 
+// Bytes between packed rows.
+__host__ __device__ __forceinline__ size_t packed_ld(size_t k) { return (k + 127) / 128 * 128; }
 // Channels of a row of parts: whole units of 16 bytes.
 __host__ __device__ __forceinline__ size_t parts_ld(size_t n) { return (n + 3) / 4 * 4; }
 
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a,
   const int slabs = (a.k + 127) / 128, first = (int)((int64_t)blockIdx.y * slabs / a.splits),
             last = (int)((int64_t)(blockIdx.y + 1) * slabs / a.splits);
 
-  // A slab row is 4 units of 16 codes; unit u of row r lies at u ^ (r / 2 & 3),
+  // A slab row is 8 units of 16 codes; unit u of row r lies at u ^ (r / 2 & 7),
   // so that rows read at one unit hit different banks.  What a slab has behind
   // k, and slabs behind the last, are other codes of the row.
   uint32_t from[PER];  // the row, of the tile's first
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a,
   constexpr std::integral_constant<int, 1> one;
   constexpr std::integral_constant<int, 2> two;
   constexpr std::integral_constant<int, 3> three;
-  constexpr int P = PER / R;  // loads of a step
+  constexpr int P = (PER + R - 1) / R;  // loads of a step
   for (int r = 0; r < R - 1; ++r) issue(first + r, 0, PER);
   issue(first + R - 1, 0, P);
   meet();
@@ -377,7 +379,9 @@ __global__ __launch_bounds__(256) void matmul_i8_join_kernel(I8Args a) {
   store4(static_cast<T*>(a.y) + i * a.ld_y + j, y, a.n - j);
 }
 
-// Rows of k codes at any byte, copied to rows of whole units with zeros behind:
+// Rows of k codes at any byte, copied to rows that begin at cache lines (at 16
+// bytes their slabs would lie in two: 1021 x 5003 x 4100 7 us more), zeros up to a
+// unit's end:
 // x's and the weights' in one launch (25 MB: 9.6 us, 5 TB/s).
 struct Packed {
   const int8_t* src;
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(256) void i8_pack_kernel(Packed x, Packed w, int k,
   if (at >= (size_t)p.rows * units) return;
   const size_t row = at / units;
   const int u = (int)(at - row * units);
-  *reinterpret_cast<i32x4_t*>(p.dst + (row * units + u) * 16) = load16(p.src + row * p.ld + 16 * u, k - 16 * u, k);
+  *reinterpret_cast<i32x4_t*>(p.dst + row * packed_ld(k) + 16 * u) = load16(p.src + row * p.ld + 16 * u, k - 16 * u, k);
 }
 
 template <class T, int MT, int NC, bool ODD>
@@ -435,6 +439,8 @@ template <class T>
 using Small = Tiles<T, 128, 128, 2, 2, 2>;
 template <class T>
 using Deep = Tiles<T, 128, 128, 2, 2, 4>;
+template <class T>
+using Tall = Tiles<T, 192, 128, 2, 2, 4>;
 
 template <class C, class T>
 Status launch_tiles(hipStream_t stream, const I8Args& a) {
@@ -455,6 +461,11 @@ template <class T>
 Status launch_typed(hipStream_t stream, const I8Args& a) {
   if (a.m <= kI8FewRows) return launch_few<T>(stream, a);
   if (large_tiles(a.m, a.n)) return launch_tiles<Large<T>, T>(stream, a);
+  // 192 rows where these get by with a workgroup a compute unit and 128 do not
+  // (1024 x 5120 x 4096: 31 us, 34 with 128 rows; 1500 x 4000 x 2048: 20 and 21,
+  // x 512: 12 and 11).
+  if (a.k >= 1024 && tiles_of(a.m, a.n, 128) > kComputeUnits && ((size_t)a.m + 191) / 192 * (((size_t)a.n + 127) / 128) <= kComputeUnits)
+    return launch_tiles<Tall<T>, T>(stream, a);
   // A workgroup a compute unit has room for four buffers (1024 x 4096 x 4096:
   // 25 us, with two 28), more than that share it with two each (1024 x 5120 x
   // 4096: 34 us, one after the other 40).
@@ -469,8 +480,7 @@ bool in_units(const void* p, size_t ld, size_t k) { return ((uintptr_t)p | ld | 
 I8Plan i8_plan(size_t m, size_t n, size_t k) {
   I8Plan p;
   if (m <= kI8FewRows) return p;
-  const size_t rows = (k + 15) / 16 * 16;
-  p.pack_bytes = ((m * rows + 255) & ~(size_t)255) + ((n * rows + 255) & ~(size_t)255);
+  p.pack_bytes = ((m * packed_ld(k) + 255) & ~(size_t)255) + n * packed_ld(k);
   if (!large_tiles(m, n)) {
     // Parts of four slabs or more, for a workgroup a compute unit: two, of half
     // the slabs each, have twice the sums to join (1024 x 4096 x 4096 37 us, so 28).
@@ -488,6 +498,8 @@ Status init_i8_attributes() {
   };
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Large<float>::kKernel), Large<float>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Large<Bf16>::kKernel), Large<Bf16>::kLds));
+  PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Tall<float>::kKernel), Tall<float>::kLds));
+  PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Tall<Bf16>::kKernel), Tall<Bf16>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Deep<float>::kKernel), Deep<float>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Deep<Bf16>::kKernel), Deep<Bf16>::kLds));
   PSSA_RETURN_IF(set(reinterpret_cast<const void*>(Small<float>::kKernel), Small<float>::kLds));
@@ -501,14 +513,14 @@ Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan&
     char* at = static_cast<char*>(scratch) + ((p.parts_bytes + 255) & ~(size_t)255);
     const size_t units = ((size_t)a.k + 15) / 16;
     Packed x{a.x, a.ld_x, reinterpret_cast<int8_t*>(at), in_units(a.x, a.ld_x, (size_t)a.k) ? 0 : a.m};
-    Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * units * 16 + 255) & ~(size_t)255)), in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
+    Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * packed_ld((size_t)a.k) + 255) & ~(size_t)255)), in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
     if (x.rows || w.rows) {
       if (((size_t)x.rows + w.rows) * units >> 32) return Status::Invalid("8-bit product: too large for rows not in units of 16 bytes");
       i8_pack_kernel<<<(uint32_t)((((size_t)x.rows + w.rows) * units + 255) / 256), 256, 0, stream>>>(x, w, a.k, (int)units);
       PSSA_LAUNCH_CHECK("i8_pack_kernel");
     }
-    if (x.rows) a.x = x.dst, a.ld_x = units * 16;
-    if (w.rows) a.w = w.dst, a.ld_w = units * 16;
+    if (x.rows) a.x = x.dst, a.ld_x = packed_ld((size_t)a.k);
+    if (w.rows) a.w = w.dst, a.ld_w = packed_ld((size_t)a.k);
     a.k = (a.k + 15) / 16 * 16;
   }
   return y_dtype == PSSA_HIP_F32 ? launch_typed<float>(stream, a) : launch_typed<Bf16>(stream, a);

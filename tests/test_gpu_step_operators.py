@@ -217,7 +217,7 @@ def test_matmul_i8(hip, m, n, k):
     check_i8(hip, m, n, k, "bf16", pads=(-k % 4, -k % 4, 1), offset=4)
 
 
-@pytest.mark.parametrize("m,n,k", [(3300, 4200, 272), (2000, 2500, 528), (1025, 2100, 1000), (70, 16400, 16)])
+@pytest.mark.parametrize("m,n,k", [(3300, 4200, 272), (2000, 2500, 528), (1150, 4300, 1040), (1025, 2100, 1000), (70, 16400, 16)])
 def test_matmul_i8_of_many_tiles(hip, m, n, k):
     """Each size of tiles, and k that ends in a slab's first and later units."""
     say("i8 tiles", m, n, k)
