@@ -736,10 +736,8 @@ int pssa_hip_linear_attention_reserve(pssa_hip_ctx* ctx, int dtype, const uint64
  * above.  out may lie in the buffer of q, k and v in columns of its own (same
  * row stride) and must not overlap them, the gates or a state otherwise.
  * d_key <= 128, d_val <= 4096, n_seqs and heads <= 65535, row strides below
- * 2^24.  The states are those of fp32 products and sums for both types; a bf16
- * call of more than 4 tokens takes the state that a chunk of 64 is entered with,
- * the corrections of its tokens and their weights in two bf16 parts for the
- * outputs, up to 2^-16 of each value off.  A value that is not finite reaches
+ * 2^24.  Outputs and states are those of fp32 products and sums for both types,
+ * outputs rounded once to `dtype`.  A value that is not finite reaches
  * the outputs from its own token on and no earlier one. */
 int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, size_t ld_q, const void* d_k,
                                  size_t ld_k, const void* d_v, size_t ld_v, const float* d_log_decay,

@@ -201,11 +201,11 @@ __device__ __forceinline__ Place place_of(const DeltaArgs& a, int chunk) {
 // of it count.  T as two bf16 parts had the products for U at half the time (a
 // chunk 0.4 us of 2.6), but what they drop comes back in every chunk's state,
 // and grows where keys are alike: states were off by 5e-6 of their size, and
-// are by 2e-7 so.  P's fragments are 16 tokens by 32 in two parts (bf16), 16 by
-// 16 (fp32): it only reaches the outputs.
+// are by 2e-7 so.  P's fragments are 16 tokens by 32 in three parts (bf16), 16 by
+// 16 (fp32).
 template <bool B16>
 struct Ahead {
-  static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3, kFrag = B16 ? 128 : 64;
+  static constexpr int C = B16 ? 64 : 32, kTiles = C / 16, kPairs = B16 ? 6 : 3, kFrag = B16 ? 192 : 64;
   static constexpr int kTriangle = kTiles * (kTiles + 1) / 2, kGamma = kTriangle * 64, kRest = kGamma + C / 4, kSum = kRest + C / 4, kUnits = kGamma + 64;
 };
 // The fragment of token tile t over keys 32 h .. (bf16), 16 h .. (fp32).
@@ -411,15 +411,15 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
 enum { DR_WHOLE, DR_LOCAL, DR_SEGMENT };
 
 // LDS units of a walk: two buffers of k | q | v | what was worked out ahead,
-// P, and what the computing waves hand over: S as operands, U (its first part
-// in v's place where it is bf16), and which waves ran token by token.
+// P, and what the walking waves hand over in fp32: S, and U (bf16: its first
+// half in v's place).
 template <bool B16, int DKP, bool LOCAL>
 struct WalkLds {
   static constexpr int C = Ahead<B16>::C, N = B16 ? 8 : 4;  // elements of a unit
   static constexpr int kK = C * DKP / N, kQ = LOCAL ? 0 : kK, kV = C * 64 / N, kBuffer = kK + kQ + kV + Ahead<B16>::kUnits;
   static constexpr int kP = 2 * kBuffer, kS = kP + (LOCAL ? 0 : Ahead<B16>::kPairs * Ahead<B16>::kFrag);
-  static constexpr int kState = LOCAL ? 0 : B16 ? DKP / 32 * 2 * 64 : DKP / 16 * 64;  // of a wave
-  static constexpr int kU = kS + 4 * kState, kOdd = kU + (LOCAL ? 0 : 4 * 128), kUnits = kOdd + (LOCAL ? 0 : 1);
+  static constexpr int kState = LOCAL ? 0 : DKP / 16 * 64;  // of a wave
+  static constexpr int kU = kS + 4 * kState, kUnits = kU + (LOCAL ? 0 : 4 * 128);
   static constexpr size_t kBytes = 16 * (size_t)kUnits;
   static_assert(kBytes <= 160 * 1024, "a compute unit's LDS");
 };
@@ -446,6 +446,23 @@ __device__ __forceinline__ u32x4_t turned(const u32x4_t* s, int row0, int c0, in
   const u32x2_t x = read(at), y = read(at + 16 * (W / 4));
   return u32x4_t{x[0], x[1], y[0], y[1]};
 }
+
+// Two of an accumulator's tiles as an operand, in three bf16 parts.
+__device__ __forceinline__ void parts_of(const f32x4_t& x, const f32x4_t& y, u32x4_t (&w)[3]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f32x4_t& v = e < 2 ? x : y;
+    uint32_t p0, p1, p2;
+    split3(v[2 * (e & 1)], v[2 * (e & 1) + 1], p0, p1, p2);
+    w[0][e] = p0;
+    w[1][e] = p1;
+    w[2][e] = p2;
+  }
+}
+
+// In U's place (a NaN, which U never holds there): the walking wave runs the
+// chunk token by token and stores its outputs.
+constexpr uint32_t kOneByOne = ~0u;
 
 // What a workgroup walks: a sequence's or segment's first chunk, its first
 // token and its tokens.
@@ -487,9 +504,13 @@ __device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
 // four turn the S and U that they are handed into outputs, and these eight
 // work out P, so that nothing but the states' own chain runs from chunk to
 // chunk (where the same waves did all, issuing the loads alone took 2.3 of a
-// chunk's 5.7 us, heads of 128).  A chunk takes 3 us at heads of 64, 4.5 at 128:
+// chunk's 5.7 us, heads of 128).  A chunk takes 3.5 us at heads of 64, 5.5 at 128:
 // the chain's matrix products 0.9 and 1.2 us, the rest its LDS reads, splits and
-// two meetings; matrix cores and VALU are 0.3 busy each.
+// two meetings; matrix cores and VALU are 0.3 busy each.  Of these 0.5 and 1 us
+// are what outputs from S, U and P in all three parts cost (two parts, 2^-17 of
+// each value off, put one bf16 output in 250 on the wrong side of a border).
+// Both outputs' helpers at once, Q S ahead of the second meeting and S handed
+// over in parts came to the same times within 3%.
 // A segment's own state and its transition need no outputs, and two waves bring
 // their chunks, so that two workgroups fit a compute unit.  The transition is
 // the state that the unit matrix becomes without values: more columns.
@@ -580,8 +601,7 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
     }
   }
   u32x4_t *sP = s_walk + Lds::kP, *sS = s_walk + Lds::kS + wave * Lds::kState, *sU = s_walk + Lds::kU + wave * 128;
-  uint32_t* s_odd = reinterpret_cast<uint32_t*>(s_walk + Lds::kOdd);
-  // U's first parts in v's place: the wave's own columns, 2 units of each row.
+  // U's first half in v's place: the wave's own columns, 2 units of each row.
   auto u_place = [&](const u32x4_t* v, int h) {
     const int i = 64 * h + lane, row = i >> 1;
     return const_cast<u32x4_t*>(v) + row * 8 + row_unit<64>(row, 2 * wave + (i & 1));
@@ -590,7 +610,7 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
     if constexpr (B16) {  // the halves of fragments that P does not reach
       if (wave < 2) {
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int part = 0; part < 3; ++part)
           reinterpret_cast<u32x2_t*>(sP + In::kFrag * pair_of<B16>(2 * wave, wave) + 64 * part + lane)[1] = u32x2_t{0, 0};
       }
     }
@@ -625,23 +645,24 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
 #pragma unroll
         for (int e = 0; e < 4; ++e) p[e] = 16 * r + col >= 16 * c + 4 * quad + e ? p[e] * d[e] : 0.0f;
         if constexpr (B16) {
-          u32x2_t hi, lo;
+          u32x2_t w[3];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t u, l;
-            split2(p[2 * e], p[2 * e + 1], u, l);
-            hi[e] = u;
-            lo[e] = l;
+            uint32_t p0, p1, p2;
+            split3(p[2 * e], p[2 * e + 1], p0, p1, p2);
+            w[0][e] = p0;
+            w[1][e] = p1;
+            w[2][e] = p2;
           }
           u32x4_t* to_p = sP + In::kFrag * pair_of<B16>(r, c >> 1) + lane;
-          reinterpret_cast<u32x2_t*>(to_p)[c & 1] = hi;
-          reinterpret_cast<u32x2_t*>(to_p + 64)[c & 1] = lo;
+#pragma unroll
+          for (int part = 0; part < 3; ++part) reinterpret_cast<u32x2_t*>(to_p + 64 * part)[c & 1] = w[part];
         } else {
           sP[In::kFrag * pair_of<B16>(r, c) + lane] = __builtin_bit_cast(u32x4_t, p);
         }
       }
       meet();  // P, S and U are there
-      if (brings || s_odd[wave]) continue;  // uniform; odd: the walking wave stores these
+      if (brings || (uint32_t)__builtin_amdgcn_readfirstlane(sU[0][0]) == kOneByOne) continue;
       // O^T = scale e^G (Q S)^T + (P U)^T.
       f32x4_t o[NT];
 #pragma unroll
@@ -649,14 +670,15 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
       if constexpr (B16) {
 #pragma unroll
         for (int kp = 0; kp < DKP / 32; ++kp) {
-          const u32x4_t hi = sS[128 * kp + lane], lo = sS[128 * kp + 64 + lane];
+          u32x4_t w[3];
+          parts_of(__builtin_bit_cast(f32x4_t, sS[128 * kp + lane]), __builtin_bit_cast(f32x4_t, sS[128 * kp + 64 + lane]), w);
           u32x4_t qf[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t) qf[t] = row_frag<DKP>(sQ, 16 * t + col, 4 * kp + quad);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) o[t] = mfma(lo, qf[t], o[t]);
+          for (int p = 2; p >= 0; --p)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) o[t] = mfma(hi, qf[t], o[t]);
+            for (int t = 0; t < NT; ++t) o[t] = mfma(w[p], qf[t], o[t]);
         }
       } else {
         const f32x4_t* Q32 = reinterpret_cast<const f32x4_t*>(sQ);
@@ -675,21 +697,23 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[t] *= a.scale * gamma[16 * t + col];
       if constexpr (B16) {
-        u32x4_t hi[2], lo[2];
+        // Parts' products down to 2^-16 of the whole; the others hold some 2^-24 of it.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          hi[h] = *u_place(sV, h);
-          lo[h] = sU[64 * h + lane];
+          u32x4_t w[3];
+          if (h == 0)
+            parts_of(__builtin_bit_cast(f32x4_t, *u_place(sV, 0)), __builtin_bit_cast(f32x4_t, *u_place(sV, 1)), w);
+          else
+            parts_of(__builtin_bit_cast(f32x4_t, sU[lane]), __builtin_bit_cast(f32x4_t, sU[64 + lane]), w);
+#pragma unroll
+          for (int part = 2; part >= 0; --part)
+#pragma unroll
+            for (int t = 2 * h; t < NT; ++t) {
+              const u32x4_t pf = sP[In::kFrag * pair_of<B16>(t, h) + 64 * part + lane];
+#pragma unroll
+              for (int p = 2 - part; p >= 0; --p) o[t] = mfma(w[p], pf, o[t]);
+            }
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int h = 0; 2 * h <= t; ++h) {
-            const u32x4_t ph = sP[128 * pair_of<B16>(t, h) + lane], pl = sP[128 * pair_of<B16>(t, h) + 64 + lane];
-            o[t] = mfma(lo[h], ph, o[t]);
-            o[t] = mfma(hi[h], pl, o[t]);
-            o[t] = mfma(hi[h], ph, o[t]);
-          }
       } else {
         f32x4_t u[NT];
 #pragma unroll
@@ -766,18 +790,11 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
     if constexpr (B16) {
 #pragma unroll
       for (int kp = 0; kp < DKP / 32; ++kp) {
-        u32x4_t w[3];  // the outputs, in bf16, do with two
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t p0, p1, p2;
-          split3(S[2 * kp + (e >> 1)][2 * (e & 1)], S[2 * kp + (e >> 1)][2 * (e & 1) + 1], p0, p1, p2);
-          w[0][e] = p0;
-          w[1][e] = p1;
-          w[2][e] = p2;
-        }
+        u32x4_t w[3];
+        parts_of(S[2 * kp], S[2 * kp + 1], w);
         if constexpr (!LOCAL) {
-          sS[128 * kp + lane] = w[0];
-          sS[128 * kp + 64 + lane] = w[1];
+          sS[128 * kp + lane] = __builtin_bit_cast(u32x4_t, S[2 * kp]);
+          sS[128 * kp + 64 + lane] = __builtin_bit_cast(u32x4_t, S[2 * kp + 1]);
         }
         u32x4_t kf[NT];
 #pragma unroll
@@ -841,25 +858,15 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
 #pragma unroll
       for (int r = 0; r < 4; ++r) odd = fmaf(u[t][r], 0.0f, odd);
     const bool one_by_one = __any(odd != odd);
-    if (!LOCAL && lane == 0) s_odd[wave] = one_by_one;
-    if (!LOCAL && !one_by_one) {
-      if constexpr (B16) {
+    if constexpr (!LOCAL) {
+      if (lane == 0) *reinterpret_cast<uint32_t*>(sU) = 0u - (uint32_t)one_by_one;  // kOneByOne, or what U then overwrites
+      if (!one_by_one) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4_t p, l;
+        for (int t = 0; t < 2; ++t) sU[64 * t + lane] = __builtin_bit_cast(u32x4_t, u[NT - 2 + t]);
+        if constexpr (B16) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t hi, lo;
-            split2(u[2 * h + (e >> 1)][2 * (e & 1)], u[2 * h + (e >> 1)][2 * (e & 1) + 1], hi, lo);
-            p[e] = hi;
-            l[e] = lo;
-          }
-          *u_place(sV, h) = p;
-          sU[64 * h + lane] = l;
+          for (int t = 0; t < 2; ++t) *u_place(sV, t) = __builtin_bit_cast(u32x4_t, u[t]);
         }
-      } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) sU[64 * t + lane] = __builtin_bit_cast(u32x4_t, u[t]);
       }
     }
     if constexpr (!LOCAL) meet();  // S and U are there
@@ -929,14 +936,7 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4_t w[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t p0, p1, p2;
-          split3(u[2 * h + (e >> 1)][2 * (e & 1)], u[2 * h + (e >> 1)][2 * (e & 1) + 1], p0, p1, p2);
-          w[0][e] = p0;
-          w[1][e] = p1;
-          w[2][e] = p2;
-        }
+        parts_of(u[2 * h], u[2 * h + 1], w);
         constexpr int BG = NB < 4 ? NB : 4;
 #pragma unroll
         for (int b0 = 0; b0 < NB; b0 += BG) {
@@ -1203,7 +1203,7 @@ Status init_delta_attributes() {
   return Status::Ok();
 }
 
-// A walk's chunk takes about 3.1 us, one of a segment's own state 2.3 us, a
+// A walk's chunk takes about 3.1 us (bf16 3.5), one of a segment's own state 2.3 us, a
 // step of the scan over the segments 1.5 us, and the passes between some 12 us
 // (at heads of 64 and the machine's 256 compute units, a workgroup each; wider
 // heads take half as much again of all, which leaves the choice).  A call is

@@ -985,3 +985,39 @@ def test_beam_search_behind_prompts_of_different_lengths(hip):
     np.testing.assert_array_equal(ids, want)
     np.testing.assert_allclose(scores, ws, rtol=0, atol=1e-4 * 4 * np.abs(ws).max())
     layer.close()
+
+
+# ---------------------------------------------------------------------------
+# What a call holds on its way to an output
+
+
+def beside_ties(shape):
+    """fp32 values a step above and a step below the middle of two bf16 neighbours: a value that was held in fewer bits
+    on its way lies on the middle, and half of these are then rounded to the wrong side."""
+    i = np.arange(np.prod(shape))
+    tie = 1 + (2 * (i // 2 % 128) + 1) * 2.0 ** -8
+    return ((tie + np.where(i % 2, 2.0 ** -23, -2.0 ** -23)) * 2.0 ** (i % 3 - 1) * np.where(i // 5 % 2, -1, 1)).reshape(shape).astype(np.float32)
+
+
+@pytest.mark.parametrize("dk", [32, 64, 128])
+@pytest.mark.parametrize("what", ["state", "update", "scale"])
+def test_delta_rule_rounds_bf16_outputs_once(hip, dk, what):
+    """Queries and keys of a single one leave one term in every sum, factors of one and powers of two leave it as it is:
+    what fp32 holds is exact, and the output is its rounding."""
+    rng = np.random.default_rng(dk)
+    n, dv = min(dk, 64), 64
+    at = rng.integers(0, np.arange(n) + 1)  # a token's query meets one key, of a token before it or its own
+    eye, two = np.eye(dk)[:n, None], 2.0 ** (np.arange(n * dv) % 5 - 2).reshape(n, 1, dv)
+    zero, one = np.zeros((n, 1)), np.ones((n, 1))
+    base = dict(g=zero, k=eye, q=np.eye(dk)[at, None], v=two, state=None, beta=one)
+    if what == "state":  # nothing is added to it
+        state = beside_ties((1, 1, dk, dv))
+        cases = [(dict(base, state=state, beta=zero), 1.0, state[0, 0, at])]
+    elif what == "update":
+        beta = np.abs(beside_ties((n, 1)))
+        cases = [(dict(base, beta=beta), 1.0, (beta[:, :, None] * two)[at, 0])]
+    else:
+        cases = [(base, float(s), s * two[at, 0]) for s in beside_ties(64)[7::9]]
+    for c, scale, want in cases:
+        out = run_delta(hip, c, [n], 1, 1, dk, dv, "bf16", scale)[3]
+        np.testing.assert_array_equal(out[:, 0], to_bf16(want)[1])
