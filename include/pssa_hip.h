@@ -762,7 +762,7 @@ int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* le
  *   scales = max|t| / 127 / sqrt(mean(h^2) + eps),
  * d_codes [rows, width] and d_scales [rows] together.  A row of zeros has
  * codes and scale 0; one whose t is not finite has codes 0 and scale NaN.
- * gamma is fp32 [width]; 1 <= width <= 65536, eps in [1e-12, 1].  d_sum and d_out may be
+ * gamma is fp32 [width]; 1 <= width <= 65536, rows <= 2^31 - 4096, eps in [1e-12, 1].  d_sum and d_out may be
  * d_x or d_residual with their row stride; outputs must not overlap the inputs
  * or each other otherwise (other columns of the same rows do not). */
 int pssa_hip_rms_norm_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, const void* d_residual,
@@ -770,7 +770,8 @@ int pssa_hip_rms_norm_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, si
                                void* d_sum, size_t ld_sum, void* d_out, size_t ld_out, int8_t* d_codes,
                                size_t ld_codes, float* d_scales, char* err, size_t err_len);
 /* 8-bit codes and scales of rows as they are (activations, or a weight's
- * channels): codes = round(x 127 / max|x|), scales = max|x| / 127. */
+ * channels): codes = round(x 127 / max|x|), scales = max|x| / 127.  Sizes as
+ * above. */
 int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, size_t ld_x, size_t rows, size_t width,
                                   int8_t* d_codes, size_t ld_codes, float* d_scales, char* err, size_t err_len);
 

@@ -2770,6 +2770,7 @@ int pssa_hip_rms_norm_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x, si
     PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
     PSSA_RETURN_IF(need(eps >= 1e-12f && eps <= 1.0f, "rms norm: eps must be in [1e-12, 1]"));
     PSSA_RETURN_IF(need(width <= pssa::kRmsWidth, "rms norm: rows above 65536 elements are not supported"));
+    PSSA_RETURN_IF(need(rows <= pssa::kRmsRows, "rms norm: too large"));
     PSSA_RETURN_IF(need(!d_codes == !d_scales, "rms norm: codes and scales belong together"));
     PSSA_RETURN_IF(need(d_sum || d_out || d_codes, "rms norm: no output asked for"));
     PSSA_RETURN_IF(check_matrix(rows, width, ld_x, "rms norm"));
@@ -2820,6 +2821,7 @@ int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x,
     PSSA_RETURN_IF(need(d_x && d_codes && d_scales, "8-bit rows: null buffer"));
     PSSA_RETURN_IF(need(dtype_ok(dtype), "unknown dtype"));
     PSSA_RETURN_IF(need(width <= pssa::kRmsWidth, "8-bit rows: above 65536 elements are not supported"));
+    PSSA_RETURN_IF(need(rows <= pssa::kRmsRows, "8-bit rows: too large"));
     PSSA_RETURN_IF(check_matrix(rows, width, ld_x, "8-bit rows"));
     PSSA_RETURN_IF(check_matrix(rows, width, ld_codes, "8-bit rows' codes"));
     const size_t size = dtype_size(dtype);

@@ -508,7 +508,7 @@ __device__ __forceinline__ Walk<C> walk_of(const DeltaArgs& a, int item) {
 // the chain's matrix products 0.9 and 1.2 us, the rest its LDS reads, splits and
 // two meetings; matrix cores and VALU are 0.3 busy each.  Of these 0.5 and 1 us
 // are what outputs from S, U and P in all three parts cost (two parts, 2^-17 of
-// each value off, put one bf16 output in 250 on the wrong side of a border).
+// each value off, put one bf16 output in some 900 on the wrong side of a border).
 // Both outputs' helpers at once, Q S ahead of the second meeting and S handed
 // over in parts came to the same times within 3%.
 // A segment's own state and its transition need no outputs, and two waves bring

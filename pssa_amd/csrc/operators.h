@@ -88,6 +88,8 @@ Status launch_linear_attention(hipStream_t stream, int dtype, const LinearArgs& 
 
 // ------------------------------------------------------------------- norms
 constexpr size_t kRmsWidth = 65536;  // the widest row: a workgroup's registers
+constexpr size_t kRmsStep = 4096;    // rows at a time, at most
+constexpr size_t kRmsRows = ((size_t)1 << 31) - kRmsStep;  // a row and a step beyond it stay below 2^31
 
 struct RmsNormArgs {
   const void *x = nullptr, *residual = nullptr;  // row r at r * ld; residual may be null

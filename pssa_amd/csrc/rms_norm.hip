@@ -279,7 +279,9 @@ template <class T, int W, int NV>
 Status launch_rows(hipStream_t stream, const RmsNormArgs& a, size_t rows) {
   constexpr int WAVES = W == 1 ? 4 : W;
   // As many workgroups as the machine holds at once, 16 waves a compute unit.
-  const size_t all = W == 1 ? (rows + 3) / 4 : rows, most = 256 * std::max(1, 16 / WAVES);
+  constexpr size_t most = 256 * std::max(1, 16 / WAVES);
+  static_assert((W == 1 ? 4 : 1) * most <= kRmsStep, "rows of a step");
+  const size_t all = W == 1 ? (rows + 3) / 4 : rows;
   rms_norm_kernel<T, W, NV><<<(uint32_t)std::min(all, most), 64 * WAVES, 0, stream>>>(a, (int)rows);
   PSSA_LAUNCH_CHECK("rms_norm_kernel");
   return Status::Ok();

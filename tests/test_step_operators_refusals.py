@@ -151,3 +151,17 @@ def test_beam_reserve_and_search_refuse():
     refused(fn, [None, 2, 65, 100, 4], "1..=64")
     ids, scores = np.empty(8, np.uint32), np.empty(4, np.float32)
     refused(_abi.lib().pssa_hip_beam_search, [None, 1, 4, 2, 2, _abi.ptr(ids, C.c_uint32), 8, _abi.ptr(scores), 4], "null argument")
+
+
+@pytest.mark.parametrize("width", [1, 2, 16])
+def test_norms_of_too_many_rows_refuse(width):
+    """A workgroup steps up to 4096 rows on from its last one, in 31 bits."""
+    most, far = 2 ** 31 - 4096, 1 << 44
+    norm = dict(NORM, dtype=_abi.BF16, width=width, residual=None, ld_x=width, ld_sum=width, sum=far, out=None, codes=None,
+                scales=None)
+    quant = dict(QUANT, width=width, ld_x=width, ld_codes=width, codes=far, scales=2 * far)
+    for fn, base in ((_abi.lib().pssa_hip_rms_norm_resident, norm), (_abi.lib().pssa_hip_quantize_i8_resident, quant)):
+        base = dict(base, x=4 * far)
+        refused(fn, changed(base, rows=most), "null context")
+        for rows in (most + 1, 2 ** 31 - 2048, 2 ** 31 - 1):
+            refused(fn, changed(base, rows=rows), "too large")
