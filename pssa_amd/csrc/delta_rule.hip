@@ -756,6 +756,12 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
     }
     return;
   }
+  // Whether a token of the segment forgets the state before it (a NaN does not).
+  float least = 0.0f;
+  if (moves)
+#pragma unroll 4
+    for (int i = lane; i < sp.len; i += 64) least = fminf(least, a.log_decay[(sp.tok + i) * a.ld_gates + head]);
+  const bool forgets = __any(expf(least) == 0.0f);
   // S: the rows of the lane's column.
   f32x4_t S[NB];
 #pragma unroll
@@ -962,11 +968,14 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
   if (LOCAL && moves) {  // whole rows and columns, zeros past d_key, as the scan's lanes read them: 16 bytes each
     const int k = B16 ? j / 32 * 2 + (j >> 2 & 1) : j / 16, at = B16 ? j >> 3 & 3 : j >> 2 & 3;  // j = state_row(k, at, j % 4)
     float* move = a.seg_move + item_head * DKP * DKP + (k * 64 + at * 16 + 4 * quad) * 4 + j % 4;
+    // Zeros are +0 where a token forgets; where the transition has only become
+    // too small for fp32, -0, and the scan multiplies by them.
+    const float zero = forgets ? 0.0f : -0.0f;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (j < DKP) move[(b * NB * 64 + r) * 4] = S[b][r];
+        if (j < DKP) move[(b * NB * 64 + r) * 4] = S[b][r] == 0.0f ? zero : S[b][r];
   } else if (LOCAL) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -1033,14 +1042,14 @@ __global__ __launch_bounds__(64 * kScanWaves<DKP>) void delta_scan_kernel(DeltaA
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     f32x4_t next[MINE];
-    uint32_t keeps = 0;  // a transition of zeros forgets whatever the state is
+    uint32_t keeps = 0;  // a transition of +0 forgets whatever the state is, one of -0 passes on what is not finite
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
       next[m] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < NB; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) keeps |= __float_as_uint(p.move[m][k][r]) << 1;
+        for (int r = 0; r < 4; ++r) keeps |= __float_as_uint(p.move[m][k][r]);
     }
     if (__any(keeps != 0)) {
 #pragma unroll

@@ -1021,3 +1021,31 @@ def test_delta_rule_rounds_bf16_outputs_once(hip, dk, what):
     for c, scale, want in cases:
         out = run_delta(hip, c, [n], 1, 1, dk, dv, "bf16", scale)[3]
         np.testing.assert_array_equal(out[:, 0], to_bf16(want)[1])
+
+
+# ---------------------------------------------------------------------------
+# Values that are not finite, across segments
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,heads,dk,dv", [([3000], 1, 64, 64), ([2177, 1300], 2, 32, 72), ([1601], 1, 100, 40), ([4100], 2, 128, 64)])
+def test_delta_rule_segments_pass_on_what_is_not_finite(hip, dtype, lens, heads, dk, dv):
+    """Decays of e^-0.5 a token take a segment's transition below what fp32 holds, but no token forgets: a NaN stays."""
+    say("segments, not finite", dtype, lens, heads, dk, dv)
+    rng = np.random.default_rng(sum(lens) + dk)
+    c = delta_case(rng, lens, heads, 1, dk, dv, True)
+    c["g"][:] = -0.5 - 0.2 * rng.random(c["g"].shape)
+    clean = run_delta(hip, c, lens, heads, 1, dk, dv, dtype, 1.0)
+    at, n = 150, lens[0]
+    c["v"][at, 0, 1] = np.nan
+    c["state"][0, 0, dk - 1, 0] = np.nan
+    c["state"][0, heads - 1, 3, dv - 1] = np.inf
+    _, _, _, out, S = run_delta(hip, c, lens, heads, 1, dk, dv, dtype, 1.0)
+    bad, gone = np.zeros(out.shape, bool), np.zeros(S.shape, bool)
+    bad[at:n, 0, 1] = bad[:n, 0, 0] = bad[:n, heads - 1, dv - 1] = True
+    gone[0, 0, :, :2] = gone[0, heads - 1, :, dv - 1] = True
+    np.testing.assert_array_equal(np.isfinite(out), ~bad)
+    np.testing.assert_array_equal(np.isfinite(S), ~gone)
+    # What it does not reach is as near the sound call's as another order of sums leaves it.
+    for got, was, there, u in ((out, clean[3], ~bad, U16 * 2 if dtype == "bf16" else 0), (S, clean[4], ~gone, 0)):
+        assert np.abs(got - was)[there].max() <= np.abs(was).max() * (u + delta_steps(dk, "f32") * 64 * U32)
