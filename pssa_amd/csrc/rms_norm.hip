@@ -213,20 +213,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNorm
       }
     }
     row_reduce<W>(ss, most, s_part);
-    float inv = 1.0f / sqrtf(ss / (float)a.width + a.eps);
+    // Squares past fp32's range: again with the row scaled down, by a power of
+    // two that lets 65536 of the largest values in (an infinity in the row comes
+    // out the same).  inv is then that of the scaled row.
+    float inv = 1.0f / sqrtf(ss / (float)a.width + a.eps), half = 1.0f;
     if (ss == INFINITY) {
-      // Squares past fp32's range: again with the row scaled down (an infinity
-      // in the row comes out the same).
-      constexpr float kDown = 5.42101086242752217e-20f;  // 2^-64
+      half = 3.5527136788005009e-15f;  // 2^-48
       float low = 0.0f, none = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int j = 0; j < N; ++j) low = fmaf(h[k][j] * kDown, h[k][j] * kDown, low);
+        for (int j = 0; j < N; ++j) {
+          const float v = h[k][j] * (half * half);
+          low = fmaf(v, v, low);
+        }
       row_reduce<W>(low, none, s_part);
-      inv = kDown / sqrtf(low / (float)a.width);
+      inv = 1.0f / sqrtf(low / (float)a.width);
     }
-    if (!a.normed) inv = 1.0f;
+    const float down = a.normed ? half * half : 1.0f;
+    if (!a.normed) inv = half = 1.0f;
 
     if (a.sum) {
       T* sum = static_cast<T*>(a.sum) + (size_t)r * a.ld_sum;
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNorm
         float v[N], g[N];
         if constexpr (!kAhead) gamma_of(k, g);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = h[k][j] * inv * (kAhead ? gamma[kAhead ? k : 0][j] : g[j]);
+        for (int j = 0; j < N; ++j) v[j] = h[k][j] * down * inv * (kAhead ? gamma[kAhead ? k : 0][j] : g[j]);
         store_vec<T>(out, c, left, v);
       }
     }
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNorm
         }
         store_codes<N>(codes, c, left, q);
       }
-      if (tid == 0) a.scales[r] = fine ? most / 127.0f * inv : NAN;
+      if (tid == 0) a.scales[r] = fine ? most / 127.0f * half * inv * half : NAN;  // halves: products inside the range
     }
   }
 }

@@ -1049,3 +1049,16 @@ def test_delta_rule_segments_pass_on_what_is_not_finite(hip, dtype, lens, heads,
     # What it does not reach is as near the sound call's as another order of sums leaves it.
     for got, was, there, u in ((out, clean[3], ~bad, U16 * 2 if dtype == "bf16" else 0), (S, clean[4], ~gone, 0)):
         assert np.abs(got - was)[there].max() <= np.abs(was).max() * (u + delta_steps(dk, "f32") * 64 * U32)
+
+
+# ---------------------------------------------------------------------------
+# Norms at the ends of fp32's range
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [4, 700, 9000])
+def test_norm_of_rows_near_the_largest_value(hip, dtype, width):
+    """Rows whose squares' mean is past fp32's range by far are normed all the same."""
+    rng = np.random.default_rng(width)
+    x = rng.choice([-1.0, 1.0], (4, width)) * rng.uniform(0.3, 1.0, (4, width)) * np.array([[3e38], [1.2e38], [2e30], [3e19]])
+    check_norm(hip, x, None, rng.uniform(0.2, 0.9, width), dtype, pad=1)
