@@ -257,8 +257,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNorm
     if (a.codes) {
       // A row that is not finite has the scale NaN, which its products take on.
       const bool fine = most < INFINITY;
-      // Maxima so small that 127 / max would overflow are scaled up, exactly.
-      const float up = most < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 2^64
+      // Small maxima are scaled up, exactly: 127 / max would overflow, max / 127 have few bits left.
+      const float up = most < 1.0f ? 18446744073709551616.0f : 1.0f;  // 2^64
       const float by = 127.0f / (most * up);
       int8_t* codes = a.codes + (size_t)r * a.ld_codes;
 #pragma unroll
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_kernel(RmsNorm
         }
         store_codes<N>(codes, c, left, q);
       }
-      if (tid == 0) a.scales[r] = fine ? most / 127.0f * half * inv * half : NAN;  // halves: products inside the range
+      if (tid == 0) a.scales[r] = fine ? most * up / 127.0f * half * inv * half / up : NAN;  // halves: products inside the range
     }
   }
 }

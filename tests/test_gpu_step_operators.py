@@ -1062,3 +1062,12 @@ def test_norm_of_rows_near_the_largest_value(hip, dtype, width):
     rng = np.random.default_rng(width)
     x = rng.choice([-1.0, 1.0], (4, width)) * rng.uniform(0.3, 1.0, (4, width)) * np.array([[3e38], [1.2e38], [2e30], [3e19]])
     check_norm(hip, x, None, rng.uniform(0.2, 0.9, width), dtype, pad=1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("eps", [1e-12, 1e-5])
+def test_norm_scales_of_rows_near_the_least_value(hip, dtype, eps):
+    """max|t| / 127 would be held in a few bits where it is below fp32's normal range, the scale itself is not."""
+    rng = np.random.default_rng(17)
+    x = rng.normal(0, 1, (4, 300)) * np.array([[1e-38], [3e-39], [4e-37], [1e-35]])
+    check_norm(hip, x, None, rng.normal(1, 0.2, 300), dtype, eps=eps)
