@@ -784,7 +784,9 @@ int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x,
 int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scales,
                                 const int8_t* d_w, size_t ld_w, const float* d_w_scales, size_t m, size_t n, size_t k,
                                 void* d_y, int y_dtype, size_t ld_y, char* err, size_t err_len);
-/* Grows the context's scratch (synchronously) to what such a call needs. */
+/* Grows the context's scratch (synchronously) to what such a call needs at most:
+ * copies of rows and weights of more than 64 rows are counted, which calls make
+ * of those that do not lie in units of 16 bytes. */
 int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, char* err, size_t err_len);
 
 /* Beam search's selection: of `groups` requests with `beams` rows of logits

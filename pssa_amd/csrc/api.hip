@@ -2873,7 +2873,7 @@ int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_
     a.m = (int)m;
     a.n = (int)n;
     a.k = (int)k;
-    const pssa::I8Plan plan = pssa::i8_plan(m, n, k);
+    const pssa::I8Plan plan = pssa::i8_plan(m, n, k, !pssa::i8_in_units(d_x, ld_x, k), !pssa::i8_in_units(d_w, ld_w, k));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     PSSA_RETURN_IF(grow_scratch(ctx, plan.bytes(), false));
@@ -2887,7 +2887,7 @@ int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, 
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
-    return grow_scratch(ctx, pssa::i8_plan(m, n, k).bytes(), false);
+    return grow_scratch(ctx, pssa::i8_plan(m, n, k, true, true).bytes(), false);
   }, err, err_len);
 }
 

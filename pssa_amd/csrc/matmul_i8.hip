@@ -472,15 +472,15 @@ Status launch_typed(hipStream_t stream, const I8Args& a) {
   return tiles_of(a.m, a.n, 128) * a.splits <= kComputeUnits ? launch_tiles<Deep<T>, T>(stream, a) : launch_tiles<Small<T>, T>(stream, a);
 }
 
-// Whole units, and offsets inside a tile's rows of 32 bits.
-bool in_units(const void* p, size_t ld, size_t k) { return ((uintptr_t)p | ld | k) % 16 == 0 && ld <= (size_t)1 << 24; }
-
 }  // namespace
 
-I8Plan i8_plan(size_t m, size_t n, size_t k) {
+// Also offsets inside a tile's rows of 32 bits.
+bool i8_in_units(const void* p, size_t ld, size_t k) { return ((uintptr_t)p | ld | k) % 16 == 0 && ld <= (size_t)1 << 24; }
+
+I8Plan i8_plan(size_t m, size_t n, size_t k, bool copy_x, bool copy_w) {
   I8Plan p;
   if (m <= kI8FewRows) return p;
-  p.pack_bytes = ((m * packed_ld(k) + 255) & ~(size_t)255) + n * packed_ld(k);
+  p.pack_bytes = (copy_x ? (m * packed_ld(k) + 255) & ~(size_t)255 : 0) + (copy_w ? n * packed_ld(k) : 0);
   if (!large_tiles(m, n)) {
     // Parts of four slabs or more, for a workgroup a compute unit: two, of half
     // the slabs each, have twice the sums to join (1024 x 4096 x 4096 37 us, so 28).
@@ -512,8 +512,8 @@ Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan&
     a.parts = static_cast<int32_t*>(scratch);
     char* at = static_cast<char*>(scratch) + ((p.parts_bytes + 255) & ~(size_t)255);
     const size_t units = ((size_t)a.k + 15) / 16;
-    Packed x{a.x, a.ld_x, reinterpret_cast<int8_t*>(at), in_units(a.x, a.ld_x, (size_t)a.k) ? 0 : a.m};
-    Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * packed_ld((size_t)a.k) + 255) & ~(size_t)255)), in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
+    Packed x{a.x, a.ld_x, reinterpret_cast<int8_t*>(at), i8_in_units(a.x, a.ld_x, (size_t)a.k) ? 0 : a.m};
+    Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * packed_ld((size_t)a.k) + 255) & ~(size_t)255)), i8_in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
     if (x.rows || w.rows) {
       if (((size_t)x.rows + w.rows) * units >> 32) return Status::Invalid("8-bit product: too large for rows not in units of 16 bytes");
       i8_pack_kernel<<<(uint32_t)((((size_t)x.rows + w.rows) * units + 255) / 256), 256, 0, stream>>>(x, w, a.k, (int)units);

@@ -118,14 +118,16 @@ struct I8Args {
   int32_t* parts = nullptr;  // [splits, m, n] sums of each, where there are several
 };
 constexpr int kI8FewRows = 64;  // up to these the weights go straight to registers
+// Whether rows of k codes lie in units of 16 bytes: many rows are copied where not.
+bool i8_in_units(const void* p, size_t ld, size_t k);
 // Parts of k of a product of these sizes, and its scratch: the parts' sums,
-// and copies of rows and weights that do not lie in units of 16 bytes.
+// and the copies of rows and weights that there are.
 struct I8Plan {
   int splits = 1;
   size_t parts_bytes = 0, pack_bytes = 0;
   size_t bytes() const { return ((parts_bytes + 255) & ~(size_t)255) + pack_bytes; }
 };
-I8Plan i8_plan(size_t m, size_t n, size_t k);
+I8Plan i8_plan(size_t m, size_t n, size_t k, bool copy_x, bool copy_w);
 Status init_i8_attributes();
 Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan& p, void* scratch);
 

@@ -4,6 +4,8 @@ bits: norms with 8-bit rows, 8-bit products, the gated delta rule, beam search's
 Tolerances count roundings: u = 2^-24 is half a step of fp32, and an output held in bf16 adds its own half step 2^-8
 relative.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -1071,3 +1073,35 @@ def test_norm_scales_of_rows_near_the_least_value(hip, dtype, eps):
     rng = np.random.default_rng(17)
     x = rng.normal(0, 1, (4, 300)) * np.array([[1e-38], [3e-39], [4e-37], [1e-35]])
     check_norm(hip, x, None, rng.normal(1, 0.2, 300), dtype, eps=eps)
+
+
+# ---------------------------------------------------------------------------
+# Scratch: what a call takes
+
+
+def free_bytes(dev):
+    dev.synchronize()
+    free, total = C.c_size_t(), C.c_size_t()
+    assert C.CDLL("libamdhip64.so").hipMemGetInfo(C.byref(free), C.byref(total)) == 0
+    return free.value
+
+
+def test_matmul_i8_in_units_takes_no_scratch_for_copies(hip):
+    m, n, k = 65, 2 ** 20, 512
+    dev = HipDevice(0)
+    try:
+        with Held(dev) as h:
+            x, w, y = h.up(np.ones((m, k), np.int8)), h.up(np.ones((n, k), np.int8)), dev.empty((m, n), np.float32)
+            h.bufs.append(y)
+            s = h.up(np.ones(n, np.float32))
+            before = free_bytes(dev)
+            dev.matmul_i8_resident(x.ptr, s.ptr, w.ptr, s.ptr, m, n, k, y.ptr)
+            assert before - free_bytes(dev) < 64 << 20
+            assert (y.to_host() == k).all()
+            # Weights that begin at an odd byte are copied, and the rows stay.
+            dev.matmul_i8_resident(x.ptr, s.ptr, w.ptr + 1, s.ptr, m, n - 1, k, y.ptr)
+            taken = before - free_bytes(dev)
+            assert n * k - (64 << 20) < taken < n * k + (64 << 20)
+            assert (y.to_host().ravel()[:m * (n - 1)] == k).all()
+    finally:
+        dev.close()
