@@ -745,8 +745,10 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
                                  size_t n_seqs, size_t seq_len, size_t heads, size_t key_heads, size_t d_key,
                                  size_t d_val, float scale, void* d_out, size_t ld_out, float* d_state_out, char* err,
                                  size_t err_len);
-/* Grows the context's scratch (synchronously) to what such a call needs, so
- * that it then allocates nothing and stays asynchronous.  More than 256
+/* Grows the context's scratch (synchronously) to what such a call needs at most,
+ * so that it then allocates nothing and stays asynchronous: with a key head for
+ * each head and copies of q, k and v, which calls of more than 4 tokens make of
+ * those whose rows and heads do not lie in units of 16 bytes.  More than 256
  * sequences of unequal lengths take a table of 8 (n_seqs + 1) bytes (12 where
  * the call is split), which goes there as linear attention's does. */
 int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len,

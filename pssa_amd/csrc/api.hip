@@ -2563,6 +2563,7 @@ namespace {
 struct DeltaPlan {
   std::vector<uint32_t> table;  // first tokens and chunks, where the arguments do not hold them
   size_t tokens = 0, longest = 0;
+  bool chunked = false;
   pssa::DeltaScratch scratch;
 
   // What is worked out ahead, row copies, the segments' states and transitions, then the table.
@@ -2583,8 +2584,8 @@ Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len
     same &= !lens || lens[i] == lens[0];
   }
   a.uniform_len = same ? (int)p.longest : -1;
-  const bool chunked = p.longest > (size_t)pssa::kDeltaSteps;
-  a.seg_chunks = chunked ? pssa::delta_segment(dtype, lens, n_seqs, p.longest, heads, d_key, d_val) : 0;
+  p.chunked = p.longest > (size_t)pssa::kDeltaSteps;
+  a.seg_chunks = p.chunked ? pssa::delta_segment(dtype, lens, n_seqs, p.longest, heads, d_key, d_val) : 0;
   const size_t seg = (size_t)a.seg_chunks * chunk;
   auto segments = [&](size_t len) { return seg ? std::max<size_t>(1, (len + seg - 1) / seg) : 1; };
   size_t chunks = 0, items = 0;
@@ -2610,7 +2611,7 @@ Status plan_delta(int dtype, const uint64_t* lens, size_t n_seqs, size_t seq_len
   a.chunks = (int)chunks;
   a.items = (int)items;
   a.uniform_segs = (int)segments(p.longest);
-  if (chunked) p.scratch = pssa::delta_scratch(dtype, p.tokens, chunks, n_seqs, seg ? items : 0, heads, d_key, d_val);
+  if (p.chunked) p.scratch = pssa::delta_scratch(dtype, chunks, n_seqs, seg ? items : 0, heads, d_key, d_val);
   return Status::Ok();
 }
 Status check_delta_heads(size_t heads, size_t d_key, size_t d_val) {
@@ -2701,6 +2702,12 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
     DeltaPlan plan;
     PSSA_RETURN_IF(plan_delta(dtype, lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
     const size_t tokens = plan.tokens;
+    if (plan.chunked) {
+      auto copied = [&](const void* p, size_t ld, size_t n, size_t width) {
+        return pssa::delta_in_units(dtype, p, ld, width) ? 0 : pssa::delta_copy_bytes(dtype, tokens, n, width);
+      };
+      plan.scratch.rows = copied(d_q, ld_q, key_heads, d_key) + copied(d_k, ld_k, key_heads, d_key) + copied(d_v, ld_v, heads, d_val);
+    }
     size_t n = 0;
     for (size_t ld : {ld_q, ld_k, ld_v, ld_out, ld_gates})
       PSSA_RETURN_IF(pssa::checked_count({tokens, ld}, &n, "delta rule"));
@@ -2754,6 +2761,8 @@ int pssa_hip_delta_rule_reserve(pssa_hip_ctx* ctx, int dtype, const uint64_t* le
     pssa::DeltaArgs a;
     DeltaPlan plan;
     PSSA_RETURN_IF(plan_delta(dtype, lens, n_seqs, seq_len, heads, d_key, d_val, a, plan));
+    if (plan.chunked)
+      plan.scratch.rows = 2 * pssa::delta_copy_bytes(dtype, plan.tokens, heads, d_key) + pssa::delta_copy_bytes(dtype, plan.tokens, heads, d_val);
     PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));

@@ -1160,10 +1160,6 @@ Status with_chunks(int dtype, int dk, F f) {
 
 size_t unit_of(int dtype) { return dtype == PSSA_HIP_BF16 ? 8 : 4; }  // elements of 16 bytes
 size_t whole(size_t width, size_t unit) { return (width + unit - 1) / unit * unit; }
-// Rows and heads in whole 16-byte units.
-bool in_units(const void* p, size_t ld, size_t width, size_t unit) {
-  return (uintptr_t)p % 16 == 0 && ld % unit == 0 && width % unit == 0;
-}
 
 template <class T>
 Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, int width, int& to, size_t tokens, char*& scratch) {
@@ -1174,7 +1170,7 @@ Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, in
   PSSA_LAUNCH_CHECK("delta_rows_kernel");
   p = scratch;
   ld = (size_t)heads * to;
-  scratch += (units * 16 + 255) & ~(size_t)255;
+  scratch += delta_copy_bytes(sizeof(T) == 2 ? PSSA_HIP_BF16 : PSSA_HIP_F32, tokens, heads, width);
   return Status::Ok();
 }
 
@@ -1182,13 +1178,19 @@ Status launch_rows(hipStream_t stream, const void*& p, size_t& ld, int heads, in
 
 int delta_chunk(int dtype) { return dtype == PSSA_HIP_BF16 ? Ahead<true>::C : Ahead<false>::C; }
 
+bool delta_in_units(int dtype, const void* p, size_t ld, size_t width) {
+  return (uintptr_t)p % 16 == 0 && ld % unit_of(dtype) == 0 && width % unit_of(dtype) == 0;
+}
+size_t delta_copy_bytes(int dtype, size_t tokens, size_t heads, size_t width) {
+  const size_t unit = unit_of(dtype);
+  return (tokens * heads * (whole(width, unit) / unit) * 16 + 255) & ~(size_t)255;
+}
+
 // What is worked out ahead takes 11 KiB a chunk and head (bf16; 4 KiB fp32):
 // past 1 GiB of it the heads run in several launches, and where a launch would
 // have 2^32 threads.
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key,
-                           size_t d_val) {
+DeltaScratch delta_scratch(int dtype, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key, size_t d_val) {
   DeltaScratch s;
-  const size_t size = dtype == PSSA_HIP_BF16 ? 2 : 4, unit = unit_of(dtype);
   const size_t one = chunks * 16 * (dtype == PSSA_HIP_BF16 ? Ahead<true>::kUnits : Ahead<false>::kUnits);
   const size_t walks = std::max(n_seqs, items) * ((d_val + 63) / 64 + (items ? (d_key + 63) / 64 : 0));
   s.heads_here = (int)std::max<size_t>(1, std::min({heads, ((size_t)1 << 30) / std::max<size_t>(one, 1), 5000000 / walks}));
@@ -1196,8 +1198,6 @@ DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t n_seq
   const size_t keys = d_key <= 32 ? 32 : d_key <= 64 ? 64 : 128;  // as the kernels hold them
   s.state = items * s.heads_here * keys * whole(d_val, 16) * 4;
   s.move = items * s.heads_here * keys * keys * 4;
-  s.rows = 2 * ((tokens * heads * whole(d_key, unit) * size + 255) & ~(size_t)255) +
-           ((tokens * heads * whole(d_val, unit) * size + 255) & ~(size_t)255);
   return s;
 }
 
@@ -1252,11 +1252,10 @@ Status launch_delta_rule(hipStream_t stream, int dtype, DeltaArgs a, size_t toke
   a.seg_state = reinterpret_cast<float*>(scratch + s.ahead + s.rows);
   a.seg_move = reinterpret_cast<float*>(scratch + s.ahead + s.rows + s.state);
   char* rows = scratch + s.ahead;
-  const size_t unit = unit_of(dtype);
   const bool b16 = dtype == PSSA_HIP_BF16;
   auto in_place = [&](const void*& p, size_t& ld, int heads, int width, int& to) -> Status {
     to = width;
-    if (in_units(p, ld, width, unit)) return Status::Ok();
+    if (delta_in_units(dtype, p, ld, width)) return Status::Ok();
     return b16 ? launch_rows<Bf16>(stream, p, ld, heads, width, to, tokens, rows)
                : launch_rows<float>(stream, p, ld, heads, width, to, tokens, rows);
   };

@@ -164,16 +164,19 @@ struct DeltaArgs {
   uint32_t inline_items[kDeltaInline + 1] = {};
 };
 // Tokens of a chunk of a type, and the scratch of a call: what is worked out
-// ahead for the heads of one launch, and copies of rows that do not lie in
-// units of 16 bytes.
+// ahead for the heads of one launch, the copies of rows that do not lie in
+// units of 16 bytes, which the caller adds, and the segments' states.
 int delta_chunk(int dtype);
 struct DeltaScratch {
   size_t ahead = 0, rows = 0, state = 0, move = 0;  // bytes
   int heads_here = 0;                               // heads of a launch
 };
 // `items` segments, 0 where the call is not split.
-DeltaScratch delta_scratch(int dtype, size_t tokens, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key,
-                           size_t d_val);
+DeltaScratch delta_scratch(int dtype, size_t chunks, size_t n_seqs, size_t items, size_t heads, size_t d_key, size_t d_val);
+// Rows of heads of `width` elements that a call in chunks reads as they are,
+// and the bytes of a copy of those that it does not.
+bool delta_in_units(int dtype, const void* p, size_t ld, size_t width);
+size_t delta_copy_bytes(int dtype, size_t tokens, size_t heads, size_t width);
 // Chunks of a segment where a call of these sizes is split, else 0.
 int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val);
 Status init_delta_attributes();

@@ -1105,3 +1105,44 @@ def test_matmul_i8_in_units_takes_no_scratch_for_copies(hip):
             assert (y.to_host().ravel()[:m * (n - 1)] == k).all()
     finally:
         dev.close()
+
+
+def test_delta_rule_takes_scratch_for_the_rows_it_copies(hip):
+    n, heads, dk, dv = 2 ** 17, 8, 128, 128
+    dev = HipDevice(0)
+    try:
+        with Held(dev) as h:
+            q, k, v = h.up(np.zeros((n + 1, dk), np.uint16)), h.up(np.zeros((n + 1, dk), np.uint16)), h.up(np.zeros((n + 1, heads * dv), np.uint16))
+            g, out = h.up(np.zeros((n, 2 * heads), np.float32)), dev.empty((n, heads * dv), np.uint16)
+            h.bufs.append(out)
+
+            def call(off):
+                dev.delta_rule_resident(q.ptr + off, k.ptr + off, v.ptr + off, g.ptr, g.ptr + 4 * heads, "bf16", heads, dk, dv,
+                                        out.ptr, n_seqs=1, seq_len=n, key_heads=1, ld_gates=2 * heads)
+
+            before = free_bytes(dev)
+            call(0)
+            own = before - free_bytes(dev)
+            # 11 KiB a chunk and head; the states and transitions of at most a segment for two chunks.
+            assert own < n // 64 * heads * (11 << 10) + n // 128 * heads * 2 * (dk * dv * 4) + (64 << 20)
+            call(2)
+            copies = 2 * n * dk * 2 + n * heads * dv * 2
+            assert copies - (32 << 20) < before - free_bytes(dev) - own < copies + (32 << 20)
+    finally:
+        dev.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,heads,key_heads,dk,dv", [([300, 70], 4, 2, 64, 64), ([2000], 2, 1, 100, 72), ([65], 3, 1, 7, 5)])
+def test_delta_rule_of_odd_rows_in_a_context_of_its_own(hip, dtype, lens, heads, key_heads, dk, dv):
+    """The first call of a context: its scratch is what this call takes."""
+    c = delta_case(np.random.default_rng(81), lens, heads, key_heads, dk, dv, True)
+    want = run_delta(hip, c, lens, heads, key_heads, dk, dv, dtype, 0.5, reserve=True)
+    for layout in ("odd", "row"):
+        dev = HipDevice(0)
+        try:
+            got = run_delta(dev, c, lens, heads, key_heads, dk, dv, dtype, 0.5, layout=layout)
+            for a, b in zip(got[3:], want[3:]):
+                np.testing.assert_array_equal(a, b)
+        finally:
+            dev.close()
