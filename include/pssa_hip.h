@@ -782,7 +782,7 @@ int pssa_hip_quantize_i8_resident(pssa_hip_ctx* ctx, int dtype, const void* d_x,
  * row [m] and channel [n]; rows at any byte, strides ld_x, ld_w >= k.  The sums
  * are exact (k <= 131071), rounded once to fp32, and y (y_dtype, stride ld_y
  * >= n) has two more roundings for the scales and one to bf16.  m <= 2^20;
- * strides below 2^31.  y must not overlap the other arrays. */
+ * strides below 2^31; rows and weights that are copied (below) up to some 64 GiB.  y must not overlap the other arrays. */
 int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scales,
                                 const int8_t* d_w, size_t ld_w, const float* d_w_scales, size_t m, size_t n, size_t k,
                                 void* d_y, int y_dtype, size_t ld_y, char* err, size_t err_len);
@@ -815,7 +815,9 @@ int pssa_hip_beam_select_reserve(pssa_hip_ctx* ctx, size_t groups, size_t beams,
  * i of group g at (g*n_in + i)*ld_src bytes, (g*n_out + j)*ld_dst bytes).  A
  * row whose parent is not below n_in (PSSA_HIP_NO_TOKEN) stays as it is.  The
  * rows may be reordered in place (d_dst = d_src, n_out = n_in, equal strides)
- * and must not overlap otherwise.  n_in, n_out <= 64. */
+ * and must not overlap otherwise.  n_in, n_out <= 64; rows of up to some 2^32
+ * pieces of 16 bytes, of 4 where 16 do not divide them or more than 16 rows are
+ * reordered in place, else of single bytes. */
 int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t ld_src, void* d_dst, size_t ld_dst,
                                   size_t row_bytes, size_t groups, size_t n_in, const uint32_t* d_parents,
                                   size_t n_out, char* err, size_t err_len);

@@ -2706,7 +2706,9 @@ int pssa_hip_delta_rule_resident(pssa_hip_ctx* ctx, int dtype, const void* d_q, 
       auto copied = [&](const void* p, size_t ld, size_t n, size_t width) {
         return pssa::delta_in_units(dtype, p, ld, width) ? 0 : pssa::delta_copy_bytes(dtype, tokens, n, width);
       };
-      plan.scratch.rows = copied(d_q, ld_q, key_heads, d_key) + copied(d_k, ld_k, key_heads, d_key) + copied(d_v, ld_v, heads, d_val);
+      const size_t q = copied(d_q, ld_q, key_heads, d_key), k = copied(d_k, ld_k, key_heads, d_key), v = copied(d_v, ld_v, heads, d_val);
+      PSSA_RETURN_IF(need(std::max({q, k, v}) / 16 <= pssa::kMostThreads, "delta rule: too large for rows not in units of 16 bytes"));
+      plan.scratch.rows = q + k + v;
     }
     size_t n = 0;
     for (size_t ld : {ld_q, ld_k, ld_v, ld_out, ld_gates})
@@ -2869,6 +2871,10 @@ int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_
     for (const Rows& r : {Rows{d_x, m, ld_x, k}, Rows{d_w, n, ld_w, k}, Rows{d_x_scales, 1, 0, m * 4},
                           Rows{d_w_scales, 1, 0, n * 4}})
       PSSA_RETURN_IF(need(apart(r, y), "8-bit product: the output overlaps its inputs"));
+    const bool copy_x = !pssa::i8_in_units(d_x, ld_x, k), copy_w = !pssa::i8_in_units(d_w, ld_w, k);
+    const pssa::I8Plan plan = pssa::i8_plan(m, n, k, copy_x, copy_w);
+    PSSA_RETURN_IF(need(m <= pssa::kI8FewRows || ((copy_x ? m : 0) + (copy_w ? n : 0)) * ((k + 15) / 16) <= pssa::kMostThreads,
+                        "8-bit product: too large for rows not in units of 16 bytes"));
     PSSA_RETURN_IF(check_ctx(ctx));
     pssa::I8Args a;
     a.x = d_x;
@@ -2882,7 +2888,6 @@ int pssa_hip_matmul_i8_resident(pssa_hip_ctx* ctx, const int8_t* d_x, size_t ld_
     a.m = (int)m;
     a.n = (int)n;
     a.k = (int)k;
-    const pssa::I8Plan plan = pssa::i8_plan(m, n, k, !pssa::i8_in_units(d_x, ld_x, k), !pssa::i8_in_units(d_w, ld_w, k));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     PSSA_RETURN_IF(grow_scratch(ctx, plan.bytes(), false));
@@ -2972,7 +2977,6 @@ int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t l
     const bool in_place = d_src == d_dst && n_in == n_out && ld_src == ld_dst;
     PSSA_RETURN_IF(need(in_place || apart(src, dst), "beam states: the rows overlap"));
     PSSA_RETURN_IF(need(apart(dst, Rows{d_parents, 1, 0, groups * n_out * 4}), "beam states: the rows overlap the parents"));
-    PSSA_RETURN_IF(check_ctx(ctx));
     pssa::GatherArgs a;
     a.src = d_src;
     a.dst = d_dst;
@@ -2983,6 +2987,8 @@ int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t l
     a.n_in = (int)n_in;
     a.n_out = (int)n_out;
     a.parents = d_parents;
+    PSSA_RETURN_IF(need(row_bytes / pssa::beam_gather_piece(a) <= pssa::kMostThreads, "beam states: too large"));
+    PSSA_RETURN_IF(check_ctx(ctx));
     std::lock_guard<std::mutex> g(ctx->mu);
     PSSA_HIP_TRY(hipSetDevice(ctx->device));
     return pssa::launch_beam_gather(ctx->stream, a);

@@ -406,7 +406,6 @@ __global__ __launch_bounds__(kThreads) void beam_feed_kernel(const uint32_t* tok
 template <class V, int MOST>
 Status launch_pieces(hipStream_t stream, const GatherArgs& a) {
   const size_t pieces = a.row_bytes / sizeof(V);
-  if (pieces >> 32) return Status::Invalid("beam states: too large");
   const dim3 grid((uint32_t)((pieces + kThreads - 1) / kThreads), (uint32_t)std::min(a.groups, 65535));
   beam_gather_kernel<V, MOST><<<grid, kThreads, 0, stream>>>(a);
   PSSA_LAUNCH_CHECK("beam_gather_kernel");
@@ -451,14 +450,18 @@ Status launch_beam_select(hipStream_t stream, int dtype, const BeamArgs& a, size
 
 // 16 bytes a thread and row up to 16 rows (64 registers), more rows in parts
 // of 16, but for those that are reordered in place: 4 bytes of up to 64 rows.
+size_t beam_gather_piece(const GatherArgs& a) {
+  if (a.row_bytes % 16 == 0 && (a.n_out <= 16 || a.src != a.dst)) return 16;
+  return a.row_bytes % 4 == 0 ? 4 : 1;
+}
 Status launch_beam_gather(hipStream_t stream, const GatherArgs& a) {
-  const bool in_place = a.src == a.dst;
-  if (a.row_bytes % 16 == 0 && (a.n_out <= 16 || !in_place)) {
+  const size_t piece = beam_gather_piece(a);
+  if (piece == 16) {
     if (a.n_out <= 4) return launch_pieces<u32x4_t, 4>(stream, a);
     if (a.n_out <= 8) return launch_pieces<u32x4_t, 8>(stream, a);
     return launch_pieces<u32x4_t, 16>(stream, a);
   }
-  if (a.row_bytes % 4 == 0) return launch_pieces<uint32_t, kMaxBeams>(stream, a);
+  if (piece == 4) return launch_pieces<uint32_t, kMaxBeams>(stream, a);
   return launch_pieces<uint8_t, kMaxBeams>(stream, a);
 }
 

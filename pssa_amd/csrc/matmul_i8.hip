@@ -515,7 +515,6 @@ Status launch_matmul_i8(hipStream_t stream, int y_dtype, I8Args a, const I8Plan&
     Packed x{a.x, a.ld_x, reinterpret_cast<int8_t*>(at), i8_in_units(a.x, a.ld_x, (size_t)a.k) ? 0 : a.m};
     Packed w{a.w, a.ld_w, reinterpret_cast<int8_t*>(at + ((x.rows * packed_ld((size_t)a.k) + 255) & ~(size_t)255)), i8_in_units(a.w, a.ld_w, (size_t)a.k) ? 0 : a.n};
     if (x.rows || w.rows) {
-      if (((size_t)x.rows + w.rows) * units >> 32) return Status::Invalid("8-bit product: too large for rows not in units of 16 bytes");
       i8_pack_kernel<<<(uint32_t)((((size_t)x.rows + w.rows) * units + 255) / 256), 256, 0, stream>>>(x, w, a.k, (int)units);
       PSSA_LAUNCH_CHECK("i8_pack_kernel");
     }

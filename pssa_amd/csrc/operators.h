@@ -7,6 +7,9 @@
 
 namespace pssa {
 
+// Threads of a launch along x: below 2^32, in workgroups of 256.
+constexpr size_t kMostThreads = ((size_t)1 << 32) - 256;
+
 // Dynamic LDS above the default limit, once for each device.
 Status init_w4_attributes();
 
@@ -216,6 +219,8 @@ struct GatherArgs {
   int groups = 0, n_in = 0, n_out = 0;
   const uint32_t* parents = nullptr;  // [groups, n_out]; a row whose parent is not below n_in stays as it is
 };
+// Bytes of a row that a thread moves.
+size_t beam_gather_piece(const GatherArgs& a);
 Status launch_beam_gather(hipStream_t stream, const GatherArgs& a);
 // Rows 0 .. groups-1 copied to rows g * beams .. + beams - 1 of the same array.
 Status launch_beam_spread(hipStream_t stream, void* rows, size_t words, size_t ld, size_t groups, size_t beams);

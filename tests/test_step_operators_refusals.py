@@ -165,3 +165,27 @@ def test_norms_of_too_many_rows_refuse(width):
         refused(fn, changed(base, rows=most), "null context")
         for rows in (most + 1, 2 ** 31 - 2048, 2 ** 31 - 1):
             refused(fn, changed(base, rows=rows), "too large")
+
+
+def test_launches_past_32_bits_refuse():
+    """A thread moves a piece of a row or copies 16 bytes of it: what 2^32 threads would not hold is refused ahead."""
+    most = 2 ** 32 - 256
+    apart, place = dict(dst=1 << 50, n_in=2, n_out=2), dict(dst=P, n_in=17, n_out=17)
+    for size, where, message in ((16 * most, apart, "null context"), (16 * (most + 1), apart, "too large"),
+                                 (4 * (most - 1), apart, "null context"), (4 * (most + 1), apart, "too large"),
+                                 (4 * most, place, "null context"), (4 * (most + 4), place, "too large"),
+                                 (most - 1, apart, "null context"), (most + 1, apart, "too large")):
+        base = dict(GATHER, parents=1 << 56, groups=1, row_bytes=size, ld_src=size, ld_dst=size)
+        refused(_abi.lib().pssa_hip_beam_gather_resident, changed(base, **where), message)
+    far = dict(I8, x=P + 1, w=1 << 50, y=1 << 55, m=100, k=131071, ld_x=131071, ld_w=131071, ld_y=1 << 24)
+    most = (2 ** 32 - 256) // 8192 - 100  # channels, beside 100 rows
+    for n, message in ((most, "null context"), (most + 1, "units of 16 bytes")):
+        refused(_abi.lib().pssa_hip_matmul_i8_resident, changed(far, n=n, x_scales=1 << 57, w_scales=1 << 58), message)
+    refused(_abi.lib().pssa_hip_matmul_i8_resident,
+            changed(far, n=most + 1, k=131056, ld_x=131072, ld_w=131072, x=P, x_scales=1 << 57, w_scales=1 << 58), "null context")
+    rows = dict(DELTA, dtype=_abi.BF16, q=1 << 50, k=1 << 51, v=1 << 52, out=1 << 53, log_decay=1 << 54, beta=1 << 55, state_out=None,
+                heads=64, key_heads=1, d_key=16, d_val=4096, ld_q=16, ld_k=16, ld_v=64 * 4096, ld_out=64 * 4096, ld_gates=64, n_seqs=1)
+    most = (2 ** 32 - 256) // (64 * 512)
+    refused(_abi.lib().pssa_hip_delta_rule_resident, changed(rows, seq_len=most + 1), "null context")
+    refused(_abi.lib().pssa_hip_delta_rule_resident, changed(rows, seq_len=most, v=(1 << 52) + 2), "null context")
+    refused(_abi.lib().pssa_hip_delta_rule_resident, changed(rows, seq_len=most + 1, v=(1 << 52) + 2), "units of 16 bytes")
