@@ -796,7 +796,11 @@ int pssa_hip_matmul_i8_reserve(pssa_hip_ctx* ctx, size_t m, size_t n, size_t k, 
  *   scores[g][b] + log softmax(logits[row])[v]
  * over b and v, in descending order, equal ones by beam, then by token:
  * d_parents (the beam b), d_tokens (v) and d_out_scores [groups, keep].  Sums
- * and values are computed in 64 bits, of exponentials in fp32, and rounded once.  d_last [groups, beams] or
+ * and values are computed in 64 bits, of exponentials in fp32, and rounded once.
+ * A beam's candidates are the `keep` largest logits of each part of its row (of
+ * 1024 tokens or more, one part where there are fewer): where a score some 2^52
+ * times the logits' differences makes their values one, the larger logits are
+ * kept, not the lower tokens.  d_last [groups, beams] or
  * NULL: a beam whose last token is `eos` has ended and has one candidate, eos
  * with its score as it is; its logits are not read.  A beam whose score is not
  * finite, or whose logits hold a NaN or +inf or nothing but -inf, has none, and
@@ -832,7 +836,8 @@ int pssa_hip_beam_gather_resident(pssa_hip_ctx* ctx, const void* d_src, size_t l
  * (PSSA_HIP_NO_TOKEN: none does) have ended, keep their score and repeat it.
  * out_ids [n_groups, beams, steps] are the tokens of the beams that are left,
  * best first, out_scores [n_groups, beams] their summed log probabilities; a
- * beam that never had a candidate holds PSSA_HIP_NO_TOKEN and -inf.  The lanes
+ * beam that never had a candidate holds PSSA_HIP_NO_TOKEN and -inf, one whose
+ * model's logits are not finite at a step has both from that step on.  The lanes
  * are left at their last step: the last token of a beam is not yet consumed.
  * beams <= 64; steps <= 2^20.  Lanes with a repetition penalty or a sampling
  * temperature are PSSA_HIP_EUNSUPPORTED. */

@@ -1146,3 +1146,81 @@ def test_delta_rule_of_odd_rows_in_a_context_of_its_own(hip, dtype, lens, heads,
                 np.testing.assert_array_equal(a, b)
         finally:
             dev.close()
+
+
+# ---------------------------------------------------------------------------
+# Two contexts, and values that are one
+
+
+def test_two_contexts_run_at_once(hip):
+    """Calls that take scratch, enqueued in turn on two contexts without a wait between them: each as if it ran alone."""
+    rng = np.random.default_rng(91)
+    m, n, k, heads, vocab, steps = 100, 300, 5001, 2, 9000, 6
+    lens = [2100, 40, 700]
+    t = sum(lens)
+    host = []
+    for _ in range(2):  # other values for each
+        c = delta_case(rng, lens, heads, 1, 64, 64, True)
+        host.append(dict(x=rng.integers(-128, 128, (m, k)).astype(np.int8), w=rng.integers(-128, 128, (n, k)).astype(np.int8),
+                         s=rng.uniform(0.1, 1, n).astype(np.float32), q=to_bf16(c["q"].reshape(t, 64))[0], kk=to_bf16(c["k"].reshape(t, 64))[0],
+                         v=to_bf16(c["v"].reshape(t, heads * 64))[0], g=np.concatenate([c["g"], c["beta"]], 1).astype(np.float32),
+                         state=c["state"], z=rng.normal(0, 2, (8, vocab)).astype(np.float32), score=rng.normal(-9, 1, 8).astype(np.float32)))
+    dev = [HipDevice(0), HipDevice(0)]
+    held = [Held(d) for d in dev]
+    try:
+        arrays = [{x: h.up(a) for x, a in of.items()} for h, of in zip(held, host)]
+
+        def outputs(h):
+            return dict(y=h.new((m, n), np.float32, 0), o=h.new((t, heads * 64), np.uint16, 0), S=h.new((len(lens), heads, 64, 64), np.float32, 0),
+                        par=h.new((2, 4), np.uint32, 0), tok=h.new((2, 4), np.uint32, 0), best=h.new((2, 4), np.float32, 0))
+
+        def calls(d, a, o):
+            yield lambda: d.matmul_i8_resident(a["x"].ptr, a["s"].ptr, a["w"].ptr, a["s"].ptr, m, n, k, o["y"].ptr)
+            yield lambda: d.delta_rule_resident(a["q"].ptr, a["kk"].ptr, a["v"].ptr, a["g"].ptr, a["g"].ptr + 4 * heads, "bf16", heads, 64,
+                                                64, o["o"].ptr, lens, key_heads=1, ld_gates=2 * heads, state_in_ptr=a["state"].ptr,
+                                                state_out_ptr=o["S"].ptr)
+            yield lambda: d.beam_select_resident(a["z"].ptr, "f32", 2, 4, vocab, a["score"].ptr, 4, o["par"].ptr, o["tok"].ptr, o["best"].ptr)
+
+        alone = []
+        for d, h, a in zip(dev, held, arrays):
+            d.matmul_i8_reserve(m, n, k)
+            d.delta_rule_reserve("bf16", heads, 64, 64, lens)
+            d.beam_select_reserve(2, 4, vocab, 4)
+            o = outputs(h)
+            for call in calls(d, a, o):
+                call()
+                d.synchronize()
+            alone.append({x: b.to_host() for x, b in o.items()})
+        together = [[outputs(h) for _ in range(steps)] for h in held]
+        for d in dev:
+            d.synchronize()
+        for i in range(steps):
+            for pair in zip(*(calls(d, a, o[i]) for d, a, o in zip(dev, arrays, together))):
+                for call in pair:
+                    call()
+        for d in dev:
+            d.synchronize()
+        for want, outs in zip(alone, together):
+            for o in outs:
+                for x, b in o.items():
+                    np.testing.assert_array_equal(b.to_host(), want[x], err_msg=x)
+        want = (host[0]["x"].astype(np.float64) @ host[0]["w"].astype(np.float64).T) * host[0]["s"][:m, None].astype(np.float64) * host[0]["s"].astype(np.float64)
+        within(alone[0]["y"], want, np.abs(want) * 3.01 * U32, "product")
+    finally:
+        for h in held:
+            h.__exit__()
+        for d in dev:
+            d.close()
+
+
+@pytest.mark.parametrize("beams,vocab,keep", [(4, 40, 16), (3, 1000, 64), (2, 10, 16)])
+def test_beam_select_keeps_the_larger_of_logits_whose_values_are_one(hip, beams, vocab, keep):
+    """A score that rounds the logits away: the first beams' places, of a beam its largest logits, in the tokens' order."""
+    z = np.random.default_rng(vocab).permutation(beams * vocab).reshape(1, beams, vocab).astype(np.float32) * 2.0 ** -20
+    with Held(hip) as h:
+        dz, ds = h.up(z), h.up(np.full((1, beams), -1e14, np.float32))
+        par, tok, out = h.new(keep, np.uint32, 7), h.new(keep, np.uint32, 7), h.new(keep, np.float32, 7.0)
+        hip.beam_select_resident(dz.ptr, "f32", 1, beams, vocab, ds.ptr, keep, par.ptr, tok.ptr, out.ptr)
+        hip.synchronize()
+        want = [b * vocab + i for b in range(beams) for i in sorted(np.argsort(-z[0, b])[:keep])][:keep]
+        np.testing.assert_array_equal(par.to_host().astype(np.int64) * vocab + tok.to_host(), want)
