@@ -197,8 +197,7 @@ __device__ __forceinline__ Place place_of(const DeltaArgs& a, int chunk) {
 
 // What is worked out ahead for a chunk and head, in units of 16 bytes: T's
 // tiles of 16 x 16 where its triangle holds anything, in fp32 for both types,
-// then of the tokens e^G, e^(G_n - G) and G itself, in 64 bits since differences
-// of it count.  T as two bf16 parts had the products for U at half the time (a
+// then of the tokens e^G, e^(G_n - G) and G itself (Power).  T as two bf16 parts had the products for U at half the time (a
 // chunk 0.4 us of 2.6), but what they drop comes back in every chunk's state,
 // and grows where keys are alike: states were off by 5e-6 of their size, and
 // are by 2e-7 so.  P's fragments are 16 tokens by 32 in three parts (bf16), 16 by
@@ -245,10 +244,26 @@ __device__ __forceinline__ f32x4_t tile_product(const u32x4_t* sx, int x, const 
   return s;
 }
 
+// e^G, G summed in 64 bits, as 2^(part + whole), part in +-1/2: in one fp32
+// number the whole part would leave the exponential of a difference off by up
+// to 22 roundings (at e^-29), so it is by 2.
+struct Power {
+  float part;
+  int whole;
+};
+__device__ __forceinline__ Power power_of(double g) {
+  const double d = g * kLog2e, whole = rint(d);
+  return Power{(float)(d - whole), (int)whole};
+}
+// From LDS as 64 bits of a type of its own: read as any other, the compiler has
+// it wait for the loads into LDS that are on their way.
+__device__ __forceinline__ Power power_in(double bits) {
+  return Power{__int_as_float(__double2loint(bits)), __double2hiint(bits)};
+}
 // e^(gi - gj) where `on`, else 0: no branch, as the loads of either would wait in it.
-__device__ __forceinline__ float decay_between(double gi, double gj, bool on) {
-  const float d = (float)((gi - gj) * kLog2e);
-  return __builtin_amdgcn_exp2f(on ? d : -INFINITY);
+__device__ __forceinline__ float decay_between(const Power& gi, const Power& gj, bool on) {
+  const float part = gi.part - gj.part;
+  return ldexpf(__builtin_amdgcn_exp2f(on ? part : -INFINITY), gi.whole - gj.whole);
 }
 
 // A chunk of one head, a wave for each 16 tokens.  A's triangle lies in LDS;
@@ -264,7 +279,7 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
   constexpr int C = Out::C, NT = Out::kTiles, LD = C + 4, N = 16 / (int)sizeof(T), ROW = DKP / N;
   __shared__ __attribute__((aligned(256))) u32x4_t s_k[C * ROW];
   __shared__ __attribute__((aligned(16))) float s_a[C * LD];
-  __shared__ double s_g[C];
+  __shared__ Power s_g[C];
   __shared__ float s_beta[C];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   const int head = a.head0 + blockIdx.y, key_head = head / (a.heads / a.key_heads);
@@ -289,12 +304,13 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
     }
     const double all = __shfl(sum, C - 1, 64);
     if (lane < C) {
-      s_g[lane] = sum;
+      const Power g_i = power_of(sum);
+      s_g[lane] = g_i;
       s_beta[lane] = on ? a.beta[(pl.tok + lane) * a.ld_gates + head] : 0.0f;
       float* f = reinterpret_cast<float*>(out + Out::kGamma);
-      f[lane] = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
-      f[C + lane] = __builtin_amdgcn_exp2f((float)((all - sum) * kLog2e));
-      reinterpret_cast<double*>(out + Out::kSum)[lane] = sum;
+      f[lane] = decay_between(g_i, Power{0.0f, 0}, true);
+      f[C + lane] = decay_between(power_of(all), g_i, true);
+      reinterpret_cast<Power*>(out + Out::kSum)[lane] = g_i;
     }
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
@@ -304,7 +320,7 @@ __global__ __launch_bounds__(B16 ? 256 : 128) void delta_ahead_kernel(DeltaArgs 
   for (int i = 0; i < (NT * (NT + 1) / 2 + NT - 1) / NT; ++i) {
     const int at = min(i * NT + wave, NT * (NT + 1) / 2 - 1), r = triangle_row(at), c = triangle_col(at);
     const f32x4_t s = tile_product<B16, DKP>(s_k, 16 * r, s_k, 16 * c, lane);
-    const double gk = s_g[16 * c + col];
+    const Power gk = s_g[16 * c + col];
     float w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -635,12 +651,12 @@ __global__ __launch_bounds__(64 * (kWalkers + kHelpers<MODE>), MODE != DR_LOCAL 
         const int at = i ? 8 + helper - 4 : helper, r = triangle_row(at), c = triangle_col(at);
         if (at < 8 * i || at >= NT * (NT + 1) / 2) continue;  // uniform
         f32x4_t p = tile_product<B16, DKP>(sK, 16 * c, sQ, 16 * r, lane);
-        const double gq = sum[16 * r + col];
+        const Power gq = power_in(sum[16 * r + col]);
         float d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = 16 * c + 4 * quad + e;
-          d[e] = a.scale * decay_between(gq, sum[key], 16 * r + col >= key);
+          d[e] = a.scale * decay_between(gq, power_in(sum[key]), 16 * r + col >= key);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) p[e] = 16 * r + col >= 16 * c + 4 * quad + e ? p[e] * d[e] : 0.0f;

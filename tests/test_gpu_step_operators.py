@@ -1224,3 +1224,31 @@ def test_beam_select_keeps_the_larger_of_logits_whose_values_are_one(hip, beams,
         hip.synchronize()
         want = [b * vocab + i for b in range(beams) for i in sorted(np.argsort(-z[0, b])[:keep])][:keep]
         np.testing.assert_array_equal(par.to_host().astype(np.int64) * vocab + tok.to_host(), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pace", [0.01, 0.3, 0.9])
+def test_delta_rule_decays_to_the_last_bits(hip, dtype, pace):
+    """The decays themselves: of a state of ones that nothing is added to, and of ones that tokens add.  An exponential
+    is within a step of fp32 and the rounding of a fraction, three half steps; a chunk's two products and what the chunks
+    before it left are four of them."""
+    rng = np.random.default_rng(int(pace * 100))
+    n, dk, dv = 64, 64, 64  # two chunks in fp32
+    g = -pace * rng.uniform(0.8, 1.2, (n, 1))
+    total = np.cumsum(g.astype(np.float32).astype(np.float64))
+    tol = 4 * 4 * U32 + (U16 if dtype == "bf16" else 0)
+    # The state.
+    q = np.zeros((n, 1, dk))
+    q[:, 0, 5] = 1
+    c = dict(q=q, k=np.zeros((n, 1, dk)), v=np.zeros((n, 1, dv)), g=g, beta=np.zeros((n, 1)), state=np.ones((1, 1, dk, dv), np.float32))
+    _, _, _, out, S = run_delta(hip, c, [n], 1, 1, dk, dv, dtype, 1.0)
+    within(out[:, 0], np.exp(total)[:, None] + 0 * out[:, 0], tol * np.exp(total)[:, None], "state")
+    within(S[0, 0], np.exp(total[-1]) + 0 * S[0, 0], 16 * U32 * np.exp(total[-1]), "last state")
+    # Updates: token j adds ones to its own row, token i reads that of one before it.
+    at = rng.integers(0, np.arange(n) + 1)
+    c = dict(q=np.eye(dk)[at, None], k=np.eye(dk)[:n, None], v=np.ones((n, 1, dv)), g=g, beta=np.ones((n, 1)), state=None)
+    _, _, _, out, S = run_delta(hip, c, [n], 1, 1, dk, dv, dtype, 1.0)
+    want = np.exp(total - total[at])
+    within(out[:, 0], want[:, None] + 0 * out[:, 0], tol * want[:, None], "updates")
+    want = np.exp(total[-1] - total)
+    within(S[0, 0], want[:, None] + 0 * S[0, 0], 16 * U32 * want[:, None], "states of updates")
