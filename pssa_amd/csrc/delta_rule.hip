@@ -1233,9 +1233,10 @@ Status init_delta_attributes() {
 // (at heads of 64 and the machine's 256 compute units, a workgroup each; wider
 // heads take half as much again of all, which leaves the choice).  A call is
 // split where that makes it the faster, into segments of whichever length
-// costs least: ten calls of 600 to 16 x 1000 tokens ran within 5% of the best of
-// segments of 4, 8, 12, 16 and 32 chunks and of none (8192 tokens, 8 heads of 128:
-// 132 us, unsplit 480; 600 tokens, 2 heads of 64: 29 us, unsplit 34).
+// costs least: nine of ten calls of 600 to 16 x 1024 tokens ran within 5% of the
+// best of segments of 2, 4, 6, 8, 12, 16 and 32 chunks and of none, one within 9
+// (8192 tokens, 8 heads of 128: 137 us, unsplit 569; 600 tokens, 2 heads of 64: 31
+// us, unsplit 38).
 constexpr size_t kComputeUnits = 256;
 int delta_segment(int dtype, const uint64_t* lens, size_t n_seqs, size_t longest, size_t heads, size_t d_key, size_t d_val) {
   const size_t chunk = (size_t)delta_chunk(dtype), most = (longest + chunk - 1) / chunk;

@@ -75,7 +75,7 @@ __device__ __forceinline__ i32x4_t load16(const int8_t* p, int left, int k) {
 
 // ---------------------------------------------------------------- few rows
 // A wave multiplies 16 MT rows by 16 NC channels over its part of k: WK waves
-// of a workgroup share the channels, 4 / WK... of them lie side by side, and
+// of a workgroup share the channels, 4 / WK such groups lie side by side, and
 // the parts meet in LDS.  Rows at any dword, or (ODD) at any byte.  Bound by the
 // weights' way from memory (24 x 8192 x 8192: 16 us, 4.2 TB/s) or by the launch (1 x
 // 16384 x 768: 5.1 us).
@@ -188,8 +188,8 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int& 
 // the slab R - 1 ahead go out over R steps between the products: the L1 takes
 // 16 cycles for each, all at once they held the products up.  At the end a
 // wave's 32 rows at a time turn in LDS, so that what it stores is whole lines.
-// 8192 x 8192 x 8192: 475 to 550 us, by the card's clock, which falls to 1.7
-// GHz under this load (2.0 to 2.3 POP/s; stores of 8 bytes a row took 70 us
+// 8192 x 8192 x 8192: 455 to 550 us, by the card's clock, which falls to 1.7
+// GHz under this load (2.0 to 2.4 POP/s; stores of 8 bytes a row took 70 us
 // more, rows whose units lay two to a bank 20).
 template <class T, int BM, int BN, int WM, int WN, int R>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a, int tiles_m, int tiles_n) {
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_i8_tiles_kernel(I8Args a,
     for (int t = 0; t < TM; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[b][t][e] = 0;
-  // Slab s is there for all waves, and s - 1 read by them.  Slabs behind the last are of zeros.
+  // Slab s is there for all waves, and s - 1 read by them.  Slabs behind the last are the last again.
   auto meet = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(vmcnt_only((R - 2) * PER) & kLdsDone);
